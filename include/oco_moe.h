@@ -58,7 +58,11 @@ typedef enum {
 typedef enum { OCO_ARCH_GPT_OSS = 0, OCO_ARCH_NEMOTRON = 1, OCO_ARCH_QWEN = 2 } oco_arch;
 
 /* GGUF tensor type codes (reference `src/tensor.rs:9-22`). */
-typedef enum { OCO_FMT_Q4_0 = 2, OCO_FMT_Q4_K = 12, OCO_FMT_MXFP4 = 39 } oco_weight_format;
+typedef enum {
+    OCO_FMT_Q4_0 = 2, OCO_FMT_Q4_K = 12, OCO_FMT_MXFP4 = 39,
+    OCO_FMT_F8_E4M3 = 128   /* no GGUF type: e4m3 codes with f32 scales of 128 x 128 blocks beside them (dense products
+                               and oco_moe_f8_plan; the reference has no 8-bit floating-point weights) */
+} oco_weight_format;
 
 /* Geometry lowered once per model, as the reference's `ExpertPlan::new`
  * (feed_forward.rs:43-72) and `ReluExpertPlan::new` (compute/nemotron.rs:142-184). */
@@ -360,10 +364,134 @@ void oco_dense_plan_destroy(oco_dense_plan* plan);
 size_t oco_dense_workspace_bytes(const oco_dense_plan* plan, int max_rows);
 int oco_dense_bind_workspace(oco_dense_plan* plan, void* workspace, size_t bytes, int max_rows);
 int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* weights);
+/* OCO_FMT_F8_E4M3 (OCO_DENSE_PROJECTION and OCO_DENSE_FFN_SILU_GATE; hidden and ffn multiples of 32, codes 16-byte
+ * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes. The arithmetic
+ * is that of the oco_moe_f8_plan calls at every row count: no single-token numerics of its own. */
+typedef struct {
+    const float* up_s;
+    const float* gate_s;
+    const float* down_s;
+} oco_dense_scales;
+int oco_dense_bind_scales(oco_dense_plan* plan, const oco_dense_scales* scales);
 int oco_dense_forward(oco_dense_plan* plan, const uint16_t* x_bf16, uint16_t* y_bf16, int rows, void* cuda_stream);
 int oco_dense_poll(oco_dense_plan* plan, void* cuda_stream);
 int oco_dense_last_launch_count(const oco_dense_plan* plan);
 const char* oco_dense_last_error(const oco_dense_plan* plan);
+
+/* ---- routing with groups of experts ------------------------------------------------------------
+ * Rows or logits -> expert ids and combination weights, for layers whose experts are kept in groups. The
+ * reference's routers (softmax over the winners, sigmoid with a selection bias) know no groups and at most
+ * 128 experts; oco_moe_route serves those. For a token's logits l:
+ *     s = sigmoid(l) or softmax(l) over all experts          the score, which becomes the weight
+ *     r = s + bias                                           what the experts are ranked by (no bias: s)
+ *     worth of a group = the sum of its `group_best` largest r; the `top_groups` worthiest groups stay
+ *     ids = the top_k largest r of those groups, in falling order; equal values go to the lower index
+ *     prob = s[id] / max(sum of the winners' s, 2^-14) if normalize, else s[id]; times scale
+ * Rankings are decided in 64 bits wherever two values lie within the error of the 32-bit ones (then the
+ * logits concerned are summed again in 64 bits from x and the weights), so the ids of a token do not depend
+ * on the number of rows in the call. A non-finite logit makes the token's weights NaN while its ids stay
+ * valid and distinct (a non-finite logit ranks last). A bias may be -inf: such an expert is chosen only when
+ * nothing else is left. */
+typedef enum { OCO_SCORE_SIGMOID = 0, OCO_SCORE_SOFTMAX = 1 } oco_moe_score;
+typedef struct {
+    int32_t hidden;      /* row width, a multiple of 32 up to 16384; 0: the plan selects from given logits only */
+    int32_t experts;     /* 1 .. 512 */
+    int32_t top_k;       /* 1 .. 16, no more than the experts of top_groups groups */
+    int32_t score;       /* oco_moe_score */
+    int32_t groups;      /* 1 .. 32, divides experts; 1 = no groups */
+    int32_t top_groups;  /* 1 .. groups */
+    int32_t group_best;  /* 1 or 2 */
+    int32_t normalize;
+    float scale;
+} oco_moe_router_desc;
+typedef struct oco_moe_router oco_moe_router;
+int oco_moe_router_create(const oco_moe_router_desc* desc, oco_moe_router** out);
+void oco_moe_router_destroy(oco_moe_router* router);
+/* Workspace and weights follow the rules of oco_moe_bind_workspace / _weights: caller-owned, set-up calls on the
+ * device that stays current for every later call. router_w: f32 [experts, hidden] (NULL where hidden is 0), bias:
+ * f32 [experts] or NULL; both must stay valid and unchanged. The weights are laid out once for the tensor cores
+ * when both are bound. */
+size_t oco_moe_router_workspace_bytes(const oco_moe_router* router, int max_rows);
+int oco_moe_router_bind_workspace(oco_moe_router* router, void* workspace, size_t bytes, int max_rows);
+int oco_moe_router_bind_weights(oco_moe_router* router, const float* router_w, const float* bias);
+/* x bf16 [rows, hidden] -> ids u32 [rows, top_k], probs f32 [rows, top_k] and, where `logits` is not NULL, the
+ * logits f32 [rows, experts]. Only enqueues; 0 rows are no work. */
+int oco_moe_router_forward(oco_moe_router* router, const uint16_t* x_bf16, int rows, uint32_t* ids, float* probs, float* logits,
+                           void* cuda_stream);
+/* The selection alone, from logits f32 [rows, experts] of any origin (any number of rows). */
+int oco_moe_router_select(oco_moe_router* router, const float* logits, int rows, uint32_t* ids, float* probs, void* cuda_stream);
+int oco_moe_router_poll(oco_moe_router* router, void* cuda_stream);
+int oco_moe_router_last_launch_count(const oco_moe_router* router);
+const char* oco_moe_router_last_error(const oco_moe_router* router);
+
+/* ---- the norms around a block, with its gate and residual scale ---------------------------------
+ * What stands between two blocks (attention, a feed-forward, the experts), in one pass over the rows:
+ *     b = post(block)                     post_w NULL: b = block
+ *     h = residual_scale * hidden + block_scale * act(gate) * b          -> hidden_out
+ *     x = pre(h)                                                         -> norm_out (bf16)
+ *     RMS:   v * rsqrt(mean(v^2) + epsilon) * (weight_offset + w)
+ *     layer: (v - mean(v)) * rsqrt(var(v) + epsilon) * (weight_offset + w) + bias
+ * (oco_moe_add_norm_forward holds the plain case, with the reference's rounding, in front of a layer.) Sums are
+ * f32; x is made from h before h is rounded. pre_w NULL: x is not weighted. block NULL: h = residual_scale *
+ * hidden. hidden_out may be hidden and norm_out may be block (with the same strides); other overlaps are not
+ * allowed. Rows of zeros give zeros (epsilon > 0); a NaN or infinity spoils its own row only. */
+typedef enum { OCO_NORM_RMS = 0, OCO_NORM_LAYER = 1 } oco_moe_norm_kind;
+typedef enum { OCO_GATE_NONE = 0, OCO_GATE_BF16 = 1, OCO_GATE_F32 = 2 } oco_moe_gate_type;
+typedef enum { OCO_GATE_PLAIN = 0, OCO_GATE_SIGMOID = 1, OCO_GATE_TANH = 2 } oco_moe_gate_act;
+typedef struct {
+    int32_t width;          /* a multiple of 8, 8 .. 32768 */
+    int32_t kind;           /* oco_moe_norm_kind, of both norms */
+    int32_t wide;           /* the residual rows are f32 (0: bf16) */
+    int32_t gate_type;      /* oco_moe_gate_type */
+    int32_t gate_rows;      /* row r takes gate row r / gate_rows; 0: one gate row [width] for all */
+    int32_t gate_act;       /* oco_moe_gate_act */
+    float epsilon, weight_offset, residual_scale, block_scale;
+    const void* hidden;     /* bf16 or f32 rows */
+    const uint16_t* block;  /* bf16 rows or NULL */
+    const float *post_w, *post_b, *pre_w, *pre_b;   /* f32 [width] or NULL */
+    const void* gate;
+    void* hidden_out;       /* type of hidden, or NULL */
+    uint16_t* norm_out;     /* bf16 or NULL */
+    int64_t hidden_stride, block_stride, gate_stride, hidden_out_stride, norm_out_stride;   /* elements, multiples of 8; 0: width */
+} oco_moe_block_norm_args;
+/* Stateless: needs no plan and no workspace, runs on the current device. All pointers 16-byte aligned. A refused call
+ * leaves its reason in `err` (if given). Only enqueues; 0 rows are no work. */
+int oco_moe_block_norm(const oco_moe_block_norm_args* args, int rows, void* cuda_stream, char* err, size_t err_len);
+
+/* ---- routed experts with 8-bit floating-point weights ---------------------------------------------
+ * SiLU-gated experts whose matrices are e4m3 codes with one f32 scale per block of 128 x 128 (OCO_FMT_F8_E4M3;
+ * dense products of the same format: oco_dense_*). Rows are rounded to e4m3 under one scale per row and 128
+ * elements: scale = largest / 448, code = e4m3(x * 448 / largest). Products of codes are summed in f32 over the
+ * 128 elements of a block on the tensor cores, the blocks' sums in f32 under the product of their scales:
+ *     g = gate . x, u = up . x, a = silu(g) * u (f32), rounded to e4m3 as the rows are, y = down . a
+ *     out[t] = residual[t] + sum_r prob[t, r] * y[t, r]        (y is rounded to bf16, the sum is f32, one rounding)
+ * The ids may come from any router; an id outside 0 .. experts-1 is a route of another shard or of padding and is
+ * left out (its weight is not read). A row without any route keeps its residual. */
+typedef struct {
+    int32_t hidden;      /* multiple of 32 */
+    int32_t ffn;         /* multiple of 32 */
+    int32_t experts;     /* 1 .. 512 */
+    int32_t top_k;       /* 1 .. 16 */
+} oco_moe_f8_desc;
+/* Codes [experts][ffn][hidden] (gate, up) and [experts][hidden][ffn] (down), 16-byte aligned; scales f32
+ * [experts][ceil(rows / 128)][ceil(columns / 128)] of the same matrices. */
+typedef struct {
+    const uint8_t *gate_w, *up_w, *down_w;
+    const float *gate_s, *up_s, *down_s;
+} oco_moe_f8_weights;
+typedef struct oco_moe_f8_plan oco_moe_f8_plan;
+int oco_moe_f8_plan_create(const oco_moe_f8_desc* desc, oco_moe_f8_plan** out);
+void oco_moe_f8_plan_destroy(oco_moe_f8_plan* plan);
+size_t oco_moe_f8_workspace_bytes(const oco_moe_f8_plan* plan, int max_rows);
+int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t bytes, int max_rows);
+int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* weights);
+/* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual); ids u32, probs f32 [rows, top_k].
+ * Only enqueues; 0 rows are no work. */
+int oco_moe_f8_forward(oco_moe_f8_plan* plan, const uint16_t* x_bf16, const uint32_t* ids, const float* probs,
+                       const uint16_t* residual_bf16, uint16_t* out_bf16, int rows, void* cuda_stream);
+int oco_moe_f8_poll(oco_moe_f8_plan* plan, void* cuda_stream);
+int oco_moe_f8_last_launch_count(const oco_moe_f8_plan* plan);
+const char* oco_moe_f8_last_error(const oco_moe_f8_plan* plan);
 
 /* Expert parallelism without a collective on the rows' way. The reference is single-device; nothing
  * below has a counterpart in it.

@@ -39,6 +39,29 @@ class DenseWeights(C.Structure):
     _fields_ = [("up_w", C.POINTER(C.c_uint8)), ("gate_w", C.POINTER(C.c_uint8)), ("down_w", C.POINTER(C.c_uint8))]
 
 
+class DenseScales(C.Structure):
+    _fields_ = [("up_s", C.c_void_p), ("gate_s", C.c_void_p), ("down_s", C.c_void_p)]
+
+
+class RouterDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("hidden", "experts", "top_k", "score", "groups", "top_groups", "group_best", "normalize")] + [("scale", C.c_float)]
+
+
+class F8Desc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("hidden", "ffn", "experts", "top_k")]
+
+
+class F8Weights(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("gate_w", "up_w", "down_w", "gate_s", "up_s", "down_s")]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("width", "kind", "wide", "gate_type", "gate_rows", "gate_act")]
+                + [(n, C.c_float) for n in ("epsilon", "weight_offset", "residual_scale", "block_scale")]
+                + [(n, C.c_void_p) for n in ("hidden", "block", "post_w", "post_b", "pre_w", "pre_b", "gate", "hidden_out", "norm_out")]
+                + [(n, C.c_int64) for n in ("hidden_stride", "block_stride", "gate_stride", "hidden_out_stride", "norm_out_stride")])
+
+
 SIGNATURES = {
     "oco_moe_plan_create": (C.c_int, [C.POINTER(Desc), C.POINTER(C.c_void_p)]),
     "oco_moe_plan_destroy": (None, [C.c_void_p]),
@@ -106,6 +129,27 @@ SIGNATURES = {
     "oco_ep_window_error": (C.c_char_p, []),
     "oco_moe_experts_window": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_void_p, C.c_void_p]),
+    "oco_dense_bind_scales": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "oco_moe_router_create": (C.c_int, [C.POINTER(RouterDesc), C.POINTER(C.c_void_p)]),
+    "oco_moe_router_destroy": (None, [C.c_void_p]),
+    "oco_moe_router_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "oco_moe_router_bind_workspace": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]),
+    "oco_moe_router_bind_weights": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "oco_moe_router_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "oco_moe_router_select": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "oco_moe_router_poll": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "oco_moe_router_last_launch_count": (C.c_int, [C.c_void_p]),
+    "oco_moe_router_last_error": (C.c_char_p, [C.c_void_p]),
+    "oco_moe_block_norm": (C.c_int, [C.POINTER(BlockNormArgs), C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "oco_moe_f8_plan_create": (C.c_int, [C.POINTER(F8Desc), C.POINTER(C.c_void_p)]),
+    "oco_moe_f8_plan_destroy": (None, [C.c_void_p]),
+    "oco_moe_f8_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "oco_moe_f8_bind_workspace": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]),
+    "oco_moe_f8_bind_weights": (C.c_int, [C.c_void_p, C.POINTER(F8Weights)]),
+    "oco_moe_f8_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "oco_moe_f8_poll": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "oco_moe_f8_last_launch_count": (C.c_int, [C.c_void_p]),
+    "oco_moe_f8_last_error": (C.c_char_p, [C.c_void_p]),
     "oco_moe_version": (C.c_char_p, []),
 }
 

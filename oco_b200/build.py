@@ -8,8 +8,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liboco_moe.so")
-SOURCES = ["api.cu", "route_static.cu", "peaks.cu", "window.cu"]
+SOURCES = ["api.cu", "route_static.cu", "peaks.cu", "window.cu", "f8.cu", "router_groups.cu", "block_norm.cu"]
 HEADERS = ["common.cuh", "router.cuh", "plan.cuh", "decode.cuh", "batch.cuh", "gemm.cuh", "gemm_wide.cuh", "gemm_pair.cuh", "token_deal.h", "mx.cuh", "mx_pieces.cuh", "gemm_mx.cuh",
+           "host.cuh", "f8.cuh", "f8.h", "select.cuh",
            "../../include/oco_moe.h"]
 
 
@@ -31,7 +32,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not (force or stale()):
         return LIB
     cmd = [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v" if verbose else "-O3",
+           "-Xcompiler", "-fPIC", "-shared", "--threads", "0", "-Xptxas", "-v" if verbose else "-O3",
            "-o", LIB] + [os.path.join(CSRC, f) for f in SOURCES]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -11,6 +11,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "host.cuh"
 #include "decode.cuh"
 #include "batch.cuh"
 #include "gemm.cuh"
@@ -18,6 +19,7 @@
 #include "gemm_pair.cuh"
 #include "mx.cuh"
 #include "gemm_mx.cuh"
+#include "f8.h"
 #include <cmath>
 #include "plan.cuh"
 #include "router.cuh"
@@ -154,14 +156,6 @@ int fail(oco_moe_plan* p, int code, const char* fmt, ...) {
         if (e_ != cudaSuccess) return fail(plan, OCO_CUDA_ERROR, "%s: %s", #call, cudaGetErrorString(e_)); \
     } while (0)
 
-// A kernel's opt-in to large dynamic shared memory is a per-device attribute: this remembers, per
-// launch site, on which devices it has been set (bit d = device d). Two threads may both find the
-// bit clear and set the attribute twice, which is harmless; a set bit is never lost.
-struct DeviceOnce {
-    std::atomic<uint64_t> done{0};
-    bool need(int dev) const { return dev < 0 || dev >= 64 || !((done.load(std::memory_order_acquire) >> dev) & 1u); }
-    void mark(int dev) { if (dev >= 0 && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release); }
-};
 #define ALLOW_SMEM_ONCE(kernel)                                   \
     do {                                                          \
         static DeviceOnce once_;                                  \
@@ -190,8 +184,6 @@ uint32_t packed_row_bytes(int fmt, int k) {
     return 0;
 }
 int block_elems(int fmt) { return fmt == OCO_FMT_Q4_K ? 256 : 32; }
-
-size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // CTAs that a split dense product may use, whatever the GPU has: bounds its partial sums in the workspace.
 constexpr int kSplitCtas = 148;
@@ -270,51 +262,17 @@ Workspace carve(const oco_moe_desc& d, int split_width, int max_rows, unsigned c
     return w;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 int make_row_map(oco_moe_plan* plan, CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-    // looked up once per process (initialisation of a function-local static is thread-safe)
-    static const EncodeTiledFn encode = [] {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return (EncodeTiledFn)fn;
-    }();
-    if (!encode) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
-    cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {cols * 2};
-    cuuint32_t box[2] = {64, box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return OCO_OK;
+    if (!encode_tiled()) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    CUresult r = encode_rows(map, base, rows, cols, 2, box_rows);
+    return r == CUDA_SUCCESS ? OCO_OK : fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
 // The same over rows of bytes (e2m1 pairs): box 128 bytes x box_rows.
 int make_byte_map(oco_moe_plan* plan, CUtensorMap* map, void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows) {
-    static const EncodeTiledFn encode = [] {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return (EncodeTiledFn)fn;
-    }();
-    if (!encode) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
-    cuuint64_t dims[2] = {row_bytes, rows};
-    cuuint64_t strides[1] = {row_bytes};
-    cuuint32_t box[2] = {128, box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled (byte rows) failed (%d)", (int)r);
-    return OCO_OK;
+    if (!encode_tiled()) return fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    CUresult r = encode_rows(map, base, rows, row_bytes, 1, box_rows);
+    return r == CUDA_SUCCESS ? OCO_OK : fail(plan, OCO_CUDA_ERROR, "cuTensorMapEncodeTiled (byte rows) failed (%d)", (int)r);
 }
 
 // Only the wide tile kernel splits a contraction; a plan that was asked for the generic kernels never reaches it.
@@ -332,47 +290,6 @@ int pick_tile_index(int routes, int experts, int wide_min_avg) {
 }
 
 // ---- launch helpers ---------------------------------------------------------------------------
-// Opts a kernel into the full 227 KB of dynamic shared memory; each launch then asks for what it needs.
-constexpr size_t kMaxDynamicSmem = 232448;
-template <typename Kern>
-cudaError_t allow_smem(Kern k) {
-    cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, k);
-    if (e != cudaSuccess) return e;
-    // static and dynamic shared memory share the 227 KB a CTA may opt into
-    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(kMaxDynamicSmem - attr.sharedSizeBytes));
-}
-
-// Launches a kernel with programmatic stream serialization: it may be scheduled (and, where it does so
-// before its griddepcontrol.wait, set up its shared memory and barriers) while its predecessor in the stream
-// still runs, and waits for it inside. Every kernel launched this way calls pdl_wait() before it touches
-// anything a predecessor wrote or still reads.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-}
-
-// The same for a kernel that runs in clusters of two CTAs.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-}
-
 template <int FMT, int EPI, int NT>
 int launch_gemm(oco_moe_plan* plan, const GemmParams& gp, const CUtensorMap& map, int max_tiles, cudaStream_t st) {
     using S = GemmShape<EPI, NT>;
@@ -402,7 +319,7 @@ int launch_gemm_wide(oco_moe_plan* plan, GemmParams gp, const CUtensorMap* maps,
         ALLOW_SMEM_ONCE((grouped_gemm_pair_kernel<FMT, EPI>));
         const int per = epi_gated(EPI) ? 128 : 256;
         const int pairs = std::min(plan->sm_count / 2, ((gp.n + per - 1) / per) * max_tiles);
-        CK(launch_dependent_pairs(grouped_gemm_pair_kernel<FMT, EPI>, dim3(2 * pairs), dim3(PairShapeT<FMT>::kThreads), PairShapeT<FMT>::kSmemBytes, st, gp,
+        CK(launch_dependent_clusters(grouped_gemm_pair_kernel<FMT, EPI>, 2u, dim3(2 * pairs), dim3(PairShapeT<FMT>::kThreads), PairShapeT<FMT>::kSmemBytes, st, gp,
                                   maps[0], maps[1], maps[2]));
         plan->launches++;
         CK(cudaGetLastError());
@@ -1581,6 +1498,7 @@ int oco_moe_routing(const oco_moe_plan* plan, oco_moe_routing_view* out) {
 // is a route to expert 0, the tiles run in their dense mode, the single-token kernels take a null id list.
 struct oco_dense_plan {
     oco_moe_plan* inner = nullptr;
+    oco_moe_f8_plan* f8 = nullptr;   // OCO_FMT_F8_E4M3: the plan of its own kernels (f8.cu), inner stays null
     oco_dense_desc d{};
 };
 
@@ -1652,6 +1570,7 @@ int oco_dense_plan_create(const oco_dense_desc* desc, oco_dense_plan** out) {
     if (!dp) return OCO_INVALID_ARGUMENT;
     dp->d = *desc;
     *out = dp;   // handed out even on failure so that the caller can read the message, then destroy
+    if (desc->weight_format == OCO_FMT_F8_E4M3) return f8_dense_create(*desc, &dp->f8);
     oco_moe_desc md{};
     md.hidden = desc->hidden; md.ffn = desc->ffn; md.experts = 1; md.top_k = 1; md.weight_format = desc->weight_format;
     md.scale = 1.0f;
@@ -1680,19 +1599,23 @@ int oco_dense_plan_create(const oco_dense_desc* desc, oco_dense_plan** out) {
 void oco_dense_plan_destroy(oco_dense_plan* plan) {
     if (!plan) return;
     oco_moe_plan_destroy(plan->inner);
+    oco_moe_f8_plan_destroy(plan->f8);
     delete plan;
 }
 
 size_t oco_dense_workspace_bytes(const oco_dense_plan* plan, int max_rows) {
+    if (plan && plan->f8) return oco_moe_f8_workspace_bytes(plan->f8, max_rows);
     return plan && plan->inner ? oco_moe_workspace_bytes(plan->inner, max_rows) : 0;
 }
 
 int oco_dense_bind_workspace(oco_dense_plan* plan, void* workspace, size_t bytes, int max_rows) {
+    if (plan && plan->f8) return oco_moe_f8_bind_workspace(plan->f8, workspace, bytes, max_rows);
     if (!plan || !plan->inner) return OCO_INVALID_ARGUMENT;
     return oco_moe_bind_workspace(plan->inner, workspace, bytes, max_rows);
 }
 
 int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* w) {
+    if (plan && plan->f8) return f8_dense_bind_codes(plan->f8, w ? *w : oco_dense_weights{});
     if (!plan || !plan->inner) return OCO_INVALID_ARGUMENT;
     oco_moe_plan* in = plan->inner;
     if (!w || !w->up_w) return fail(in, OCO_INVALID_ARGUMENT, "up_w is required");
@@ -1707,7 +1630,14 @@ int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* w) {
     return OCO_OK;
 }
 
+int oco_dense_bind_scales(oco_dense_plan* plan, const oco_dense_scales* s) {
+    if (plan && plan->f8) return f8_dense_bind_scales(plan->f8, s ? *s : oco_dense_scales{});
+    if (!plan || !plan->inner) return OCO_INVALID_ARGUMENT;
+    return fail(plan->inner, OCO_INVALID_ARGUMENT, "this weight format carries its scales in its blocks");
+}
+
 int oco_dense_forward(oco_dense_plan* dp, const uint16_t* x_bf16, uint16_t* y_bf16, int rows, void* cuda_stream) {
+    if (dp && dp->f8) return f8_dense_forward(dp->f8, x_bf16, y_bf16, rows, cuda_stream);
     if (!dp || !dp->inner) return OCO_INVALID_ARGUMENT;
     oco_moe_plan* plan = dp->inner;
     if (!plan->have_ws || !plan->have_w) return fail(plan, OCO_INVALID_ARGUMENT, "bind a workspace and weights first");
@@ -1726,9 +1656,9 @@ int oco_dense_forward(oco_dense_plan* dp, const uint16_t* x_bf16, uint16_t* y_bf
     return rc;
 }
 
-int oco_dense_poll(oco_dense_plan* plan, void* cuda_stream) { return plan && plan->inner ? oco_moe_poll(plan->inner, cuda_stream) : OCO_INVALID_ARGUMENT; }
-int oco_dense_last_launch_count(const oco_dense_plan* plan) { return plan && plan->inner ? plan->inner->launches : 0; }
-const char* oco_dense_last_error(const oco_dense_plan* plan) { return plan && plan->inner ? plan->inner->err : "null plan"; }
+int oco_dense_poll(oco_dense_plan* plan, void* cuda_stream) { return plan && plan->f8 ? oco_moe_f8_poll(plan->f8, cuda_stream) : plan && plan->inner ? oco_moe_poll(plan->inner, cuda_stream) : OCO_INVALID_ARGUMENT; }
+int oco_dense_last_launch_count(const oco_dense_plan* plan) { return plan && plan->f8 ? oco_moe_f8_last_launch_count(plan->f8) : plan && plan->inner ? plan->inner->launches : 0; }
+const char* oco_dense_last_error(const oco_dense_plan* plan) { return plan && plan->f8 ? oco_moe_f8_last_error(plan->f8) : plan && plan->inner ? plan->inner->err : "null plan"; }
 
 const char* oco_moe_last_error(const oco_moe_plan* plan) { return plan ? plan->err : "null plan"; }
 int oco_moe_last_launch_count(const oco_moe_plan* plan) { return plan ? plan->launches : 0; }

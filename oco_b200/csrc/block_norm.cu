@@ -1,0 +1,261 @@
+// The step between two blocks of a layer, in one pass over the rows: the finished block's output is normalised
+// (post-norm, optional), gated and scaled onto the residual rows, and the result is normalised for the next block:
+//
+//     b  = post(block)                          RMS:   v * rsqrt(mean(v^2) + eps) * (offset + w)
+//     h  = residual_scale * hidden              layer: (v - mean(v)) * rsqrt(var(v) + eps) * (offset + w) + bias
+//        + block_scale * act(gate) * b
+//     x  = pre(h)
+//
+// Bound: memory. Rows are read once and written once (hidden, block and a per-element gate in; hidden and x out); a
+// row lives in the registers of the threads that share it, so the statistics cost no second read. They are sums in
+// f32; the variance of the layer form is the mean square of the centred values (two sums over registers), not a
+// difference of large sums. x is made from the f32 value of h, not from its rounded copy: one rounding per output.
+#include "host.cuh"
+
+using namespace oco;
+
+namespace {
+
+constexpr int kMaxWidth = 32768;
+
+struct NormParams {
+    const void* hidden;
+    const uint16_t* block;
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    const void* gate;
+    void* hidden_out;
+    uint16_t* norm_out;
+    long long hidden_stride, block_stride, gate_stride, hidden_out_stride, norm_out_stride;
+    int n, rows, gate_type, gate_rows, gate_act;
+    float eps, offset, residual_scale, block_scale;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<uint32_t*>(&p);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// Sum over the THREADS threads that share a row; every one of them gets it. `slot`: shared memory, a fresh one per call.
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float s, float* slot) {
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (THREADS == 32) return s;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = s;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; i++) t += slot[i];
+    return t;
+}
+
+// Normalises the row held in v (elements at or past n are zero and stay out of the sums). LAYER: centred first.
+template <int THREADS, int ITER, bool LAYER>
+__device__ __forceinline__ void normalise(float (&v)[ITER][8], const bool (&live)[ITER], const float* w, const float* b, int col0, const NormParams& p,
+                                          float* slots) {
+    const float inv_n = 1.0f / (float)p.n;
+    if (LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITER; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) s += v[i][j];
+        const float mean = row_sum<THREADS>(s, slots) * inv_n;
+#pragma unroll
+        for (int i = 0; i < ITER; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = live[i] ? v[i][j] - mean : 0.f;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITER; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) s = fmaf(v[i][j], v[i][j], s);
+    const float inv = 1.0f / sqrtf(row_sum<THREADS>(s, slots + 32) * inv_n + p.eps);
+#pragma unroll
+    for (int i = 0; i < ITER; i++) {
+        if (live[i]) {
+            const int at = col0 + i * THREADS * 8;
+            if (w) {
+                float t[8];
+                load8(w + at, t);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * inv * (t[j] + p.offset);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] *= inv;
+            }
+            if (LAYER && b) {
+                float t[8];
+                load8(b + at, t);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] += t[j];
+            }
+        }
+    }
+}
+
+// THREADS threads share a row, each holds ITER pieces of eight elements (piece i of thread t: elements
+// 8 * (t + i * THREADS)). THREADS == 32: a warp per row, four rows per CTA; else a CTA per row.
+template <int THREADS, int ITER, bool LAYER, bool WIDE>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kernel(const NormParams p) {
+    __shared__ float slots[4 * 32];
+    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
+    pdl_wait();                // the kernel before has completed and its writes are visible
+    const int row = THREADS == 32 ? (int)(blockIdx.x * 4 + (threadIdx.x >> 5)) : (int)blockIdx.x;
+    const int t = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    if (row >= p.rows) return;                 // whole warps (THREADS == 32); never in the other forms
+    const int col0 = 8 * t;
+    bool live[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; i++) live[i] = col0 + i * THREADS * 8 < p.n;
+
+    float h[ITER][8], b[ITER][8];
+    uint4 raw[ITER][WIDE ? 2 : 1], braw[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; i++) {
+        const int at = col0 + i * THREADS * 8;
+        if (live[i]) {
+            const char* src = (const char*)p.hidden + ((long long)row * p.hidden_stride + at) * (WIDE ? 4 : 2);
+            raw[i][0] = *reinterpret_cast<const uint4*>(src);
+            if (WIDE) raw[i][WIDE ? 1 : 0] = *reinterpret_cast<const uint4*>(src + 16);
+            if (p.block) braw[i] = *reinterpret_cast<const uint4*>(p.block + (long long)row * p.block_stride + at);
+        } else {
+            raw[i][0] = raw[i][WIDE ? 1 : 0] = make_uint4(0, 0, 0, 0);
+        }
+        if (!p.block || !live[i]) braw[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (p.block) {
+#pragma unroll
+        for (int i = 0; i < ITER; i++) unpack8(braw[i], b[i]);
+        if (p.post_w) normalise<THREADS, ITER, LAYER>(b, live, p.post_w, p.post_b, col0, p, slots);
+        if (p.gate_type) {
+            const long long grow = p.gate_rows > 0 ? (long long)(row / p.gate_rows) * p.gate_stride : 0;
+#pragma unroll
+            for (int i = 0; i < ITER; i++) {
+                if (live[i]) {
+                    const long long at = grow + col0 + i * THREADS * 8;
+                    float g[8];
+                    if (p.gate_type == 2) load8(reinterpret_cast<const float*>(p.gate) + at, g);
+                    else unpack8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + at)), g);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (p.gate_act == 1) g[j] = 1.0f / (1.0f + __expf(-g[j]));
+                        else if (p.gate_act == 2) g[j] = tanhf(g[j]);
+                        b[i][j] *= g[j];
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITER; i++) {
+        if (WIDE) {
+            const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
+                                   raw[i][WIDE].x, raw[i][WIDE].y, raw[i][WIDE].z, raw[i][WIDE].w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] = __uint_as_float(w[j]);
+        } else {
+            unpack8(raw[i][0], h[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] *= p.residual_scale;
+        if (p.block) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] = fmaf(p.block_scale, b[i][j], h[i][j]);
+        }
+        if (p.hidden_out && live[i]) {
+            char* dst = (char*)p.hidden_out + ((long long)row * p.hidden_out_stride + col0 + i * THREADS * 8) * (WIDE ? 4 : 2);
+            if (WIDE) {
+                *reinterpret_cast<float4*>(dst) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
+                *reinterpret_cast<float4*>(dst + 16) = make_float4(h[i][4], h[i][5], h[i][6], h[i][7]);
+            } else {
+                *reinterpret_cast<uint4*>(dst) = pack8(h[i]);
+            }
+        }
+    }
+    if (!p.norm_out) return;
+    normalise<THREADS, ITER, LAYER>(h, live, p.pre_w, p.pre_b, col0, p, slots + 64);
+#pragma unroll
+    for (int i = 0; i < ITER; i++)
+        if (live[i]) *reinterpret_cast<uint4*>(p.norm_out + (long long)row * p.norm_out_stride + col0 + i * THREADS * 8) = pack8(h[i]);
+}
+
+int say(char* err, size_t len, int code, const char* text) {
+    if (err && len) snprintf(err, len, "%s", text);
+    return code;
+}
+
+template <int THREADS, int ITER>
+cudaError_t launch(const NormParams& p, bool layer, bool wide, cudaStream_t st) {
+    const dim3 grid(THREADS == 32 ? (p.rows + 3) / 4 : p.rows), block(THREADS == 32 ? 128 : THREADS);
+    if (layer) return wide ? launch_dependent(block_norm_kernel<THREADS, ITER, true, true>, grid, block, 0, st, p)
+                           : launch_dependent(block_norm_kernel<THREADS, ITER, true, false>, grid, block, 0, st, p);
+    return wide ? launch_dependent(block_norm_kernel<THREADS, ITER, false, true>, grid, block, 0, st, p)
+                : launch_dependent(block_norm_kernel<THREADS, ITER, false, false>, grid, block, 0, st, p);
+}
+
+}  // namespace
+
+extern "C" int oco_moe_block_norm(const oco_moe_block_norm_args* a, int rows, void* cuda_stream, char* err, size_t err_len) {
+    if (err && err_len) err[0] = 0;
+    if (!a) return OCO_INVALID_ARGUMENT;
+    if (a->width < 8 || a->width % 8 || a->width > kMaxWidth) return say(err, err_len, OCO_UNSUPPORTED_SHAPE, "width must be a multiple of 8, 8 .. 32768");
+    if (rows < 0) return say(err, err_len, OCO_INVALID_ARGUMENT, "rows must not be negative");
+    if (!a->hidden || (!a->hidden_out && !a->norm_out)) return say(err, err_len, OCO_INVALID_ARGUMENT, "hidden and one of hidden_out, norm_out are required");
+    if (a->kind != OCO_NORM_RMS && a->kind != OCO_NORM_LAYER) return say(err, err_len, OCO_INVALID_ARGUMENT, "unknown kind of norm");
+    if (a->gate_type < OCO_GATE_NONE || a->gate_type > OCO_GATE_F32 || a->gate_act < OCO_GATE_PLAIN || a->gate_act > OCO_GATE_TANH || a->gate_rows < 0)
+        return say(err, err_len, OCO_INVALID_ARGUMENT, "unknown gate_type or gate_act, or negative gate_rows");
+    if ((a->gate_type != OCO_GATE_NONE) != (a->gate != nullptr)) return say(err, err_len, OCO_INVALID_ARGUMENT, "gate and gate_type do not agree");
+    if (!a->block && (a->gate || a->post_w || a->post_b)) return say(err, err_len, OCO_INVALID_ARGUMENT, "a gate or post-norm without a block output");
+    if (a->kind == OCO_NORM_RMS && (a->post_b || a->pre_b)) return say(err, err_len, OCO_INVALID_ARGUMENT, "biases belong to the layer norm");
+    if ((a->post_b && !a->post_w) || (a->pre_b && !a->pre_w)) return say(err, err_len, OCO_INVALID_ARGUMENT, "a bias without its weight");
+    if (!(a->epsilon >= 0.0f)) return say(err, err_len, OCO_INVALID_ARGUMENT, "epsilon must not be negative");
+    const void* aligned[] = {a->hidden, a->block, a->post_w, a->post_b, a->pre_w, a->pre_b, a->gate, a->hidden_out, a->norm_out};
+    for (const void* q : aligned)
+        if ((uintptr_t)q & 15u) return say(err, err_len, OCO_INVALID_ARGUMENT, "pointers must be 16-byte aligned");
+    const int64_t strides[] = {a->hidden_stride, a->block_stride, a->gate_stride, a->hidden_out_stride, a->norm_out_stride};
+    for (int64_t s : strides)
+        if (s != 0 && (s < a->width || s % 8)) return say(err, err_len, OCO_INVALID_ARGUMENT, "strides are multiples of 8 and at least the width (0: the width)");
+    if (rows == 0) return OCO_OK;
+
+    NormParams p{};
+    auto pitch = [&](int64_t s) { return s ? (long long)s : (long long)a->width; };
+    p.hidden = a->hidden; p.block = a->block; p.post_w = a->post_w; p.post_b = a->post_b; p.pre_w = a->pre_w; p.pre_b = a->pre_b;
+    p.gate = a->gate; p.hidden_out = a->hidden_out; p.norm_out = a->norm_out;
+    p.hidden_stride = pitch(a->hidden_stride); p.block_stride = pitch(a->block_stride); p.gate_stride = pitch(a->gate_stride);
+    p.hidden_out_stride = pitch(a->hidden_out_stride); p.norm_out_stride = pitch(a->norm_out_stride);
+    p.n = a->width; p.rows = rows; p.gate_type = a->gate_type; p.gate_rows = a->gate_rows; p.gate_act = a->gate_act;
+    p.eps = a->epsilon; p.offset = a->weight_offset; p.residual_scale = a->residual_scale; p.block_scale = a->block_scale;
+    const bool layer = a->kind == OCO_NORM_LAYER, wide = a->wide != 0;
+    const int pieces = a->width / 8;
+    cudaStream_t st = (cudaStream_t)cuda_stream;
+    cudaError_t e;
+    if (pieces <= 32) e = launch<32, 1>(p, layer, wide, st);
+    else if (pieces <= 64) e = launch<32, 2>(p, layer, wide, st);
+    else if (pieces <= 128) e = launch<128, 1>(p, layer, wide, st);
+    else if (pieces <= 256) e = launch<256, 1>(p, layer, wide, st);
+    else if (pieces <= 512) e = launch<256, 2>(p, layer, wide, st);
+    else if (pieces <= 1024) e = launch<512, 2>(p, layer, wide, st);
+    else if (pieces <= 2048) e = launch<1024, 2>(p, layer, wide, st);
+    else e = launch<1024, 4>(p, layer, wide, st);
+    if (e != cudaSuccess) return say(err, err_len, OCO_CUDA_ERROR, cudaGetErrorString(e));
+    return OCO_OK;
+}

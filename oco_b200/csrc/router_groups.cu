@@ -1,0 +1,177 @@
+// Routing with groups of experts: the router product and the selection (select.cuh) behind oco_moe_router_*.
+#include <new>
+
+#include "host.cuh"
+#include "select.cuh"
+
+using namespace oco;
+
+struct oco_moe_router : PlanBase {
+    oco_moe_router_desc d{};
+    const float* w = nullptr;
+    const float* bias = nullptr;
+    uint32_t* status = nullptr;
+    float* logits = nullptr;
+};
+
+namespace {
+
+struct RouterSpace { size_t status, logits, total; };
+RouterSpace carve(const oco_moe_router_desc& d, int max_rows) {
+    RouterSpace s{};
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off = align_up(off + bytes, 256); return at; };
+    s.status = take(256);
+    s.logits = take(d.hidden ? (size_t)max_rows * d.experts * 4 : 0);
+    s.total = off;
+    return s;
+}
+
+// logits[t][e] = sum_k x[t][k] w[e][k]: a warp per expert and four tokens, f32.
+__global__ void __launch_bounds__(256) router_rows_kernel(const uint16_t* __restrict__ x, const float* __restrict__ w, float* __restrict__ logits,
+                                                          int rows, int E, int H) {
+    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
+    pdl_wait();                // the kernel before has completed and its writes are visible
+    const int e = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t0 = blockIdx.x * 4;
+    if (e >= E) return;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = lane * 4; k < H; k += 128) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(w + (size_t)e * H + k));
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint2 q = *reinterpret_cast<const uint2*>(x + (size_t)min(t0 + t, rows - 1) * H + k);
+            acc[t] = fmaf(v.x, __uint_as_float(q.x << 16), acc[t]);
+            acc[t] = fmaf(v.y, __uint_as_float(q.x & 0xffff0000u), acc[t]);
+            acc[t] = fmaf(v.z, __uint_as_float(q.y << 16), acc[t]);
+            acc[t] = fmaf(v.w, __uint_as_float(q.y & 0xffff0000u), acc[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const float s = warp_sum_f(acc[t]);
+        if (lane == 0 && t0 + t < rows) logits[(size_t)(t0 + t) * E + e] = s;
+    }
+}
+
+int launch_select(oco_moe_router* r, const SelectParams& p, cudaStream_t st) {
+    const dim3 grid((p.rows + 7) / 8), block(256);
+    const int per_lane = (p.E + 31) / 32;
+    cudaError_t e;
+    if (per_lane <= 1) e = launch_dependent(select_kernel<1>, grid, block, 0, st, p);
+    else if (per_lane <= 2) e = launch_dependent(select_kernel<2>, grid, block, 0, st, p);
+    else if (per_lane <= 4) e = launch_dependent(select_kernel<4>, grid, block, 0, st, p);
+    else if (per_lane <= 8) e = launch_dependent(select_kernel<8>, grid, block, 0, st, p);
+    else e = launch_dependent(select_kernel<16>, grid, block, 0, st, p);
+    if (e != cudaSuccess) return r->fail(OCO_CUDA_ERROR, "select: %s", cudaGetErrorString(e));
+    r->launches++;
+    return OCO_OK;
+}
+
+SelectParams select_params(const oco_moe_router* r, const float* logits, int rows, uint32_t* ids, float* probs) {
+    const oco_moe_router_desc& d = r->d;
+    SelectParams p{};
+    p.logits = logits; p.bias = r->bias; p.ids = ids; p.probs = probs; p.status = nullptr;
+    p.rows = rows; p.E = d.experts; p.H = d.hidden; p.K = d.top_k; p.G = d.groups; p.TG = d.top_groups; p.best = d.group_best;
+    p.score = d.score; p.normalize = d.normalize; p.scale = d.scale;
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int oco_moe_router_create(const oco_moe_router_desc* desc, oco_moe_router** out) {
+    if (!desc || !out) return OCO_INVALID_ARGUMENT;
+    oco_moe_router* r = new (std::nothrow) oco_moe_router();
+    if (!r) return OCO_OUT_OF_MEMORY;
+    *out = r;   // handed out even on failure so that the caller can read the message, then destroy
+    r->d = *desc;
+    const oco_moe_router_desc& d = *desc;
+    if (d.hidden < 0 || d.hidden > 16384 || d.hidden % 32) return r->fail(OCO_UNSUPPORTED_SHAPE, "hidden must be a multiple of 32, up to 16384 (0: logits only)");
+    if (d.experts < 1 || d.experts > kSelMaxExperts) return r->fail(OCO_UNSUPPORTED_SHAPE, "experts must be 1 .. %d", kSelMaxExperts);
+    if (d.groups < 1 || d.groups > kSelMaxGroups || d.experts % d.groups) return r->fail(OCO_UNSUPPORTED_SHAPE, "groups must be 1 .. %d and divide the experts", kSelMaxGroups);
+    if (d.top_groups < 1 || d.top_groups > d.groups) return r->fail(OCO_INVALID_ARGUMENT, "top_groups must be 1 .. groups");
+    if (d.top_k < 1 || d.top_k > kSelMaxTopK) return r->fail(OCO_UNSUPPORTED_SHAPE, "top_k must be 1 .. %d", kSelMaxTopK);
+    if (d.top_k > d.top_groups * (d.experts / d.groups)) return r->fail(OCO_INVALID_ARGUMENT, "top_k is more than the experts of top_groups groups");
+    if (d.group_best != 1 && d.group_best != 2) return r->fail(OCO_INVALID_ARGUMENT, "group_best must be 1 or 2");
+    if (d.score != OCO_SCORE_SIGMOID && d.score != OCO_SCORE_SOFTMAX) return r->fail(OCO_INVALID_ARGUMENT, "unknown score");
+    return OCO_OK;
+}
+
+void oco_moe_router_destroy(oco_moe_router* r) { delete r; }
+
+size_t oco_moe_router_workspace_bytes(const oco_moe_router* r, int max_rows) { return r && max_rows >= 1 ? carve(r->d, max_rows).total : 0; }
+
+int oco_moe_router_bind_workspace(oco_moe_router* r, void* workspace, size_t bytes, int max_rows) {
+    if (!r) return OCO_INVALID_ARGUMENT;
+    if (!workspace || max_rows < 1) return r->fail(OCO_INVALID_ARGUMENT, "null workspace or max_rows < 1");
+    if ((uintptr_t)workspace & 255u) return r->fail(OCO_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    const RouterSpace s = carve(r->d, max_rows);
+    if (bytes < s.total) return r->fail(OCO_INVALID_ARGUMENT, "workspace too small: %zu < %zu", bytes, s.total);
+    OCO_CK(r, cudaMemset(workspace, 0, 256));
+    OCO_CK(r, cudaDeviceSynchronize());
+    if (int rc = r->note_device()) return rc;
+    unsigned char* base = (unsigned char*)workspace;
+    r->status = (uint32_t*)(base + s.status);
+    r->logits = (float*)(base + s.logits);
+    r->max_rows = max_rows;
+    r->have_ws = true;
+    return OCO_OK;
+}
+
+int oco_moe_router_bind_weights(oco_moe_router* r, const float* w, const float* bias) {
+    if (!r) return OCO_INVALID_ARGUMENT;
+    if ((r->d.hidden != 0) != (w != nullptr)) return r->fail(OCO_INVALID_ARGUMENT, "router_w goes with hidden: both or neither");
+    if (((uintptr_t)w & 15u) || ((uintptr_t)bias & 3u)) return r->fail(OCO_INVALID_ARGUMENT, "router_w must be 16-byte aligned, bias 4-byte");
+    r->w = w; r->bias = bias;
+    r->have_w = true;
+    return OCO_OK;
+}
+
+int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint32_t* ids, float* probs, float* logits, void* cuda_stream) {
+    if (!r) return OCO_INVALID_ARGUMENT;
+    r->launches = 0;
+    if (!r->d.hidden) return r->fail(OCO_INVALID_ARGUMENT, "this router selects from logits only");
+    if (!r->have_ws || !r->have_w) return r->fail(OCO_INVALID_ARGUMENT, "bind a workspace and weights first");
+    if (int rc = r->check_device()) return rc;
+    if (rows < 0 || rows > r->max_rows) return r->fail(OCO_INVALID_ARGUMENT, "rows %d outside 0..%d", rows, r->max_rows);
+    if (rows == 0) return OCO_OK;
+    if (!x || !ids || !probs) return r->fail(OCO_INVALID_ARGUMENT, "null x, ids or probs");
+    if (((uintptr_t)x & 15u) || (((uintptr_t)ids | (uintptr_t)probs | (uintptr_t)logits) & 3u))
+        return r->fail(OCO_INVALID_ARGUMENT, "x must be 16-byte aligned; ids, probs and logits 4-byte");
+    cudaStream_t st = (cudaStream_t)cuda_stream;
+    float* lg = logits ? logits : r->logits;
+    const oco_moe_router_desc& d = r->d;
+    OCO_CK(r, launch_dependent(router_rows_kernel, dim3((rows + 3) / 4, (d.experts + 7) / 8), dim3(256), 0, st, x, r->w, lg, rows, d.experts, d.hidden));
+    r->launches++;
+    SelectParams p = select_params(r, lg, rows, ids, probs);
+    p.x = x; p.w = r->w;
+    return launch_select(r, p, st);
+}
+
+int oco_moe_router_select(oco_moe_router* r, const float* logits, int rows, uint32_t* ids, float* probs, void* cuda_stream) {
+    if (!r) return OCO_INVALID_ARGUMENT;
+    r->launches = 0;
+    if (!r->have_w) return r->fail(OCO_INVALID_ARGUMENT, "bind weights first (NULL for what the plan has not)");
+    if (rows < 0) return r->fail(OCO_INVALID_ARGUMENT, "rows must not be negative");
+    if (rows == 0) return OCO_OK;
+    if (!logits || !ids || !probs) return r->fail(OCO_INVALID_ARGUMENT, "null logits, ids or probs");
+    if (((uintptr_t)logits | (uintptr_t)ids | (uintptr_t)probs) & 3u) return r->fail(OCO_INVALID_ARGUMENT, "logits, ids and probs must be 4-byte aligned");
+    return launch_select(r, select_params(r, logits, rows, ids, probs), (cudaStream_t)cuda_stream);
+}
+
+int oco_moe_router_poll(oco_moe_router* r, void* cuda_stream) {
+    if (!r) return OCO_INVALID_ARGUMENT;
+    OCO_CK(r, cudaStreamSynchronize((cudaStream_t)cuda_stream));
+    if (!r->have_ws) return OCO_OK;
+    uint32_t word = 0;
+    OCO_CK(r, cudaMemcpy(&word, r->status, 4, cudaMemcpyDeviceToHost));
+    if (!word) return OCO_OK;
+    OCO_CK(r, cudaMemset(r->status, 0, 4));
+    return r->fail(OCO_DEVICE_TIMEOUT, "a device-side wait gave up");
+}
+
+int oco_moe_router_last_launch_count(const oco_moe_router* r) { return r ? r->launches : 0; }
+const char* oco_moe_router_last_error(const oco_moe_router* r) { return r ? r->err : "null plan"; }
+
+}  // extern "C"

@@ -11,8 +11,8 @@ from typing import Optional
 import numpy as np
 import torch
 
-from . import _lib
-from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr
+from . import _lib, synth
+from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr, f8_matrix, need
 
 PROJECTION, FFN_RELU2, FFN_SILU_GATE = 0, 1, 2
 
@@ -47,8 +47,23 @@ class DensePlan:
         self._check(_lib.lib().oco_dense_bind_workspace(self.handle, _ptr(self.workspace), nbytes, max_rows))
         self.max_rows = max_rows
 
-    def bind(self, up_w: np.ndarray, gate_w: Optional[np.ndarray] = None, down_w: Optional[np.ndarray] = None, device="cuda"):
-        """Packed rows as they sit in the file: up_w [ffn][hidden], gate_w the same, down_w [hidden][ffn]."""
+    def bind(self, up_w, gate_w=None, down_w=None, device="cuda", up_scale=None, gate_scale=None, down_scale=None):
+        """Packed rows as they sit in the file: up_w [ffn][hidden], gate_w the same, down_w [hidden][ffn].
+        FMT_F8_E4M3: tensors of e4m3 codes (or their bytes) with the f32 scales [ceil(rows / 128)][ceil(columns / 128)]
+        of each matrix; CUDA tensors are used where they are, host arrays are uploaded."""
+        if self.fmt == synth.FMT_F8_E4M3:
+            out = self.ffn, self.hidden
+            gated = self.kind != PROJECTION
+            shapes = [("up", up_w, up_scale, out)] + ([("gate", gate_w, gate_scale, out), ("down", down_w, down_scale, out[::-1])] if gated else [])
+            if not gated and any(t is not None for t in (gate_w, down_w, gate_scale, down_scale)):
+                raise OcoError(_lib.INVALID_ARGUMENT, "a projection has one matrix")
+            got = {name: f8_matrix(codes, scales, (), n, k, device, name) for name, codes, scales, (n, k) in shapes}
+            ptr = lambda name, i: C.c_void_p(got[name][i].data_ptr()) if name in got else None  # noqa: E731
+            cw = _lib.DenseWeights(*[C.cast(ptr(n, 0), C.POINTER(C.c_uint8)) if n in got else None for n in ("up", "gate", "down")])
+            self._check(_lib.lib().oco_dense_bind_weights(self.handle, C.byref(cw)))
+            self._check(_lib.lib().oco_dense_bind_scales(self.handle, C.byref(_lib.DenseScales(*[ptr(n, 1) for n in ("up", "gate", "down")]))))
+            self._weights = got
+            return
         staged = tuple(_dev_bytes(a, device) for a in (up_w, gate_w, down_w))
         cw = _lib.DenseWeights(*[C.cast(C.c_void_p(t.data_ptr()), C.POINTER(C.c_uint8)) if t is not None else None for t in staged])
         self._check(_lib.lib().oco_dense_bind_weights(self.handle, C.byref(cw)))
@@ -56,6 +71,9 @@ class DensePlan:
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, rows: int):
         """x: bf16 bit patterns [rows, hidden]; y receives [rows, ffn] (projection) or [rows, hidden]."""
+        if self.fmt == synth.FMT_F8_E4M3 and rows > 0:
+            need(x, "x", 2, rows * self.hidden, self.workspace)
+            need(y, "y", 2, rows * (self.ffn if self.kind == PROJECTION else self.hidden), self.workspace)
         self._check(_lib.lib().oco_dense_forward(self.handle, _ptr(x), _ptr(y), rows, _stream_ptr()))
 
     def poll(self):

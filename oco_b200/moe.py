@@ -328,6 +328,233 @@ class Routing:
         return out
 
 
+def need(t: torch.Tensor, name: str, size: int, count: int, like: Optional[torch.Tensor]):
+    """Refuses a tensor that the kernels could not read as `count` contiguous elements of `size` bytes on the plan's device
+    (`like`: the plan's workspace)."""
+    if not t.is_cuda or not t.is_contiguous() or t.element_size() != size or t.numel() < count:
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {size} bytes is needed, "
+                                              f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if like is not None and t.device != like.device:
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name} is on {t.device}, the plan on {like.device}")
+
+
+def _on_current(t: torch.Tensor, name: str):
+    if t.device.index != torch.cuda.current_device():
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _staged(a, device) -> torch.Tensor:
+    if isinstance(a, np.ndarray):
+        return _dev_bytes(a, device)
+    return a if a.is_cuda else a.to(device)
+
+
+def f8_matrix(codes, scales, lead, n: int, k: int, device, name: str):
+    """Codes [*lead, n, k] of one byte and f32 scales [*lead, ceil(n / 128), ceil(k / 128)] on the device, checked."""
+    if codes is None or scales is None:
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: codes and scales are required")
+    count, blocks = n * k, -(-n // 128) * -(-k // 128)
+    for d in lead:
+        count, blocks = count * d, blocks * d
+    codes, scales = _staged(codes, device), _staged(scales, device)
+    if scales.dtype == torch.uint8 and scales.numel() == 4 * blocks:      # bytes of a host array
+        scales = scales.view(torch.float32)
+    for t, size, want, what in ((codes, 1, count, "codes"), (scales, 4, blocks, "scales")):
+        if t.numel() != want or t.element_size() != size or not t.is_contiguous():
+            raise OcoError(_lib.INVALID_ARGUMENT, f"{name} {what}: {want} contiguous elements of {size} bytes are needed, got {tuple(t.shape)} {t.dtype}")
+    return codes, scales
+
+
+class _GroupPlan:
+    """What the plans of grouped routing and of 8-bit float experts share: handle, workspace, errors."""
+    _prefix = ""
+
+    def _open(self, create, desc):
+        self.desc, self.handle = desc, C.c_void_p()
+        self._fn = {n: getattr(_lib.lib(), self._prefix + n) for n in ("workspace_bytes", "bind_workspace", "bind_weights", "forward", "poll",
+                                                                      "last_error", "last_launch_count")}
+        self.workspace, self.max_rows, self._weights = None, 0, None
+        rc = create(C.byref(desc), C.byref(self.handle))
+        if rc != _lib.OK:
+            raise OcoError(rc, self._fn["last_error"](self.handle).decode())
+
+    def _check(self, rc):
+        if rc != _lib.OK:
+            raise OcoError(rc, self._fn["last_error"](self.handle).decode())
+
+    def reserve(self, max_rows: int, device="cuda"):
+        if self.workspace is not None and max_rows <= self.max_rows:
+            return
+        nbytes = self._fn["workspace_bytes"](self.handle, max_rows)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        self._check(self._fn["bind_workspace"](self.handle, _ptr(ws), nbytes, max_rows))
+        self.workspace, self.max_rows = ws, max_rows
+
+    def poll(self):
+        self._check(self._fn["poll"](self.handle, _stream_ptr()))
+
+    def launch_count(self) -> int:
+        return self._fn["last_launch_count"](self.handle)
+
+    def __del__(self):
+        try:
+            if self.handle:
+                getattr(_lib.lib(), self._destroy)(self.handle)
+                self.handle = C.c_void_p()
+        except Exception:
+            pass
+
+
+SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+class RouterPlan(_GroupPlan):
+    """Routing with groups of experts (oco_moe_router_*): rows or logits -> expert ids and weights. The definition stands
+    at the declarations in include/oco_moe.h."""
+    _prefix, _destroy = "oco_moe_router_", "oco_moe_router_destroy"
+
+    @classmethod
+    def new(cls, hidden: int, experts: int, active: int, score: str = "sigmoid", groups: int = 1, top_groups: int = 1,
+            group_best: int = 1, normalize: bool = True, scale: float = 1.0) -> "RouterPlan":
+        """hidden 0: a plan that selects from given logits only."""
+        if score not in SCORES:
+            raise OcoError(_lib.INVALID_ARGUMENT, f"score is one of {sorted(SCORES)}")
+        self = cls()
+        self._open(_lib.lib().oco_moe_router_create,
+                   _lib.RouterDesc(hidden=hidden, experts=experts, top_k=active, score=SCORES[score], groups=groups, top_groups=top_groups,
+                                   group_best=group_best, normalize=int(bool(normalize)), scale=float(scale)))
+        return self
+
+    def bind(self, router_w: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None):
+        """f32 CUDA tensors [experts, hidden] and [experts]; they must stay unchanged."""
+        d = self.desc
+        for t, name, count in ((router_w, "router_w", d.experts * d.hidden), (bias, "bias", d.experts)):
+            if t is not None:
+                need(t, name, 4, count, self.workspace)
+        self._check(self._fn["bind_weights"](self.handle, _ptr(router_w), _ptr(bias)))
+        self._weights = (router_w, bias)
+
+    def forward(self, x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int, logits: Optional[torch.Tensor] = None):
+        """x bf16 [rows, hidden] -> ids (32-bit) and probs f32 [rows, active], and the logits f32 [rows, experts] if asked for."""
+        d = self.desc
+        need(x, "x", 2, rows * d.hidden, self.workspace)
+        need(ids, "ids", 4, rows * d.top_k, self.workspace)
+        need(probs, "probs", 4, rows * d.top_k, self.workspace)
+        if logits is not None:
+            need(logits, "logits", 4, rows * d.experts, self.workspace)
+        self._check(self._fn["forward"](self.handle, x.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(),
+                                        logits.data_ptr() if logits is not None else None, _stream_ptr()))
+
+    def select(self, logits: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int):
+        """The selection alone, from logits f32 [rows, experts] of any origin."""
+        d = self.desc
+        need(logits, "logits", 4, rows * d.experts, self.workspace)
+        _on_current(logits, "logits")
+        need(ids, "ids", 4, rows * d.top_k, logits)
+        need(probs, "probs", 4, rows * d.top_k, logits)
+        self._check(_lib.lib().oco_moe_router_select(self.handle, logits.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), _stream_ptr()))
+
+
+@dataclass
+class F8Experts:
+    """Codes (e4m3, or their bytes) [experts, ffn, hidden] (gate, up) and [experts, hidden, ffn] (down) with the f32 scales
+    [experts, ceil(rows / 128), ceil(columns / 128)] of the same matrices."""
+    gate_w: object
+    gate_s: object
+    up_w: object
+    up_s: object
+    down_w: object
+    down_s: object
+
+
+class F8ExpertPlan(_GroupPlan):
+    """SiLU-gated experts with e4m3 weights and block scales (oco_moe_f8_*)."""
+    _prefix, _destroy = "oco_moe_f8_", "oco_moe_f8_plan_destroy"
+
+    @classmethod
+    def new(cls, hidden: int, ffn: int, experts: int, active: int) -> "F8ExpertPlan":
+        self = cls()
+        self._open(_lib.lib().oco_moe_f8_plan_create, _lib.F8Desc(hidden=hidden, ffn=ffn, experts=experts, top_k=active))
+        return self
+
+    def bind(self, w: F8Experts, device="cuda"):
+        d = self.desc
+        got = {}
+        for name, n, k in (("gate", d.ffn, d.hidden), ("up", d.ffn, d.hidden), ("down", d.hidden, d.ffn)):
+            got[name + "_w"], got[name + "_s"] = f8_matrix(getattr(w, name + "_w"), getattr(w, name + "_s"), (d.experts,), n, k, device, name)
+        cw = _lib.F8Weights(**{n: t.data_ptr() for n, t in got.items()})
+        self._check(self._fn["bind_weights"](self.handle, C.byref(cw)))
+        self._weights = got
+
+    def forward(self, x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, residual: torch.Tensor, rows: int,
+                out: Optional[torch.Tensor] = None):
+        """out = residual + the weighted expert outputs (bf16 rows; out None: in place). Ids outside 0 .. experts - 1 are left out."""
+        d = self.desc
+        out = residual if out is None else out
+        need(x, "x", 2, rows * d.hidden, self.workspace)
+        need(ids, "ids", 4, rows * d.top_k, self.workspace)
+        need(probs, "probs", 4, rows * d.top_k, self.workspace)
+        need(residual, "residual", 2, rows * d.hidden, self.workspace)
+        need(out, "out", 2, rows * d.hidden, self.workspace)
+        self._check(self._fn["forward"](self.handle, x.data_ptr(), ids.data_ptr(), probs.data_ptr(), residual.data_ptr(), out.data_ptr(), rows,
+                                        _stream_ptr()))
+
+
+NORMS = {"rms": 0, "layer": 1}
+GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
+
+
+def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hidden_out: Optional[torch.Tensor] = None,
+               norm_out: Optional[torch.Tensor] = None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None,
+               gate: Optional[torch.Tensor] = None, gate_rows: Optional[int] = None, gate_act: str = "none", kind: str = "rms",
+               weight_offset: float = 0.0, residual_scale: float = 1.0, block_scale: float = 1.0, epsilon: float = 1e-6):
+    """The step between two blocks (oco_moe_block_norm): h = residual_scale * hidden + block_scale * act(gate) * post(block)
+    into hidden_out, pre(h) into norm_out; hidden_out may be hidden, norm_out may be block. Rows are [rows, width] with unit
+    stride inside a row; hidden bf16 or f32, block and norm_out bf16, weights f32 [width]. The gate is [width] (for all rows)
+    or [gates, width], of which row r takes gate r // gate_rows (default: rows / gates), bf16 or f32."""
+    def refuse(text):
+        raise OcoError(_lib.INVALID_ARGUMENT, text)
+
+    if hidden.dim() != 2 or not hidden.is_cuda or hidden.dtype not in (torch.bfloat16, torch.float32):
+        refuse("hidden: CUDA rows [rows, width], bf16 or f32")
+    _on_current(hidden, "hidden")
+    rows, width = hidden.shape
+    if kind not in NORMS or gate_act not in GATE_ACTS:
+        refuse(f"kind is one of {sorted(NORMS)}, gate_act one of {sorted(GATE_ACTS)}")
+    a = _lib.BlockNormArgs(width=width, kind=NORMS[kind], wide=int(hidden.dtype == torch.float32), gate_act=GATE_ACTS[gate_act], epsilon=epsilon,
+                           weight_offset=weight_offset, residual_scale=residual_scale, block_scale=block_scale)
+    for t, name, dtype in ((hidden, "hidden", hidden.dtype), (block, "block", torch.bfloat16), (hidden_out, "hidden_out", hidden.dtype),
+                           (norm_out, "norm_out", torch.bfloat16)):
+        if t is None:
+            continue
+        if t.shape != hidden.shape or t.dtype != dtype or t.device != hidden.device or t.stride(1) != 1:
+            refuse(f"{name}: rows {tuple(hidden.shape)} of {dtype} on {hidden.device} with unit stride inside a row are needed")
+        setattr(a, name, t.data_ptr())
+        if rows > 1:
+            setattr(a, name + "_stride", t.stride(0))
+    for t, name in ((pre_weight, "pre_w"), (pre_bias, "pre_b"), (post_weight, "post_w"), (post_bias, "post_b")):
+        if t is not None:
+            need(t, name, 4, width, hidden)
+            setattr(a, name, t.data_ptr())
+    if gate is not None:
+        if gate.dtype not in (torch.bfloat16, torch.float32) or gate.device != hidden.device or gate.shape[-1] != width or gate.stride(-1) != 1 or gate.dim() > 2:
+            refuse("gate: [width] or [gates, width], bf16 or f32, unit stride inside a row")
+        a.gate, a.gate_type = gate.data_ptr(), 2 if gate.dtype == torch.float32 else 1
+        if gate.dim() == 2:
+            gates = gate.shape[0]
+            a.gate_rows = gate_rows if gate_rows is not None else (rows // gates if gates and rows % gates == 0 else 0)
+            if rows and (a.gate_rows < 1 or (rows - 1) // a.gate_rows >= gates):
+                refuse("gate: fewer gate rows than the rows need")
+            if gates > 1:
+                a.gate_stride = gate.stride(0)
+    if rows == 0:      # an empty tensor has no address
+        return
+    err = C.create_string_buffer(160)
+    rc = _lib.lib().oco_moe_block_norm(C.byref(a), rows, _stream_ptr(), err, len(err))
+    if rc != _lib.OK:
+        raise OcoError(rc, err.value.decode())
+
+
 @dataclass
 class Scratch:
     """The slice of the reference's `CommonScratch` this path reads (src/weights/state.rs:148-177)."""

@@ -20,6 +20,7 @@ from typing import Optional
 import numpy as np
 
 FMT_Q4_0, FMT_Q4_K, FMT_MXFP4 = 2, 12, 39
+FMT_F8_E4M3 = 128   # no GGUF type: e4m3 codes, f32 scales of 128 x 128 blocks in a tensor of their own
 ARCH_GPT_OSS, ARCH_NEMOTRON, ARCH_QWEN = 0, 1, 2
 
 BLOCK = {FMT_MXFP4: (32, 17), FMT_Q4_0: (32, 18), FMT_Q4_K: (256, 144)}

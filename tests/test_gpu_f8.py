@@ -1,0 +1,339 @@
+"""8-bit float products with block scales (dense and routed) against their 64-bit form."""
+import numpy as np
+import pytest
+import torch
+
+from oco_b200 import _lib, synth
+from tests import opref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from oco_b200 import build, dense, moe
+    build.build()
+
+    class Mods:
+        pass
+    m = Mods()
+    m.moe, m.dense = moe, dense
+    return m
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def bf16(g, *shape):
+    return torch.randn(shape, device="cuda", generator=g).to(torch.bfloat16)
+
+
+def projection(lib, up, up_s, x, rows=None, max_rows=None):
+    F, H = up.shape
+    rows = x.shape[0] if rows is None else rows
+    plan = lib.dense.DensePlan(lib.dense.PROJECTION, synth.FMT_F8_E4M3, H, F)
+    plan.reserve(max_rows or rows)
+    plan.bind(up, up_scale=up_s)
+    y = torch.full((x.shape[0], F), 7.0, dtype=torch.bfloat16, device="cuda")
+    plan.forward(x, y, rows)
+    plan.poll()
+    return plan, y
+
+
+# the result: one rounding to bf16 (2^-8), and sums of exact products: f32 inside a block of 128 and over the blocks.
+# 2^-14 of the terms' sizes allows the tensor cores any order and truncation of 128 terms (128 * 2^-23 = 2^-16) and the
+# f32 sum of up to 64 blocks' scaled sums
+def within(y, want, terms):
+    assert ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * terms).all(), ((y.double() - want).abs() / (terms + 1e-30)).max()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 8, 15, 16, 17, 33, 64, 100, 128, 129, 257, 600])
+@pytest.mark.parametrize("hidden,ffn", [(32, 32), (128, 128), (160, 96), (512, 384), (2880, 320), (1056, 1312)])
+def test_projection(lib, rows, hidden, ffn):
+    g = gen(rows * 7 + hidden)
+    up, up_s = opref.weights(g, (), ffn, hidden)
+    x = bf16(g, rows, hidden)
+    _, y = projection(lib, up, up_s, x)
+    within(y, *opref.product(*opref.quantize(x.double()), up, up_s))
+
+
+@pytest.mark.parametrize("rows,hidden,ffn", [(1, 4096, 6144), (5, 8192, 512), (40, 4096, 4096), (300, 4096, 2048), (1100, 1024, 4096)])
+def test_projection_larger(lib, rows, hidden, ffn):
+    g = gen(5)
+    up, up_s = opref.weights(g, (), ffn, hidden)
+    x = bf16(g, rows, hidden)
+    _, y = projection(lib, up, up_s, x)
+    within(y, *opref.product(*opref.quantize(x.double()), up, up_s))
+
+
+@pytest.mark.parametrize("rows", [1, 20, 70, 300])
+def test_integers_are_exact(lib, rows):
+    """Codes that are small whole numbers and scales of 1: every sum is exact in f32, the result is its bf16 rounding."""
+    H, F = 1184, 416
+    g = gen(rows)
+    x = torch.randint(-8, 9, (rows, H), device="cuda", generator=g).double()
+    x[:, ::128] = 448.0                                            # every block's scale is 1
+    up = torch.randint(-4, 5, (F, H), device="cuda", generator=g).double()
+    up_s = torch.ones((-(-F // 128), -(-H // 128)), device="cuda")
+    _, y = projection(lib, up.float().to(torch.float8_e4m3fn), up_s, x.to(torch.bfloat16))
+    assert torch.equal(y, (x @ up.t()).to(torch.bfloat16))
+
+
+def test_rounding_of_rows_halfway_between_codes(lib):
+    """Rows whose quotients lie halfway between two codes; the identity as weights shows the codes themselves."""
+    H = 128
+    rows = 240
+    x = torch.zeros((rows, H), dtype=torch.float64)
+    tops = torch.arange(128, 248).double()
+    for i in range(rows):
+        top = tops[i % 120] * 2.0 ** (i % 7 - 3)
+        x[i, 0] = top
+        mid = torch.tensor([17.0, 19.0, 21.0, 23.0, 25.0, 27.0, 29.0, 31.0]) / 16          # halfway between neighbours of a binade
+        x[i, 1:9] = (mid * top / 448 * 64)
+        x[i, 9:128] = torch.linspace(-1, 1, 119) * top
+    x = x.to(torch.bfloat16).cuda()
+    eye = torch.eye(H, device="cuda").to(torch.float8_e4m3fn)
+    _, y = projection(lib, eye, torch.ones((1, 1), device="cuda"), x)
+    codes, scales = opref.quantize(x.double())
+    assert torch.equal(y, (codes.float() * scales.float()).to(torch.bfloat16))
+
+
+def ffn_near(y, want, extra=0.0):
+    """Two more roundings than a projection: activations to e4m3 (the same on both sides but where f32 and f64 lie on
+    different sides of a border between codes) and bf16. Of n activations a share of about (error 2^-14) / (step 2^-3)
+    = 2^-11 may land on the neighbouring code, off by at most 2^-3: 2^-3 * sqrt(2^-11) < 2^-8 of the result's norm."""
+    err = (y.double() - want).norm() / want.norm()
+    assert err <= 2.0 ** -8 + 2.0 ** -8 + extra, err
+
+
+@pytest.mark.parametrize("rows", [1, 3, 16, 40, 129, 400])
+@pytest.mark.parametrize("hidden,ffn", [(64, 32), (256, 384), (2048, 768), (416, 2080)])
+def test_gated_feed_forward(lib, rows, hidden, ffn):
+    g = gen(rows + ffn)
+    w = dict(zip(("gate", "gate_s", "up", "up_s", "down", "down_s"),
+                 (*opref.weights(g, (), ffn, hidden), *opref.weights(g, (), ffn, hidden), *opref.weights(g, (), hidden, ffn))))
+    x = bf16(g, rows, hidden)
+    plan = lib.dense.DensePlan(lib.dense.FFN_SILU_GATE, synth.FMT_F8_E4M3, hidden, ffn)
+    plan.reserve(rows)
+    plan.bind(w["up"], w["gate"], w["down"], up_scale=w["up_s"], gate_scale=w["gate_s"], down_scale=w["down_s"])
+    y = torch.empty_like(x)
+    plan.forward(x, y, rows)
+    plan.poll()
+    ffn_near(y, opref.ffn(x.double(), **w))
+
+
+def expert_layer(lib, seed, H, F, E, K, max_rows):
+    g = gen(seed)
+    names = ("gate", "up", "down")
+    w = {}
+    for n in names:
+        w[n], w[n + "_s"] = opref.weights(g, (E,), *((H, F) if n == "down" else (F, H)))
+    plan = lib.moe.F8ExpertPlan.new(H, F, E, K)
+    plan.reserve(max_rows)
+    plan.bind(lib.moe.F8Experts(**{k2: w[k1] for n in names for k1, k2 in ((n, n + "_w"), (n + "_s", n + "_s"))}))
+    return plan, w, g
+
+
+def experts_want(w, x, ids, probs, residual):
+    out = residual.double().clone()
+    E = w["gate"].shape[0]
+    for e in range(E):
+        t, j = torch.nonzero(ids == e, as_tuple=True)
+        if t.numel():
+            y = opref.ffn(x[t].double(), **{n: w[n][e] for n in ("gate", "gate_s", "up", "up_s", "down", "down_s")})
+            out.index_add_(0, t, y * probs[t, j].double().unsqueeze(1))
+    return out
+
+
+@pytest.mark.parametrize("H,F,E,K", [(64, 32, 4, 2), (256, 160, 8, 3), (2048, 768, 32, 8), (320, 256, 300, 6), (416, 96, 1, 1), (128, 128, 512, 16)])
+@pytest.mark.parametrize("rows", [1, 2, 9, 64, 333])
+def test_experts(lib, H, F, E, K, rows):
+    plan, w, g = expert_layer(lib, rows + E, H, F, E, K, rows)
+    x, res = bf16(g, rows, H), bf16(g, rows, H)
+    ids = torch.topk(torch.rand((rows, E), device="cuda", generator=g), K, 1).indices.to(torch.int32)
+    ids[torch.rand((rows, K), device="cuda", generator=g) < 0.15] = -1                       # routes of other shards
+    probs = torch.rand((rows, K), device="cuda", generator=g)
+    out = torch.empty_like(res)
+    plan.forward(x, ids, probs, res, rows, out=out)
+    plan.poll()
+    want = experts_want(w, x, ids, probs, res)
+    ffn_near(out, want, 2.0 ** -8)
+    keep = (ids < 0).all(1)
+    assert torch.equal(out[keep], res[keep])
+    again = res.clone()
+    plan.forward(x, ids, probs, again, rows)                                                  # in place
+    assert torch.equal(again, out)
+
+
+def test_one_expert_takes_all_and_an_expert_twice(lib):
+    plan, w, g = expert_layer(lib, 3, 256, 256, 16, 4, 300)
+    x, res = bf16(g, 300, 256), bf16(g, 300, 256)
+    probs = torch.rand((300, 4), device="cuda", generator=g)
+    for ids in (torch.full((300, 4), 5), torch.tensor([[3, 3, -1, 3]]).repeat(300, 1), torch.full((300, 4), -1), torch.full((300, 4), 16),
+                torch.tensor([[0, 15, 2**31 - 1, -2**31]]).repeat(300, 1)):
+        ids = ids.to(torch.int32).cuda()
+        out = torch.empty_like(res)
+        plan.forward(x, ids, probs, res, 300, out=out)
+        ffn_near(out, experts_want(w, x, ids, probs, res), 2.0 ** -8)
+        if not ((ids >= 0) & (ids < 16)).any():
+            assert torch.equal(out, res)
+
+
+def test_weights_of_absent_routes_are_not_read(lib):
+    plan, w, g = expert_layer(lib, 4, 128, 128, 4, 2, 5)
+    x, res = bf16(g, 5, 128), bf16(g, 5, 128)
+    ids = torch.tensor([[0, -1]] * 5, dtype=torch.int32, device="cuda")
+    probs = torch.tensor([[0.5, float("nan")]] * 5, device="cuda")
+    out = torch.empty_like(res)
+    plan.forward(x, ids, probs, res, 5, out=out)
+    assert out.isfinite().all()
+
+
+def test_rows_of_zeros_and_bad_values_stay_in_their_row(lib):
+    plan, w, g = expert_layer(lib, 5, 384, 128, 4, 2, 40)
+    x, res = bf16(g, 40, 384), bf16(g, 40, 384)
+    ids = torch.topk(torch.rand((40, 4), device="cuda", generator=g), 2, 1).indices.to(torch.int32)
+    probs = torch.rand((40, 2), device="cuda", generator=g)
+    x[7] = 0
+    x[9, 130] = float("nan")
+    x[11, 5] = float("inf")
+    x[13] = torch.finfo(torch.bfloat16).tiny / 64          # subnormal rows
+    x[15] *= 1e38
+    out = torch.empty_like(res)
+    plan.forward(x, ids, probs, res, 40, out=out)
+    assert torch.equal(out[7], res[7])
+    assert out[9].isnan().all() and out[11].isnan().all()
+    rows = [r for r in range(40) if r not in (9, 11, 15)]
+    assert out[rows].isfinite().all()
+    want = experts_want(w, x[rows], ids[rows], probs[rows], res[rows])
+    ffn_near(out[rows], want, 2.0 ** -8)
+
+
+def test_a_row_does_not_depend_on_its_neighbours(lib):
+    """The same row alone, among few and among many: the sums run in the same order up to the parts of a split contraction."""
+    plan, w, g = expert_layer(lib, 6, 512, 256, 8, 2, 500)
+    x, res = bf16(g, 500, 512), bf16(g, 500, 512)
+    ids = torch.topk(torch.rand((500, 8), device="cuda", generator=g), 2, 1).indices.to(torch.int32)
+    probs = torch.rand((500, 2), device="cuda", generator=g)
+    out = torch.empty_like(res)
+    plan.forward(x, ids, probs, res, 500, out=out)
+    for rows in (1, 30, 200):
+        part = torch.empty_like(res)
+        plan.forward(x, ids, probs, res, rows, out=part)
+        ffn_near(part[:rows], out[:rows].double(), 0.0)
+
+
+def test_rows_behind_the_last_one_are_left_alone(lib):
+    g = gen(7)
+    up, up_s = opref.weights(g, (), 96, 160)
+    x = bf16(g, 50, 160)
+    plan, y = projection(lib, up, up_s, x, rows=37, max_rows=64)
+    assert (y[37:] == 7.0).all() and not (y[:37] == 7.0).all()
+    y.fill_(7.0)
+    plan.forward(x, y, 0)
+    assert (y == 7.0).all() and plan.launch_count() == 0
+    eplan, w, g = expert_layer(lib, 8, 160, 96, 4, 2, 64)
+    out = torch.full((50, 160), 7.0, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros((50, 2), dtype=torch.int32, device="cuda")
+    probs = torch.ones((50, 2), device="cuda")
+    eplan.forward(x, ids, probs, x, 37, out=out)
+    assert (out[37:] == 7.0).all()
+    out.fill_(7.0)
+    eplan.forward(x, ids, probs, x, 0, out=out)
+    assert (out == 7.0).all()
+
+
+def test_streams_graphs_and_calls_in_a_row(lib):
+    plan, w, g = expert_layer(lib, 9, 512, 256, 16, 4, 200)
+    x, res = bf16(g, 200, 512), bf16(g, 200, 512)
+    ids = torch.topk(torch.rand((200, 16), device="cuda", generator=g), 4, 1).indices.to(torch.int32)
+    probs = torch.rand((200, 4), device="cuda", generator=g)
+    want = {}
+    for rows in (1, 8, 60, 200):
+        want[rows] = torch.empty_like(res)
+        plan.forward(x, ids, probs, res, rows, out=want[rows])
+    torch.cuda.synchronize()
+    got = {r: torch.empty_like(res) for r in want}
+    for _ in range(3):                                       # back to back, nothing waits between
+        for rows in (200, 1, 60, 8):
+            plan.forward(x, ids, probs, res, rows, out=got[rows])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    for rows in want:
+        assert torch.equal(got[rows][:rows], want[rows][:rows])
+    with torch.cuda.stream(s):
+        plan.forward(x, ids, probs, res, 60, out=got[60])
+    s.synchronize()
+    assert torch.equal(got[60][:60], want[60][:60])
+    graphs = []
+    for rows in want:                                        # several graphs over one workspace, replayed in any order
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.forward(x, ids, probs, res, rows, out=got[rows])
+        graphs.append((rows, graph))
+    for rows, graph in graphs + graphs[::-1]:
+        got[rows].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[rows][:rows], want[rows][:rows])
+
+
+def test_refused_tensors(lib):
+    plan, w, g = expert_layer(lib, 10, 128, 128, 4, 2, 8)
+    x = bf16(g, 8, 128)
+    ids, probs = torch.zeros((8, 2), dtype=torch.int32, device="cuda"), torch.ones((8, 2), device="cuda")
+    for args in ((x.float(), ids, probs, x), (x, ids.long(), probs, x), (x, ids, probs.half(), x), (x, ids, probs, x[:4]), (x.cpu(), ids, probs, x)):
+        with pytest.raises(_lib.OcoError):
+            plan.forward(*args, 8)
+    with pytest.raises(_lib.OcoError, match="rows"):
+        big = bf16(g, 9, 128)
+        plan.forward(big, ids.new_zeros((9, 2)), probs.new_ones((9, 2)), big, 9)
+    with pytest.raises(_lib.OcoError, match="scales"):
+        plan.bind(lib.moe.F8Experts(w["gate"], w["gate_s"][:, :, :0], w["up"], w["up_s"], w["down"], w["down_s"]))
+    shifted = torch.zeros(8 * 128 + 4, dtype=torch.bfloat16, device="cuda")[4:]
+    plan2 = lib.dense.DensePlan(lib.dense.PROJECTION, synth.FMT_F8_E4M3, 128, 64)
+    plan2.reserve(8)
+    with pytest.raises(_lib.OcoError, match="bind"):
+        plan2.forward(x, x, 8)
+    plan2.bind(np.zeros((64, 128), np.uint8), up_scale=np.ones((1, 1), np.float32))           # host arrays are uploaded
+    y = torch.ones((8, 64), dtype=torch.bfloat16, device="cuda")
+    plan2.forward(x, y, 8)
+    assert not y.any()
+    with pytest.raises(_lib.OcoError, match="aligned"):
+        plan2.forward(shifted, y, 8)
+
+
+def test_a_layer_of_the_operators(lib):
+    """Norm, routing with groups, experts and the next norm, as a layer runs them, for a prefill batch and a token."""
+    H, F, E, K = 512, 256, 64, 6
+    plan, w, g = expert_layer(lib, 11, H, F, E, K, 150)
+    router = lib.moe.RouterPlan.new(H, E, K, groups=8, top_groups=3, group_best=2, scale=2.5)
+    router.reserve(150)
+    rw = torch.randn((E, H), device="cuda", generator=g) * 0.05
+    rb = torch.randn(E, device="cuda", generator=g) * 0.1
+    router.bind(rw, rb)
+    pre, post = (1 + 0.1 * torch.randn(H, device="cuda", generator=g) for _ in range(2))
+    for rows in (150, 1):
+        hidden, block = bf16(g, rows, H), bf16(g, rows, H)
+        x, ids, probs = torch.empty_like(hidden), torch.empty((rows, K), dtype=torch.int32, device="cuda"), torch.empty((rows, K), device="cuda")
+        zero = torch.zeros_like(hidden)
+        h0 = hidden.clone()
+        lib.moe.block_norm(hidden, block, hidden_out=hidden, norm_out=x, pre_weight=pre, post_weight=post)
+        router.forward(x, ids, probs, rows)
+        moe_out = torch.empty_like(hidden)
+        plan.forward(x, ids, probs, zero, rows, out=moe_out)
+        nxt = torch.empty_like(hidden)
+        lib.moe.block_norm(hidden, moe_out, hidden_out=hidden, norm_out=nxt, pre_weight=pre, post_weight=post, residual_scale=0.5)
+        plan.poll()
+        # the same from the rows the operators handed on: each stage is held to its own rounding
+        wid, wp = opref.route((x.double() @ rw.double().t()).cpu().numpy(), rb.double().cpu().numpy(), E, K, "sigmoid", 8, 3, 2, True, 2.5)
+        assert np.array_equal(ids.cpu().numpy(), wid)
+        ffn_near(moe_out, experts_want(w, x, ids, probs, zero), 2.0 ** -8)
+        h1, _ = opref.block_norm(h0, block, pre, None, post)
+        h2, n2 = opref.block_norm(h1.to(torch.bfloat16), moe_out, pre, None, post, residual_scale=0.5)
+        assert (hidden.double() - h2).norm() <= 2.0 ** -7 * h2.norm() and (nxt.double() - n2).norm() <= 2.0 ** -7 * n2.norm()

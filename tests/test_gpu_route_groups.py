@@ -1,0 +1,247 @@
+"""Routing with groups of experts against the 64-bit definition: ids exact, weights within their 32-bit rounding."""
+import numpy as np
+import pytest
+import torch
+
+from oco_b200 import _lib
+from tests import opref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def moe():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from oco_b200 import build, moe as m
+    build.build()
+    return m
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+# experts, active, score, groups, top_groups, best, bias, normalize, scale
+SHAPES = [
+    (8, 2, "softmax", 1, 1, 1, False, True, 1.0),
+    (32, 4, "sigmoid", 1, 1, 1, True, False, 2.5),
+    (64, 6, "softmax", 8, 3, 1, False, True, 1.0),
+    (128, 8, "softmax", 1, 1, 1, False, True, 1.0),
+    (160, 6, "sigmoid", 5, 2, 2, True, True, 2.5),
+    (256, 8, "sigmoid", 8, 4, 2, True, True, 2.5),
+    (270, 9, "softmax", 5, 1, 2, True, True, 1.0),
+    (384, 16, "sigmoid", 1, 1, 1, True, True, 1.0),
+    (512, 16, "softmax", 32, 31, 2, True, False, 1.0),
+    (16, 1, "sigmoid", 16, 1, 2, True, True, 1.0),      # groups of one expert
+    (1, 1, "softmax", 1, 1, 1, False, True, 1.0),
+    (10, 10, "sigmoid", 2, 2, 1, False, True, 1.0),     # every expert chosen
+]
+
+
+def make(moe, shape, hidden, rows, seed):
+    E, K, score, G, TG, best, bias, normalize, scale = shape
+    r = moe.RouterPlan.new(hidden, E, K, score=score, groups=G, top_groups=TG, group_best=best, normalize=normalize, scale=scale)
+    r.reserve(max(rows, 1))
+    g = gen(seed)
+    b = torch.randn(E, device="cuda", generator=g) * 0.1 if bias else None
+    w = torch.randn((E, hidden), device="cuda", generator=g) * (1.3 / max(hidden, 1) ** 0.5) if hidden else None
+    r.bind(w, b)
+    return r, w, b, g
+
+
+def outputs(shape, rows):
+    K = shape[1]
+    return torch.full((rows, K), -7, dtype=torch.int32, device="cuda"), torch.full((rows, K), -7.0, device="cuda")
+
+
+def expect(shape, logits, b):
+    E, K, score, G, TG, best, _, normalize, scale = shape
+    return opref.route(logits.cpu().numpy(), None if b is None else b.double().cpu().numpy(), E, K, score, G, TG, best, normalize, scale)
+
+
+# a weight is a quotient of scores: exponential, sum and quotient in f32, each within a few units in the last place, and
+# the logit's own error through the slope (at most its size times 2^-22); 2^-20 relative holds all of it
+REL = 2.0 ** -20
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("rows", [1, 7, 130])
+def test_select_matches_the_definition(moe, shape, rows):
+    r, _, b, g = make(moe, shape, 0, rows, 1)
+    logits = torch.randn((rows, shape[0]), device="cuda", generator=g) * 1.5
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    r.poll()
+    want, p = expect(shape, logits.double(), b)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL, atol=0)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("hidden,rows", [(32, 3), (96, 65), (2688, 1), (2080, 9), (1024, 200), (4096, 513)])
+def test_forward_matches_the_definition(moe, shape, hidden, rows):
+    r, w, b, g = make(moe, shape, hidden, rows, 2)
+    x = torch.randn((rows, hidden), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, rows)
+    logits = torch.empty((rows, shape[0]), device="cuda")
+    r.forward(x, ids, probs, rows, logits=logits)
+    r.poll()
+    exact = x.double() @ w.double().t()
+    # the product: f32 accumulation of exact products of row and weight; 2^-21 of the sum of the terms' sizes
+    assert ((logits.double() - exact).abs() <= 2.0 ** -21 * (x.double().abs() @ w.double().abs().t())).all()
+    want, p = expect(shape, exact, b)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    # the logit's error enters the weight through its slope: at most 2^-21 of the terms' sizes (here below 2^5)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=2.0 ** -16, atol=0)
+
+
+def test_equal_values_go_to_the_lower_index(moe):
+    shape = (256, 8, "sigmoid", 8, 4, 2, False, True, 1.0)
+    r, _, _, _ = make(moe, shape, 0, 4, 3)
+    logits = torch.zeros((4, 256), device="cuda")
+    logits[1, 100:] = 0.5
+    logits[2] = torch.arange(256, device="cuda") // 2 * 0.25 - 20      # pairs of equal logits
+    logits[3, ::2] = -0.0                                              # the two zeros are equal
+    ids, probs = outputs(shape, 4)
+    r.select(logits, ids, probs, 4)
+    want, p = expect(shape, logits.double(), None)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
+
+
+def test_scores_that_32_bits_cannot_tell_apart(moe):
+    """Logits near 20 have sigmoids within 2e-9 of 1: the order is decided in 64 bits."""
+    shape = (64, 8, "sigmoid", 4, 2, 2, True, True, 1.0)
+    r, _, b, g = make(moe, shape, 0, 50, 4)
+    r.bind(None, None)
+    logits = 20.0 + torch.rand((50, 64), device="cuda", generator=g)
+    ids, probs = outputs(shape, 50)
+    r.select(logits, ids, probs, 50)
+    want, p = expect(shape, logits.double(), None)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_near_ties_of_the_product_are_decided_in_64_bits(moe, score, bias):
+    """Weight rows that differ in their last bits give logits that 32-bit sums cannot order."""
+    E, H, rows = 64, 1024, 40
+    shape = (E, 8, score, 4, 2, 2, bias, True, 1.0)
+    r, w, b, g = make(moe, shape, H, rows, 5)
+    w = w[:8].repeat(8, 1)
+    w *= 1.0 + (torch.rand((E, H), device="cuda", generator=g) - 0.5) * 2e-7
+    if bias:
+        b = b[:8].repeat(8)
+    r.bind(w, b)
+    x = torch.randn((rows, H), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, rows)
+    r.forward(x, ids, probs, rows)
+    want, p = expect(shape, x.double() @ w.double().t(), b)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=2.0 ** -16)
+
+
+def test_ids_do_not_depend_on_the_rows_of_the_call(moe):
+    shape = (256, 8, "sigmoid", 8, 4, 2, True, True, 2.5)
+    r, w, b, g = make(moe, shape, 2048, 400, 6)
+    x = torch.randn((400, 2048), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, 400)
+    r.forward(x, ids, probs, 400)
+    for rows in (1, 5, 33, 100):
+        i2, p2 = outputs(shape, rows)
+        r.forward(x[:rows], i2, p2, rows)
+        assert torch.equal(i2, ids[:rows])
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_values_that_are_not_finite(moe, score):
+    """A non-finite logit: NaN weights, valid distinct ids, other rows untouched. A bias of -inf keeps an expert out."""
+    shape = (32, 4, score, 4, 2, 2, True, True, 1.0)
+    r, _, b, g = make(moe, shape, 0, 6, 7)
+    b = b.clone()
+    b[::2] = -float("inf")
+    r.bind(None, b)
+    logits = torch.randn((6, 32), device="cuda", generator=g)
+    clean = logits.clone()
+    logits[1, 5] = float("nan")
+    logits[2, 6] = float("inf")
+    logits[3, :] = -float("inf")
+    logits[4, 1] = -3.0e38
+    clean[4, 1] = -3.0e38
+    ids, probs = outputs(shape, 6)
+    r.select(logits, ids, probs, 6)
+    ids, probs = ids.cpu().numpy(), probs.cpu().numpy()
+    assert np.isnan(probs[1:4]).all() and np.isfinite(probs[[0, 4, 5]]).all()
+    assert all(len(set(row)) == 4 and (row >= 0).all() and (row < 32).all() for row in ids)
+    want, p = expect(shape, clean.double(), b)
+    assert np.array_equal(ids[[0, 4, 5]], want[[0, 4, 5]])
+    np.testing.assert_allclose(probs[[0, 4, 5]], p[[0, 4, 5]], rtol=REL)
+
+
+def test_rows_of_zeros_and_of_nan(moe):
+    shape = (128, 8, "sigmoid", 8, 4, 2, False, True, 1.0)
+    r, w, b, g = make(moe, shape, 512, 64, 8)
+    x = torch.zeros((64, 512), device="cuda", dtype=torch.bfloat16)
+    x[5, 7] = float("nan")
+    ids, probs = outputs(shape, 64)
+    r.forward(x, ids, probs, 64)
+    p = probs.cpu().numpy()
+    assert np.isnan(p[5]).all() and np.all(np.delete(p, 5, 0) == 0.125)
+    want, _ = expect(shape, torch.zeros((1, 128), dtype=torch.float64), None)
+    assert (np.delete(ids.cpu().numpy(), 5, 0) == want).all()
+
+
+def test_rows_behind_the_last_one_are_left_alone_and_no_rows_are_no_work(moe):
+    shape = (64, 6, "softmax", 1, 1, 1, False, True, 1.0)
+    r, w, b, g = make(moe, shape, 256, 16, 9)
+    x = torch.randn((16, 256), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, 16)
+    r.forward(x, ids, probs, 0)
+    assert r.launch_count() == 0 and (ids == -7).all()
+    r.forward(x, ids, probs, 11)
+    assert (ids[11:] == -7).all() and (probs[11:] == -7.0).all() and (ids[:11] >= 0).all()
+    with pytest.raises(_lib.OcoError, match="rows 17 outside"):
+        r.forward(torch.zeros((17, 256), device="cuda", dtype=torch.bfloat16), *outputs(shape, 17), 17)
+
+
+def test_a_side_stream_and_a_replayed_graph(moe):
+    shape = (256, 8, "sigmoid", 8, 4, 2, True, True, 2.5)
+    r, w, b, g = make(moe, shape, 1024, 40, 10)
+    x = torch.randn((40, 1024), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, 40)
+    r.forward(x, ids, probs, 40)
+    torch.cuda.synchronize()
+    i2, p2 = outputs(shape, 40)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        r.forward(x, i2, p2, 40)
+    s.synchronize()
+    assert torch.equal(ids, i2) and torch.equal(probs, p2)
+    xs = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r.forward(xs, i2, p2, 40)
+    xs.copy_(x)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(ids, i2) and torch.equal(probs, p2)
+
+
+def test_refused_tensors(moe):
+    shape = (64, 6, "softmax", 1, 1, 1, False, True, 1.0)
+    r, w, b, g = make(moe, shape, 256, 4, 11)
+    x = torch.zeros((4, 256), device="cuda", dtype=torch.bfloat16)
+    ids, probs = outputs(shape, 4)
+    for bad in (x.cpu(), x.float(), x[:2], torch.zeros((256, 4), device="cuda", dtype=torch.bfloat16).t()):
+        with pytest.raises(_lib.OcoError, match="x"):
+            r.forward(bad, ids, probs, 4)
+    with pytest.raises(_lib.OcoError, match="ids"):
+        r.forward(x, ids.long(), probs, 4)
+    shifted = torch.zeros(4 * 256 + 1, device="cuda", dtype=torch.bfloat16)[1:]
+    with pytest.raises(_lib.OcoError, match="aligned"):
+        r.forward(shifted, ids, probs, 4)
