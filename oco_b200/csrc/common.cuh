@@ -189,6 +189,13 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
     mbar_wait_for(bar, parity, abort_flag, status_word, kWaitCycles);
 }
 
+// The same for the end of a kernel whose wait has given up: copies and MMAs that are in flight come to their end, or the
+// limit does, before the CTA frees what they use.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - start <= kWaitCycles) {}
+}
+
 // Programmatic dependent launch: a kernel launched with the programmatic-serialization attribute may
 // start while its predecessor in the stream still runs; pdl_wait() returns when the predecessor has
 // completed and its writes are visible. pdl_launch_dependents() lets the successor start launching.

@@ -4,11 +4,14 @@
 
 #include "f8.cuh"
 #include "f8.h"
+#include "f8_tiles.cuh"
 #include "host.cuh"
 
 using namespace oco;
 
 namespace {
+constexpr int kRowBoxes[4] = {16, 32, 64, 128};   // rows per tile: the narrow heights, then f8_wide_kernel's
+constexpr int kWideIndex = 3;
 enum F8Kind { kF8Projection = OCO_DENSE_PROJECTION, kF8Gated = OCO_DENSE_FFN_SILU_GATE, kF8Experts = 100 };
 
 struct F8Space {
@@ -19,7 +22,6 @@ struct F8Space {
     uint32_t* route_of_row = nullptr;
     uint8_t* xq = nullptr;        // codes of the input rows [R][H] (expert-sorted for routed products)
     float* xs = nullptr;          // their scales [H blocks][pitch]
-    float* act = nullptr;
     uint8_t* aq = nullptr;        // codes of the activations [R][F]
     float* as = nullptr;
     uint16_t* y = nullptr;        // bf16 [R][H], route order
@@ -34,6 +36,8 @@ struct oco_moe_f8_plan : PlanBase {
     oco_moe_f8_weights w{};
     bool have_codes = false;
     F8Space ws{};
+    // rows as TMA reads them (boxes of kRowBoxes rows) and the matrices (boxes of 128 rows)
+    CUtensorMap map_x[4], map_a[4], map_gate, map_up, map_down;
 };
 
 namespace {
@@ -58,7 +62,6 @@ F8Space carve(int kind, const oco_moe_f8_desc& d, int max_rows, unsigned char* b
     w.xq = take(R * H);
     w.xs = (float*)take((H + 127) / 128 * w.pitch * 4);
     if (kind != kF8Projection) {
-        w.act = (float*)take(R * F * 4);
         w.aq = take(R * F);
         w.as = (float*)take((F + 127) / 128 * w.pitch * 4);
     }
@@ -89,6 +92,55 @@ int check_scales(oco_moe_f8_plan* p) {
     return OCO_OK;
 }
 
+int make_maps(oco_moe_f8_plan* plan) {
+    const oco_moe_f8_desc& d = plan->d;
+    const uint64_t E = (uint64_t)d.experts, H = (uint64_t)d.hidden, F = (uint64_t)d.ffn;
+    if (!encode_tiled()) return plan->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    CUresult r = encode_rows(&plan->map_up, (void*)plan->w.up_w, E * F, H, 1, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (plan->kind != kF8Projection) {
+        if (r == CUDA_SUCCESS) r = encode_rows(&plan->map_gate, (void*)plan->w.gate_w, E * F, H, 1, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+        if (r == CUDA_SUCCESS) r = encode_rows(&plan->map_down, (void*)plan->w.down_w, E * H, F, 1, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    }
+    return r == CUDA_SUCCESS ? OCO_OK : plan->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+// Rows per tile (index into kRowBoxes) for `rows` rows of `experts` experts that some row may choose.
+int tile_index(int rows, int experts) {
+    const int avg = (rows + experts - 1) / experts;
+    if (experts == 1) return avg <= 16 ? 0 : avg <= 32 ? 1 : avg <= 256 ? 2 : kWideIndex;
+    return avg <= 8 ? 0 : avg <= 20 ? 1 : avg <= 64 ? 2 : kWideIndex;
+}
+
+template <int NT, bool GATED>
+int launch_thin(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap& rows, const CUtensorMap& w0, const CUtensorMap& w1, int tiles, int expected,
+                cudaStream_t st) {
+    using S = F8Thin<NT, GATED>;
+    auto kernel = f8_thin_kernel<NT, GATED>;
+    OCO_ALLOW_SMEM_ONCE(plan, kernel);
+    const int nfeat = (p.n + 127) / 128, nkb = (p.K + 127) / 128;
+    // parts of the contraction: as many as fill the SMs twice, two blocks of 128 or more each
+    unsigned split = 1;
+    while (split < 8 && (long long)expected * nfeat * split * 2 <= 2LL * plan->sm_count && nkb >= 4 * (int)split) split *= 2;
+    OCO_CK(plan, launch_dependent_clusters(kernel, split, dim3((unsigned)((long long)tiles * nfeat * split)), dim3(S::kThreads), S::kSmem, st, p, rows, w0, w1));
+    plan->launches++;
+    return OCO_OK;
+}
+
+// One product over the rows of a call. `maps`: the rows' maps by tile height.
+template <bool GATED>
+int product(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap* maps, const CUtensorMap& w0, const CUtensorMap& w1, int index, int tiles, int expected,
+            cudaStream_t st) {
+    if (index == 0) return launch_thin<16, GATED>(plan, p, maps[0], w0, w1, tiles, expected, st);
+    if (index == 1) return launch_thin<32, GATED>(plan, p, maps[1], w0, w1, tiles, expected, st);
+    if (index == 2) return launch_thin<64, GATED>(plan, p, maps[2], w0, w1, tiles, expected, st);
+    auto kernel = f8_wide_kernel<GATED>;
+    OCO_ALLOW_SMEM_ONCE(plan, kernel);
+    const long long items = (long long)tiles * ((p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+    OCO_CK(plan, launch_dependent(kernel, dim3((unsigned)std::min<long long>(items, plan->sm_count)), dim3(F8Wide::kThreads), F8Wide::kSmem, st, p, maps[kWideIndex], w0, w1));
+    plan->launches++;
+    return OCO_OK;
+}
+
 // The rows of one call through the plan's products. ids null: dense.
 int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, const float* probs, const uint16_t* residual, uint16_t* out, int rows,
              cudaStream_t st) {
@@ -96,38 +148,31 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     F8Space& ws = plan->ws;
     const bool routed = ids != nullptr;
     const int R = rows * d.top_k, H = d.hidden, F = d.ffn, E = d.experts;
+    const int index = tile_index(R, routed ? std::min(E, R) : 1), nt = kRowBoxes[index];
+    // tiles: exact for a dense product; for routed rows as many as the worst choice of experts makes, and the usual number
+    const int tiles = routed ? R / nt + std::min(E, R) : (R + nt - 1) / nt, expected = routed ? std::max(std::min(E, R), R / nt) : tiles;
     const uint32_t* live = routed ? ws.offsets + E : nullptr;
     if (routed) {
-        F8PlanParams pp{ids, ws.offsets, ws.route_of_row, ws.tiles, ws.tile_count, R, E, 128};
+        F8PlanParams pp{ids, ws.offsets, ws.route_of_row, ws.tiles, ws.tile_count, R, E, nt};
         OCO_CK(plan, launch_dependent(f8_plan_kernel, dim3(1), dim3(1024), 0, st, pp));
         plan->launches++;
     }
-    auto grid_for = [&](int k) { return dim3((unsigned)std::min<long long>(((long long)R * ((k + 127) / 128) + 7) / 8, 16LL * plan->sm_count)); };
-    OCO_CK(plan, launch_dependent(f8_rows_kernel, grid_for(H), dim3(256), 0, st, x, routed ? ws.route_of_row : nullptr, live, d.top_k, R, H, ws.xq, ws.xs, ws.pitch));
+    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)R * ((H + 127) / 128) + 7) / 8, 16LL * plan->sm_count);
+    OCO_CK(plan, launch_dependent(f8_rows_kernel, dim3(row_ctas), dim3(256), 0, st, x, routed ? ws.route_of_row : nullptr, live, d.top_k, R, H, ws.xq, ws.xs, ws.pitch));
     plan->launches++;
-    F8Params p{};
-    p.rows = ws.xq; p.row_scales = ws.xs; p.scale_pitch = ws.pitch; p.K = H; p.n = F; p.experts = E; p.dense_rows = R;
-    p.offsets = routed ? ws.offsets : nullptr;
-    const unsigned row_tiles = (unsigned)std::min(64, (R + 15) / 16);
+    F8TileParams p{};
+    p.row_scales = ws.xs; p.pitch = ws.pitch; p.K = H; p.n = F; p.rows = R; p.status = ws.status;
+    if (routed) { p.tiles = ws.tiles; p.tile_count = ws.tile_count; p.offsets = ws.offsets; }
     if (plan->kind == kF8Projection) {
-        p.w0 = plan->w.up_w; p.s0 = plan->w.up_s; p.out = out;
-        f8_product_kernel<<<dim3((F + 15) / 16, row_tiles, E), 256, 0, st>>>(p);
-        OCO_CK(plan, cudaGetLastError());
-        plan->launches++;
-        return OCO_OK;
+        p.s0 = plan->w.up_s; p.out = out;
+        return product<false>(plan, p, plan->map_x, plan->map_up, plan->map_up, index, tiles, expected, st);
     }
-    p.w0 = plan->w.gate_w; p.s0 = plan->w.gate_s; p.w1 = plan->w.up_w; p.s1 = plan->w.up_s; p.act = ws.act;
-    f8_product_kernel<<<dim3((F + 15) / 16, row_tiles, E), 256, 0, st>>>(p);
-    OCO_CK(plan, cudaGetLastError());
-    f8_act_kernel<<<grid_for(F), 256, 0, st>>>(ws.act, live, R, F, ws.aq, ws.as, ws.pitch);
-    OCO_CK(plan, cudaGetLastError());
-    F8Params q{};
-    q.rows = ws.aq; q.row_scales = ws.as; q.scale_pitch = ws.pitch; q.K = F; q.n = H; q.experts = E; q.dense_rows = R;
-    q.offsets = p.offsets; q.route_of_row = routed ? ws.route_of_row : nullptr;
-    q.w0 = plan->w.down_w; q.s0 = plan->w.down_s; q.out = routed ? ws.y : out;
-    f8_product_kernel<<<dim3((H + 15) / 16, row_tiles, E), 256, 0, st>>>(q);
-    OCO_CK(plan, cudaGetLastError());
-    plan->launches += 3;
+    F8TileParams q = p;
+    p.s0 = plan->w.gate_s; p.s1 = plan->w.up_s; p.codes = ws.aq; p.code_scales = ws.as;
+    if (int rc = product<true>(plan, p, plan->map_x, plan->map_gate, plan->map_up, index, tiles, expected, st)) return rc;
+    q.row_scales = ws.as; q.K = F; q.n = H; q.s0 = plan->w.down_s;
+    q.out = routed ? ws.y : out; q.route_of_row = routed ? ws.route_of_row : nullptr;
+    if (int rc = product<false>(plan, q, plan->map_a, plan->map_down, plan->map_down, index, tiles, expected, st)) return rc;
     if (routed) {
         const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (H / 8) + 255) / 256, 16LL * plan->sm_count);
         OCO_CK(plan, launch_dependent(f8_combine_kernel, dim3(grid), dim3(256), 0, st, ws.y, ids, probs, residual, out, rows, d.top_k, H, E));
@@ -175,6 +220,7 @@ int f8_dense_bind_scales(oco_moe_f8_plan* p, const oco_dense_scales& s) {
     p->w.up_s = s.up_s;
     if (p->kind == kF8Gated) { p->w.gate_s = s.gate_s; p->w.down_s = s.down_s; }
     if (int rc = check_scales(p)) return rc;
+    if (int rc = make_maps(p)) return rc;
     p->have_w = true;
     return OCO_OK;
 }
@@ -216,6 +262,13 @@ int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t byt
     OCO_CK(plan, cudaMemset(ws.status, 0, 256));
     OCO_CK(plan, cudaDeviceSynchronize());
     if (int rc = plan->note_device()) return rc;
+    const uint64_t R = (uint64_t)max_rows * plan->d.top_k;
+    if (!encode_tiled()) return plan->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    for (int i = 0; i < 4; i++) {
+        CUresult r = encode_rows(&plan->map_x[i], ws.xq, R, plan->d.hidden, 1, (uint32_t)kRowBoxes[i]);
+        if (r == CUDA_SUCCESS && ws.aq) r = encode_rows(&plan->map_a[i], ws.aq, R, plan->d.ffn, 1, (uint32_t)kRowBoxes[i]);
+        if (r != CUDA_SUCCESS) return plan->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    }
     plan->ws = ws;
     plan->max_rows = max_rows;
     plan->have_ws = true;
@@ -229,6 +282,7 @@ int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* w) 
     plan->w = *w;
     if (int rc = check_codes(plan)) return rc;
     if (int rc = check_scales(plan)) return rc;
+    if (int rc = make_maps(plan)) return rc;
     plan->have_w = true;
     return OCO_OK;
 }

@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
 __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict__ x, const uint32_t* __restrict__ route_of_row,
                                                       const uint32_t* __restrict__ live_rows, int top_k, int rows, int K,
                                                       uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
-    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
     pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();   // only now: the next kernel reads weights before it waits for this one
     const int lane = threadIdx.x & 31, nkb = (K + 127) / 128;
     const int n = live_rows ? (int)*live_rows : rows;
     for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < (long long)n * nkb; u += (long long)gridDim.x * 8) {
@@ -92,59 +92,6 @@ __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = __fdiv_rn(v[j] * 0.875f, div) * 512.0f;
         if (k < K) *reinterpret_cast<uint32_t*>(codes + (size_t)row * K + k) = f8x4(v[0], v[1], v[2], v[3]);
-        if (lane == 0) scales[(size_t)kb * scale_pitch + row] = __fdiv_rn(top, 448.0f);
-    }
-}
-
-// ---- the product ----------------------------------------------------------------------------------------------------
-struct F8Params {
-    const uint8_t* rows;        // codes [rows][K]
-    const float* row_scales;    // [K blocks][scale_pitch]
-    const uint8_t* w0;          // codes [experts][n][K]: gate (gated) or the one matrix
-    const uint8_t* w1;          // up (gated)
-    const float* s0;            // [experts][ceil(n / 128)][K blocks]
-    const float* s1;
-    const uint32_t* offsets;    // null: dense (one expert, dense_rows rows)
-    const uint32_t* route_of_row;   // rows of the result go to these rows (null: in place)
-    uint16_t* out;              // bf16 [..][n]
-    float* act;                 // gated: f32 [rows][n]
-    int n, K, scale_pitch, dense_rows, experts;
-};
-// Plain CUDA-core form: a thread per output, tiles of 16 rows x 16 features.
-__global__ void __launch_bounds__(256) f8_product_kernel(const F8Params p) {
-    const int nkb = (p.K + 127) / 128, nfb = (p.n + 127) / 128;
-    const int f = blockIdx.x * 16 + (threadIdx.x & 15), e = blockIdx.z;
-    const int begin = p.offsets ? (int)p.offsets[e] : 0, end = p.offsets ? (int)p.offsets[e + 1] : p.dense_rows;
-    for (int row = begin + blockIdx.y * 16 + (threadIdx.x >> 4); row < end; row += gridDim.y * 16) {
-        if (f >= p.n) continue;
-        float acc[2] = {0.f, 0.f};
-        for (int m = 0; m < (p.w1 ? 2 : 1); m++) {
-            const uint8_t* w = (m ? p.w1 : p.w0) + ((size_t)e * p.n + f) * p.K;
-            const float* ws = (m ? p.s1 : p.s0) + ((size_t)e * nfb + f / 128) * nkb;
-            for (int kb = 0; kb < nkb; kb++) {
-                float d = 0.f;
-                for (int k = kb * 128; k < min(p.K, kb * 128 + 128); k++) d = fmaf(f8_value(w[k]), f8_value(p.rows[(size_t)row * p.K + k]), d);
-                acc[m] = fmaf(d, ws[kb] * p.row_scales[(size_t)kb * p.scale_pitch + row], acc[m]);
-            }
-        }
-        if (p.w1) p.act[(size_t)row * p.n + f] = acc[0] / (1.0f + expf(-acc[0])) * acc[1];
-        else p.out[(size_t)(p.route_of_row ? p.route_of_row[row] : row) * p.n + f] = f32_to_bf16_bits(acc[0]);
-    }
-}
-// Activations (f32) to codes: a warp per row and block.
-__global__ void __launch_bounds__(256) f8_act_kernel(const float* __restrict__ act, const uint32_t* __restrict__ live_rows, int rows, int K,
-                                                     uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
-    const int lane = threadIdx.x & 31, nkb = (K + 127) / 128;
-    const int n = live_rows ? (int)*live_rows : rows;
-    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < (long long)n * nkb; u += (long long)gridDim.x * 8) {
-        const int row = (int)(u / nkb), kb = (int)(u - (long long)row * nkb), k = kb * 128 + 4 * lane;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k < K) v = *reinterpret_cast<const float4*>(act + (size_t)row * K + k);
-        uint32_t m = max(max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y))), max(__float_as_uint(fabsf(v.z)), __float_as_uint(fabsf(v.w))));
-        m = __reduce_max_sync(0xffffffffu, m);
-        const float top = __uint_as_float(m), div = m ? top : 1.0f;
-        auto code = [&](float a) { return __fdiv_rn(a * 0.875f, div) * 512.0f; };
-        if (k < K) *reinterpret_cast<uint32_t*>(codes + (size_t)row * K + k) = f8x4(code(v.x), code(v.y), code(v.z), code(v.w));
         if (lane == 0) scales[(size_t)kb * scale_pitch + row] = __fdiv_rn(top, 448.0f);
     }
 }
