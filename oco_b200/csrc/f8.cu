@@ -10,8 +10,10 @@
 using namespace oco;
 
 namespace {
-constexpr int kRowBoxes[4] = {16, 32, 64, 128};   // rows per tile: the narrow heights, then f8_wide_kernel's
-constexpr int kWideIndex = 3;
+// Rows per tile: the heights of f8_thin_kernel, then f8_wide_kernel's on one SM and on a pair of them. Row maps have boxes
+// of as many rows, the pair's two of 128.
+constexpr int kTileRows[5] = {16, 32, 64, 128, 256}, kRowBoxes[4] = {16, 32, 64, 128};
+constexpr int kWideIndex = 3, kPairIndex = 4;
 enum F8Kind { kF8Projection = OCO_DENSE_PROJECTION, kF8Gated = OCO_DENSE_FFN_SILU_GATE, kF8Experts = 100 };
 
 struct F8Space {
@@ -20,6 +22,7 @@ struct F8Space {
     uint32_t* tile_count = nullptr;
     uint32_t* tiles = nullptr;
     uint32_t* route_of_row = nullptr;
+    uint32_t* row_of_route = nullptr;
     uint8_t* xq = nullptr;        // codes of the input rows [R][H] (expert-sorted for routed products)
     float* xs = nullptr;          // their scales [H blocks][pitch]
     uint8_t* aq = nullptr;        // codes of the activations [R][F]
@@ -58,6 +61,7 @@ F8Space carve(int kind, const oco_moe_f8_desc& d, int max_rows, unsigned char* b
         w.tile_count = (uint32_t*)take(4);
         w.tiles = (uint32_t*)take(2 * (R / 16 + std::min(E, R)) * 4);
         w.route_of_row = (uint32_t*)take(R * 4);
+        w.row_of_route = (uint32_t*)take(R * 4);
     }
     w.xq = take(R * H);
     w.xs = (float*)take((H + 127) / 128 * w.pitch * 4);
@@ -104,11 +108,11 @@ int make_maps(oco_moe_f8_plan* plan) {
     return r == CUDA_SUCCESS ? OCO_OK : plan->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
-// Rows per tile (index into kRowBoxes) for `rows` rows of `experts` experts that some row may choose.
+// Rows per tile (index into kTileRows) for `rows` rows of `experts` experts that some row may choose.
 int tile_index(int rows, int experts) {
     const int avg = (rows + experts - 1) / experts;
-    if (experts == 1) return avg <= 16 ? 0 : avg <= 32 ? 1 : avg <= 256 ? 2 : kWideIndex;
-    return avg <= 8 ? 0 : avg <= 20 ? 1 : avg <= 64 ? 2 : kWideIndex;
+    if (experts == 1) return avg <= 16 ? 0 : avg <= 32 ? 1 : avg <= 256 ? 2 : avg <= 512 ? kWideIndex : kPairIndex;
+    return avg <= 8 ? 0 : avg <= 20 ? 1 : avg <= 64 ? 2 : avg <= 128 ? kWideIndex : kPairIndex;
 }
 
 template <int NT, bool GATED>
@@ -133,10 +137,18 @@ int product(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap* map
     if (index == 0) return launch_thin<16, GATED>(plan, p, maps[0], w0, w1, tiles, expected, st);
     if (index == 1) return launch_thin<32, GATED>(plan, p, maps[1], w0, w1, tiles, expected, st);
     if (index == 2) return launch_thin<64, GATED>(plan, p, maps[2], w0, w1, tiles, expected, st);
-    auto kernel = f8_wide_kernel<GATED>;
-    OCO_ALLOW_SMEM_ONCE(plan, kernel);
     const long long items = (long long)tiles * ((p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
-    OCO_CK(plan, launch_dependent(kernel, dim3((unsigned)std::min<long long>(items, plan->sm_count)), dim3(F8Wide::kThreads), F8Wide::kSmem, st, p, maps[kWideIndex], w0, w1));
+    if (index == kWideIndex) {
+        auto kernel = f8_wide_kernel<GATED, false>;
+        OCO_ALLOW_SMEM_ONCE(plan, kernel);
+        OCO_CK(plan, launch_dependent(kernel, dim3((unsigned)std::min<long long>(items, plan->sm_count)), dim3(F8Wide<false>::kThreads), F8Wide<false>::kSmem, st, p,
+                                      maps[kWideIndex], w0, w1));
+    } else {
+        auto kernel = f8_wide_kernel<GATED, true>;
+        OCO_ALLOW_SMEM_ONCE(plan, kernel);
+        OCO_CK(plan, launch_dependent_clusters(kernel, 2u, dim3((unsigned)(2 * std::min<long long>(items, plan->sm_count / 2))), dim3(F8Wide<true>::kThreads),
+                                               F8Wide<true>::kSmem, st, p, maps[kWideIndex], w0, w1));
+    }
     plan->launches++;
     return OCO_OK;
 }
@@ -148,17 +160,16 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     F8Space& ws = plan->ws;
     const bool routed = ids != nullptr;
     const int R = rows * d.top_k, H = d.hidden, F = d.ffn, E = d.experts;
-    const int index = tile_index(R, routed ? std::min(E, R) : 1), nt = kRowBoxes[index];
+    const int index = tile_index(R, routed ? std::min(E, R) : 1), nt = kTileRows[index];
     // tiles: exact for a dense product; for routed rows as many as the worst choice of experts makes, and the usual number
     const int tiles = routed ? R / nt + std::min(E, R) : (R + nt - 1) / nt, expected = routed ? std::max(std::min(E, R), R / nt) : tiles;
-    const uint32_t* live = routed ? ws.offsets + E : nullptr;
     if (routed) {
-        F8PlanParams pp{ids, ws.offsets, ws.route_of_row, ws.tiles, ws.tile_count, R, E, nt};
+        F8PlanParams pp{ids, ws.offsets, ws.route_of_row, ws.row_of_route, ws.tiles, ws.tile_count, R, E, nt};
         OCO_CK(plan, launch_dependent(f8_plan_kernel, dim3(1), dim3(1024), 0, st, pp));
         plan->launches++;
     }
-    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)R * ((H + 127) / 128) + 7) / 8, 16LL * plan->sm_count);
-    OCO_CK(plan, launch_dependent(f8_rows_kernel, dim3(row_ctas), dim3(256), 0, st, x, routed ? ws.route_of_row : nullptr, live, d.top_k, R, H, ws.xq, ws.xs, ws.pitch));
+    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)rows * ((H + 127) / 128) + 15) / 16, 8LL * plan->sm_count);
+    OCO_CK(plan, launch_dependent(f8_rows_kernel, dim3(row_ctas), dim3(256), 0, st, x, routed ? ws.row_of_route : nullptr, d.top_k, rows, H, ws.xq, ws.xs, ws.pitch));
     plan->launches++;
     F8TileParams p{};
     p.row_scales = ws.xs; p.pitch = ws.pitch; p.K = H; p.n = F; p.rows = R; p.status = ws.status;
@@ -255,7 +266,9 @@ size_t oco_moe_f8_workspace_bytes(const oco_moe_f8_plan* plan, int max_rows) {
 int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t bytes, int max_rows) {
     if (!plan) return OCO_INVALID_ARGUMENT;
     if (!workspace || max_rows < 1) return plan->fail(OCO_INVALID_ARGUMENT, "null workspace or max_rows < 1");
-    if ((long long)max_rows * plan->d.top_k > (1LL << 30)) return plan->fail(OCO_UNSUPPORTED_SHAPE, "max_rows * top_k is more than 2^30");
+    // rows, tokens' blocks and pieces of eight columns are counted in 32 bits
+    if ((long long)max_rows * plan->d.top_k > (1LL << 28) || (long long)max_rows * plan->d.hidden > (1LL << 33))
+        return plan->fail(OCO_UNSUPPORTED_SHAPE, "max_rows * top_k is more than 2^28 or max_rows * hidden more than 2^33");
     if ((uintptr_t)workspace & 255u) return plan->fail(OCO_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
     const F8Space ws = carve(plan->kind, plan->d, max_rows, (unsigned char*)workspace);
     if (bytes < ws.total) return plan->fail(OCO_INVALID_ARGUMENT, "workspace too small: %zu < %zu", bytes, ws.total);

@@ -27,6 +27,7 @@ struct F8PlanParams {
     const uint32_t* ids;      // [R]; outside 0 .. E-1: no route of this plan
     uint32_t* offsets;        // [E + 1]
     uint32_t* route_of_row;   // [R]
+    uint32_t* row_of_route;   // [R]; 0xffffffff: a route without a row
     uint32_t* tiles;          // pairs (expert, first sorted row), tile_rows rows each
     uint32_t* tile_count;
     int R, E, tile_rows;
@@ -64,35 +65,70 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
     __syncthreads();
     for (int i = tid; i < p.R; i += 1024) {
         const uint32_t e = p.ids[i];
-        if (e < (uint32_t)p.E) p.route_of_row[atomicAdd(&next[e], 1u)] = (uint32_t)i;
+        uint32_t row = 0xffffffffu;
+        if (e < (uint32_t)p.E) {
+            row = atomicAdd(&next[e], 1u);
+            p.route_of_row[row] = (uint32_t)i;
+        }
+        p.row_of_route[i] = row;
     }
 }
 
 // ---- rows to codes ------------------------------------------------------------------------------------------------
-// A warp per row and block of 128 elements, four a lane. code = e4m3(x * 448 / largest) with one rounding before e4m3's:
-// x * 0.875 is exact for bf16 x, the division rounds correctly and the power of two is exact, so an element halfway
-// between two codes is decided as such. Scales lie [block][row].
-__global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict__ x, const uint32_t* __restrict__ route_of_row,
-                                                      const uint32_t* __restrict__ live_rows, int top_k, int rows, int K,
-                                                      uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
+// code = e4m3(x * 448 / largest), the quotient rounded once before e4m3's own rounding, so that an element halfway between
+// two codes is decided as such; scale = largest / 448. x * 448 is exact for bf16 x. The quotient is the product with the
+// rounded reciprocal, corrected once by its exact residual (Markstein's method: the correction of a correctly rounded
+// reciprocal's product rounds correctly while nothing leaves the normal range; a block outside 2^-100 .. 2^100 divides).
+// A block whose largest is NaN or infinite gives NaN codes or a scale that makes its products NaN.
+struct F8Divider {
+    float top, rcp;
+    bool plain;
+    __device__ __forceinline__ explicit F8Divider(float largest) {
+        top = largest;
+        plain = largest > 7.9e-31f && largest < 1.2e30f;
+        rcp = plain ? __frcp_rn(largest) : 0.0f;
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        if (plain) {
+            const float n = x * 448.0f, q = n * rcp;
+            return fmaf(fmaf(-q, top, n), rcp, q);
+        }
+        return __fdiv_rn(x * 0.875f, top == 0.0f ? 1.0f : top) * 512.0f;
+    }
+};
+
+// Rows to codes: half a warp per token and block of 128 elements, eight elements a lane. A routed token is read and
+// rounded once and its codes written to the row of each of its routes. Scales lie [block][row].
+__global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict__ x, const uint32_t* __restrict__ row_of_route, int top_k,
+                                                      int tokens, int K, uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();   // only now: the next kernel reads weights before it waits for this one
-    const int lane = threadIdx.x & 31, nkb = (K + 127) / 128;
-    const int n = live_rows ? (int)*live_rows : rows;
-    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < (long long)n * nkb; u += (long long)gridDim.x * 8) {
-        const int row = (int)(u / nkb), kb = (int)(u - (long long)row * nkb), k = kb * 128 + 4 * lane;
-        const size_t token = route_of_row ? route_of_row[row] / (uint32_t)top_k : (uint32_t)row;
-        uint2 q = make_uint2(0, 0);
-        if (k < K) q = *reinterpret_cast<const uint2*>(x + token * K + k);
-        float v[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
+    const int lane = threadIdx.x & 15, nkb = (K + 127) / 128;
+    const uint32_t half = 0xffffu << (threadIdx.x & 16);
+    const uint32_t units = (uint32_t)tokens * (uint32_t)nkb, step = gridDim.x * 16;
+    for (uint32_t u = blockIdx.x * 16 + (threadIdx.x >> 4); u < units; u += step) {
+        const uint32_t token = u / (uint32_t)nkb;
+        const int kb = (int)(u - token * (uint32_t)nkb), k = kb * 128 + 8 * lane;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (k < K) q = __ldg(reinterpret_cast<const uint4*>(x + (size_t)token * K + k));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
         // the largest as bits: for non-negative floats the order of the bits, a NaN above everything
-        uint32_t m = max(max(__float_as_uint(fabsf(v[0])), __float_as_uint(fabsf(v[1]))), max(__float_as_uint(fabsf(v[2])), __float_as_uint(fabsf(v[3]))));
-        m = __reduce_max_sync(0xffffffffu, m);
-        const float top = __uint_as_float(m), div = m ? top : 1.0f;
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = __fdiv_rn(v[j] * 0.875f, div) * 512.0f;
-        if (k < K) *reinterpret_cast<uint32_t*>(codes + (size_t)row * K + k) = f8x4(v[0], v[1], v[2], v[3]);
-        if (lane == 0) scales[(size_t)kb * scale_pitch + row] = __fdiv_rn(top, 448.0f);
+        for (int j = 0; j < 4; j++) m = max(m, max((w[j] << 16) & 0x7fff0000u, w[j] & 0x7fff0000u));
+        m = __reduce_max_sync(half, m);
+        const float top = __uint_as_float(m);
+        const F8Divider code(top);
+        uint2 c;
+        c.x = f8x4(code(__uint_as_float(w[0] << 16)), code(__uint_as_float(w[0] & 0xffff0000u)), code(__uint_as_float(w[1] << 16)), code(__uint_as_float(w[1] & 0xffff0000u)));
+        c.y = f8x4(code(__uint_as_float(w[2] << 16)), code(__uint_as_float(w[2] & 0xffff0000u)), code(__uint_as_float(w[3] << 16)), code(__uint_as_float(w[3] & 0xffff0000u)));
+        const float scale = __fdiv_rn(top, 448.0f);
+        for (int r = 0; r < top_k; r++) {
+            const uint32_t row = row_of_route ? row_of_route[(size_t)token * top_k + r] : token;
+            if (row == 0xffffffffu) continue;
+            if (k < K) *reinterpret_cast<uint2*>(codes + (size_t)row * K + k) = c;
+            if (lane == 0) scales[(size_t)kb * scale_pitch + row] = scale;
+        }
     }
 }
 
@@ -103,30 +139,35 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* __restr
                                                          const uint16_t* residual, uint16_t* out, int rows, int top_k, int H, int E) {
     pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
     pdl_wait();                // the kernel before has completed and its writes are visible
-    const int per_row = H / 8;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * per_row; i += (long long)gridDim.x * 256) {
-        const int t = (int)(i / per_row), c = (int)(i - (long long)t * per_row) * 8;
-        float acc[8];
+    const uint32_t per_row = (uint32_t)H / 8, units = (uint32_t)rows * per_row;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < units; i += gridDim.x * 256) {
+        const uint32_t t = i / per_row, c = (i - t * per_row) * 8;
         const uint4 q = *reinterpret_cast<const uint4*>(residual + (size_t)t * H + c);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
         float sum[8] = {};
-        for (int r = 0; r < top_k; r++) {
-            if (ids[(size_t)t * top_k + r] >= (uint32_t)E) continue;
-            const float pr = probs[(size_t)t * top_k + r];
-            const uint4 v = *reinterpret_cast<const uint4*>(y + ((size_t)t * top_k + r) * H + c);
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        for (int r0 = 0; r0 < top_k; r0 += 4) {                        // four routes' rows on their way at a time
+            uint4 v[4];
+            float pr[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sum[2 * j] = fmaf(pr, __uint_as_float(u[j] << 16), sum[2 * j]);
-                sum[2 * j + 1] = fmaf(pr, __uint_as_float(u[j] & 0xffff0000u), sum[2 * j + 1]);
+            for (int r = 0; r < 4; r++) {
+                const bool live = r0 + r < top_k && __ldg(ids + (size_t)t * top_k + r0 + r) < (uint32_t)E;
+                pr[r] = live ? __ldg(probs + (size_t)t * top_k + r0 + r) : 0.f;
+                v[r] = live ? __ldg(reinterpret_cast<const uint4*>(y + ((size_t)t * top_k + r0 + r) * H + c)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t u[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    sum[2 * j] = fmaf(pr[r], __uint_as_float(u[j] << 16), sum[2 * j]);
+                    sum[2 * j + 1] = fmaf(pr[r], __uint_as_float(u[j] & 0xffff0000u), sum[2 * j + 1]);
+                }
             }
         }
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            acc[2 * j] = __uint_as_float(w[j] << 16) + sum[2 * j];
-            acc[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) + sum[2 * j + 1];
-            const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(w[j] << 16) + sum[2 * j], __uint_as_float(w[j] & 0xffff0000u) + sum[2 * j + 1]);
             o[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
         *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = make_uint4(o[0], o[1], o[2], o[3]);

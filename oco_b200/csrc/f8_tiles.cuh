@@ -16,7 +16,7 @@
 // Every wait is bounded (mbar_wait); one that gives up sets the status word and the kernel runs on to its end.
 #pragma once
 #include "f8.cuh"
-#include "gemm.cuh"
+#include "cluster.cuh"
 
 namespace oco {
 
@@ -45,38 +45,85 @@ __device__ __forceinline__ void f8_act_scale(float top, float& scale, float& lif
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
+// PAIR: two SMs multiply one tile of 256 rows (tcgen05.mma.cta_group::2): each brings its own 128 rows and half of the 256
+// features, so that an SM fetches 32 KB instead of 48 KB for the same 128 x 256 products of 128 terms.
+// Two warpgroups read the accumulators and hold the sums; the third one's warps feed them: TMA, MMA, scales. The 168
+// registers a thread starts with are dealt anew, 224 to the sums and 56 to the rest (2 * 224 + 56 = 3 * 168).
+template <bool PAIR>
 struct F8Wide {
-    static constexpr int kStages = 4, kA = 128 * 128, kB = 256 * 128, kStage = kA + kB;
-    static constexpr int kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;
-    static constexpr int kCtrl = 256 + 2 * 128 * 4;
-    static constexpr int kSmem = kStages * kStage + kCtrl + 1024;
+    static constexpr int kRows = PAIR ? 256 : 128;                      // rows of a tile
+    static constexpr int kA = 128 * 128, kB = (PAIR ? 128 : 256) * 128, kStage = kA + kB, kStages = PAIR ? 4 : 3;
+    static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10, kThreads = 384;
+    static constexpr int kScales = 8;                                   // blocks whose scales are on their way
+    static constexpr int kScaleBytes = (128 + 4) * 4;                   // 128 rows, gate and up block
+    static constexpr int kOutPitch = 256 + 16;                          // a row's 128 results, spread over the banks
+    static constexpr int kOut = kStages * kStage, kCtrlAt = kOut + 8 * 32 * kOutPitch;
+    static constexpr int kTops = 512, kRing = kTops + 2 * 128 * 4, kCtrl = kRing + kScales * kScaleBytes;
+    static constexpr int kSmem = kCtrlAt + kCtrl + 1024;
+    static_assert(kSmem <= 232448, "shared memory of one CTA");
+    static_assert(8 * (2 * kStages + 2 + 2 * kScales) + 8 <= kTops, "barriers");
 };
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void cp_async4(uint32_t smem_dst, const void* gsrc) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(gsrc) : "memory");
+}
+// One arrival on `bar` when this thread's copies so far have landed (counted among the barrier's expected arrivals).
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void umma_f8f6f4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // GATED: the 256 columns of a tile are 128 gate and the same 128 up features, the result is silu(gate) * up as codes.
-template <bool GATED>
-__global__ void __launch_bounds__(F8Wide::kThreads, 1) f8_wide_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
-                                                                     const __grid_constant__ CUtensorMap w0_map, const __grid_constant__ CUtensorMap w1_map) {
-    using S = F8Wide;
+// Launched in clusters of two where PAIR; persistent: CTA (pair) c takes items c, c + CTAs (pairs), ...
+template <bool GATED, bool PAIR>
+__global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
+                                                                           const __grid_constant__ CUtensorMap w0_map, const __grid_constant__ CUtensorMap w1_map) {
+    using S = F8Wide<PAIR>;
     extern __shared__ unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0u;                   // 0: the CTA that issues the MMAs
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t ctrl = base + S::kStages * S::kStage;
-    auto full = [&](int s) { return ctrl + 8u * s; };
-    auto empty = [&](int s) { return ctrl + 8u * (S::kStages + s); };
-    auto tfull = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };
-    auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + 2 + b); };
-    uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kStages * S::kStage + 8 * (2 * S::kStages + 4));
+    const uint32_t ctrl = base + S::kCtrlAt;
+    auto full = [&](int s) { return ctrl + 8u * s; };                   // of the issuing CTA: the stage of both has landed
+    auto done = [&](int s) { return ctrl + 8u * (S::kStages + s); };    // the MMAs of the stage: its sums are there, its room is free
+    auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };   // of the issuing CTA: both have read
+    auto sfull = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + q); };
+    auto sempty = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + S::kScales + q); };
+    auto ring = [&](int q) { return ctrl + S::kRing + (uint32_t)q * S::kScaleBytes; };   // [128] rows, then gate and up
+    uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + 8 * (2 * S::kStages + 2 + 2 * S::kScales));
     volatile uint32_t* abort_flag = slot + 1;
-    uint32_t* tops = reinterpret_cast<uint32_t*>(gen + S::kStages * S::kStage + 256);   // [2][128]
+    uint32_t* tops = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + S::kTops);   // [2][128]
+    const uint32_t lead = PAIR ? map_to_cta(ctrl, 0) : ctrl;
+    auto at_lead = [&](uint32_t bar) { return lead + (bar - ctrl); };
     if (tid == 0) {
-        for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(tfull(b), 1); mbar_init(tempty(b), 8); }
+        for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(done(s), 1); }
+        for (int q = 0; q < S::kScales; q++) { mbar_init(sfull(q), 32); mbar_init(sempty(q), 8); }
+        for (int b = 0; b < 2; b++) mbar_init(tempty(b), PAIR ? 16 : 8);
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == S::kMmaWarp) { tmem_alloc(smem_u32(slot), 512); tmem_relinquish(); }
+    if (warp == S::kMmaWarp) {
+        if (PAIR) { tmem_alloc_pair(smem_u32(slot), 512); tmem_relinquish_pair(); }
+        else { tmem_alloc(smem_u32(slot), 512); tmem_relinquish(); }
+    }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();   // both CTAs' barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = *slot;
     pdl_wait();                // the kernel before has completed and its writes are visible
@@ -84,69 +131,94 @@ __global__ void __launch_bounds__(F8Wide::kThreads, 1) f8_wide_kernel(const F8Ti
 
     constexpr int kFeat = GATED ? 128 : 256;
     const int nfeat = (p.n + kFeat - 1) / kFeat, nkb = (p.K + 127) / 128, nfb = (p.n + 127) / 128;
-    const int ntiles = p.tiles ? (int)*p.tile_count : (p.rows + 127) / 128;
+    const int ntiles = p.tiles ? (int)*p.tile_count : (p.rows + S::kRows - 1) / S::kRows;
     const int total = ntiles * nfeat;
-    struct Item { int expert, row0, nv, f0; };
+    const int first = PAIR ? (int)blockIdx.x >> 1 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
+    struct Item { int expert, row0, nv, f0; };                          // rows of this CTA's part
     auto item_of = [&](int i) {
         Item r;
         const int t = i / nfeat;
         r.f0 = (i - t * nfeat) * kFeat;
+        int end = p.rows;
+        r.expert = 0; r.row0 = t * S::kRows;
         if (p.tiles) {
             r.expert = (int)p.tiles[2 * t];
             r.row0 = (int)p.tiles[2 * t + 1];
-            r.nv = min(128, (int)p.offsets[r.expert + 1] - r.row0);
-        } else {
-            r.expert = 0; r.row0 = t * 128; r.nv = min(128, p.rows - r.row0);
+            end = (int)p.offsets[r.expert + 1];
         }
+        r.row0 += 128 * (int)rank;
+        r.nv = max(0, min(128, end - r.row0));
         return r;
     };
 
     if (warp < 8) {
+        more_registers<224>();
         // ===== epilogue: thread = row (32 * (warp & 3) + lane), half of the columns (warp >> 2) ====================
         const int erow = (warp & 3) * 32 + lane, half = warp >> 2;
         const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t col0 = GATED ? 64u * half : 128u * half, col1 = GATED ? 128u + 64u * half : 128u * half + 64u;
+        // results leave through shared memory: a row's part is one bulk copy (a thread's own 16-byte stores would touch
+        // 32 rows an instruction, which took as long as the MMAs of an item)
+        const uint32_t out_row = base + S::kOut + (uint32_t)(warp * 32 + lane) * S::kOutPitch;
+        auto send = [&](void* dst, uint32_t bytes, bool live) {
+            fence_proxy_async_smem();
+            if (live) asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(out_row), "r"(bytes) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        };
+        auto store16 = [&](int c, const uint32_t (&w)[4]) {
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(out_row + 16u * c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        };
         int g = 0;
-        for (int i = blockIdx.x; i < total; i += gridDim.x) {
+        for (int i = first; i < total; i += step) {
             const Item it = item_of(i);
-            const float* xs = p.row_scales + min(it.row0 + erow, p.pitch - 1);
-            const int fb = it.f0 / 128 + (GATED ? 0 : min(half, nfb - 1 - it.f0 / 128));
-            const float* ws0 = p.s0 + ((size_t)it.expert * nfb + fb) * nkb;
-            const float* ws1 = GATED ? p.s1 + ((size_t)it.expert * nfb + fb) * nkb : ws0;
             uint64_t acc[64];
 #pragma unroll
             for (int j = 0; j < 64; j++) acc[j] = 0;
-            float x1 = xs[0], x2 = nkb > 1 ? xs[p.pitch] : 0.f, a1 = ws0[0], a2 = nkb > 1 ? ws0[1] : 0.f;
-            float b1 = GATED ? ws1[0] : 0.f, b2 = GATED && nkb > 1 ? ws1[1] : 0.f;
-            for (int kb = 0; kb < nkb; kb++, g++) {
-                const float s0 = x1 * a1, s1 = GATED ? x1 * b1 : s0;
-                x1 = x2; a1 = a2; b1 = b2;
-                if (kb + 2 < nkb) {
-                    x2 = xs[(size_t)(kb + 2) * p.pitch];
-                    a2 = ws0[kb + 2];
-                    if (GATED) b2 = ws1[kb + 2];
-                }
-                const int b = g & 1;
-                if (lane == 0) mbar_wait(tfull(b), (uint32_t)(g >> 1) & 1u, abort_flag, p.status);
+            // scales of a block: gate columns under the gate's, up columns under up's; else under this half's feature block's
+            uint64_t t0, t1;
+            auto scales = [&](int k) {
+                const int q = k % S::kScales;
+                mbar_wait(sfull(q), (uint32_t)(k / S::kScales) & 1u, abort_flag, p.status);
+                const float x = lds_f32(ring(q) + 4u * erow);
+                const float s0 = x * lds_f32(ring(q) + 512u + (GATED ? 0u : 4u * half)), s1 = GATED ? x * lds_f32(ring(q) + 516u) : s0;
+                t0 = f32x2(s0, s0);
+                t1 = f32x2(s1, s1);
                 __syncwarp();
+                if (lane == 0) mbar_arrive(sempty(q));
+            };
+            scales(g);
+            for (int kb = 0; kb < nkb; kb++, g++) {
+                const int b = g & 1, s = g % S::kStages;
+                mbar_wait(done(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, p.status);
                 tc_fence_after();
-                const uint64_t t0 = f32x2(s0, s0), t1 = f32x2(s1, s1);
-#pragma unroll
-                for (int h = 0; h < 4; h++) {                         // 32 columns in registers at a time, beside 128 sums
-                    uint32_t r[32];
-                    tmem_ld32(taddr + 256u * b + (h < 2 ? col0 : col1) + 32u * (h & 1), r);
-                    tmem_ld_wait();
-                    if (h == 3) {                                     // all of it is in registers: the buffer is free
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(tempty(b));
-                    }
+                const uint32_t at0 = taddr + 256u * b + col0, at1 = taddr + 256u * b + col1;
+                uint32_t r[32], u[32];
+                auto add = [&](const uint32_t (&v)[32], uint64_t t, int j0) {
 #pragma unroll
                     for (int j = 0; j < 16; j++)
-                        acc[16 * h + j] = fma_f32x2(f32x2_bits(r[2 * j], r[2 * j + 1]), h < 2 ? t0 : t1, acc[16 * h + j]);
+                        asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[j0 + j]) : "l"(f32x2_bits(v[2 * j], v[2 * j + 1])), "l"(t));
+                };
+                tmem_ld32(at0, r);
+                tmem_ld32(at0 + 32u, u);
+                tmem_ld_wait();
+                add(r, t0, 0);
+                tmem_ld32(at1, r);                                    // travels while the columns before it are added
+                add(u, t0, 16);
+                tmem_ld32(at1 + 32u, u);
+                tmem_ld_wait();
+                tc_fence_before();                                    // all of it is in registers: the buffer is free
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_peer(at_lead(tempty(b)));
+                    else mbar_arrive(tempty(b));
                 }
+                const uint64_t last = t1;
+                if (kb + 1 < nkb) scales(g + 1);
+                add(r, last, 32);
+                add(u, last, 48);
             }
             const bool live = erow < it.nv;
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // the item before has left its rows
             if (GATED) {
                 const int f = it.f0 + 64 * half;                      // this thread's 64 features
                 uint32_t top = 0;
@@ -166,9 +238,9 @@ __global__ void __launch_bounds__(F8Wide::kThreads, 1) f8_wide_kernel(const F8Ti
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
                 float scale, lift, factor;
                 f8_act_scale(__uint_as_float(top), scale, lift, factor);
-                if (live) {
-                    const size_t row = (size_t)it.row0 + erow;
-                    if (half == 0) p.code_scales[(size_t)(it.f0 / 128) * p.pitch + row] = scale;
+                const size_t row = (size_t)it.row0 + erow;
+                if (live && half == 0) p.code_scales[(size_t)(it.f0 / 128) * p.pitch + row] = scale;
+                {
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         uint32_t w[4];
@@ -181,12 +253,13 @@ __global__ void __launch_bounds__(F8Wide::kThreads, 1) f8_wide_kernel(const F8Ti
                             for (int e = 0; e < 4; e++) v[e] = v[e] * lift * factor;
                             w[k] = f8x4(v[0], v[1], v[2], v[3]);
                         }
-                        if (f + 16 * c < p.n) *reinterpret_cast<uint4*>(p.codes + row * p.n + f + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        store16(c, w);
                     }
                 }
-            } else if (live) {
+                send(p.codes + row * p.n + f, (uint32_t)max(0, min(64, p.n - f)), live && f < p.n);
+            } else {
                 const int f = it.f0 + 128 * half;
-                const size_t row = p.route_of_row ? p.route_of_row[it.row0 + erow] : (uint32_t)(it.row0 + erow);
+                const size_t row = !live ? 0 : p.route_of_row ? p.route_of_row[it.row0 + erow] : (uint32_t)(it.row0 + erow);
 #pragma unroll
                 for (int c = 0; c < 16; c++) {
                     uint32_t w[4];
@@ -197,56 +270,99 @@ __global__ void __launch_bounds__(F8Wide::kThreads, 1) f8_wide_kernel(const F8Ti
                         const __nv_bfloat162 o = __floats2bfloat162_rn(v0, v1);
                         w[k] = *reinterpret_cast<const uint32_t*>(&o);
                     }
-                    if (f + 8 * c < p.n) *reinterpret_cast<uint4*>(p.out + row * p.n + f + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    store16(c, w);
                 }
+                send(p.out + row * p.n + f, 2u * (uint32_t)max(0, min(128, p.n - f)), live && f < p.n);
             }
         }
-    } else if (warp == S::kTmaWarp) {
-        if (lane == 0) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else {
+        fewer_registers<56>();
+        if (warp == S::kScaleWarp) {
+            // ===== scales: four rows a lane and the two blocks of the weights, a block of K at a time ====================
             int g = 0;
-            for (int i = blockIdx.x; i < total; i += gridDim.x) {
+            for (int i = first; i < total; i += step) {
+                const Item it = item_of(i);
+                const int fb = it.f0 / 128;
+                const float* ws = lane == 0 || !GATED ? p.s0 : p.s1;   // lane 0: gate or the first block, lane 1: up or the second
+                ws += ((size_t)it.expert * nfb + (GATED ? fb : min(fb + lane, nfb - 1))) * nkb;
+                for (int kb = 0; kb < nkb; kb++, g++) {
+                    const int q = g % S::kScales;
+                    mbar_wait(sempty(q), ((uint32_t)(g / S::kScales) & 1u) ^ 1u, abort_flag, p.status);
+                    const float* xs = p.row_scales + (size_t)kb * p.pitch;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) cp_async4(ring(q) + 4u * (lane + 32 * r), xs + min(it.row0 + lane + 32 * r, p.pitch - 1));
+                    if (lane < 2) cp_async4(ring(q) + 512u + 4u * lane, ws + kb);
+                    cp_async_arrive(sfull(q));
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else if (warp == S::kTmaWarp && lane == 0) {
+            // ===== operands: this CTA's 128 rows, and its half (PAIR) or all of the features ==============================
+            int g = 0;
+            for (int i = first; i < total && !*abort_flag; i += step) {
                 const Item it = item_of(i);
                 const int wrow = it.expert * p.n + it.f0;
                 for (int kb = 0; kb < nkb; kb++, g++) {
                     const int s = g % S::kStages;
-                    mbar_wait(empty(s), ((uint32_t)(g / S::kStages) & 1u) ^ 1u, abort_flag, p.status);
+                    mbar_wait(done(s), ((uint32_t)(g / S::kStages) & 1u) ^ 1u, abort_flag, p.status);
                     if (*abort_flag) break;
                     const uint32_t at = base + (uint32_t)s * S::kStage;
-                    mbar_arrive_expect_tx(full(s), S::kStage);
-                    tma_load_2d(at, &rows_map, kb * 128, it.row0, full(s));
-                    tma_load_2d(at + S::kA, &w0_map, kb * 128, wrow, full(s));
-                    tma_load_2d(at + S::kA + S::kB / 2, GATED ? &w1_map : &w0_map, kb * 128, GATED ? wrow : wrow + 128, full(s));
+                    if (PAIR) {
+                        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * S::kStage);
+                        tma_load_2d_pair(at, &rows_map, kb * 128, it.row0, at_lead(full(s)));
+                        if (GATED) tma_load_2d_pair(at + S::kA, rank ? &w1_map : &w0_map, kb * 128, wrow, at_lead(full(s)));
+                        else tma_load_2d_pair(at + S::kA, &w0_map, kb * 128, wrow + 128 * (int)rank, at_lead(full(s)));
+                    } else {
+                        mbar_arrive_expect_tx(full(s), S::kStage);
+                        tma_load_2d(at, &rows_map, kb * 128, it.row0, full(s));
+                        tma_load_2d(at + S::kA, &w0_map, kb * 128, wrow, full(s));
+                        tma_load_2d(at + S::kA + S::kB / 2, GATED ? &w1_map : &w0_map, kb * 128, GATED ? wrow : wrow + 128, full(s));
+                    }
                 }
-                if (*abort_flag) break;
             }
-            if (*abort_flag)
-                for (int k = max(0, g - S::kStages); k < g; k++) mbar_drain(full(k % S::kStages), (uint32_t)(k / S::kStages) & 1u);
-        }
-    } else if (lane == 0) {
-        const uint32_t idesc = umma_idesc_f16(256);                  // e4m3 x e4m3, f32, M = 128, N = 256
-        int g = 0;
-        for (int i = blockIdx.x; i < total; i += gridDim.x) {
-            for (int kb = 0; kb < nkb; kb++, g++) {
-                const int s = g % S::kStages, b = g & 1;
+        } else if (warp == S::kMmaWarp && rank == 0) {
+            // e4m3 x e4m3, f32; M = 128 (256 over the pair), N = 256: columns of this CTA's features, then of the other's.
+            // The whole warp waits, one lane issues: what the MMAs of a block cost this warp has to stay below their own time.
+            const uint32_t idesc = PAIR ? umma_idesc_f16_pair(256) : umma_idesc_f16(256);
+            const uint64_t a0 = umma_desc(base), w0 = umma_desc(base + S::kA);
+            const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+            const int blocks = total > first ? (total - first + step - 1) / step * nkb : 0;
+            int s = 0;
+            uint32_t turn = 0;                                          // parity of the stages' turn
+            for (int g = 0; g < blocks; g++) {
+                const int b = g & 1;
+                mbar_wait(full(s), turn, abort_flag, p.status);
                 mbar_wait(tempty(b), ((uint32_t)(g >> 1) & 1u) ^ 1u, abort_flag, p.status);
-                mbar_wait(full(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, p.status);
-                if (*abort_flag) break;
                 tc_fence_after();
-                const uint64_t a = umma_desc(base + (uint32_t)s * S::kStage), w = umma_desc(base + (uint32_t)s * S::kStage + S::kA);
+                if (elect_one()) {
+                    const uint64_t a = a0 + (uint64_t)(s * (S::kStage >> 4)), w = w0 + (uint64_t)(s * (S::kStage >> 4));
 #pragma unroll
-                for (int k = 0; k < 4; k++) umma_f8f6f4(tmem + 256u * b, a + 2u * k, w + 2u * k, idesc, k ? 1u : 0u);
-                umma_commit(empty(s));
-                umma_commit(tfull(b));
+                    for (int k = 0; k < 4; k++) {
+                        if (PAIR) umma_f8f6f4_pair(d0 + 256u * b, a + 2u * k, w + 2u * k, idesc, k ? 1u : 0u);
+                        else umma_f8f6f4(d0 + 256u * b, a + 2u * k, w + 2u * k, idesc, k ? 1u : 0u);
+                    }
+                    if (PAIR) umma_commit_both(done(s));
+                    else umma_commit(done(s));
+                }
+                __syncwarp();
+                if (++s == S::kStages) { s = 0; turn ^= 1u; }
             }
-            if (*abort_flag) break;
         }
-        if (*abort_flag && g > 0) mbar_drain(tfull((g - 1) & 1), (uint32_t)((g - 1) >> 1) & 1u);
     }
-    __syncwarp();
-    tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 64; i++) __nanosleep(1000);   // let copies and MMAs in flight end before the CTA retires
+        __syncthreads();
+    }
+    tc_fence_before();
+    if (PAIR) cluster_sync_all();   // neither CTA retires, or gives its tensor memory back, while the other may still signal or multiply
+    else __syncthreads();
     tc_fence_after();
-    if (warp == S::kMmaWarp) tmem_dealloc(tmem, 512);
+    if (warp == S::kMmaWarp) {
+        if (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
+    }
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------
@@ -263,24 +379,14 @@ struct F8Thin {
     static_assert(kMats * NT * 128 * 4 <= kStages * kStage, "the parts of a split contraction lie where the stages were");
     static_assert(8 * (2 * kStages + 2 * kBufs) + 8 <= 256, "barriers");
 };
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ uint32_t cluster_size() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float peer_f32(uint32_t local, uint32_t rank) {      // this CTA's shared address `local`, in CTA `rank`
-    uint32_t at;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(local, rank)) : "memory");
     return v;
 }
 
@@ -441,7 +547,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
             if (*abort_flag && g > 0) mbar_drain(tfull((g - 1) % S::kBufs), (uint32_t)((g - 1) / S::kBufs) & 1u);
         }
         __syncwarp();
-        if (split > 1) cluster_sync(); else __syncthreads();
+        if (split > 1) cluster_sync_all(); else __syncthreads();
         // ===== join: this CTA's share of the rows, thread = feature ===================================================
         if (warp < 4) {
             const uint32_t mine = base + 4u * tid;
@@ -471,7 +577,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
                 }
             }
         }
-        if (split > 1) cluster_sync();                                   // nobody leaves while its parts are read
+        if (split > 1) cluster_sync_all();                                   // nobody leaves while its parts are read
     }
     tc_fence_before();
     __syncthreads();

@@ -374,6 +374,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
         : "memory");
 }
 
+// One lane of a converged warp, the same one every time. Code under it keeps what is uniform in uniform registers, which
+// a branch on the lane's number does not (an MMA's operands then move one by one ahead of each instruction).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
 // K-major, 128-byte swizzle: 8-row groups of 1024 bytes (stride byte offset), descriptor version 1.
 __device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr) {
     uint32_t lo = ((smem_addr & 0x3ffffu) >> 4) | (1u << 16);

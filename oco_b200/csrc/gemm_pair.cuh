@@ -28,92 +28,10 @@
 // far more). Every load has one destination CTA. All mbarrier waits are bounded (see mbar_wait); the two cluster
 // barriers (after set-up, before the end) are reached by every thread on every path.
 #pragma once
+#include "cluster.cuh"
 #include "gemm_wide.cuh"
 
 namespace oco {
-
-// ---- what crosses the pair ------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// The address, in the cluster's shared window, of CTA `rank`'s copy of this CTA's shared address.
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// mbar_wait for a barrier on which the other CTA of the pair arrives: the same bound, cluster-scope acquire.
-__device__ __forceinline__ void mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                                  uint32_t* status_word) {
-    if (mbar_try_wait_cluster(bar, parity)) return;
-    long long start = clock64();
-    while (!mbar_try_wait_cluster(bar, parity)) {
-        if (*abort_flag) return;
-        if (clock64() - start > kWaitCycles) {
-            *abort_flag = 1u;
-            atomicExch(status_word, (uint32_t)kDevBarrierTimeout);
-            return;
-        }
-    }
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_dst, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish_pair() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// D (256 rows: 128 in each CTA's tensor memory) += A (128 rows in each CTA) x B (N / 2 rows in each CTA)
-__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ uint32_t umma_idesc_f16_pair(uint32_t n) {
-    return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
-}
-// One arrival, when the MMAs issued so far have retired, on the barrier at `bar` of both CTAs (one instruction
-// per CTA; a single instruction that signals both measured the same).
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-    const uint32_t b0 = map_to_cta(bar, 0), b1 = map_to_cta(bar, 1);
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b0) : "memory");
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b1) : "memory");
-}
-// This CTA's box of route rows into its own shared memory; the bytes are counted on the barrier at `cluster_bar`
-// (an address in the cluster's shared window: the even CTA's).
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, int c0, int c1, uint32_t cluster_bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(smem_dst), "l"(map), "r"(c0), "r"(c1), "r"(cluster_bar)
-        : "memory");
-}
 
 template <int FMT>
 struct PairShapeT {
