@@ -54,11 +54,11 @@ struct F8Wide {
     static constexpr int kRows = PAIR ? 256 : 128;                      // rows of a tile
     static constexpr int kA = 128 * 128, kB = (PAIR ? 128 : 256) * 128, kStage = kA + kB, kStages = PAIR ? 4 : 3;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10, kThreads = 384;
-    static constexpr int kScales = 8;                                   // blocks whose scales are on their way
-    static constexpr int kScaleBytes = (128 + 4) * 4;                   // 128 rows, gate and up block
+    static constexpr int kScaleRun = 4, kScales = 3;                    // scales travel in runs of four blocks, three runs
+    static constexpr int kScaleBytes = (128 + 4) * 4;                   // of a block: 128 rows, gate and up block
     static constexpr int kOutPitch = 256 + 16;                          // a row's 128 results, spread over the banks
     static constexpr int kOut = kStages * kStage, kCtrlAt = kOut + 8 * 32 * kOutPitch;
-    static constexpr int kTops = 512, kRing = kTops + 2 * 128 * 4, kCtrl = kRing + kScales * kScaleBytes;
+    static constexpr int kTops = 512, kRing = kTops + 2 * 128 * 4, kCtrl = kRing + kScales * kScaleRun * kScaleBytes;
     static constexpr int kSmem = kCtrlAt + kCtrl + 1024;
     static_assert(kSmem <= 232448, "shared memory of one CTA");
     static_assert(8 * (2 * kStages + 2 + 2 * kScales) + 8 <= kTops, "barriers");
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
     auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };   // of the issuing CTA: both have read
     auto sfull = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + q); };
     auto sempty = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + S::kScales + q); };
-    auto ring = [&](int q) { return ctrl + S::kRing + (uint32_t)q * S::kScaleBytes; };   // [128] rows, then gate and up
+    auto ring = [&](int q, int k) { return ctrl + S::kRing + (uint32_t)(q * S::kScaleRun + k) * S::kScaleBytes; };   // [128] rows, gate, up
     uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + 8 * (2 * S::kStages + 2 + 2 * S::kScales));
     volatile uint32_t* abort_flag = slot + 1;
     uint32_t* tops = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + S::kTops);   // [2][128]
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
         auto store16 = [&](int c, const uint32_t (&w)[4]) {
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(out_row + 16u * c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         };
-        int g = 0;
+        int g = 0, run = 0;
         for (int i = first; i < total; i += step) {
             const Item it = item_of(i);
             uint64_t acc[64];
@@ -176,20 +176,24 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
             for (int j = 0; j < 64; j++) acc[j] = 0;
             // scales of a block: gate columns under the gate's, up columns under up's; else under this half's feature block's
             uint64_t t0, t1;
-            auto scales = [&](int k) {
-                const int q = k % S::kScales;
-                mbar_wait(sfull(q), (uint32_t)(k / S::kScales) & 1u, abort_flag, p.status);
-                const float x = lds_f32(ring(q) + 4u * erow);
-                const float s0 = x * lds_f32(ring(q) + 512u + (GATED ? 0u : 4u * half)), s1 = GATED ? x * lds_f32(ring(q) + 516u) : s0;
+            auto scales = [&](int kb) {
+                const int k = kb % S::kScaleRun, q = run % S::kScales;
+                if (k == 0) mbar_wait(sfull(q), (uint32_t)(run / S::kScales) & 1u, abort_flag, p.status);
+                const float x = lds_f32(ring(q, k) + 4u * erow);
+                const float s0 = x * lds_f32(ring(q, k) + 512u + (GATED ? 0u : 4u * half)), s1 = GATED ? x * lds_f32(ring(q, k) + 516u) : s0;
                 t0 = f32x2(s0, s0);
                 t1 = f32x2(s1, s1);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sempty(q));
+                if (k == S::kScaleRun - 1 || kb == nkb - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sempty(q));
+                    run++;
+                }
             };
-            scales(g);
+            scales(0);
+            bool there = mbar_try_wait(done(g % S::kStages), (uint32_t)(g / S::kStages) & 1u);
             for (int kb = 0; kb < nkb; kb++, g++) {
                 const int b = g & 1, s = g % S::kStages;
-                mbar_wait(done(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, p.status);
+                if (!there) mbar_wait(done(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, p.status);
                 tc_fence_after();
                 const uint32_t at0 = taddr + 256u * b + col0, at1 = taddr + 256u * b + col1;
                 uint32_t r[32], u[32];
@@ -213,7 +217,11 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
                     else mbar_arrive(tempty(b));
                 }
                 const uint64_t last = t1;
-                if (kb + 1 < nkb) scales(g + 1);
+                // the next block's scales and a first look at its barrier, under the sums of this one
+                if (kb + 1 < nkb) {
+                    scales(kb + 1);
+                    there = mbar_try_wait(done((g + 1) % S::kStages), (uint32_t)((g + 1) / S::kStages) & 1u);
+                }
                 add(r, last, 32);
                 add(u, last, 48);
             }
@@ -280,19 +288,21 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
         fewer_registers<56>();
         if (warp == S::kScaleWarp) {
             // ===== scales: four rows a lane and the two blocks of the weights, a block of K at a time ====================
-            int g = 0;
+            int run = 0;
             for (int i = first; i < total; i += step) {
                 const Item it = item_of(i);
                 const int fb = it.f0 / 128;
                 const float* ws = lane == 0 || !GATED ? p.s0 : p.s1;   // lane 0: gate or the first block, lane 1: up or the second
                 ws += ((size_t)it.expert * nfb + (GATED ? fb : min(fb + lane, nfb - 1))) * nkb;
-                for (int kb = 0; kb < nkb; kb++, g++) {
-                    const int q = g % S::kScales;
-                    mbar_wait(sempty(q), ((uint32_t)(g / S::kScales) & 1u) ^ 1u, abort_flag, p.status);
-                    const float* xs = p.row_scales + (size_t)kb * p.pitch;
+                for (int kb = 0; kb < nkb; kb += S::kScaleRun, run++) {
+                    const int q = run % S::kScales;
+                    mbar_wait(sempty(q), ((uint32_t)(run / S::kScales) & 1u) ^ 1u, abort_flag, p.status);
+                    for (int k = 0; k < S::kScaleRun && kb + k < nkb; k++) {
+                        const float* xs = p.row_scales + (size_t)(kb + k) * p.pitch;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) cp_async4(ring(q) + 4u * (lane + 32 * r), xs + min(it.row0 + lane + 32 * r, p.pitch - 1));
-                    if (lane < 2) cp_async4(ring(q) + 512u + 4u * lane, ws + kb);
+                        for (int r = 0; r < 4; r++) cp_async4(ring(q, k) + 4u * (lane + 32 * r), xs + min(it.row0 + lane + 32 * r, p.pitch - 1));
+                        if (lane < 2) cp_async4(ring(q, k) + 512u + 4u * lane, ws + kb + k);
+                    }
                     cp_async_arrive(sfull(q));
                 }
             }
