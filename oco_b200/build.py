@@ -10,7 +10,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liboco_moe.so")
 SOURCES = ["api.cu", "route_static.cu", "peaks.cu", "window.cu", "f8.cu", "router_groups.cu", "block_norm.cu"]
 HEADERS = ["common.cuh", "router.cuh", "plan.cuh", "decode.cuh", "batch.cuh", "gemm.cuh", "gemm_wide.cuh", "gemm_pair.cuh", "token_deal.h", "mx.cuh", "mx_pieces.cuh", "gemm_mx.cuh",
-           "host.cuh", "cluster.cuh", "f8.cuh", "f8_tiles.cuh", "f8.h", "select.cuh",
+           "host.cuh", "cluster.cuh", "f8.cuh", "f8_tiles.cuh", "f8.h", "select.cuh", "router_tiles.cuh",
            "../../include/oco_moe.h"]
 
 

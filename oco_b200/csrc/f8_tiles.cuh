@@ -389,17 +389,6 @@ struct F8Thin {
     static_assert(kMats * NT * 128 * 4 <= kStages * kStage, "the parts of a split contraction lie where the stages were");
     static_assert(8 * (2 * kStages + 2 * kBufs) + 8 <= 256, "barriers");
 };
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ float peer_f32(uint32_t local, uint32_t rank) {      // this CTA's shared address `local`, in CTA `rank`
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(local, rank)) : "memory");
-    return v;
-}
-
 // One item (a tile of up to NT rows of one expert, 128 features) per cluster; CTA r of its S takes the blocks
 // [r * per, ..) of the contraction. x = S * (item), items: feature tile fastest.
 template <int NT, bool GATED>

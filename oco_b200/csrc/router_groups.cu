@@ -1,7 +1,9 @@
 // Routing with groups of experts: the router product and the selection (select.cuh) behind oco_moe_router_*.
+#include <algorithm>
 #include <new>
 
 #include "host.cuh"
+#include "router_tiles.cuh"
 #include "select.cuh"
 
 using namespace oco;
@@ -12,20 +14,45 @@ struct oco_moe_router : PlanBase {
     const float* bias = nullptr;
     uint32_t* status = nullptr;
     float* logits = nullptr;
+    uint16_t* pieces = nullptr;       // the weights as three bf16 pieces [3][experts rounded up to 128][hidden]
+    CUtensorMap map_w;
+    bool laid_out = false;            // pieces and map match the bound weights and workspace
 };
 
 namespace {
 
-struct RouterSpace { size_t status, logits, total; };
+int padded(int experts) { return (experts + 127) / 128 * 128; }
+
+struct RouterSpace { size_t status, logits, pieces, total; };
 RouterSpace carve(const oco_moe_router_desc& d, int max_rows) {
     RouterSpace s{};
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off = align_up(off + bytes, 256); return at; };
     s.status = take(256);
     s.logits = take(d.hidden ? (size_t)max_rows * d.experts * 4 : 0);
+    s.pieces = take((size_t)3 * padded(d.experts) * d.hidden * 2);
     s.total = off;
     return s;
 }
+
+// Lays the weights out for the tensor cores once both they and the workspace are bound.
+int lay_out(oco_moe_router* r) {
+    r->laid_out = false;
+    const oco_moe_router_desc& d = r->d;
+    if (!r->have_ws || !r->have_w || !d.hidden) return OCO_OK;
+    if (int rc = r->check_device()) return rc;
+    const int Ep = padded(d.experts);
+    router_pieces_kernel<<<4 * r->sm_count, 256>>>(r->w, r->pieces, d.experts, Ep, d.hidden);
+    OCO_CK(r, cudaGetLastError());
+    OCO_CK(r, cudaDeviceSynchronize());
+    const CUresult e = encode_rows(&r->map_w, r->pieces, (uint64_t)3 * Ep, (uint64_t)d.hidden, 2, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (e != CUDA_SUCCESS) return r->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)e);
+    r->laid_out = true;
+    return OCO_OK;
+}
+
+// Rows up to which the logits are made by router_rows_kernel, above by router_tile_kernel.
+constexpr int kRowsMax = 16;
 
 // logits[t][e] = sum_k x[t][k] w[e][k]: a warp per expert and four tokens, f32.
 __global__ void __launch_bounds__(256) router_rows_kernel(const uint16_t* __restrict__ x, const float* __restrict__ w, float* __restrict__ logits,
@@ -114,9 +141,10 @@ int oco_moe_router_bind_workspace(oco_moe_router* r, void* workspace, size_t byt
     unsigned char* base = (unsigned char*)workspace;
     r->status = (uint32_t*)(base + s.status);
     r->logits = (float*)(base + s.logits);
+    r->pieces = (uint16_t*)(base + s.pieces);
     r->max_rows = max_rows;
     r->have_ws = true;
-    return OCO_OK;
+    return lay_out(r);
 }
 
 int oco_moe_router_bind_weights(oco_moe_router* r, const float* w, const float* bias) {
@@ -125,14 +153,14 @@ int oco_moe_router_bind_weights(oco_moe_router* r, const float* w, const float* 
     if (((uintptr_t)w & 15u) || ((uintptr_t)bias & 3u)) return r->fail(OCO_INVALID_ARGUMENT, "router_w must be 16-byte aligned, bias 4-byte");
     r->w = w; r->bias = bias;
     r->have_w = true;
-    return OCO_OK;
+    return lay_out(r);
 }
 
 int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint32_t* ids, float* probs, float* logits, void* cuda_stream) {
     if (!r) return OCO_INVALID_ARGUMENT;
     r->launches = 0;
     if (!r->d.hidden) return r->fail(OCO_INVALID_ARGUMENT, "this router selects from logits only");
-    if (!r->have_ws || !r->have_w) return r->fail(OCO_INVALID_ARGUMENT, "bind a workspace and weights first");
+    if (!r->laid_out) return r->fail(OCO_INVALID_ARGUMENT, "bind a workspace and weights first");
     if (int rc = r->check_device()) return rc;
     if (rows < 0 || rows > r->max_rows) return r->fail(OCO_INVALID_ARGUMENT, "rows %d outside 0..%d", rows, r->max_rows);
     if (rows == 0) return OCO_OK;
@@ -142,10 +170,22 @@ int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint3
     cudaStream_t st = (cudaStream_t)cuda_stream;
     float* lg = logits ? logits : r->logits;
     const oco_moe_router_desc& d = r->d;
-    OCO_CK(r, launch_dependent(router_rows_kernel, dim3((rows + 3) / 4, (d.experts + 7) / 8), dim3(256), 0, st, x, r->w, lg, rows, d.experts, d.hidden));
+    if (rows <= kRowsMax) {
+        OCO_CK(r, launch_dependent(router_rows_kernel, dim3((rows + 3) / 4, (d.experts + 7) / 8), dim3(256), 0, st, x, r->w, lg, rows, d.experts, d.hidden));
+    } else {
+        CUtensorMap map_x;
+        const CUresult e = encode_rows(&map_x, (void*)x, (uint64_t)rows, (uint64_t)d.hidden, 2, 128);
+        if (e != CUDA_SUCCESS) return r->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)e);
+        OCO_ALLOW_SMEM_ONCE(r, router_tile_kernel);
+        const int Ep = padded(d.experts), items = (rows + 127) / 128 * (Ep / 128), chunks = (d.hidden + 63) / 64;
+        unsigned split = 1;      // parts of the contraction, four stages of 64 or more each, while they find idle SMs
+        while (split < 8 && items * (int)split * 2 <= r->sm_count && chunks >= 8 * (int)split) split *= 2;
+        OCO_CK(r, launch_dependent_clusters(router_tile_kernel, split, dim3((unsigned)items * split), dim3(RouterTile::kThreads), RouterTile::kSmem, st, map_x, r->map_w,
+                                            lg, rows, d.experts, Ep, d.hidden, r->status));
+    }
     r->launches++;
     SelectParams p = select_params(r, lg, rows, ids, probs);
-    p.x = x; p.w = r->w;
+    p.x = x; p.w = r->w; p.status = r->status;
     return launch_select(r, p, st);
 }
 

@@ -1,0 +1,171 @@
+// The router product on the tensor cores: logits[t][e] = sum_k x[t][k] w[e][k] to the accuracy of f32 sums.
+//
+// The rows are bf16; an f32 weight is the exact sum of three bf16 pieces of falling size (8 bits of its 24 each), laid
+// out once when the weights are bound. Three kind::f16 products with bf16 operands then add exact terms into one f32
+// accumulator. What is left is the rounding of the sums: after every 512 terms of the contraction the accumulator is
+// read out of tensor memory and added, rounding to nearest, to sums in registers, so that no chain of roundings in
+// tensor memory is long.
+//
+// One item = 128 rows x 128 experts; a contraction is split over the CTAs of a cluster while items do not fill the SMs,
+// and the parts are added through distributed shared memory in the order of their ranks. Each stage of shared memory
+// holds 64 columns of the rows and of the three pieces (64 KB). All waits are bounded (mbar_wait).
+#pragma once
+#include "cluster.cuh"
+
+namespace oco {
+
+struct RouterTile {
+    static constexpr int kTile = 128 * 128, kStage = 4 * kTile, kStages = 3;
+    static constexpr int kRun = 8;                       // stages between two readings of the accumulator
+    static constexpr int kPitch = 129;                   // f32 of a row of the parts: neighbouring rows in other banks
+    static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
+    static constexpr int kCtrl = 256, kSmem = kStages * kStage + kCtrl + 1024;
+    static_assert(128 * kPitch * 4 <= kStages * kStage, "the parts lie where the stages were");
+};
+
+// Weights -> three bf16 pieces [piece][Ep][H], Ep = experts rounded up to 128 (rows behind the last expert are zero).
+__global__ void __launch_bounds__(256) router_pieces_kernel(const float* __restrict__ w, uint16_t* __restrict__ pieces, int E, int Ep, int H) {
+    const size_t n = (size_t)Ep * H;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const float v = i < (size_t)E * H ? w[i] : 0.0f;
+        const float a = bf16_round(v);
+        const bool whole = !nonfinite(a);                // an infinite or NaN weight stands in its first piece alone
+        const float b = whole ? bf16_round(v - a) : 0.0f, c = whole ? v - a - b : 0.0f;
+        pieces[i] = f32_to_bf16_bits(a);
+        pieces[n + i] = f32_to_bf16_bits(b);
+        pieces[2 * n + i] = f32_to_bf16_bits(c);
+    }
+}
+
+__global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
+                                                                             float* __restrict__ logits, int rows, int E, int Ep, int H, uint32_t* status) {
+    using S = RouterTile;
+    extern __shared__ unsigned char smem_raw[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t ctrl = base + S::kStages * S::kStage;
+    auto full = [&](int s) { return ctrl + 8u * s; };
+    auto empty = [&](int s) { return ctrl + 8u * (S::kStages + s); };
+    auto tfull = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };
+    auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + 2 + b); };
+    uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kStages * S::kStage + 8 * (2 * S::kStages + 4));
+    volatile uint32_t* abort_flag = slot + 1;
+    const int split = (int)cluster_size(), rank = (int)cluster_rank();
+    const int chunks = (H + 63) / 64, per = (chunks + split - 1) / split, c0 = min(chunks, rank * per), c1 = min(chunks, c0 + per);
+    const int etiles = Ep / 128, item = (int)blockIdx.x / split, row0 = item / etiles * 128, e0 = item % etiles * 128;
+    if (tid == 0) {
+        for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(tfull(b), 1); mbar_init(tempty(b), 4); }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == S::kMmaWarp) { tmem_alloc(smem_u32(slot), 256); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    auto load_pieces = [&](int c, int s) {
+        const uint32_t at = base + (uint32_t)s * S::kStage;
+        mbar_arrive_expect_tx(full(s), S::kStage);
+#pragma unroll
+        for (int q = 0; q < 3; q++) tma_load_2d(at + (1 + q) * S::kTile, &w_map, c * 64, q * Ep + e0, full(s));
+    };
+    // the pieces were laid out when the weights were bound: their first tiles travel while the kernel before still runs
+    const int first = min(S::kStages, c1 - c0);
+    if (warp == S::kTmaWarp && lane == 0)
+        for (int k = 0; k < first; k++) load_pieces(c0 + k, k);
+    pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();
+
+    float* part = reinterpret_cast<float*>(gen);
+    if (warp < 4) {
+        // thread = row
+        float sum[128];
+#pragma unroll
+        for (int j = 0; j < 128; j++) sum[j] = 0.f;
+        const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+        for (int c = c0, run = 0; c < c1; c += S::kRun, run++) {
+            const int b = run & 1;
+            mbar_wait(tfull(b), (uint32_t)(run >> 1) & 1u, abort_flag, status);
+            tc_fence_after();
+#pragma unroll
+            for (int j0 = 0; j0 < 128; j0 += 32) {
+                uint32_t r[32];
+                tmem_ld32(taddr + 128u * b + j0, r);
+                tmem_ld_wait();
+                if (j0 == 96) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty(b));
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j++) sum[j0 + j] += __uint_as_float(r[j]);
+            }
+        }
+        // every MMA of this CTA is done: the parts go where the stages were
+#pragma unroll
+        for (int j = 0; j < 128; j++) part[tid * S::kPitch + j] = sum[j];
+    } else if (warp == S::kTmaWarp) {
+        if (lane == 0) {
+            int g = 0;
+            for (int c = c0; c < c1; c++, g++) {
+                const int s = g % S::kStages;
+                if (g >= first) {
+                    mbar_wait(empty(s), ((uint32_t)(g / S::kStages) & 1u) ^ 1u, abort_flag, status);
+                    if (*abort_flag) break;
+                    load_pieces(c, s);
+                }
+                tma_load_2d(base + (uint32_t)s * S::kStage, &x_map, c * 64, row0, full(s));
+            }
+            if (*abort_flag)
+                for (int k = max(0, g - S::kStages); k < g; k++) mbar_drain(full(k % S::kStages), (uint32_t)(k / S::kStages) & 1u);
+        }
+    } else {
+        const uint32_t idesc = umma_idesc_f16(128) | (1u << 7) | (1u << 10);       // both operands bf16
+        const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t x0 = umma_desc(base), w0 = umma_desc(base + S::kTile);
+        for (int c = c0, g = 0; c < c1; c++, g++) {
+            const int s = g % S::kStages, run = g / S::kRun, b = run & 1;
+            const bool begins = g % S::kRun == 0, ends = g % S::kRun == S::kRun - 1 || c == c1 - 1;
+            if (begins) mbar_wait(tempty(b), ((uint32_t)(run >> 1) & 1u) ^ 1u, abort_flag, status);
+            mbar_wait(full(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, status);
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t at = (uint64_t)(s * (S::kStage >> 4));
+#pragma unroll
+                for (int q = 2; q >= 0; q--)                           // the smallest piece first
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        umma_f16(d0 + 128u * b, x0 + at + 2u * k, w0 + at + (uint64_t)(q * (S::kTile >> 4)) + 2u * k, idesc, begins && q == 2 && k == 0 ? 0u : 1u);
+                umma_commit(empty(s));
+                if (ends) umma_commit(tfull(b));
+            }
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 64; i++) __nanosleep(1000);   // let copies and MMAs in flight end before the CTA goes on
+        __syncthreads();
+    }
+    if (split > 1) cluster_sync_all();
+    // join: this CTA's share of the rows, a warp per row
+    const int live = min(128, rows - row0), cols = min(128, E - e0);
+    for (int r = rank + split * warp; r < live; r += split * (S::kThreads / 32)) {
+        for (int c = lane; c < cols; c += 32) {
+            float v = 0.f;
+            if (split == 1) v = part[r * S::kPitch + c];
+            else
+                for (int q = 0; q < split; q++) v += peer_f32(base + 4u * (uint32_t)(r * S::kPitch + c), (uint32_t)q);
+            logits[(size_t)(row0 + r) * E + e0 + c] = v;
+        }
+    }
+    tc_fence_before();
+    if (split > 1) cluster_sync_all();                   // nobody leaves while its parts are read
+    else __syncthreads();
+    tc_fence_after();
+    if (warp == S::kMmaWarp) tmem_dealloc(tmem, 256);
+}
+
+}  // namespace oco
