@@ -383,7 +383,7 @@ const char* oco_dense_last_error(const oco_dense_plan* plan);
  * reference's routers (softmax over the winners, sigmoid with a selection bias) know no groups and at most
  * 128 experts; oco_moe_route serves those. For a token's logits l:
  *     s = sigmoid(l) or softmax(l) over all experts          the score, which becomes the weight
- *     r = s + bias                                           what the experts are ranked by (no bias: s)
+ *     r = s + bias                                           what the experts are ranked by (no bias: l, in the same order)
  *     worth of a group = the sum of its `group_best` largest r; the `top_groups` worthiest groups stay
  *     ids = the top_k largest r of those groups, in falling order; equal values go to the lower index
  *     prob = s[id] / max(sum of the winners' s, 2^-14) if normalize, else s[id]; times scale

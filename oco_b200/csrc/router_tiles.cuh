@@ -1,10 +1,11 @@
 // The router product on the tensor cores: logits[t][e] = sum_k x[t][k] w[e][k] to the accuracy of f32 sums.
 //
 // The rows are bf16; an f32 weight is the exact sum of three bf16 pieces of falling size (8 bits of its 24 each), laid
-// out once when the weights are bound. Three kind::f16 products with bf16 operands then add exact terms into one f32
-// accumulator. What is left is the rounding of the sums: after every 512 terms of the contraction the accumulator is
-// read out of tensor memory and added, rounding to nearest, to sums in registers, so that no chain of roundings in
-// tensor memory is long.
+// out once when the weights are bound. Three kind::f16 products with bf16 operands then add exact terms into f32
+// accumulators. What is left is the rounding of the sums, which tensor memory cuts off instead of rounding to nearest
+// (with one accumulator read out every 512 terms, 96 additions, the logits came out 1.6e-6 too small): the largest pieces
+// have an accumulator of their own, and after every 256 terms (16 additions to it) both are read out and added, rounding
+// to nearest, to sums in registers.
 //
 // One item = 128 rows x 128 experts; a contraction is split over the CTAs of a cluster while items do not fill the SMs,
 // and the parts are added through distributed shared memory in the order of their ranks. Each stage of shared memory
@@ -16,7 +17,7 @@ namespace oco {
 
 struct RouterTile {
     static constexpr int kTile = 128 * 128, kStage = 4 * kTile, kStages = 3;
-    static constexpr int kRun = 8;                       // stages between two readings of the accumulator
+    static constexpr int kRun = 4;                       // stages between two readings of the accumulator
     static constexpr int kPitch = 129;                   // f32 of a row of the parts: neighbouring rows in other banks
     static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
     static constexpr int kCtrl = 256, kSmem = kStages * kStage + kCtrl + 1024;
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == S::kMmaWarp) { tmem_alloc(smem_u32(slot), 256); tmem_relinquish(); }
+    if (warp == S::kMmaWarp) { tmem_alloc(smem_u32(slot), 512); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -91,8 +92,9 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
             tc_fence_after();
 #pragma unroll
             for (int j0 = 0; j0 < 128; j0 += 32) {
-                uint32_t r[32];
-                tmem_ld32(taddr + 128u * b + j0, r);
+                uint32_t r[32], u[32];
+                tmem_ld32(taddr + 256u * b + j0, r);
+                tmem_ld32(taddr + 256u * b + 128u + j0, u);
                 tmem_ld_wait();
                 if (j0 == 96) {
                     tc_fence_before();
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
                     if (lane == 0) mbar_arrive(tempty(b));
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j++) sum[j0 + j] += __uint_as_float(r[j]);
+                for (int j = 0; j < 32; j++) sum[j0 + j] += __uint_as_float(r[j]) + __uint_as_float(u[j]);
             }
         }
         // every MMA of this CTA is done: the parts go where the stages were
@@ -134,10 +136,11 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
             if (elect_one()) {
                 const uint64_t at = (uint64_t)(s * (S::kStage >> 4));
 #pragma unroll
-                for (int q = 2; q >= 0; q--)                           // the smallest piece first
+                for (int q = 0; q < 3; q++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        umma_f16(d0 + 128u * b, x0 + at + 2u * k, w0 + at + (uint64_t)(q * (S::kTile >> 4)) + 2u * k, idesc, begins && q == 2 && k == 0 ? 0u : 1u);
+                        umma_f16(d0 + 256u * b + (q ? 128u : 0u), x0 + at + 2u * k, w0 + at + (uint64_t)(q * (S::kTile >> 4)) + 2u * k, idesc,
+                                 begins && q < 2 && k == 0 ? 0u : 1u);
                 umma_commit(empty(s));
                 if (ends) umma_commit(tfull(b));
             }
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
     if (split > 1) cluster_sync_all();                   // nobody leaves while its parts are read
     else __syncthreads();
     tc_fence_after();
-    if (warp == S::kMmaWarp) tmem_dealloc(tmem, 256);
+    if (warp == S::kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace oco

@@ -5,8 +5,8 @@
 //
 // Everything is first done in 32 bits. Two ranking values that lie within each other's error (rounding of the score, of
 // score + bias, and the error of the logit where it came from the router product) leave their order open; such a token
-// goes through the same steps in 64 bits, where the logits that matter are summed again from x and the weights. With
-// continuous logits that is a token in a few hundred, so the 64-bit path costs time only as a tail.
+// is settled in 64 bits, where the logits that matter are summed again from x and the weights by the whole CTA (one warp
+// alone took 10 to 20 us for it). With continuous logits that is a token in a few hundred.
 #pragma once
 #include "common.cuh"
 
@@ -48,11 +48,59 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 
-// Error of a logit that came from the router product: a sum of H products whose partial sums are of the size of the
-// row's logits, taken in 32-bit accumulators (relative to the larger of the logit and the row's root mean square).
-constexpr float kLogitError = 1.6e-6f;
-// Relative error of a 32-bit score: two roundings and the exponential's two units in the last place, with room.
-constexpr float kScoreError = 6e-7f, kHalfUlp = 6e-8f;
+// Error of a logit that came from the router product, relative to the largest logit of its row: a sum of exact products
+// whose partial sums are of the size of the row's logits, in 32-bit accumulators.
+constexpr float kLogitError = 1.5e-6f;
+// A sigmoid in 32 bits: s (1 - s) 2^-22 from the exponential's two units in the last place, the sum's rounding and the
+// quotient's two units: below 4e-7.
+// A softmax score relative to the largest one: the same and the rounding of l - top (x e^-x < 0.37), the sum and its
+// reciprocal. kHalfUlp: the rounding of score + bias.
+constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f;
+
+// ---- exact logits, summed by a whole CTA ------------------------------------------------------------------------------
+struct SelectShared {
+    int rows[8];                 // rows of the CTA's warps that need exact logits, -1: none
+    int row, a, b, work;         // what is asked for: the logits of experts a and b of a row; work 0: nothing more
+    double part[2][8];
+};
+__device__ __forceinline__ void dots_share(const SelectParams& p, SelectShared* sh) {
+    const float4* wa = reinterpret_cast<const float4*>(p.w + (size_t)sh->a * p.H);
+    const float4* wb = reinterpret_cast<const float4*>(p.w + (size_t)sh->b * p.H);
+    const uint2* xr = reinterpret_cast<const uint2*>(p.x + (size_t)sh->row * p.H);
+    double a0 = 0, a1 = 0, b0 = 0, b1 = 0;
+#pragma unroll 2
+    for (int k = threadIdx.x; k < p.H / 4; k += 256) {
+        const float4 u = __ldg(wa + k), v = __ldg(wb + k);
+        const uint2 q = __ldg(xr + k);
+        const double x0 = (double)__uint_as_float(q.x << 16), x1 = (double)__uint_as_float(q.x & 0xffff0000u);
+        const double x2 = (double)__uint_as_float(q.y << 16), x3 = (double)__uint_as_float(q.y & 0xffff0000u);
+        a0 = fma((double)u.x, x0, a0); a1 = fma((double)u.y, x1, a1); a0 = fma((double)u.z, x2, a0); a1 = fma((double)u.w, x3, a1);
+        b0 = fma((double)v.x, x0, b0); b1 = fma((double)v.y, x1, b1); b0 = fma((double)v.z, x2, b0); b1 = fma((double)v.w, x3, b1);
+    }
+    const double da = warp_sum_d(a0 + a1), db = warp_sum_d(b0 + b1);
+    if ((threadIdx.x & 31) == 0) { sh->part[0][threadIdx.x >> 5] = da; sh->part[1][threadIdx.x >> 5] = db; }
+}
+// Warp 0 asks, the other warps wait in dots_serve.
+__device__ __noinline__ void dots_ask(const SelectParams& p, SelectShared* sh, int row, int a, int b, double& da, double& db) {
+    if (threadIdx.x == 0) { sh->row = row; sh->a = a; sh->b = b; sh->work = 1; }
+    __syncthreads();
+    dots_share(p, sh);
+    __syncthreads();
+    da = db = 0.0;
+    for (int w = 0; w < 8; w++) { da += sh->part[0][w]; db += sh->part[1][w]; }
+}
+__device__ __noinline__ void dots_serve(const SelectParams& p, SelectShared* sh) {
+    while (true) {
+        __syncthreads();
+        if (!sh->work) return;
+        dots_share(p, sh);
+        __syncthreads();
+    }
+}
+__device__ __forceinline__ void dots_end(SelectShared* sh) {
+    if (threadIdx.x == 0) sh->work = 0;
+    __syncthreads();
+}
 
 // ---- 64-bit path ---------------------------------------------------------------------------------------------------
 struct Best { double v; int i; float e; };
@@ -71,31 +119,24 @@ __device__ __forceinline__ Best warp_best(Best b) {
 // Writes ids and weights of one token; called by a whole warp. `l`: the lane's logits, `bad`: lanes' elements whose logit
 // is not finite never come here. Not inlined: it is rare and would cost the 32-bit path registers.
 template <int VPL>
-__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane) {
+__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, SelectShared* sh) {
     const int E = p.E, gs = p.E / p.G;
-    const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = p.x != nullptr;
+    const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = sh != nullptr;
     double l[VPL], s[VPL], r[VPL];
     float e[VPL];
     uint32_t precise = 0;                                              // bit i: element i's logit is exact
     double top = -1e300;
-    float sq = 0.f;
+    float big = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         const int x = lane * VPL + i;
         l[i] = x < E ? (double)lrow[x] : 0.0;
-        if (x < E) { top = fmax(top, l[i]); sq += (float)(l[i] * l[i]); }
+        if (x < E) { top = fmax(top, l[i]); big = fmaxf(big, fabsf((float)l[i])); }
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float rms = sqrtf(warp_sum_f(sq) / (float)E);
+    const float d = kLogitError * __uint_as_float(warp_max(__float_as_uint(big)));
     if (!remake) precise = 0xffffffffu;
-    else {
-        // a row of zeros has exact logits, and it is what padding looks like
-        uint32_t any = 0;
-        const uint4* xr = reinterpret_cast<const uint4*>(p.x + (size_t)row * p.H);
-        for (int k = lane; k < p.H / 8; k += 32) { const uint4 q = xr[k]; any |= (q.x | q.y | q.z | q.w) & 0x7fff7fffu; }
-        if (!__any_sync(0xffffffffu, any != 0)) precise = 0xffffffffu;
-    }
     while (true) {
         // scores and ranks from the present logits
         double z = 1.0;
@@ -118,7 +159,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
         for (int i = 0; i < VPL; i++) {
             const int x = lane * VPL + i;
             s[i] /= z;
-            const float d = kLogitError * fmaxf(fabsf((float)l[i]), rms), sf = (float)s[i];
+            const float sf = (float)s[i];
             e[i] = ((precise >> i) & 1u) ? 0.f : sf * (1.f - sf) * d * 1.01f;
             // the sum of the softmax is not exact before all logits are; it shifts ranks only against a bias
             if (soft && p.bias && !all) e[i] += sf * kLogitError * 0.25f;
@@ -209,195 +250,356 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
             }
             return;
         }
-        // sum the wanted logits again, one after the other, the warp over the row
+        // sum the wanted logits again, two at a time
+        int first = -1;
+        auto keep = [&](int x, double v) {
+#pragma unroll
+            for (int q = 0; q < VPL; q++)
+                if (lane * VPL + q == x) l[q] = v;
+        };
         for (int i = 0; i < VPL; i++) {
             uint32_t lanes = __ballot_sync(0xffffffffu, ((want >> i) & 1u) && lane * VPL + i < E);
             while (lanes) {
-                const int src = __ffs((int)lanes) - 1;
+                const int x = (__ffs((int)lanes) - 1) * VPL + i;
                 lanes &= lanes - 1;
-                const float4* wr = reinterpret_cast<const float4*>(p.w + (size_t)(src * VPL + i) * p.H);
-                const uint2* xr = reinterpret_cast<const uint2*>(p.x + (size_t)row * p.H);
-                double a0 = 0, a1 = 0, a2 = 0, a3 = 0;
-#pragma unroll 4
-                for (int k = lane; k < p.H / 4; k += 32) {
-                    const float4 w = __ldg(wr + k);
-                    const uint2 q = xr[k];
-                    a0 = fma((double)w.x, (double)__uint_as_float(q.x << 16), a0);
-                    a1 = fma((double)w.y, (double)__uint_as_float(q.x & 0xffff0000u), a1);
-                    a2 = fma((double)w.z, (double)__uint_as_float(q.y << 16), a2);
-                    a3 = fma((double)w.w, (double)__uint_as_float(q.y & 0xffff0000u), a3);
-                }
-                const double sum = warp_sum_d((a0 + a1) + (a2 + a3));
-#pragma unroll
-                for (int q = 0; q < VPL; q++)
-                    if (q == i && lane == src) l[q] = sum;
+                if (first < 0) { first = x; continue; }
+                double da, db;
+                dots_ask(p, sh, row, first, x, da, db);
+                keep(first, da);
+                keep(x, db);
+                first = -1;
             }
+        }
+        if (first >= 0) {
+            double da, db;
+            dots_ask(p, sh, row, first, first, da, db);
+            keep(first, da);
         }
         precise |= want;
     }
 }
 
 // ---- 32-bit path -----------------------------------------------------------------------------------------------------
-template <int VPL>
-__device__ __forceinline__ void select_row(const SelectParams& p, int row, int lane) {
+// The ranking values r and scores s (64 bits) of two experts, made by a whole warp. `z`: the softmax's sum.
+__device__ __noinline__ void exact_pair(const SelectParams& p, SelectShared* sh, int row, const float* lrow, int lane, int a, int b, double top, double z, double (&r)[2], double (&s)[2]) {
+    double la = (double)lrow[a], lb = (double)lrow[b];
+    if (sh) dots_ask(p, sh, row, a, b, la, lb);
+    // lane 0 takes a, lane 1 takes b
+    const double l = lane == 0 ? la : lb;
+    const double v = p.score == OCO_SCORE_SOFTMAX ? exp(l - top) / z : 1.0 / (1.0 + exp(-l));
+    const double w = p.bias ? v + (double)p.bias[lane == 0 ? a : b] : v;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        r[i] = __shfl_sync(0xffffffffu, w, i);
+        s[i] = __shfl_sync(0xffffffffu, v, i);
+    }
+}
+
+// Largest first (Batcher's merge exchange).
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; i++)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t a = k[i + j], b = k[i + j + q];
+                        k[i + j] = max(a, b);
+                        k[i + j + q] = min(a, b);
+                    }
+}
+
+// A lane's keys carry the element's index in place of their last bits (VPL - 1 - i, so that of equal ones the lower index
+// comes first): sorted once, a lane's best is its first key, and taking it is a shift. What the bits hid belongs to the
+// margin below which two values are not told apart here.
+//
+// Returns 0, or, before anything is written, what an open decision needs (only where !EXACT): 1 the exact values of the
+// logits as they are, 2 exact logits too. EXACT settles it: with `sh`, warp 0 while the others serve, else any warp.
+template <int VPL, bool EXACT>
+__device__ __forceinline__ int select_row(const SelectParams& p, int row, int lane, SelectShared* sh) {
+    constexpr uint32_t kIndex = VPL - 1;
     const int E = p.E, gs = E / p.G, K = p.K;
     const float* lrow = p.logits + (size_t)row * E;
     const bool soft = p.score == OCO_SCORE_SOFTMAX;
-    float l[VPL], s[VPL];
-    uint32_t key[VPL];
+    float l[VPL];
     if (VPL >= 4 && E % 4 == 0 && ((uintptr_t)p.logits & 15u) == 0) {
 #pragma unroll
         for (int i = 0; i < VPL; i += 4) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane * VPL + i < E) v = *reinterpret_cast<const float4*>(lrow + lane * VPL + i);
+            if (lane * VPL + i < E) v = __ldg(reinterpret_cast<const float4*>(lrow + lane * VPL + i));
             l[i] = v.x; l[(i + 1) % VPL] = v.y; l[(i + 2) % VPL] = v.z; l[(i + 3) % VPL] = v.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) l[i] = lane * VPL + i < E ? lrow[lane * VPL + i] : 0.f;
+        for (int i = 0; i < VPL; i++) l[i] = lane * VPL + i < E ? __ldg(lrow + lane * VPL + i) : 0.f;
     }
-    uint32_t bad = 0;
-    float top = 0.f, sq = 0.f;
+    uint32_t big = 0;                                                  // largest magnitude of a logit, as bits
 #pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        const bool in = lane * VPL + i < E;
-        if (in && nonfinite(l[i])) bad |= 1u << i;
-        if ((bad >> i) & 1u) l[i] = -3.4e38f;                          // ranks last; the weights become NaN below
-        sq = fmaf(l[i], l[i], sq);
+    for (int i = 0; i < VPL; i++) big = max(big, __float_as_uint(fabsf(l[i])));
+    big = warp_max(big);
+    const bool any_bad = big >= 0x7f800000u;                           // a logit is infinite or NaN: the weights will be NaN
+    if (any_bad) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (nonfinite(l[i])) l[i] = -3.4e38f;
     }
-    const bool any_bad = __any_sync(0xffffffffu, bad != 0);
+    // largest error of a logit of this row (0: they are exact as given)
+    const float dl = p.x && !any_bad ? kLogitError * __uint_as_float(big) : 0.f;   // rows of zeros have exact ones
+    const bool pairs = p.TG < p.G && p.best == 2 && gs > 1;            // groups are worth two scores
+    float top = 0.f, inv = 1.f;
     if (soft) {
         float m = -3.4e38f;
 #pragma unroll
         for (int i = 0; i < VPL; i++)
             if (lane * VPL + i < E) m = fmaxf(m, l[i]);
         top = key_rank(warp_max(rank_key(m)));
+    }
+    // What is ranked: score + bias; without a bias the logit itself, which has the same order. ek: the largest error of a
+    // ranking value, es: of a score (a softmax's relative to the largest score, which is inv).
+    float ek = dl;
+    const float es = soft ? kScoreError + dl : kSigmoidError + 0.25f * dl;
+    float r[VPL];
+    uint32_t wide = 0;                                                 // largest magnitude of score + bias, as bits
+    if (p.bias || (soft && !p.normalize)) {
         float z = 0.f;
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
-            const float d = l[i] - top;
-            s[i] = lane * VPL + i < E ? expf(d) : 0.f;
-            z += s[i];
+            if (soft) {
+                r[i] = lane * VPL + i < E ? expf(l[i] - top) : 0.f;
+                z += r[i];
+            } else {
+                r[i] = __fdividef(1.0f, 1.0f + expf(fminf(-l[i], 80.0f)));
+            }
         }
-        const float inv = 1.0f / warp_sum_f(z);
+        if (soft) inv = 1.0f / warp_sum_f(z);
+    }
+    if (p.bias) {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] *= inv;
+        for (int i = 0; i < VPL; i++) {
+            const int x = lane * VPL + i;
+            r[i] = r[i] * inv + (x < E ? __ldg(p.bias + x) : 0.f);
+            if (!nonfinite(r[i])) wide = max(wide, __float_as_uint(fabsf(r[i])));
+        }
+        wide = warp_max(wide);
+        ek = (soft ? inv * es : es) + kHalfUlp * __uint_as_float(wide);
     } else {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = 1.0f / (1.0f + expf(-l[i]));
+        for (int i = 0; i < VPL; i++) r[i] = l[i];
     }
-    const float rms = p.x ? sqrtf(warp_sum_f(sq) / (float)E) : 0.f;
+    uint32_t key[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
-        const int x = lane * VPL + i;
-        float r = s[i];
-        if (p.bias && x < E) r += __ldg(p.bias + x);
-        key[i] = x < E ? ((bad >> i) & 1u ? 1u : rank_key(r)) : 0u;
+        uint32_t k = rank_key(r[i]);
+        if (any_bad && l[i] == -3.4e38f) k = 1u;
+        key[i] = lane * VPL + i < E ? (max(k, 16u) & ~kIndex) | (kIndex - i) : 0u;
     }
-    // error of a ranking value with score sv: its own roundings, and its logit's error through the score's slope.
-    // softmax: exp(l - top) also carries the rounding of l - top (|ln s| bounds it up to the sum)
-    auto error_of = [&](float r, float sv) {
-        float er = kScoreError * sv + kHalfUlp * fabsf(r);
-        if (soft) er += kHalfUlp * sv * (16.f + fabsf(__logf(fmaxf(sv, 1e-37f))));
-        if (p.x) {
-            const float lv = soft ? fabsf(top) + 1.f : fabsf(__logf(fmaxf(sv, 1e-37f)) - __logf(fmaxf(1.f - sv, 1e-37f)));
-            er += sv * ((1.f - sv) + (soft && p.bias ? 0.25f : 0.f) + 1e-6f) * kLogitError * fmaxf(rms, lv);
-        }
-        return er;
-    };
-    bool open = false;
-
-    uint32_t groups = 0xffffffffu;
-    if (p.TG < p.G) {
-        float worth = 0.f, werr = 0.f;                                 // lane g: group g
-        for (int g = 0; g < p.G; g++) {
-            uint32_t m1 = 0, m2 = 0;
-            float s1 = 0.f, s2 = 0.f;
+    sort_keys(key);
+    // the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
+    auto value = [&](uint32_t k) { return k < 0x00800000u ? -INFINITY : key_rank(k); };
+    auto margin = [&](float v) { return 2.f * ek + (VPL > 1 ? 2.f * VPL * kHalfUlp * 2.f * fabsf(v) : 0.f); };
+    // two values, the first not below the second, that are not told apart (also two of -inf)
+    auto too_near = [&](float a, float b) { return (VPL > 1 || ek > 0.f) && !(a - b > margin(a)); };
+    auto expert_of = [&](uint32_t k, int from) { return from * VPL + (int)(kIndex - (k & kIndex)); };
+    double z64 = 0.0;                                                  // the softmax's sum in 64 bits, made when it is needed
+    auto sum64 = [&]() {
+        if (!soft || z64 != 0.0) return;
+        double z = 0.0;
 #pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                const uint32_t k = (lane * VPL + i) / gs == g ? key[i] : 0u;
-                if (k > m1) { m2 = m1; s2 = s1; m1 = k; s1 = s[i]; }
-                else if (k > m2) { m2 = k; s2 = s[i]; }
+        for (int i = 0; i < VPL; i++)
+            if (lane * VPL + i < E) z += exp((double)lrow[lane * VPL + i] - (double)top);
+        z64 = warp_sum_d(z);
+    };
+
+    bool open = false;                                                 // left to select_exact
+    if (p.TG < p.G) {
+        const bool whole = gs % VPL == 0;                              // a lane's experts are all of one group
+        // the three best of group g: values, and the experts of the first two
+        auto best_of = [&](int g, float (&v)[3], int (&id)[2]) {
+            uint32_t m[3] = {0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (key[i] && expert_of(key[i], lane) / gs == g) {
+                    if (!m[0]) m[0] = key[i];
+                    else if (!m[1]) m[1] = key[i];
+                    else if (!m[2]) m[2] = key[i];
+                }
+#pragma unroll
+            for (int t = 0; t < 3; t++) {
+                const uint32_t a = warp_max(m[0]);
+                const int from = __ffs((int)__ballot_sync(0xffffffffu, m[0] == a)) - 1;
+                v[t] = a ? value(a) : -INFINITY;
+                if (t < 2) id[t] = a ? expert_of(a, from) : g * gs;
+                if (lane == from) { m[0] = m[1]; m[1] = m[2]; m[2] = 0; }
             }
-            const uint32_t a = warp_max(m1);
-            const int la = __ffs((int)__ballot_sync(0xffffffffu, m1 == a)) - 1;
-            float w = key_rank(a), er = error_of(w, __shfl_sync(0xffffffffu, s1, la));
-            if (a <= 1u) { w = -INFINITY; er = 0.f; }                  // nothing finite in the group
-            if (p.best == 2 && gs > 1) {
-                if (lane == la) { m1 = m2; s1 = s2; }
-                const uint32_t b = warp_max(m1);
-                const int lb = __ffs((int)__ballot_sync(0xffffffffu, m1 == b)) - 1;
-                const float v = b <= 1u ? -INFINITY : key_rank(b);
-                er += error_of(v, __shfl_sync(0xffffffffu, s1, lb)) + kHalfUlp * fabsf(w + v);
-                w += v;
+        };
+        auto worth_of = [&](float a, float b) {                        // without a bias of scores, a softmax's relative to the largest
+            if (!pairs) return a;
+            if (p.bias) return a + b;
+            return soft ? expf(a - top) + expf(b - top) : __fdividef(1.0f, 1.0f + expf(fminf(-a, 80.0f))) + __fdividef(1.0f, 1.0f + expf(fminf(-b, 80.0f)));
+        };
+        float worth = -INFINITY;                                       // lane g: group g
+        const int lanes = gs / VPL;
+        if (whole && (lanes & (lanes - 1)) == 0) {
+            // a group is 2^n lanes: the two best of every group at once
+            uint32_t m1 = key[0], m2 = VPL > 1 ? key[VPL > 1] : 0u;
+            for (int d = 1; d < lanes; d <<= 1) {
+                const uint32_t o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+                m2 = max(max(m2, o2), min(m1, o1));
+                m1 = max(m1, o1);
             }
-            if (lane == g) { worth = w; werr = er; }
+            worth = __shfl_sync(0xffffffffu, worth_of(value(m1), value(m2)), min(31, lane * lanes));
+        } else {
+            for (int g = 0; g < p.G; g++) {
+                float v[3];
+                int id[2];
+                best_of(g, v, id);
+                const float w = worth_of(v[0], v[1]);
+                if (lane == g) worth = w;
+            }
         }
         const uint32_t wkey = lane < p.G ? rank_key(worth) : 0u;
-        uint32_t left = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u, k = 0;
+        uint32_t left = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u, kprev = 0, kt = 0;
         int at = 0;
         for (int t = 0; t < p.TG; t++) {
             const uint32_t mine = (left >> lane) & 1u ? wkey : 0u;
-            k = warp_max(mine);
-            at = __ffs((int)__ballot_sync(0xffffffffu, mine == k && ((left >> lane) & 1u))) - 1;
+            kprev = kt;
+            kt = warp_max(mine);
+            at = __ffs((int)__ballot_sync(0xffffffffu, mine == kt && ((left >> lane) & 1u))) - 1;
             left &= ~(1u << at);
         }
         const uint32_t mine = (left >> lane) & 1u ? wkey : 0u, k2 = warp_max(mine);
         const int at2 = __ffs((int)__ballot_sync(0xffffffffu, mine == k2 && ((left >> lane) & 1u))) - 1;
-        const float er = __shfl_sync(0xffffffffu, werr, at) + __shfl_sync(0xffffffffu, werr, at2);
-        open = key_rank(k) - key_rank(k2) <= er;
-        groups = ~left;
+        const float wa = key_rank(kt), wb = key_rank(k2);
+        // error of a worth: of one value, or of two and the rounding of their sum
+        const float size = !pairs ? fabsf(wa) : p.bias ? __uint_as_float(wide) : 1.f;
+        const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size : 0.f) + kHalfUlp * size;
+        const float near_w = pairs ? 4.f * one : 2.f * one;
+        if ((VPL > 1 || ek > 0.f || pairs) && !(wa - wb > near_w) && !any_bad) {
+            // the border lies between two groups: their exact worths decide, unless a third one is as near or what a group
+            // is worth is not clear
+            if constexpr (!EXACT) return dl > 0.f ? 2 : 1;
+            const uint32_t k3 = warp_max((left >> lane) & 1u && lane != at2 ? wkey : 0u);
+            open = (p.TG > 1 && !(key_rank(kprev) - wb > near_w)) || (k3 != 0u && !(wa - key_rank(k3) > near_w));
+            if (!open) {
+                float a[3], b[3];
+                int ia[2], ib[2];
+                best_of(at, a, ia);
+                best_of(at2, b, ib);
+                const int t = pairs ? 1 : 0;
+                open = (gs > t + 1 && (too_near(a[t], a[t + 1]) || too_near(b[t], b[t + 1])));
+                if (!open) {
+                    sum64();
+                    double r1[2], v1[2], r2[2] = {0.0, 0.0}, v2[2] = {0.0, 0.0};
+                    exact_pair(p, sh, row, lrow, lane, ia[0], ib[0], (double)top, z64, r1, v1);
+                    if (pairs) exact_pair(p, sh, row, lrow, lane, ia[1], ib[1], (double)top, z64, r2, v2);
+                    const double da = r1[0] + r2[0], db = r1[1] + r2[1];
+                    // the softmax's sum is not exact where the logits are not: it shifts the scores' difference
+                    if (sh && soft && p.bias && fabs(da - db) <= (double)dl * fabs((v1[0] + v2[0]) - (v1[1] + v2[1]))) open = true;
+                    else if (db > da || (db == da && at2 < at)) left = (left | (1u << at)) & ~(1u << at2);
+                }
+            }
+        }
+        if (whole) {
+            if ((left >> min(31, lane * VPL / gs)) & 1u) {
 #pragma unroll
-        for (int i = 0; i < VPL; i++)
-            if (lane * VPL + i >= E || !((groups >> ((lane * VPL + i) / gs)) & 1u)) key[i] = 0u;
-    }
-
-    int my_id = 0;
-    float my_s = 0.f, prev_r = 0.f, prev_e = 0.f;
-    for (int j = 0; j <= K; j++) {
-        uint32_t lm = 0;
-#pragma unroll
-        for (int i = 0; i < VPL; i++) lm = max(lm, key[i]);
-        const uint32_t m = warp_max(lm);
-        if (m == 0u) break;                                            // fewer experts than K + 1
-        const int src = __ffs((int)__ballot_sync(0xffffffffu, lm == m)) - 1;
-        int at = 0;
-        float sv = 0.f;
-#pragma unroll
-        for (int i = VPL - 1; i >= 0; i--)
-            if (key[i] == m) { at = i; sv = s[i]; }
-        if (lane == src) {
+                for (int i = 0; i < VPL; i++) key[i] = 0u;
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < VPL; i++)
-                if (i == at) key[i] = 0u;
+                if (key[i] && ((left >> (expert_of(key[i], lane) / gs)) & 1u)) key[i] = 0u;
+            sort_keys(key);
         }
-        at = __shfl_sync(0xffffffffu, at, src);
-        sv = __shfl_sync(0xffffffffu, sv, src);
-        const float r = key_rank(m), er = error_of(r, sv);
-        if (j > 0 && prev_r - r <= prev_e + er) open = true;
-        prev_r = r; prev_e = er;
-        if (lane == j && j < K) { my_id = src * VPL + at; my_s = sv; }
     }
-    if (open && !any_bad) {
-        select_exact<VPL>(p, row, lrow, lane);
-        return;
+
+    // top-k: lane j keeps the j-th key and the lane it came from
+    uint32_t my_key = 0;
+    int my_from = 0;
+    for (int j = 0; j <= K; j++) {
+        const uint32_t m = warp_max(key[0]);
+        const int from = __ffs((int)__ballot_sync(0xffffffffu, key[0] == m)) - 1;
+        if (lane == j) { my_key = m; my_from = from; }
+        if (lane == from) {
+#pragma unroll
+            for (int i = 0; i + 1 < VPL; i++) key[i] = key[i + 1];
+            key[VPL - 1] = 0u;
+        }
+    }
+    int my_id = expert_of(my_key, my_from);
+    const float mine = my_key ? value(my_key) : 0.f, before = __shfl_up_sync(0xffffffffu, mine, 1);
+    uint32_t near = __ballot_sync(0xffffffffu, lane > 0 && lane <= K && my_key && too_near(before, mine));   // bit j: not told apart from j - 1
+    if (near && !any_bad && !open) {
+        if constexpr (!EXACT) return dl > 0.f ? 2 : 1;
+        // neighbours that are too near change places if their exact values say so; three in a row go to select_exact
+        open = (near & (near << 1)) != 0u;
+        if ((near >> K) & 1u) {
+            const uint32_t m = warp_max(key[0]);                       // the next one behind the border
+            open = open || (m != 0u && too_near(__shfl_sync(0xffffffffu, mine, K), value(m)));
+        }
+        if (!open) {
+            sum64();
+            while (near) {
+                const int j = __ffs((int)near) - 1;
+                near &= near - 1;
+                const int a = __shfl_sync(0xffffffffu, my_id, j - 1), b = __shfl_sync(0xffffffffu, my_id, j);
+                double rr[2], v[2];
+                exact_pair(p, sh, row, lrow, lane, a, b, (double)top, z64, rr, v);
+                if (sh && soft && p.bias && fabs(rr[0] - rr[1]) <= (double)dl * fabs(v[0] - v[1])) open = true;
+                if (rr[1] > rr[0] || (rr[1] == rr[0] && b < a)) {
+                    if (lane == j - 1) my_id = b;
+                    if (lane == j) my_id = a;
+                }
+            }
+        }
+    }
+    if (EXACT && open) {
+        select_exact<VPL>(p, row, lrow, lane, sh);
+        return 0;
+    }
+    float s = 0.f;
+    if (lane < K) {
+        const float v = __ldg(lrow + my_id);
+        s = soft ? expf(v - top) * inv : 1.0f / (1.0f + expf(-v));
     }
     float sum = 1.0f;
-    if (p.normalize) sum = fmaxf(warp_sum_f(lane < K ? my_s : 0.f), 6.103515625e-5f);
+    if (p.normalize) {
+        sum = warp_sum_f(s);
+        if (!soft || p.bias) sum = fmaxf(sum, 6.103515625e-5f);        // of a softmax's largest scores: never below top_k / experts
+    }
     if (lane < K) {
         p.ids[(size_t)row * K + lane] = (uint32_t)my_id;
-        p.probs[(size_t)row * K + lane] = any_bad ? qnan() : my_s / sum * p.scale;
+        p.probs[(size_t)row * K + lane] = any_bad ? qnan() : s / sum * p.scale;
     }
+    return 0;
 }
+
+template <int VPL>
+__device__ __noinline__ void settle_row(const SelectParams& p, int row, int lane, SelectShared* sh) { select_row<VPL, true>(p, row, lane, sh); }
 
 // A warp per token, eight tokens per CTA.
 template <int VPL>
-__global__ void __launch_bounds__(256) select_kernel(const SelectParams p) {
-    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
+__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2) select_kernel(const SelectParams p) {
+    __shared__ SelectShared sh;
     pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();
     if (p.status && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) return;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row < p.rows) select_row<VPL>(p, row, threadIdx.x & 31);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 8 + warp;
+    const int left = row < p.rows ? select_row<VPL, false>(p, row, lane, nullptr) : 0;
+    if (left == 1) settle_row<VPL>(p, row, lane, nullptr);
+    if (!p.x || !__syncthreads_or(left == 2)) return;
+    if (lane == 0) sh.rows[warp] = left == 2 ? row : -1;
+    __syncthreads();
+    if (warp == 0) {
+        for (int w = 0; w < 8; w++)
+            if (sh.rows[w] >= 0) settle_row<VPL>(p, sh.rows[w], lane, &sh);
+        dots_end(&sh);
+    } else {
+        dots_serve(p, &sh);
+    }
 }
 
 }  // namespace oco
