@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
     for (int i = 0; i < ITER; i++) live[i] = col0 + i * THREADS * 8 < p.n;
 
     float h[ITER][8], b[ITER][8];
-    uint4 raw[ITER][WIDE ? 2 : 1], braw[ITER];
+    uint4 raw[ITER][WIDE ? 2 : 1], braw[ITER], graw[ITER];
+    const long long grow = p.gate_rows > 0 ? (long long)(row / p.gate_rows) * p.gate_stride : 0;
 #pragma unroll
     for (int i = 0; i < ITER; i++) {
         const int at = col0 + i * THREADS * 8;
@@ -137,6 +138,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
             raw[i][0] = *reinterpret_cast<const uint4*>(src);
             if (WIDE) raw[i][WIDE ? 1 : 0] = *reinterpret_cast<const uint4*>(src + 16);
             if (p.block) braw[i] = *reinterpret_cast<const uint4*>(p.block + (long long)row * p.block_stride + at);
+            // a gate in bf16 may be as long as the rows: it travels with them
+            if (p.gate_type == OCO_GATE_BF16) graw[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + grow + at));
         } else {
             raw[i][0] = raw[i][WIDE ? 1 : 0] = make_uint4(0, 0, 0, 0);
         }
@@ -147,14 +150,12 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
         for (int i = 0; i < ITER; i++) unpack8(braw[i], b[i]);
         if (p.post_w) normalise<THREADS, ITER, LAYER>(b, live, p.post_w, p.post_b, col0, p, slots);
         if (p.gate_type) {
-            const long long grow = p.gate_rows > 0 ? (long long)(row / p.gate_rows) * p.gate_stride : 0;
 #pragma unroll
             for (int i = 0; i < ITER; i++) {
                 if (live[i]) {
-                    const long long at = grow + col0 + i * THREADS * 8;
                     float g[8];
-                    if (p.gate_type == 2) load8(reinterpret_cast<const float*>(p.gate) + at, g);
-                    else unpack8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + at)), g);
+                    if (p.gate_type == OCO_GATE_F32) load8(reinterpret_cast<const float*>(p.gate) + grow + col0 + i * THREADS * 8, g);
+                    else unpack8(graw[i], g);
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         if (p.gate_act == 1) g[j] = 1.0f / (1.0f + __expf(-g[j]));

@@ -14,6 +14,8 @@ namespace {
 // of as many rows, the pair's two of 128.
 constexpr int kTileRows[5] = {16, 32, 64, 128, 256}, kRowBoxes[4] = {16, 32, 64, 128};
 constexpr int kWideIndex = 3, kPairIndex = 4;
+// Tokens of a routed call up to which every route is a tile of its own.
+constexpr int kOwnTokens = 1;
 enum F8Kind { kF8Projection = OCO_DENSE_PROJECTION, kF8Gated = OCO_DENSE_FFN_SILU_GATE, kF8Experts = 100 };
 
 struct F8Space {
@@ -118,16 +120,20 @@ int tile_index(int rows, int experts) {
     return avg <= 8 ? 0 : avg <= 20 ? 1 : avg <= 64 ? 2 : kWideIndex;
 }
 
-template <int NT, bool GATED>
-int launch_thin(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap& rows, const CUtensorMap& w0, const CUtensorMap& w1, int tiles, int expected,
-                cudaStream_t st) {
-    using S = F8Thin<NT, GATED>;
-    auto kernel = f8_thin_kernel<NT, GATED>;
-    OCO_ALLOW_SMEM_ONCE(plan, kernel);
-    const int nfeat = (p.n + 127) / 128, nkb = (p.K + 127) / 128;
-    // parts of the contraction: as many as fill the SMs twice, two blocks of 128 or more each
+// Parts of the contraction of an f8_thin_kernel item: as many as fill the SMs twice, two blocks of 128 or more each.
+unsigned thin_split(const oco_moe_f8_plan* plan, long long items, int blocks) {
     unsigned split = 1;
-    while (split < 8 && (long long)expected * nfeat * split * 2 <= 2LL * plan->sm_count && nkb >= 4 * (int)split) split *= 2;
+    while (split < 8 && items * split * 2 <= 2LL * plan->sm_count && blocks >= 4 * (int)split) split *= 2;
+    return split;
+}
+
+template <int NT, bool GATED, int FORM>
+int launch_thin(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap& rows, const CUtensorMap& w0, const CUtensorMap& w1, int tiles, unsigned split,
+                cudaStream_t st) {
+    using S = F8Thin<NT, GATED, FORM>;
+    auto kernel = f8_thin_kernel<NT, GATED, FORM>;
+    OCO_ALLOW_SMEM_ONCE(plan, kernel);
+    const int nfeat = (p.n + 127) / 128;
     OCO_CK(plan, launch_dependent_clusters(kernel, split, dim3((unsigned)((long long)tiles * nfeat * split)), dim3(S::kThreads), S::kSmem, st, p, rows, w0, w1));
     plan->launches++;
     return OCO_OK;
@@ -137,9 +143,10 @@ int launch_thin(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap&
 template <bool GATED>
 int product(oco_moe_f8_plan* plan, const F8TileParams& p, const CUtensorMap* maps, const CUtensorMap& w0, const CUtensorMap& w1, int index, int tiles, int expected,
             cudaStream_t st) {
-    if (index == 0) return launch_thin<16, GATED>(plan, p, maps[0], w0, w1, tiles, expected, st);
-    if (index == 1) return launch_thin<32, GATED>(plan, p, maps[1], w0, w1, tiles, expected, st);
-    if (index == 2) return launch_thin<64, GATED>(plan, p, maps[2], w0, w1, tiles, expected, st);
+    const unsigned split = thin_split(plan, (long long)expected * ((p.n + 127) / 128), (p.K + 127) / 128);
+    if (index == 0) return launch_thin<16, GATED, kF8Tiles>(plan, p, maps[0], w0, w1, tiles, split, st);
+    if (index == 1) return launch_thin<32, GATED, kF8Tiles>(plan, p, maps[1], w0, w1, tiles, split, st);
+    if (index == 2) return launch_thin<64, GATED, kF8Tiles>(plan, p, maps[2], w0, w1, tiles, split, st);
     const long long items = (long long)tiles * ((p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
     if (index == kWideIndex) {
         auto kernel = f8_wide_kernel<GATED, false>;
@@ -163,6 +170,27 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     F8Space& ws = plan->ws;
     const bool routed = ids != nullptr;
     const int R = rows * d.top_k, H = d.hidden, F = d.ffn, E = d.experts;
+    F8TileParams p{};
+    p.row_scales = ws.xs; p.pitch = ws.pitch; p.K = H; p.n = F; p.rows = R; p.status = ws.status; p.top_k = d.top_k; p.experts = E;
+    // Few rows: the first product rounds them itself, and a few routed tokens need no sorted rows either (a tile per route;
+    // the second product sums a token's routes). Both read an expert once per route.
+    const int own_tiles = routed ? R : (rows + 15) / 16, nkb = (H + 127) / 128;
+    const unsigned own_split = thin_split(plan, (long long)own_tiles * ((F + 127) / 128), nkb);
+    if (rows <= (routed ? kOwnTokens : 16) && (nkb + (int)own_split - 1) / (int)own_split <= F8Thin<16, true, kF8Rows>::kBlocks) {
+        p.x = x; p.ids = ids;
+        if (plan->kind == kF8Projection) {
+            p.s0 = plan->w.up_s; p.out = out;
+            return launch_thin<16, false, kF8Rows>(plan, p, plan->map_x[0], plan->map_up, plan->map_up, own_tiles, own_split, st);
+        }
+        F8TileParams q = p;
+        p.s0 = plan->w.gate_s; p.s1 = plan->w.up_s; p.codes = ws.aq; p.code_scales = ws.as;
+        if (int rc = launch_thin<16, true, kF8Rows>(plan, p, plan->map_x[0], plan->map_gate, plan->map_up, own_tiles, own_split, st)) return rc;
+        q.row_scales = ws.as; q.K = F; q.n = H; q.s0 = plan->w.down_s; q.out = out;
+        if (!routed) return product<false>(plan, q, plan->map_a, plan->map_down, plan->map_down, 0, own_tiles, own_tiles, st);
+        q.probs = probs; q.residual = residual;
+        return launch_thin<16, false, kF8Concat>(plan, q, plan->map_a[0], plan->map_down, plan->map_down, rows,
+                                                 thin_split(plan, (long long)rows * ((H + 127) / 128), d.top_k * ((F + 127) / 128)), st);
+    }
     const int index = tile_index(R, routed ? std::min(E, R) : 1), nt = kTileRows[index];
     // tiles: exact for a dense product; for routed rows as many as the worst choice of experts makes, and the usual number
     const int tiles = routed ? R / nt + std::min(E, R) : (R + nt - 1) / nt, expected = routed ? std::max(std::min(E, R), R / nt) : tiles;
@@ -171,11 +199,9 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
         OCO_CK(plan, launch_dependent(f8_plan_kernel, dim3(1), dim3(1024), 0, st, pp));
         plan->launches++;
     }
-    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)rows * ((H + 127) / 128) + 15) / 16, 8LL * plan->sm_count);
+    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)rows * ((H + 255) / 256) + 15) / 16, 8LL * plan->sm_count);
     OCO_CK(plan, launch_dependent(f8_rows_kernel, dim3(row_ctas), dim3(256), 0, st, x, routed ? ws.row_of_route : nullptr, d.top_k, rows, H, ws.xq, ws.xs, ws.pitch));
     plan->launches++;
-    F8TileParams p{};
-    p.row_scales = ws.xs; p.pitch = ws.pitch; p.K = H; p.n = F; p.rows = R; p.status = ws.status;
     if (routed) { p.tiles = ws.tiles; p.tile_count = ws.tile_count; p.offsets = ws.offsets; }
     if (plan->kind == kF8Projection) {
         p.s0 = plan->w.up_s; p.out = out;

@@ -88,6 +88,12 @@ struct F8Divider {
         plain = largest > 7.9e-31f && largest < 1.2e30f;
         rcp = plain ? __frcp_rn(largest) : 0.0f;
     }
+    // largest / 448, by the same method
+    __device__ __forceinline__ float scale() const {
+        constexpr float kPart = 1.0f / 448.0f;
+        const float q = top * kPart;
+        return plain ? fmaf(fmaf(-q, 448.0f, top), kPart, q) : __fdiv_rn(top, 448.0f);
+    }
     __device__ __forceinline__ float operator()(float x) const {
         if (plain) {
             const float n = x * 448.0f, q = n * rcp;
@@ -97,37 +103,55 @@ struct F8Divider {
     }
 };
 
-// Rows to codes: half a warp per token and block of 128 elements, eight elements a lane. A routed token is read and
-// rounded once and its codes written to the row of each of its routes. Scales lie [block][row].
+// Half a warp's block of 128 bf16 elements (eight a lane) -> codes and their scale. `half`: the lanes' mask.
+__device__ __forceinline__ float f8_block(const uint4& q, uint32_t half, uint2& codes) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    // the largest as bits: for non-negative floats the order of the bits, a NaN above everything
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) m = max(m, max((w[j] << 16) & 0x7fff0000u, w[j] & 0x7fff0000u));
+    m = __reduce_max_sync(half, m);
+    const F8Divider code(__uint_as_float(m));
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        v[2 * j] = code(__uint_as_float(w[j] << 16));
+        v[2 * j + 1] = code(__uint_as_float(w[j] & 0xffff0000u));
+    }
+    codes = make_uint2(f8x4(v[0], v[1], v[2], v[3]), f8x4(v[4], v[5], v[6], v[7]));
+    return code.scale();
+}
+
+// Rows to codes: half a warp per token and two blocks of 128 elements, eight elements of each a lane (two loads on their
+// way). A routed token is read and rounded once and its codes written to the row of each of its routes. Scales lie
+// [block][row].
 __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict__ x, const uint32_t* __restrict__ row_of_route, int top_k,
                                                       int tokens, int K, uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();   // only now: the next kernel reads weights before it waits for this one
-    const int lane = threadIdx.x & 15, nkb = (K + 127) / 128;
+    const int lane = threadIdx.x & 15, npairs = (K + 255) / 256;
     const uint32_t half = 0xffffu << (threadIdx.x & 16);
-    const uint32_t units = (uint32_t)tokens * (uint32_t)nkb, step = gridDim.x * 16;
+    const uint32_t units = (uint32_t)tokens * (uint32_t)npairs, step = gridDim.x * 16;
     for (uint32_t u = blockIdx.x * 16 + (threadIdx.x >> 4); u < units; u += step) {
-        const uint32_t token = u / (uint32_t)nkb;
-        const int kb = (int)(u - token * (uint32_t)nkb), k = kb * 128 + 8 * lane;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (k < K) q = __ldg(reinterpret_cast<const uint4*>(x + (size_t)token * K + k));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        // the largest as bits: for non-negative floats the order of the bits, a NaN above everything
-        uint32_t m = 0;
+        const uint32_t token = u / (uint32_t)npairs;
+        const int pair = (int)(u - token * (uint32_t)npairs), k = pair * 256 + 8 * lane;
+        const uint16_t* src = x + (size_t)token * K + k;
+        const bool in[2] = {k < K, k + 128 < K};
+        uint4 q[2];
 #pragma unroll
-        for (int j = 0; j < 4; j++) m = max(m, max((w[j] << 16) & 0x7fff0000u, w[j] & 0x7fff0000u));
-        m = __reduce_max_sync(half, m);
-        const float top = __uint_as_float(m);
-        const F8Divider code(top);
-        uint2 c;
-        c.x = f8x4(code(__uint_as_float(w[0] << 16)), code(__uint_as_float(w[0] & 0xffff0000u)), code(__uint_as_float(w[1] << 16)), code(__uint_as_float(w[1] & 0xffff0000u)));
-        c.y = f8x4(code(__uint_as_float(w[2] << 16)), code(__uint_as_float(w[2] & 0xffff0000u)), code(__uint_as_float(w[3] << 16)), code(__uint_as_float(w[3] & 0xffff0000u)));
-        const float scale = __fdiv_rn(top, 448.0f);
+        for (int b = 0; b < 2; b++) q[b] = in[b] ? __ldg(reinterpret_cast<const uint4*>(src + 128 * b)) : make_uint4(0, 0, 0, 0);
+        uint2 c[2];
+        float scale[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) scale[b] = f8_block(q[b], half, c[b]);
         for (int r = 0; r < top_k; r++) {
-            const uint32_t row = row_of_route ? row_of_route[(size_t)token * top_k + r] : token;
+            const uint32_t row = row_of_route ? __ldg(row_of_route + (size_t)token * top_k + r) : token;
             if (row == 0xffffffffu) continue;
-            if (k < K) *reinterpret_cast<uint2*>(codes + (size_t)row * K + k) = c;
-            if (lane == 0) scales[(size_t)kb * scale_pitch + row] = scale;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                if (in[b]) *reinterpret_cast<uint2*>(codes + (size_t)row * K + k + 128 * b) = c[b];
+                if (lane == 0 && in[b]) scales[(size_t)(2 * pair + b) * scale_pitch + row] = scale[b];
+            }
         }
     }
 }

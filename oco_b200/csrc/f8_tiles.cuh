@@ -32,7 +32,12 @@ struct F8TileParams {
     uint8_t* codes;                 // gated: codes of the activations [row][n]
     float* code_scales;             // and their scales [ceil(n / 128)][pitch]
     uint32_t* status;
-    int n, K, rows, pitch;
+    // f8_thin_kernel's other forms: bf16 rows to be rounded (kF8Rows), routes (ids may be null there: dense), the token's sum
+    const uint16_t* x;              // bf16 [..][K]
+    const uint32_t* ids;            // [tokens][top_k]
+    const float* probs;
+    const uint16_t* residual;
+    int n, K, rows, pitch, top_k, experts;
 };
 
 __device__ __forceinline__ float silu_times(float g, float u) { return sigmoid_times(g, 1.0f) * g * u; }
@@ -376,42 +381,63 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------
-template <int NT, bool GATED>
+// What a CTA's rows are:
+//   kF8Tiles   codes and scales in memory (f8_rows_kernel, or the gated form of a product before); rows by TMA
+//   kF8Rows    bf16 rows, up to 16, that the CTA rounds to codes itself, the blocks of its part of the contraction: no
+//              kernel before it. Dense, or one tile per route (one row: the route's token)
+//   kF8Concat  one token's routes one behind the other as one long contraction, the weights of the routes in the scales:
+//              out = residual + sum_r prob_r (down_r . a_r), no kernel behind it
+enum F8Form { kF8Tiles, kF8Rows, kF8Concat };
+
+template <int NT, bool GATED, int FORM>
 struct F8Thin {
-    static constexpr int kA = 128 * 128, kMats = GATED ? 2 : 1, kB = NT * 128, kStage = kMats * kA + kB;
-    static constexpr int kRoom = 108 * 1024;                            // two CTAs on an SM
-    static constexpr int kStages = kRoom / kStage;
+    static_assert(FORM == kF8Tiles || NT == 16, "the other forms have up to 16 rows");
+    static_assert(FORM != kF8Concat || !GATED, "");
+    static constexpr int kA = 128 * 128, kMats = GATED ? 2 : 1, kB = FORM == kF8Rows ? 0 : NT * 128, kStage = kMats * kA + kB;
+    static constexpr int kCols = FORM == kF8Concat ? 1 : NT;            // columns that are rows
+    static constexpr int kBlocks = 16;                                  // kF8Rows: blocks of a CTA's part at most
+    static constexpr int kOwn = FORM == kF8Rows ? kBlocks * NT * (128 + 4) : 0;   // their codes, then their scales
+    // Shared memory for two CTAs an SM; narrow tiles get by with less, and three or four CTAs hide one another's start and end
+    // (64 tokens over 128 experts: 138 -> KSPEED us).
+    static constexpr int kRoom = (NT == 16 ? (GATED ? 70 : 54) : 108) * 1024;
+    static constexpr int kStages = (kRoom - kOwn) / kStage > 2 ? (kRoom - kOwn) / kStage : 2;
     static constexpr int kBufs = 2, kTmemUsed = kBufs * kMats * NT;
     static constexpr int kTmem = kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : 256;
     static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
     static constexpr int kCtrl = 512;
-    static constexpr int kSmem = kStages * kStage + kCtrl + 1024;
-    static_assert(kMats * NT * 128 * 4 <= kStages * kStage, "the parts of a split contraction lie where the stages were");
+    static constexpr int kSmem = kStages * kStage + kOwn + kCtrl + 1024;
+    static_assert(kMats * kCols * 128 * 4 <= kStages * kStage, "the parts of a split contraction lie where the stages were");
     static_assert(8 * (2 * kStages + 2 * kBufs) + 8 <= 256, "barriers");
 };
+
 // One item (a tile of up to NT rows of one expert, 128 features) per cluster; CTA r of its S takes the blocks
 // [r * per, ..) of the contraction. x = S * (item), items: feature tile fastest.
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
-                                                                             const __grid_constant__ CUtensorMap w0_map,
-                                                                             const __grid_constant__ CUtensorMap w1_map) {
-    using S = F8Thin<NT, GATED>;
-    constexpr int MATS = S::kMats;
+//
+// Weights travel before the kernel before is waited for: they, the tiles and (kF8Concat) the ids come from before the call
+// or from a kernel that has ended when this one may start, since every kernel of a call lets the next one start only after
+// its own wait. kF8Rows with ids (a router may just have written them) waits first.
+template <int NT, bool GATED, int FORM>
+__global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads) f8_thin_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
+                                                                                   const __grid_constant__ CUtensorMap w0_map,
+                                                                                   const __grid_constant__ CUtensorMap w1_map) {
+    using S = F8Thin<NT, GATED, FORM>;
+    constexpr int MATS = S::kMats, COLS = S::kCols;
     extern __shared__ unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t ctrl = base + S::kStages * S::kStage;
+    const uint32_t own = base + S::kStages * S::kStage, ctrl = own + S::kOwn;
+    unsigned char* gctrl = gen + (ctrl - base);
     auto full = [&](int s) { return ctrl + 8u * s; };
     auto empty = [&](int s) { return ctrl + 8u * (S::kStages + s); };
     auto tfull = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };
     auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + S::kBufs + b); };
-    uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kStages * S::kStage + 8 * (2 * S::kStages + 2 * S::kBufs));
+    uint32_t* slot = reinterpret_cast<uint32_t*>(gctrl + 8 * (2 * S::kStages + 2 * S::kBufs));
     volatile uint32_t* abort_flag = slot + 1;
-    uint32_t* tops = reinterpret_cast<uint32_t*>(gen + S::kStages * S::kStage + 256);   // [2][4]
+    uint32_t* tops = reinterpret_cast<uint32_t*>(gctrl + 256);          // [2][4]
+    volatile uint32_t* routes = reinterpret_cast<uint32_t*>(gctrl + 320);   // kF8Concat: how many, then (expert, route) of each
     const int split = (int)cluster_size(), rank = (int)cluster_rank();
-    const int nfeat = (p.n + 127) / 128, nkb = (p.K + 127) / 128, per = (nkb + split - 1) / split;
-    const int kb0 = min(nkb, rank * per), kb1 = min(nkb, kb0 + per);
+    const int nfeat = (p.n + 127) / 128, nkb = (p.K + 127) / 128;
     const int item = (int)blockIdx.x / split, tile = item / nfeat, f0 = (item - tile * nfeat) * 128;
     if (tid == 0) {
         for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -419,26 +445,22 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
         *abort_flag = 0;
         fence_barrier_init();
     }
-    // a dense product's weights are known already: their first tiles travel while the kernel before still runs
-    const bool early = p.tiles == nullptr;
+    if (FORM == kF8Concat && warp == 0) {                               // the token's routes that have an expert here
+        const uint32_t e = lane < p.top_k ? p.ids[(size_t)tile * p.top_k + lane] : 0xffffffffu;
+        const uint32_t live = __ballot_sync(0xffffffffu, e < (uint32_t)p.experts);
+        const int at = __popc(live & ((1u << lane) - 1u));
+        if ((live >> lane) & 1u) { routes[1 + 2 * at] = e; routes[2 + 2 * at] = lane; }
+        if (lane == 0) routes[0] = __popc(live);
+    }
     if (warp == S::kMmaWarp) { tmem_alloc(smem_u32(slot), S::kTmem); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    auto load_weights = [&](int kb, int s, int expert) {
-        const uint32_t at = base + (uint32_t)s * S::kStage;
-        mbar_arrive_expect_tx(full(s), S::kStage);
-        tma_load_2d(at, &w0_map, kb * 128, expert * p.n + f0, full(s));
-        if (GATED) tma_load_2d(at + S::kA, &w1_map, kb * 128, expert * p.n + f0, full(s));
-    };
-    const int first = min(S::kStages, kb1 - kb0);                       // stages filled before anything is waited for
-    if (early && warp == S::kTmaWarp && lane == 0)
-        for (int k = 0; k < first; k++) load_weights(kb0 + k, k, 0);
-    pdl_wait();                // the kernel before has completed and its writes are visible
-    pdl_launch_dependents();
+    // ---- what this CTA multiplies: rows [row0, row0 + nv) of codes with blocks [q0, q1) of the contraction -----------------
     int expert = 0, row0 = tile * NT, nv = min(NT, p.rows - row0);
-    if (p.tiles) {
+    const bool early = FORM != kF8Rows || !p.ids;
+    if (FORM == kF8Tiles && p.tiles) {
         if (tile >= (int)*p.tile_count) nv = 0;                         // the whole cluster
         else {
             expert = (int)p.tiles[2 * tile];
@@ -446,28 +468,88 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
             nv = min(NT, (int)p.offsets[expert + 1] - row0);
         }
     }
+    if (FORM == kF8Concat) nv = 1;
+    if (!early) {
+        pdl_wait();            // the kernel before has completed and its writes are visible
+        pdl_launch_dependents();
+        const uint32_t e = p.ids[tile];                                 // a tile per route, its row
+        row0 = tile;
+        nv = e < (uint32_t)p.experts ? 1 : 0;
+        expert = nv ? (int)e : 0;
+    }
+    const int blocks = FORM == kF8Concat ? (int)routes[0] * nkb : nkb, per = (blocks + split - 1) / split;
+    const int q0 = min(blocks, rank * per), q1 = nv > 0 ? min(blocks, q0 + per) : q0;
+    auto load_weights = [&](int q, int s) {
+        const uint32_t at = base + (uint32_t)s * S::kStage;
+        int e = expert, kb = q;
+        if (FORM == kF8Concat) { const int r = q / nkb; kb = q - r * nkb; e = (int)routes[1 + 2 * r]; }
+        mbar_arrive_expect_tx(full(s), S::kStage);
+        tma_load_2d(at, &w0_map, kb * 128, e * p.n + f0, full(s));
+        if (GATED) tma_load_2d(at + S::kA, &w1_map, kb * 128, e * p.n + f0, full(s));
+    };
+    const int first = min(S::kStages, q1 - q0);                         // stages filled before anything is waited for
+    if (warp == S::kTmaWarp && lane == 0)
+        for (int k = 0; k < first; k++) load_weights(q0 + k, k);
+    if (early) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     if (nv > 0) {
         if (warp < 4) {
+            if (FORM == kF8Rows) {
+                // ===== rows to codes: half a warp per row and block (the swizzled layout that TMA would have written) =======
+                const int hl = lane & 15, nb = q1 - q0, units = nv * nb;
+                const uint32_t half = 0xffffu << (lane & 16);
+                auto fetch = [&](int u) {
+                    if (u >= units) return make_uint4(0, 0, 0, 0);
+                    const int c = u / nb, k = (q0 + u - c * nb) * 128 + 8 * hl;
+                    const size_t row = p.ids ? (size_t)(tile / p.top_k) : (size_t)(row0 + c);
+                    return k < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + row * p.K + k)) : make_uint4(0, 0, 0, 0);
+                };
+                uint4 next = fetch(tid >> 4);
+                for (int u = tid >> 4; u < units; u += 8) {
+                    const uint4 v = next;
+                    next = fetch(u + 8);
+                    uint2 code;
+                    const float scale = f8_block(v, half, code);
+                    const int c = u / nb, i = u - c * nb;
+                    const uint32_t at = own + (uint32_t)(i * NT * 128 + (c >> 3) * 1024 + (c & 7) * 128) + ((((uint32_t)hl >> 1) ^ (uint32_t)(c & 7)) << 4) + 8u * (hl & 1);
+                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(code.x), "r"(code.y) : "memory");
+                    if (hl == 0) reinterpret_cast<float*>(gen + (own - base) + S::kBlocks * NT * 128)[i * NT + c] = scale;
+                }
+                fence_proxy_async_smem();
+                asm volatile("bar.sync 2, 160;" ::: "memory");          // with the MMA warp
+            }
             // ===== thread = feature, columns = rows ===============================================================
             const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
-            const float* ws0 = p.s0 + ((size_t)expert * nfeat + f0 / 128) * nkb;
-            const float* ws1 = GATED ? p.s1 + ((size_t)expert * nfeat + f0 / 128) * nkb : ws0;
             constexpr int L = (NT + 31) / 32;                           // row scales a lane holds
-            float acc[MATS][NT], x1[L], x2[L], a1 = 0.f, a2 = 0.f, b1 = 0.f, b2 = 0.f;
+            float acc[MATS][COLS], x1[L], x2[L], a1 = 0.f, a2 = 0.f, b1 = 0.f, b2 = 0.f;
 #pragma unroll
             for (int m = 0; m < MATS; m++)
 #pragma unroll
-                for (int c = 0; c < NT; c++) acc[m][c] = 0.f;
-            auto fetch = [&](int kb, float (&x)[L], float& a, float& b) {
-                if (kb >= kb1) return;
+                for (int c = 0; c < COLS; c++) acc[m][c] = 0.f;
+            auto fetch = [&](int q, float (&x)[L], float& a, float& b) {
+                if (q >= q1) return;
+                int kb = q, e = expert;
+                if (FORM == kF8Concat) {
+                    const int r = q / nkb;
+                    kb = q - r * nkb;
+                    e = (int)routes[1 + 2 * r];
+                    const size_t row = (size_t)tile * p.top_k + routes[2 + 2 * r];
+                    x[0] = p.row_scales[(size_t)kb * p.pitch + row] * p.probs[row];
+                } else if (FORM == kF8Rows) {
+                    x[0] = reinterpret_cast<const float*>(gen + (own - base) + S::kBlocks * NT * 128)[(q - q0) * NT + lane % NT];
+                } else {
 #pragma unroll
-                for (int l = 0; l < L; l++) x[l] = p.row_scales[(size_t)kb * p.pitch + min(row0 + 32 * l + (NT < 32 ? lane % NT : lane), p.pitch - 1)];
-                a = ws0[kb];
-                if (GATED) b = ws1[kb];
+                    for (int l = 0; l < L; l++) x[l] = p.row_scales[(size_t)kb * p.pitch + min(row0 + 32 * l + (NT < 32 ? lane % NT : lane), p.pitch - 1)];
+                }
+                const size_t at = ((size_t)e * nfeat + f0 / 128) * nkb + kb;
+                a = p.s0[at];
+                if (GATED) b = p.s1[at];
             };
-            fetch(kb0, x1, a1, b1);
-            fetch(kb0 + 1, x2, a2, b2);
-            for (int kb = kb0, g = 0; kb < kb1; kb++, g++) {
+            fetch(q0, x1, a1, b1);
+            fetch(q0 + 1, x2, a2, b2);
+            for (int q = q0, g = 0; q < q1; q++, g++) {
                 float t[MATS][L];
 #pragma unroll
                 for (int l = 0; l < L; l++) {
@@ -476,9 +558,9 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
                     x1[l] = x2[l];
                 }
                 a1 = a2; b1 = b2;
-                fetch(kb + 2, x2, a2, b2);
+                fetch(q + 2, x2, a2, b2);
                 const int b = g % S::kBufs;
-                if (lane == 0) mbar_wait(tfull(b), (uint32_t)(g / S::kBufs) & 1u, abort_flag, p.status);
+                mbar_wait(tfull(b), (uint32_t)(g / S::kBufs) & 1u, abort_flag, p.status);
                 __syncwarp();
                 tc_fence_after();
                 constexpr int CH = NT < 32 ? NT : 32;                   // columns in registers at a time
@@ -496,9 +578,12 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
                             __syncwarp();
                             if (lane == 0) mbar_arrive(tempty(b));
                         }
+                        if (FORM == kF8Concat) acc[0][0] = fmaf(__uint_as_float(r[0]), t[0][0], acc[0][0]);
+                        else {
 #pragma unroll
-                        for (int c = 0; c < CH; c++)
-                            acc[m][c0 + c] = fmaf(__uint_as_float(r[c]), __shfl_sync(0xffffffffu, t[m][(c0 + c) / 32], (c0 + c) % 32), acc[m][c0 + c]);
+                            for (int c = 0; c < CH; c++)
+                                if (c0 + c < COLS) acc[m][(c0 + c) % COLS] = fmaf(__uint_as_float(r[c]), __shfl_sync(0xffffffffu, t[m][(c0 + c) / 32], (c0 + c) % 32), acc[m][(c0 + c) % COLS]);
+                        }
                     }
             }
             // every MMA and copy of this CTA is done: the parts go where the stages were, [matrix][row][feature]
@@ -506,48 +591,55 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
 #pragma unroll
             for (int m = 0; m < MATS; m++)
 #pragma unroll
-                for (int c = 0; c < NT; c++)
-                    if (c < nv) part[(m * NT + c) * 128 + tid] = acc[m][c];
+                for (int c = 0; c < COLS; c++)
+                    if (c < nv) part[(m * COLS + c) * 128 + tid] = acc[m][c];
         } else if (warp == S::kTmaWarp) {
             if (lane == 0) {
                 int g = 0;
-                for (int kb = kb0; kb < kb1; kb++, g++) {
+                for (int q = q0; q < q1; q++, g++) {
                     const int s = g % S::kStages;
-                    if (!(early && g < first)) {
+                    if (g >= first) {
                         mbar_wait(empty(s), ((uint32_t)(g / S::kStages) & 1u) ^ 1u, abort_flag, p.status);
                         if (*abort_flag) break;
-                        load_weights(kb, s, expert);
+                        load_weights(q, s);
                     }
-                    tma_load_2d(base + (uint32_t)s * S::kStage + MATS * S::kA, &rows_map, kb * 128, row0, full(s));
+                    if (FORM == kF8Tiles) tma_load_2d(base + (uint32_t)s * S::kStage + MATS * S::kA, &rows_map, q * 128, row0, full(s));
+                    if (FORM == kF8Concat) {
+                        const int r = q / nkb;
+                        tma_load_2d(base + (uint32_t)s * S::kStage + S::kA, &rows_map, (q - r * nkb) * 128, tile * p.top_k + (int)routes[2 + 2 * r], full(s));
+                    }
                 }
                 if (*abort_flag)
                     for (int k = max(0, g - S::kStages); k < g; k++) mbar_drain(full(k % S::kStages), (uint32_t)(k / S::kStages) & 1u);
             }
-        } else if (lane == 0) {
-            const uint32_t idesc = umma_idesc_f16(NT);
+        } else {
+            if (FORM == kF8Rows) asm volatile("bar.sync 2, 160;" ::: "memory");
+            const uint32_t idesc = umma_idesc_f16(NT), d0 = __shfl_sync(0xffffffffu, tmem, 0);
             int g = 0;
-            for (int kb = kb0; kb < kb1; kb++, g++) {
+            for (int q = q0; q < q1; q++, g++) {
                 const int s = g % S::kStages, b = g % S::kBufs;
                 mbar_wait(tempty(b), ((uint32_t)(g / S::kBufs) & 1u) ^ 1u, abort_flag, p.status);
                 mbar_wait(full(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, p.status);
-                if (*abort_flag) break;
                 tc_fence_after();
-                const uint32_t at = base + (uint32_t)s * S::kStage;
-                const uint64_t rows = umma_desc(at + MATS * S::kA);
+                if (elect_one()) {
+                    const uint32_t at = base + (uint32_t)s * S::kStage;
+                    const uint64_t rows = umma_desc(FORM == kF8Rows ? own + (uint32_t)(q - q0) * NT * 128 : at + MATS * S::kA);
 #pragma unroll
-                for (int m = 0; m < MATS; m++) {
-                    const uint64_t w = umma_desc(at + m * S::kA);
+                    for (int m = 0; m < MATS; m++) {
+                        const uint64_t w = umma_desc(at + m * S::kA);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) umma_f8f6f4(tmem + (uint32_t)((b * MATS + m) * NT), w + 2u * k, rows + 2u * k, idesc, k ? 1u : 0u);
+                        for (int k = 0; k < 4; k++) umma_f8f6f4(d0 + (uint32_t)((b * MATS + m) * NT), w + 2u * k, rows + 2u * k, idesc, k ? 1u : 0u);
+                    }
+                    umma_commit(empty(s));
+                    umma_commit(tfull(b));
                 }
-                umma_commit(empty(s));
-                umma_commit(tfull(b));
+                __syncwarp();
             }
             if (*abort_flag && g > 0) mbar_drain(tfull((g - 1) % S::kBufs), (uint32_t)((g - 1) / S::kBufs) & 1u);
         }
         __syncwarp();
         if (split > 1) cluster_sync_all(); else __syncthreads();
-        // ===== join: this CTA's share of the rows, thread = feature ===================================================
+        // ===== join: this CTA's share of the rows, thread = feature ================
         if (warp < 4) {
             const uint32_t mine = base + 4u * tid;
             const int f = f0 + tid;
@@ -556,7 +648,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
 #pragma unroll
                 for (int m = 0; m < MATS; m++) {
                     v[m] = 0.f;
-                    for (int q = 0; q < split; q++) v[m] += peer_f32(mine + (uint32_t)(m * NT + c) * 512u, (uint32_t)q);
+                    for (int q = 0; q < split; q++) v[m] += peer_f32(mine + (uint32_t)(m * COLS + c) * 512u, (uint32_t)q);
                 }
                 if (GATED) {
                     const float a = f < p.n ? silu_times(v[0], v[MATS - 1]) : 0.f;
@@ -571,8 +663,13 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED>::kThreads) f8_thin_kernel(co
                     if (f < p.n) p.codes[(size_t)(row0 + c) * p.n + f] = (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
                     if (tid == 0) p.code_scales[(size_t)(f0 / 128) * p.pitch + row0 + c] = scale;
                 } else if (f < p.n) {
-                    const size_t row = p.route_of_row ? p.route_of_row[row0 + c] : (uint32_t)(row0 + c);
-                    p.out[row * p.n + f] = f32_to_bf16_bits(v[0]);
+                    if (FORM == kF8Concat) {
+                        const size_t at = (size_t)tile * p.n + f;
+                        p.out[at] = f32_to_bf16_bits(bf16_bits_to_f32(p.residual[at]) + v[0]);
+                    } else {
+                        const size_t row = p.route_of_row ? p.route_of_row[row0 + c] : (uint32_t)(row0 + c);
+                        p.out[row * p.n + f] = f32_to_bf16_bits(v[0]);
+                    }
                 }
             }
         }
