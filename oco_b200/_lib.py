@@ -140,7 +140,7 @@ SIGNATURES = {
     "oco_moe_router_poll": (C.c_int, [C.c_void_p, C.c_void_p]),
     "oco_moe_router_last_launch_count": (C.c_int, [C.c_void_p]),
     "oco_moe_router_last_error": (C.c_char_p, [C.c_void_p]),
-    "oco_moe_block_norm": (C.c_int, [C.POINTER(BlockNormArgs), C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "oco_moe_block_norm": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
     "oco_moe_f8_plan_create": (C.c_int, [C.POINTER(F8Desc), C.POINTER(C.c_void_p)]),
     "oco_moe_f8_plan_destroy": (None, [C.c_void_p]),
     "oco_moe_f8_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),

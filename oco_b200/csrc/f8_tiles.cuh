@@ -395,6 +395,7 @@ struct F8Thin {
     static_assert(FORM != kF8Concat || !GATED, "");
     static constexpr int kA = 128 * 128, kMats = GATED ? 2 : 1, kB = FORM == kF8Rows ? 0 : NT * 128, kStage = kMats * kA + kB;
     static constexpr int kCols = FORM == kF8Concat ? 1 : NT;            // columns that are rows
+    static constexpr bool kTight = GATED && NT == 64;                   // 128 sums a thread: fewer columns at a time, or one CTA fills an SM's registers
     static constexpr int kBlocks = 16;                                  // kF8Rows: blocks of a CTA's part at most
     static constexpr int kOwn = FORM == kF8Rows ? kBlocks * NT * (128 + 4) : 0;   // their codes, then their scales
     // Shared memory for two CTAs an SM; narrow tiles get by with less, and three or four CTAs hide one another's start and end
@@ -417,7 +418,7 @@ struct F8Thin {
 // or from a kernel that has ended when this one may start, since every kernel of a call lets the next one start only after
 // its own wait. kF8Rows with ids (a router may just have written them) waits first.
 template <int NT, bool GATED, int FORM>
-__global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads) f8_thin_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
+__global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
                                                                                    const __grid_constant__ CUtensorMap w0_map,
                                                                                    const __grid_constant__ CUtensorMap w1_map) {
     using S = F8Thin<NT, GATED, FORM>;
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads) f8_thin_ker
                 mbar_wait(tfull(b), (uint32_t)(g / S::kBufs) & 1u, abort_flag, p.status);
                 __syncwarp();
                 tc_fence_after();
-                constexpr int CH = NT < 32 ? NT : 32;                   // columns in registers at a time
+                constexpr int CH = NT < 32 || S::kTight ? 16 : 32;      // columns in registers at a time
 #pragma unroll
                 for (int m = 0; m < MATS; m++)
 #pragma unroll

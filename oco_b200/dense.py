@@ -32,6 +32,7 @@ class DensePlan:
                 self.handle = C.c_void_p()
             raise OcoError(rc, msg)
         self.workspace = None
+        self.device = -2                  # of the workspace
         self.max_rows = 0
         self._weights = None
 
@@ -46,6 +47,7 @@ class DensePlan:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         self._check(_lib.lib().oco_dense_bind_workspace(self.handle, _ptr(self.workspace), nbytes, max_rows))
         self.max_rows = max_rows
+        self.device = self.workspace.get_device()
 
     def bind(self, up_w, gate_w=None, down_w=None, device="cuda", up_scale=None, gate_scale=None, down_scale=None):
         """Packed rows as they sit in the file: up_w [ffn][hidden], gate_w the same, down_w [hidden][ffn].
@@ -72,9 +74,11 @@ class DensePlan:
     def forward(self, x: torch.Tensor, y: torch.Tensor, rows: int):
         """x: bf16 bit patterns [rows, hidden]; y receives [rows, ffn] (projection) or [rows, hidden]."""
         if self.fmt == synth.FMT_F8_E4M3 and rows > 0:
-            need(x, "x", 2, rows * self.hidden, self.workspace)
-            need(y, "y", 2, rows * (self.ffn if self.kind == PROJECTION else self.hidden), self.workspace)
-        self._check(_lib.lib().oco_dense_forward(self.handle, _ptr(x), _ptr(y), rows, _stream_ptr()))
+            need(x, "x", 2, rows * self.hidden, self.device)
+            need(y, "y", 2, rows * (self.ffn if self.kind == PROJECTION else self.hidden), self.device)
+        rc = _lib.lib().oco_dense_forward(self.handle, x.data_ptr(), y.data_ptr(), rows, _stream_ptr())
+        if rc:
+            self._check(rc)
 
     def poll(self):
         self._check(_lib.lib().oco_dense_poll(self.handle, _stream_ptr()))

@@ -19,6 +19,7 @@ streams; every computation happens inside liboco_moe.so.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import warnings
 from dataclasses import dataclass
 from typing import Optional
@@ -38,7 +39,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream_ptr():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device. (torch.cuda.current_stream() builds an object for it, 3 us a call.)"""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _dev_bytes(a: Optional[np.ndarray], device, misalign: int = 0) -> Optional[torch.Tensor]:
@@ -328,19 +330,16 @@ class Routing:
         return out
 
 
-def need(t: torch.Tensor, name: str, size: int, count: int, like: Optional[torch.Tensor]):
-    """Refuses a tensor that the kernels could not read as `count` contiguous elements of `size` bytes on the plan's device
-    (`like`: the plan's workspace)."""
-    if not t.is_cuda or not t.is_contiguous() or t.element_size() != size or t.numel() < count:
-        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {size} bytes is needed, "
+def need(t: torch.Tensor, name: str, size: int, count: int, device: int):
+    """Refuses a tensor that the kernels could not read as `count` contiguous elements of `size` bytes on the CUDA device
+    of that number."""
+    if t.get_device() != device or t.element_size() != size or not t.is_contiguous() or t.numel() < count:
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {size} bytes on cuda:{device} is needed, "
                                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if like is not None and t.device != like.device:
-        raise OcoError(_lib.INVALID_ARGUMENT, f"{name} is on {t.device}, the plan on {like.device}")
 
 
-def _on_current(t: torch.Tensor, name: str):
-    if t.device.index != torch.cuda.current_device():
-        raise OcoError(_lib.INVALID_ARGUMENT, f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _current_device() -> int:
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
 
 
 def _staged(a, device) -> torch.Tensor:
@@ -374,6 +373,7 @@ class _GroupPlan:
         self._fn = {n: getattr(_lib.lib(), self._prefix + n) for n in ("workspace_bytes", "bind_workspace", "bind_weights", "forward", "poll",
                                                                       "last_error", "last_launch_count")}
         self.workspace, self.max_rows, self._weights = None, 0, None
+        self.device = -2                                                   # of the workspace
         rc = create(C.byref(desc), C.byref(self.handle))
         if rc != _lib.OK:
             raise OcoError(rc, self._fn["last_error"](self.handle).decode())
@@ -388,7 +388,7 @@ class _GroupPlan:
         nbytes = self._fn["workspace_bytes"](self.handle, max_rows)
         ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
         self._check(self._fn["bind_workspace"](self.handle, _ptr(ws), nbytes, max_rows))
-        self.workspace, self.max_rows = ws, max_rows
+        self.workspace, self.max_rows, self.device = ws, max_rows, ws.get_device()
 
     def poll(self):
         self._check(self._fn["poll"](self.handle, _stream_ptr()))
@@ -430,29 +430,34 @@ class RouterPlan(_GroupPlan):
         d = self.desc
         for t, name, count in ((router_w, "router_w", d.experts * d.hidden), (bias, "bias", d.experts)):
             if t is not None:
-                need(t, name, 4, count, self.workspace)
+                need(t, name, 4, count, self.device if self.workspace is not None else _current_device())
         self._check(self._fn["bind_weights"](self.handle, _ptr(router_w), _ptr(bias)))
         self._weights = (router_w, bias)
 
     def forward(self, x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int, logits: Optional[torch.Tensor] = None):
         """x bf16 [rows, hidden] -> ids (32-bit) and probs f32 [rows, active], and the logits f32 [rows, experts] if asked for."""
-        d = self.desc
-        need(x, "x", 2, rows * d.hidden, self.workspace)
-        need(ids, "ids", 4, rows * d.top_k, self.workspace)
-        need(probs, "probs", 4, rows * d.top_k, self.workspace)
+        d, dev = self.desc, self.device
+        k = rows * d.top_k
+        need(x, "x", 2, rows * d.hidden, dev)
+        need(ids, "ids", 4, k, dev)
+        need(probs, "probs", 4, k, dev)
         if logits is not None:
-            need(logits, "logits", 4, rows * d.experts, self.workspace)
-        self._check(self._fn["forward"](self.handle, x.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(),
-                                        logits.data_ptr() if logits is not None else None, _stream_ptr()))
+            need(logits, "logits", 4, rows * d.experts, dev)
+            logits = logits.data_ptr()
+        rc = self._fn["forward"](self.handle, x.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), logits, _stream_ptr())
+        if rc:
+            self._check(rc)
 
     def select(self, logits: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int):
         """The selection alone, from logits f32 [rows, experts] of any origin."""
-        d = self.desc
-        need(logits, "logits", 4, rows * d.experts, self.workspace)
-        _on_current(logits, "logits")
-        need(ids, "ids", 4, rows * d.top_k, logits)
-        need(probs, "probs", 4, rows * d.top_k, logits)
-        self._check(_lib.lib().oco_moe_router_select(self.handle, logits.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), _stream_ptr()))
+        d, dev = self.desc, _current_device()
+        k = rows * d.top_k
+        need(logits, "logits", 4, rows * d.experts, dev)
+        need(ids, "ids", 4, k, dev)
+        need(probs, "probs", 4, k, dev)
+        rc = _lib.lib().oco_moe_router_select(self.handle, logits.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), _stream_ptr())
+        if rc:
+            self._check(rc)
 
 
 @dataclass
@@ -489,17 +494,20 @@ class F8ExpertPlan(_GroupPlan):
     def forward(self, x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, residual: torch.Tensor, rows: int,
                 out: Optional[torch.Tensor] = None):
         """out = residual + the weighted expert outputs (bf16 rows; out None: in place). Ids outside 0 .. experts - 1 are left out."""
-        d = self.desc
+        d, dev = self.desc, self.device
         out = residual if out is None else out
-        need(x, "x", 2, rows * d.hidden, self.workspace)
-        need(ids, "ids", 4, rows * d.top_k, self.workspace)
-        need(probs, "probs", 4, rows * d.top_k, self.workspace)
-        need(residual, "residual", 2, rows * d.hidden, self.workspace)
-        need(out, "out", 2, rows * d.hidden, self.workspace)
-        self._check(self._fn["forward"](self.handle, x.data_ptr(), ids.data_ptr(), probs.data_ptr(), residual.data_ptr(), out.data_ptr(), rows,
-                                        _stream_ptr()))
+        n, k = rows * d.hidden, rows * d.top_k
+        need(x, "x", 2, n, dev)
+        need(ids, "ids", 4, k, dev)
+        need(probs, "probs", 4, k, dev)
+        need(residual, "residual", 2, n, dev)
+        need(out, "out", 2, n, dev)
+        rc = self._fn["forward"](self.handle, x.data_ptr(), ids.data_ptr(), probs.data_ptr(), residual.data_ptr(), out.data_ptr(), rows, _stream_ptr())
+        if rc:
+            self._check(rc)
 
 
+_NORM_ARGS = struct.Struct("@6i4f9P5q")     # oco_moe_block_norm_args
 NORMS = {"rms": 0, "layer": 1}
 GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
 
@@ -515,43 +523,54 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
     def refuse(text):
         raise OcoError(_lib.INVALID_ARGUMENT, text)
 
-    if hidden.dim() != 2 or not hidden.is_cuda or hidden.dtype not in (torch.bfloat16, torch.float32):
+    dev = hidden.get_device()
+    wide = hidden.dtype is torch.float32
+    if hidden.dim() != 2 or dev < 0 or not (wide or hidden.dtype is torch.bfloat16):
         refuse("hidden: CUDA rows [rows, width], bf16 or f32")
-    _on_current(hidden, "hidden")
-    rows, width = hidden.shape
+    if dev != _current_device():
+        refuse(f"hidden is on {hidden.device}, the current device is cuda:{_current_device()}")
+    rows, width = shape = hidden.shape
     if kind not in NORMS or gate_act not in GATE_ACTS:
         refuse(f"kind is one of {sorted(NORMS)}, gate_act one of {sorted(GATE_ACTS)}")
-    a = _lib.BlockNormArgs(width=width, kind=NORMS[kind], wide=int(hidden.dtype == torch.float32), gate_act=GATE_ACTS[gate_act], epsilon=epsilon,
-                           weight_offset=weight_offset, residual_scale=residual_scale, block_scale=block_scale)
-    for t, name, dtype in ((hidden, "hidden", hidden.dtype), (block, "block", torch.bfloat16), (hidden_out, "hidden_out", hidden.dtype),
-                           (norm_out, "norm_out", torch.bfloat16)):
+
+    def rows_of(t, name, dtype):
         if t is None:
-            continue
-        if t.shape != hidden.shape or t.dtype != dtype or t.device != hidden.device or t.stride(1) != 1:
-            refuse(f"{name}: rows {tuple(hidden.shape)} of {dtype} on {hidden.device} with unit stride inside a row are needed")
-        setattr(a, name, t.data_ptr())
-        if rows > 1:
-            setattr(a, name + "_stride", t.stride(0))
-    for t, name in ((pre_weight, "pre_w"), (pre_bias, "pre_b"), (post_weight, "post_w"), (post_bias, "post_b")):
-        if t is not None:
-            need(t, name, 4, width, hidden)
-            setattr(a, name, t.data_ptr())
+            return 0, 0
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or t.stride(1) != 1:
+            refuse(f"{name}: rows {tuple(shape)} of {dtype} on {hidden.device} with unit stride inside a row are needed")
+        return t.data_ptr(), t.stride(0) if rows > 1 else 0
+
+    def vector(t, name):
+        if t is None:
+            return 0
+        need(t, name, 4, width, dev)
+        return t.data_ptr()
+
+    h, hs = rows_of(hidden, "hidden", hidden.dtype)
+    b, bs = rows_of(block, "block", torch.bfloat16)
+    ho, hos = rows_of(hidden_out, "hidden_out", hidden.dtype)
+    no, nos = rows_of(norm_out, "norm_out", torch.bfloat16)
+    g = gs = gate_type = per = 0
     if gate is not None:
-        if gate.dtype not in (torch.bfloat16, torch.float32) or gate.device != hidden.device or gate.shape[-1] != width or gate.stride(-1) != 1 or gate.dim() > 2:
+        if gate.dim() not in (1, 2) or gate.dtype not in (torch.bfloat16, torch.float32) or gate.get_device() != dev or gate.shape[-1] != width or gate.stride(-1) != 1:
             refuse("gate: [width] or [gates, width], bf16 or f32, unit stride inside a row")
-        a.gate, a.gate_type = gate.data_ptr(), 2 if gate.dtype == torch.float32 else 1
+        g, gate_type = gate.data_ptr(), 2 if gate.dtype is torch.float32 else 1
         if gate.dim() == 2:
             gates = gate.shape[0]
-            a.gate_rows = gate_rows if gate_rows is not None else (rows // gates if gates and rows % gates == 0 else 0)
-            if rows and (a.gate_rows < 1 or (rows - 1) // a.gate_rows >= gates):
+            per = gate_rows if gate_rows is not None else (rows // gates if gates and rows % gates == 0 else 0)
+            if rows and (per < 1 or (rows - 1) // per >= gates):
                 refuse("gate: fewer gate rows than the rows need")
-            if gates > 1:
-                a.gate_stride = gate.stride(0)
+            gs = gate.stride(0) if gates > 1 else 0
+    args = _NORM_ARGS.pack(width, NORMS[kind], wide, gate_type, per, GATE_ACTS[gate_act], epsilon, weight_offset, residual_scale, block_scale,
+                           h, b, vector(post_weight, "post_weight"), vector(post_bias, "post_bias"), vector(pre_weight, "pre_weight"),
+                           vector(pre_bias, "pre_bias"), g, ho, no, hs, bs, gs, hos, nos)
     if rows == 0:      # an empty tensor has no address
         return
-    err = C.create_string_buffer(160)
-    rc = _lib.lib().oco_moe_block_norm(C.byref(a), rows, _stream_ptr(), err, len(err))
-    if rc != _lib.OK:
+    rc = _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(), None, 0)
+    if rc:
+        err = C.create_string_buffer(160)
+        if rc in (_lib.INVALID_ARGUMENT, _lib.UNSUPPORTED_SHAPE):      # refused before anything ran: asked again for the reason
+            _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(), err, len(err))
         raise OcoError(rc, err.value.decode())
 
 
