@@ -396,11 +396,11 @@ struct F8Thin {
     static constexpr int kA = 128 * 128, kMats = GATED ? 2 : 1, kB = FORM == kF8Rows ? 0 : NT * 128, kStage = kMats * kA + kB;
     static constexpr int kCols = FORM == kF8Concat ? 1 : NT;            // columns that are rows
     static constexpr bool kTight = GATED && NT == 64;                   // 128 sums a thread: fewer columns at a time, or one CTA fills an SM's registers
-    static constexpr int kBlocks = 16;                                  // kF8Rows: blocks of a CTA's part at most
+    static constexpr int kBlocks = 8;                                   // kF8Rows: blocks of a CTA's part at most
     static constexpr int kOwn = FORM == kF8Rows ? kBlocks * NT * (128 + 4) : 0;   // their codes, then their scales
     // Shared memory for two CTAs an SM; narrow tiles get by with less, and three or four CTAs hide one another's start and end
     // (64 tokens over 128 experts: 138 -> KSPEED us).
-    static constexpr int kRoom = (NT == 16 ? (GATED ? 70 : 54) : 108) * 1024;
+    static constexpr int kRoom = (NT == 16 && FORM == kF8Tiles ? (GATED ? 70 : 54) : 108) * 1024;
     static constexpr int kStages = (kRoom - kOwn) / kStage > 2 ? (kRoom - kOwn) / kStage : 2;
     static constexpr int kBufs = 2, kTmemUsed = kBufs * kMats * NT;
     static constexpr int kTmem = kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : 256;
@@ -435,8 +435,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
     auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + S::kBufs + b); };
     uint32_t* slot = reinterpret_cast<uint32_t*>(gctrl + 8 * (2 * S::kStages + 2 * S::kBufs));
     volatile uint32_t* abort_flag = slot + 1;
-    uint32_t* tops = reinterpret_cast<uint32_t*>(gctrl + 256);          // [2][4]
-    volatile uint32_t* routes = reinterpret_cast<uint32_t*>(gctrl + 320);   // kF8Concat: how many, then (expert, route) of each
+    volatile uint32_t* routes = reinterpret_cast<uint32_t*>(gctrl + 256);   // kF8Concat: how many, then (expert, route) of each
     const int split = (int)cluster_size(), rank = (int)cluster_rank();
     const int nfeat = (p.n + 127) / 128, nkb = (p.K + 127) / 128;
     const int item = (int)blockIdx.x / split, tile = item / nfeat, f0 = (item - tile * nfeat) * 128;
@@ -640,38 +639,42 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
         }
         __syncwarp();
         if (split > 1) cluster_sync_all(); else __syncthreads();
-        // ===== join: this CTA's share of the rows, thread = feature ================
-        if (warp < 4) {
-            const uint32_t mine = base + 4u * tid;
-            const int f = f0 + tid;
-            for (int c = rank; c < nv; c += split) {
-                float v[MATS];
+        // ===== join: this CTA's share of the rows, a warp per row, four features a lane ================================
+        const int f = f0 + 4 * lane;
+        for (int c = rank + split * warp; c < nv; c += split * (S::kThreads / 32)) {
+            float4 v[MATS];
 #pragma unroll
-                for (int m = 0; m < MATS; m++) {
-                    v[m] = 0.f;
-                    for (int q = 0; q < split; q++) v[m] += peer_f32(mine + (uint32_t)(m * COLS + c) * 512u, (uint32_t)q);
+            for (int m = 0; m < MATS; m++) {
+                const uint32_t at = base + (uint32_t)(m * COLS + c) * 512u + 16u * lane;
+                v[m] = peer_f32x4(at, 0);
+#pragma unroll 4
+                for (int q = 1; q < split; q++) {
+                    const float4 w = peer_f32x4(at, (uint32_t)q);
+                    v[m].x += w.x; v[m].y += w.y; v[m].z += w.z; v[m].w += w.w;
                 }
-                if (GATED) {
-                    const float a = f < p.n ? silu_times(v[0], v[MATS - 1]) : 0.f;
-                    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(a)));
-                    uint32_t* t = tops + ((c / split) & 1) * 4;
-                    if (lane == 0) t[warp] = top;
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    top = max(max(t[0], t[1]), max(t[2], t[3]));
-                    float scale, lift, factor;
-                    f8_act_scale(__uint_as_float(top), scale, lift, factor);
-                    const float q = a * lift * factor;
-                    if (f < p.n) p.codes[(size_t)(row0 + c) * p.n + f] = (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-                    if (tid == 0) p.code_scales[(size_t)(f0 / 128) * p.pitch + row0 + c] = scale;
-                } else if (f < p.n) {
-                    if (FORM == kF8Concat) {
-                        const size_t at = (size_t)tile * p.n + f;
-                        p.out[at] = f32_to_bf16_bits(bf16_bits_to_f32(p.residual[at]) + v[0]);
-                    } else {
-                        const size_t row = p.route_of_row ? p.route_of_row[row0 + c] : (uint32_t)(row0 + c);
-                        p.out[row * p.n + f] = f32_to_bf16_bits(v[0]);
-                    }
+            }
+            if (GATED) {
+                const bool in = f < p.n;                                // n is a multiple of 32
+                const float4 u = v[MATS - 1];
+                const float a[4] = {in ? silu_times(v[0].x, u.x) : 0.f, in ? silu_times(v[0].y, u.y) : 0.f, in ? silu_times(v[0].z, u.z) : 0.f,
+                                    in ? silu_times(v[0].w, u.w) : 0.f};
+                const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(fabsf(a[0])), __float_as_uint(fabsf(a[1]))),
+                                                                        max(__float_as_uint(fabsf(a[2])), __float_as_uint(fabsf(a[3])))));
+                float scale, lift, factor;
+                f8_act_scale(__uint_as_float(top), scale, lift, factor);
+                if (in) *reinterpret_cast<uint32_t*>(p.codes + (size_t)(row0 + c) * p.n + f) =
+                    f8x4(a[0] * lift * factor, a[1] * lift * factor, a[2] * lift * factor, a[3] * lift * factor);
+                if (lane == 0) p.code_scales[(size_t)(f0 / 128) * p.pitch + row0 + c] = scale;
+            } else if (f < p.n) {
+                size_t row = FORM == kF8Concat ? (size_t)tile : (size_t)(row0 + c);
+                if (FORM == kF8Tiles && p.route_of_row) row = p.route_of_row[row0 + c];
+                if (FORM == kF8Concat) {
+                    const uint2 q = *reinterpret_cast<const uint2*>(p.residual + row * p.n + f);
+                    v[0].x += __uint_as_float(q.x << 16); v[0].y += __uint_as_float(q.x & 0xffff0000u);
+                    v[0].z += __uint_as_float(q.y << 16); v[0].w += __uint_as_float(q.y & 0xffff0000u);
                 }
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0].x, v[0].y), hi = __floats2bfloat162_rn(v[0].z, v[0].w);
+                *reinterpret_cast<uint2*>(p.out + row * p.n + f) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
             }
         }
         if (split > 1) cluster_sync_all();                                   // nobody leaves while its parts are read
