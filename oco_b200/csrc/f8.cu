@@ -14,8 +14,10 @@ namespace {
 // of as many rows, the pair's two of 128.
 constexpr int kTileRows[5] = {16, 32, 64, 128, 256}, kRowBoxes[4] = {16, 32, 64, 128};
 constexpr int kWideIndex = 3, kPairIndex = 4;
-// Tokens of a routed call up to which every route is a tile of its own.
-constexpr int kOwnTokens = 1;
+// Rows up to which a dense product rounds them itself (one launch less; 4096 -> 6144 features, 1 / 4 / 8 / 16 rows: 7.1 / 8.8 /
+// 11.5 / 17.1 us against 10.2 / 9.6 / 9.5 / 9.9), and tokens of a routed call up to which every route is a tile of its own (two
+// launches instead of five; eight of 128 experts, 2 / 3 / 4 tokens: 23.5 / 26.8 / 36.9 us against 28.6 / 32.5 / 37.2).
+constexpr int kOwnRows = 4, kOwnTokens = 3;
 enum F8Kind { kF8Projection = OCO_DENSE_PROJECTION, kF8Gated = OCO_DENSE_FFN_SILU_GATE, kF8Experts = 100 };
 
 struct F8Space {
@@ -176,7 +178,7 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     // the second product sums a token's routes). Both read an expert once per route.
     const int own_tiles = routed ? R : (rows + 15) / 16, nkb = (H + 127) / 128;
     const unsigned own_split = thin_split(plan, (long long)own_tiles * ((F + 127) / 128), nkb);
-    if (rows <= (routed ? kOwnTokens : 16) && (nkb + (int)own_split - 1) / (int)own_split <= F8Thin<16, true, kF8Rows>::kBlocks) {
+    if (rows <= (routed ? kOwnTokens : kOwnRows) && (nkb + (int)own_split - 1) / (int)own_split <= F8Thin<16, true, kF8Rows>::kBlocks) {
         p.x = x; p.ids = ids;
         if (plan->kind == kF8Projection) {
             p.s0 = plan->w.up_s; p.out = out;
@@ -196,7 +198,8 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     const int tiles = routed ? R / nt + std::min(E, R) : (R + nt - 1) / nt, expected = routed ? std::max(std::min(E, R), R / nt) : tiles;
     if (routed) {
         F8PlanParams pp{ids, ws.offsets, ws.route_of_row, ws.row_of_route, ws.tiles, ws.tile_count, R, E, nt};
-        OCO_CK(plan, launch_dependent(f8_plan_kernel, dim3(1), dim3(1024), 0, st, pp));
+        const unsigned ctas = R > 4096 ? 8 : 1;                            // 24576 routes: 28 us on one CTA, 6 on a cluster of eight
+        OCO_CK(plan, launch_dependent_clusters(f8_plan_kernel, ctas, dim3(ctas), dim3(1024), 0, st, pp));
         plan->launches++;
     }
     const unsigned row_ctas = (unsigned)std::min<long long>(((long long)rows * ((H + 255) / 256) + 15) / 16, 8LL * plan->sm_count);

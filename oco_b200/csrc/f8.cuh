@@ -3,7 +3,7 @@
 #pragma once
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "cluster.cuh"
 
 namespace oco {
 
@@ -21,8 +21,9 @@ __device__ __forceinline__ float f8_value(uint8_t c) {
 }
 
 // ---- expert-sorted order of the routes ----------------------------------------------------------------------------
-// One CTA: counts the routes of each expert, then gives every route its row. The order inside an expert follows the
-// atomics and may differ from call to call; rows are independent and leave through their route, so no result does.
+// One cluster of CTAs: each counts the routes of each expert in its share of the ids, all add up the counts of all, then
+// every route gets its row. The order inside an expert follows the atomics and may differ from call to call; rows are
+// independent and leave through their route, so no result does.
 struct F8PlanParams {
     const uint32_t* ids;      // [R]; outside 0 .. E-1: no route of this plan
     uint32_t* offsets;        // [E + 1]
@@ -33,19 +34,28 @@ struct F8PlanParams {
     int R, E, tile_rows;
 };
 __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
-    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
     pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();
     __shared__ uint32_t count[kF8MaxExperts], next[kF8MaxExperts], warp_rows[32], warp_tiles[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+    const int per = (p.R + ctas - 1) / ctas, i0 = min(p.R, rank * per), i1 = min(p.R, i0 + per);
     if (tid < kF8MaxExperts) count[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < p.R; i += 1024) {
+    for (int i = i0 + tid; i < i1; i += 1024) {
         const uint32_t e = p.ids[i];
         if (e < (uint32_t)p.E) atomicAdd(&count[e], 1u);
     }
-    __syncthreads();
-    // exclusive scans of rows and tiles over the experts (thread e: expert e)
-    const uint32_t c = tid < p.E ? count[tid] : 0u, nt = (c + p.tile_rows - 1) / p.tile_rows;
+    cluster_sync_all();
+    // thread e: the routes of expert e, and those in the shares before this one; exclusive scans of rows and tiles
+    uint32_t c = 0, before = 0;
+    if (tid < p.E)
+        for (int q = 0; q < ctas; q++) {
+            const uint32_t n = __float_as_uint(peer_f32(smem_u32(&count[tid]), (uint32_t)q));
+            if (q < rank) before += n;
+            c += n;
+        }
+    const uint32_t nt = (c + p.tile_rows - 1) / p.tile_rows;
     uint32_t sc = c, st = nt;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -55,15 +65,15 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
     if (lane == 31) { warp_rows[warp] = sc; warp_tiles[warp] = st; }
     __syncthreads();
     uint32_t r0 = sc - c, t0 = st - nt;
-    for (int w = 0; w < warp; w++) { r0 += warp_rows[w]; t0 += warp_tiles[w]; }
+    for (int w = 0; w < min(warp, (kF8MaxExperts + 31) / 32); w++) { r0 += warp_rows[w]; t0 += warp_tiles[w]; }
     if (tid < p.E) {
-        next[tid] = r0;
-        p.offsets[tid] = r0;
-        for (uint32_t t = 0; t < nt; t++) { p.tiles[2 * (t0 + t)] = tid; p.tiles[2 * (t0 + t) + 1] = r0 + t * p.tile_rows; }
-        if (tid == p.E - 1) { p.offsets[p.E] = r0 + c; *p.tile_count = t0 + nt; }
+        next[tid] = r0 + before;
+        if (rank == 0) p.offsets[tid] = r0;
+        for (uint32_t t = rank; t < nt; t += ctas) { p.tiles[2 * (t0 + t)] = tid; p.tiles[2 * (t0 + t) + 1] = r0 + t * p.tile_rows; }
+        if (rank == 0 && tid == p.E - 1) { p.offsets[p.E] = r0 + c; *p.tile_count = t0 + nt; }
     }
     __syncthreads();
-    for (int i = tid; i < p.R; i += 1024) {
+    for (int i = i0 + tid; i < i1; i += 1024) {
         const uint32_t e = p.ids[i];
         uint32_t row = 0xffffffffu;
         if (e < (uint32_t)p.E) {
@@ -72,6 +82,7 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
         }
         p.row_of_route[i] = row;
     }
+    cluster_sync_all();        // nobody leaves while its counts are read
 }
 
 // ---- rows to codes ------------------------------------------------------------------------------------------------
