@@ -258,7 +258,9 @@ extern "C" int oco_moe_block_norm(const oco_moe_block_norm_args* a, int rows, vo
     else if (pieces <= 64) e = launch<32, 2>(p, layer, wide, st);
     else if (pieces <= 128) e = launch<128, 1>(p, layer, wide, st);
     else if (pieces <= 256) e = launch<256, 1>(p, layer, wide, st);
+    else if (pieces <= 384) e = launch<192, 2>(p, layer, wide, st);
     else if (pieces <= 512) e = launch<256, 2>(p, layer, wide, st);
+    else if (pieces <= 768) e = launch<384, 2>(p, layer, wide, st);
     else if (pieces <= 1024) e = launch<512, 2>(p, layer, wide, st);
     else if (pieces <= 2048) e = launch<1024, 2>(p, layer, wide, st);
     else e = launch<1024, 4>(p, layer, wide, st);
