@@ -273,6 +273,8 @@ int f8_dense_forward(oco_moe_f8_plan* plan, const uint16_t* x, uint16_t* y, int 
     if (rows == 0) return OCO_OK;
     if (!x || !y) return plan->fail(OCO_INVALID_ARGUMENT, "null x or y");
     if (((uintptr_t)x | (uintptr_t)y) & 15u) return plan->fail(OCO_INVALID_ARGUMENT, "x and y must be 16-byte aligned");
+    const uintptr_t xe = (uintptr_t)x + (size_t)rows * plan->d.hidden * 2, ye = (uintptr_t)y + (size_t)rows * plan->d.ffn * 2;
+    if (plan->kind == kF8Projection && (uintptr_t)x < ye && (uintptr_t)y < xe) return plan->fail(OCO_INVALID_ARGUMENT, "y must not overlap x");
     return run_rows(plan, x, nullptr, nullptr, nullptr, y, rows, (cudaStream_t)cuda_stream);
 }
 
@@ -304,6 +306,7 @@ int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t byt
     if ((uintptr_t)workspace & 255u) return plan->fail(OCO_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
     const F8Space ws = carve(plan->kind, plan->d, max_rows, (unsigned char*)workspace);
     if (bytes < ws.total) return plan->fail(OCO_INVALID_ARGUMENT, "workspace too small: %zu < %zu", bytes, ws.total);
+    OCO_CK(plan, cudaDeviceSynchronize());     // whoever had this memory before is done with it
     OCO_CK(plan, cudaMemset(ws.status, 0, 256));
     OCO_CK(plan, cudaDeviceSynchronize());
     if (int rc = plan->note_device()) return rc;

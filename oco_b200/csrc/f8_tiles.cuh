@@ -399,7 +399,7 @@ struct F8Thin {
     static constexpr int kBlocks = 8;                                   // kF8Rows: blocks of a CTA's part at most
     static constexpr int kOwn = FORM == kF8Rows ? kBlocks * NT * (128 + 4) : 0;   // their codes, then their scales
     // Shared memory for two CTAs an SM; narrow tiles get by with less, and three or four CTAs hide one another's start and end
-    // (64 tokens over 128 experts: 138 -> KSPEED us).
+    // (64 tokens over 128 experts: 136 -> 114 us).
     static constexpr int kRoom = (NT == 16 && FORM == kF8Tiles ? (GATED ? 70 : 54) : 108) * 1024;
     static constexpr int kStages = (kRoom - kOwn) / kStage > 2 ? (kRoom - kOwn) / kStage : 2;
     static constexpr int kBufs = 2, kTmemUsed = kBufs * kMats * NT;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
         fence_barrier_init();
     }
     if (FORM == kF8Concat && warp == 0) {                               // the token's routes that have an expert here
-        const uint32_t e = lane < p.top_k ? p.ids[(size_t)tile * p.top_k + lane] : 0xffffffffu;
+        const uint32_t e = lane < p.top_k ? __ldcg(p.ids + (size_t)tile * p.top_k + lane) : 0xffffffffu;
         const uint32_t live = __ballot_sync(0xffffffffu, e < (uint32_t)p.experts);
         const int at = __popc(live & ((1u << lane) - 1u));
         if ((live >> lane) & 1u) { routes[1 + 2 * at] = e; routes[2 + 2 * at] = lane; }
@@ -461,11 +461,11 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
     int expert = 0, row0 = tile * NT, nv = min(NT, p.rows - row0);
     const bool early = FORM != kF8Rows || !p.ids;
     if (FORM == kF8Tiles && p.tiles) {
-        if (tile >= (int)*p.tile_count) nv = 0;                         // the whole cluster
+        if (tile >= (int)__ldcg(p.tile_count)) nv = 0;                  // the whole cluster (read past L1: not waited for yet)
         else {
-            expert = (int)p.tiles[2 * tile];
-            row0 = (int)p.tiles[2 * tile + 1];
-            nv = min(NT, (int)p.offsets[expert + 1] - row0);
+            expert = (int)__ldcg(p.tiles + 2 * tile);
+            row0 = (int)__ldcg(p.tiles + 2 * tile + 1);
+            nv = min(NT, (int)__ldcg(p.offsets + expert + 1) - row0);
         }
     }
     if (FORM == kF8Concat) nv = 1;

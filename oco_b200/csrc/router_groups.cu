@@ -13,6 +13,7 @@ struct oco_moe_router : PlanBase {
     const float* w = nullptr;
     const float* bias = nullptr;
     uint32_t* status = nullptr;
+    uint32_t* arrivals = nullptr;     // route_rows_kernel's counters, left at zero by every call
     float* logits = nullptr;
     uint16_t* pieces = nullptr;       // the weights as three bf16 pieces [3][experts rounded up to 128][hidden]
     CUtensorMap map_w;
@@ -42,6 +43,7 @@ int lay_out(oco_moe_router* r) {
     if (!r->have_ws || !r->have_w || !d.hidden) return OCO_OK;
     if (int rc = r->check_device()) return rc;
     const int Ep = padded(d.experts);
+    OCO_CK(r, cudaDeviceSynchronize());     // the weights have been written, on whatever stream
     router_pieces_kernel<<<4 * r->sm_count, 256>>>(r->w, r->pieces, d.experts, Ep, d.hidden);
     OCO_CK(r, cudaGetLastError());
     OCO_CK(r, cudaDeviceSynchronize());
@@ -51,44 +53,23 @@ int lay_out(oco_moe_router* r) {
     return OCO_OK;
 }
 
-// Rows up to which the logits are made by router_rows_kernel, above by router_tile_kernel.
+// Rows up to which one kernel makes the logits and selects (route_rows_kernel); above, the tensor cores make the logits
+// (256 experts, 4096 columns, 16 / 17 rows: KROWS us a pass).
 constexpr int kRowsMax = 16;
 
-// logits[t][e] = sum_k x[t][k] w[e][k]: a warp per expert and four tokens, f32.
-__global__ void __launch_bounds__(256) router_rows_kernel(const uint16_t* __restrict__ x, const float* __restrict__ w, float* __restrict__ logits,
-                                                          int rows, int E, int H) {
-    pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
-    pdl_wait();                // the kernel before has completed and its writes are visible
-    const int e = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t0 = blockIdx.x * 4;
-    if (e >= E) return;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = lane * 4; k < H; k += 128) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(w + (size_t)e * H + k));
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint2 q = *reinterpret_cast<const uint2*>(x + (size_t)min(t0 + t, rows - 1) * H + k);
-            acc[t] = fmaf(v.x, __uint_as_float(q.x << 16), acc[t]);
-            acc[t] = fmaf(v.y, __uint_as_float(q.x & 0xffff0000u), acc[t]);
-            acc[t] = fmaf(v.z, __uint_as_float(q.y << 16), acc[t]);
-            acc[t] = fmaf(v.w, __uint_as_float(q.y & 0xffff0000u), acc[t]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const float s = warp_sum_f(acc[t]);
-        if (lane == 0 && t0 + t < rows) logits[(size_t)(t0 + t) * E + e] = s;
-    }
-}
-
-int launch_select(oco_moe_router* r, const SelectParams& p, cudaStream_t st) {
-    const dim3 grid((p.rows + 7) / 8), block(256);
+// The selection; fused: with the product before it, for few rows.
+int launch_select(oco_moe_router* r, const SelectParams& p, bool fused, cudaStream_t st) {
     const int per_lane = (p.E + 31) / 32;
+    const dim3 grid = fused ? dim3((p.rows + 3) / 4, (p.E + 7) / 8) : dim3((p.rows + 7) / 8), block(256);
+    auto launch = [&](auto select, auto route) {
+        return fused ? launch_dependent(route, grid, block, 0, st, p, const_cast<float*>(p.logits), r->arrivals) : launch_dependent(select, grid, block, 0, st, p);
+    };
     cudaError_t e;
-    if (per_lane <= 1) e = launch_dependent(select_kernel<1>, grid, block, 0, st, p);
-    else if (per_lane <= 2) e = launch_dependent(select_kernel<2>, grid, block, 0, st, p);
-    else if (per_lane <= 4) e = launch_dependent(select_kernel<4>, grid, block, 0, st, p);
-    else if (per_lane <= 8) e = launch_dependent(select_kernel<8>, grid, block, 0, st, p);
-    else e = launch_dependent(select_kernel<16>, grid, block, 0, st, p);
+    if (per_lane <= 1) e = launch(select_kernel<1>, route_rows_kernel<1>);
+    else if (per_lane <= 2) e = launch(select_kernel<2>, route_rows_kernel<2>);
+    else if (per_lane <= 4) e = launch(select_kernel<4>, route_rows_kernel<4>);
+    else if (per_lane <= 8) e = launch(select_kernel<8>, route_rows_kernel<8>);
+    else e = launch(select_kernel<16>, route_rows_kernel<16>);
     if (e != cudaSuccess) return r->fail(OCO_CUDA_ERROR, "select: %s", cudaGetErrorString(e));
     r->launches++;
     return OCO_OK;
@@ -135,11 +116,13 @@ int oco_moe_router_bind_workspace(oco_moe_router* r, void* workspace, size_t byt
     if ((uintptr_t)workspace & 255u) return r->fail(OCO_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
     const RouterSpace s = carve(r->d, max_rows);
     if (bytes < s.total) return r->fail(OCO_INVALID_ARGUMENT, "workspace too small: %zu < %zu", bytes, s.total);
+    OCO_CK(r, cudaDeviceSynchronize());     // whoever had this memory before is done with it
     OCO_CK(r, cudaMemset(workspace, 0, 256));
     OCO_CK(r, cudaDeviceSynchronize());
     if (int rc = r->note_device()) return rc;
     unsigned char* base = (unsigned char*)workspace;
     r->status = (uint32_t*)(base + s.status);
+    r->arrivals = r->status + 16;
     r->logits = (float*)(base + s.logits);
     r->pieces = (uint16_t*)(base + s.pieces);
     r->max_rows = max_rows;
@@ -170,9 +153,9 @@ int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint3
     cudaStream_t st = (cudaStream_t)cuda_stream;
     float* lg = logits ? logits : r->logits;
     const oco_moe_router_desc& d = r->d;
-    if (rows <= kRowsMax) {
-        OCO_CK(r, launch_dependent(router_rows_kernel, dim3((rows + 3) / 4, (d.experts + 7) / 8), dim3(256), 0, st, x, r->w, lg, rows, d.experts, d.hidden));
-    } else {
+    SelectParams p = select_params(r, lg, rows, ids, probs);
+    p.x = x; p.w = r->w; p.status = r->status;
+    if (rows > kRowsMax) {
         CUtensorMap map_x;
         const CUresult e = encode_rows(&map_x, (void*)x, (uint64_t)rows, (uint64_t)d.hidden, 2, 128);
         if (e != CUDA_SUCCESS) return r->fail(OCO_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)e);
@@ -182,11 +165,9 @@ int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint3
         while (split < 8 && items * (int)split * 2 <= r->sm_count && chunks >= 8 * (int)split) split *= 2;
         OCO_CK(r, launch_dependent_clusters(router_tile_kernel, split, dim3((unsigned)items * split), dim3(RouterTile::kThreads), RouterTile::kSmem, st, map_x, r->map_w,
                                             lg, rows, d.experts, Ep, d.hidden, r->status));
+        r->launches++;
     }
-    r->launches++;
-    SelectParams p = select_params(r, lg, rows, ids, probs);
-    p.x = x; p.w = r->w; p.status = r->status;
-    return launch_select(r, p, st);
+    return launch_select(r, p, rows <= kRowsMax, st);
 }
 
 int oco_moe_router_select(oco_moe_router* r, const float* logits, int rows, uint32_t* ids, float* probs, void* cuda_stream) {
@@ -197,7 +178,7 @@ int oco_moe_router_select(oco_moe_router* r, const float* logits, int rows, uint
     if (rows == 0) return OCO_OK;
     if (!logits || !ids || !probs) return r->fail(OCO_INVALID_ARGUMENT, "null logits, ids or probs");
     if (((uintptr_t)logits | (uintptr_t)ids | (uintptr_t)probs) & 3u) return r->fail(OCO_INVALID_ARGUMENT, "logits, ids and probs must be 4-byte aligned");
-    return launch_select(r, select_params(r, logits, rows, ids, probs), (cudaStream_t)cuda_stream);
+    return launch_select(r, select_params(r, logits, rows, ids, probs), false, (cudaStream_t)cuda_stream);
 }
 
 int oco_moe_router_poll(oco_moe_router* r, void* cuda_stream) {

@@ -130,7 +130,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         const int x = lane * VPL + i;
-        l[i] = x < E ? (double)lrow[x] : 0.0;
+        l[i] = x < E ? (double)__ldcg(lrow + x) : 0.0;
         if (x < E) { top = fmax(top, l[i]); big = fmaxf(big, fabsf((float)l[i])); }
     }
 #pragma unroll
@@ -282,7 +282,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
 // ---- 32-bit path -----------------------------------------------------------------------------------------------------
 // The ranking values r and scores s (64 bits) of two experts, made by a whole warp. `z`: the softmax's sum.
 __device__ __noinline__ void exact_pair(const SelectParams& p, SelectShared* sh, int row, const float* lrow, int lane, int a, int b, double top, double z, double (&r)[2], double (&s)[2]) {
-    double la = (double)lrow[a], lb = (double)lrow[b];
+    double la = (double)__ldcg(lrow + a), lb = (double)__ldcg(lrow + b);
     if (sh) dots_ask(p, sh, row, a, b, la, lb);
     // lane 0 takes a, lane 1 takes b
     const double l = lane == 0 ? la : lb;
@@ -323,19 +323,19 @@ template <int VPL, bool EXACT>
 __device__ __forceinline__ int select_row(const SelectParams& p, int row, int lane, SelectShared* sh) {
     constexpr uint32_t kIndex = VPL - 1;
     const int E = p.E, gs = E / p.G, K = p.K;
-    const float* lrow = p.logits + (size_t)row * E;
+    const float* lrow = p.logits + (size_t)row * E;                     // read past L1: other CTAs of this kernel may have written them
     const bool soft = p.score == OCO_SCORE_SOFTMAX;
     float l[VPL];
     if (VPL >= 4 && E % 4 == 0 && ((uintptr_t)p.logits & 15u) == 0) {
 #pragma unroll
         for (int i = 0; i < VPL; i += 4) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane * VPL + i < E) v = __ldg(reinterpret_cast<const float4*>(lrow + lane * VPL + i));
+            if (lane * VPL + i < E) v = __ldcg(reinterpret_cast<const float4*>(lrow + lane * VPL + i));
             l[i] = v.x; l[(i + 1) % VPL] = v.y; l[(i + 2) % VPL] = v.z; l[(i + 3) % VPL] = v.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) l[i] = lane * VPL + i < E ? __ldg(lrow + lane * VPL + i) : 0.f;
+        for (int i = 0; i < VPL; i++) l[i] = lane * VPL + i < E ? __ldcg(lrow + lane * VPL + i) : 0.f;
     }
     uint32_t big = 0;                                                  // largest magnitude of a logit, as bits
 #pragma unroll
@@ -364,6 +364,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     const float es = soft ? kScoreError + dl : kSigmoidError + 0.25f * dl;
     float r[VPL];
     uint32_t wide = 0;                                                 // largest magnitude of score + bias, as bits
+    bool bad_bias = false;
     if (p.bias || (soft && !p.normalize)) {
         float z = 0.f;
 #pragma unroll
@@ -382,20 +383,36 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         for (int i = 0; i < VPL; i++) {
             const int x = lane * VPL + i;
             r[i] = r[i] * inv + (x < E ? __ldg(p.bias + x) : 0.f);
-            if (!nonfinite(r[i])) wide = max(wide, __float_as_uint(fabsf(r[i])));
+            wide = max(wide, __float_as_uint(fabsf(r[i])));
         }
         wide = warp_max(wide);
+        if (wide >= 0x7f800000u) {                                     // a bias that is not finite does not widen the margins
+            uint32_t finite = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (!nonfinite(r[i])) finite = max(finite, __float_as_uint(fabsf(r[i])));
+            const bool nan = wide > 0x7f800000u;
+            wide = warp_max(finite);
+            bad_bias = nan;
+        }
         ek = (soft ? inv * es : es) + kHalfUlp * __uint_as_float(wide);
     } else {
 #pragma unroll
         for (int i = 0; i < VPL; i++) r[i] = l[i];
     }
     uint32_t key[VPL];
+    if (any_bad || bad_bias) {                               // a NaN among the values, or a logit that ranks last
 #pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        uint32_t k = rank_key(r[i]);
-        if (any_bad && l[i] == -3.4e38f) k = 1u;
-        key[i] = lane * VPL + i < E ? (max(k, 16u) & ~kIndex) | (kIndex - i) : 0u;
+        for (int i = 0; i < VPL; i++) {
+            const uint32_t k = any_bad && l[i] == -3.4e38f ? 1u : rank_key(r[i]);
+            key[i] = lane * VPL + i < E ? (max(k, 16u) & ~kIndex) | (kIndex - i) : 0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) {
+            const uint32_t u = __float_as_uint(VPL == 1 ? r[i] + 0.0f : r[i]);   // where the last bits stay, the two zeros are made one
+            key[i] = lane * VPL + i < E ? ((u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) & ~kIndex) | (kIndex - i) : 0u;
+        }
     }
     sort_keys(key);
     // the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
@@ -410,7 +427,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         double z = 0.0;
 #pragma unroll
         for (int i = 0; i < VPL; i++)
-            if (lane * VPL + i < E) z += exp((double)lrow[lane * VPL + i] - (double)top);
+            if (lane * VPL + i < E) z += exp((double)__ldcg(lrow + lane * VPL + i) - (double)top);
         z64 = warp_sum_d(z);
     };
 
@@ -562,7 +579,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     }
     float s = 0.f;
     if (lane < K) {
-        const float v = __ldg(lrow + my_id);
+        const float v = __ldcg(lrow + my_id);
         s = soft ? expf(v - top) * inv : 1.0f / (1.0f + expf(-v));
     }
     float sum = 1.0f;
@@ -580,15 +597,11 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
 template <int VPL>
 __device__ __noinline__ void settle_row(const SelectParams& p, int row, int lane, SelectShared* sh) { select_row<VPL, true>(p, row, lane, sh); }
 
-// A warp per token, eight tokens per CTA.
+// The tokens of a CTA of 256 threads, one per warp (row < 0: none).
 template <int VPL>
-__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2) select_kernel(const SelectParams p) {
-    __shared__ SelectShared sh;
-    pdl_wait();                // the kernel before has completed and its writes are visible
-    pdl_launch_dependents();
-    if (p.status && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 8 + warp;
-    const int left = row < p.rows ? select_row<VPL, false>(p, row, lane, nullptr) : 0;
+__device__ __forceinline__ void select_tokens(const SelectParams& p, int row, SelectShared& sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int left = row >= 0 ? select_row<VPL, false>(p, row, lane, nullptr) : 0;
     if (left == 1) settle_row<VPL>(p, row, lane, nullptr);
     if (!p.x || !__syncthreads_or(left == 2)) return;
     if (lane == 0) sh.rows[warp] = left == 2 ? row : -1;
@@ -600,6 +613,58 @@ __global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2) select_kernel(const Sel
     } else {
         dots_serve(p, &sh);
     }
+}
+
+template <int VPL>
+__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2) select_kernel(const SelectParams p) {
+    __shared__ SelectShared sh;
+    pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();
+    if (__syncthreads_or(p.status && threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u)) return;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    select_tokens<VPL>(p, row < p.rows ? row : -1, sh);
+}
+
+// Few rows: the product and the selection in one launch. A warp per expert and four tokens makes the logits (f32); the CTA
+// that comes last for its four tokens (counted in `arrivals`, which it leaves at zero) selects for them. No CTA waits.
+template <int VPL>
+__global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, float* logits, uint32_t* arrivals) {
+    __shared__ SelectShared sh;
+    __shared__ int last;
+    pdl_wait();                // the kernel before has completed and its writes are visible
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.y * 8 + warp, t0 = blockIdx.x * 4;
+    if (e < p.E) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = lane * 4; k < p.H; k += 128) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p.w + (size_t)e * p.H + k));
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                if (t0 + t >= p.rows) continue;
+                const uint2 q = *reinterpret_cast<const uint2*>(p.x + (size_t)(t0 + t) * p.H + k);
+                acc[t] = fmaf(v.x, __uint_as_float(q.x << 16), acc[t]);
+                acc[t] = fmaf(v.y, __uint_as_float(q.x & 0xffff0000u), acc[t]);
+                acc[t] = fmaf(v.z, __uint_as_float(q.y << 16), acc[t]);
+                acc[t] = fmaf(v.w, __uint_as_float(q.y & 0xffff0000u), acc[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float s = warp_sum_f(acc[t]);
+            if (lane == 0 && t0 + t < p.rows) logits[(size_t)(t0 + t) * p.E + e] = s;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(&arrivals[blockIdx.x], 1u) == gridDim.y - 1;
+        if (last) arrivals[blockIdx.x] = 0u;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    select_tokens<VPL>(p, warp < 4 && t0 + warp < p.rows ? t0 + warp : -1, sh);
 }
 
 }  // namespace oco

@@ -334,6 +334,8 @@ def need(t: torch.Tensor, name: str, size: int, count: int, device: int):
     """Refuses a tensor that the kernels could not read as `count` contiguous elements of `size` bytes on the CUDA device
     of that number."""
     if t.get_device() != device or t.element_size() != size or not t.is_contiguous() or t.numel() < count:
+        if device < 0 and t.is_cuda:
+            raise OcoError(_lib.INVALID_ARGUMENT, "reserve a workspace first")
         raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {size} bytes on cuda:{device} is needed, "
                                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
 
@@ -533,37 +535,35 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
     if kind not in NORMS or gate_act not in GATE_ACTS:
         refuse(f"kind is one of {sorted(NORMS)}, gate_act one of {sorted(GATE_ACTS)}")
 
-    def rows_of(t, name, dtype):
-        if t is None:
-            return 0, 0
-        if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or t.stride(1) != 1:
-            refuse(f"{name}: rows {tuple(shape)} of {dtype} on {hidden.device} with unit stride inside a row are needed")
-        return t.data_ptr(), t.stride(0) if rows > 1 else 0
-
-    def vector(t, name):
-        if t is None:
-            return 0
-        need(t, name, 4, width, dev)
-        return t.data_ptr()
-
-    h, hs = rows_of(hidden, "hidden", hidden.dtype)
-    b, bs = rows_of(block, "block", torch.bfloat16)
-    ho, hos = rows_of(hidden_out, "hidden_out", hidden.dtype)
-    no, nos = rows_of(norm_out, "norm_out", torch.bfloat16)
-    g = gs = gate_type = per = 0
+    for t, name, dtype in ((block, "block", torch.bfloat16), (hidden_out, "hidden_out", hidden.dtype), (norm_out, "norm_out", torch.bfloat16)):
+        if t is not None and (t.shape != shape or t.dtype is not dtype or t.get_device() != dev):
+            refuse(f"{name}: rows {tuple(shape)} of {dtype} on {hidden.device} are needed")
+    strides = []
+    for t in (hidden, block, hidden_out, norm_out):
+        if t is None or t.is_contiguous():
+            strides.append(0)
+        elif t.stride(1) == 1:
+            strides.append(t.stride(0) if rows > 1 else 0)
+        else:
+            refuse("the elements of a row must be neighbours")
+    for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
+        if t is not None:
+            need(t, name, 4, width, dev)
+    gs = gate_type = per = 0
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.dtype not in (torch.bfloat16, torch.float32) or gate.get_device() != dev or gate.shape[-1] != width or gate.stride(-1) != 1:
             refuse("gate: [width] or [gates, width], bf16 or f32, unit stride inside a row")
-        g, gate_type = gate.data_ptr(), 2 if gate.dtype is torch.float32 else 1
+        gate_type = 2 if gate.dtype is torch.float32 else 1
         if gate.dim() == 2:
             gates = gate.shape[0]
             per = gate_rows if gate_rows is not None else (rows // gates if gates and rows % gates == 0 else 0)
             if rows and (per < 1 or (rows - 1) // per >= gates):
                 refuse("gate: fewer gate rows than the rows need")
             gs = gate.stride(0) if gates > 1 else 0
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     args = _NORM_ARGS.pack(width, NORMS[kind], wide, gate_type, per, GATE_ACTS[gate_act], epsilon, weight_offset, residual_scale, block_scale,
-                           h, b, vector(post_weight, "post_weight"), vector(post_bias, "post_bias"), vector(pre_weight, "pre_weight"),
-                           vector(pre_bias, "pre_bias"), g, ho, no, hs, bs, gs, hos, nos)
+                           hidden.data_ptr(), at(block), at(post_weight), at(post_bias), at(pre_weight), at(pre_bias), at(gate), at(hidden_out), at(norm_out),
+                           strides[0], strides[1], gs, strides[2], strides[3])
     if rows == 0:      # an empty tensor has no address
         return
     rc = _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(), None, 0)
