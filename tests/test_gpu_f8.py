@@ -337,3 +337,92 @@ def test_a_layer_of_the_operators(lib):
         h1, _ = opref.block_norm(h0, block, pre, None, post)
         h2, n2 = opref.block_norm(h1.to(torch.bfloat16), moe_out, pre, None, post, residual_scale=0.5)
         assert (hidden.double() - h2).norm() <= 2.0 ** -7 * h2.norm() and (nxt.double() - n2).norm() <= 2.0 ** -7 * n2.norm()
+
+
+@pytest.mark.parametrize("rows,hidden,ffn", [(1, 16384, 64), (4, 10240, 160), (1030, 288, 544), (1300, 512, 96), (2049, 160, 288)])
+def test_projection_forms(lib, rows, hidden, ffn):
+    """Contractions longer than a CTA rounds by itself; tiles on SM pairs with ragged rows and features."""
+    g = gen(rows)
+    up, up_s = opref.weights(g, (), ffn, hidden)
+    x = bf16(g, rows, hidden)
+    _, y = projection(lib, up, up_s, x)
+    within(y, *opref.product(*opref.quantize(x.double()), up, up_s))
+
+
+@pytest.mark.parametrize("rows,hidden,ffn", [(4, 16384, 96), (1100, 320, 160), (1281, 256, 416)])
+def test_gated_feed_forward_forms(lib, rows, hidden, ffn):
+    g = gen(rows)
+    w = dict(zip(("gate", "gate_s", "up", "up_s", "down", "down_s"),
+                 (*opref.weights(g, (), ffn, hidden), *opref.weights(g, (), ffn, hidden), *opref.weights(g, (), hidden, ffn))))
+    x = bf16(g, rows, hidden)
+    plan = lib.dense.DensePlan(lib.dense.FFN_SILU_GATE, synth.FMT_F8_E4M3, hidden, ffn)
+    plan.reserve(rows)
+    plan.bind(w["up"], w["gate"], w["down"], up_scale=w["up_s"], gate_scale=w["gate_s"], down_scale=w["down_s"])
+    y = torch.empty_like(x)
+    plan.forward(x, y, rows)
+    ffn_near(y, opref.ffn(x.double(), **w))
+    plan.forward(x, x, rows)                     # a feed-forward reads its rows before it writes any
+    assert torch.equal(x, y)
+
+
+def test_the_least_and_the_largest_blocks(lib):
+    """Blocks whose largest magnitude is near either end of bf16's range take the division that leaves the range never."""
+    H, F = 384, 64
+    g = gen(77)
+    x = bf16(g, 6, H)
+    x[0, :128] *= 1e-36
+    x[1, 128:256] *= 3e37
+    x[2] = 0
+    x[2, 300] = 1e-38
+    x[3, :] = torch.finfo(torch.bfloat16).max
+    up, up_s = opref.weights(g, (), F, H)
+    up = (up.float() / 64).to(torch.float8_e4m3fn)
+    up_s = up_s * 1e-3
+    for rows in (6, 3):
+        _, y = projection(lib, up, up_s, x[:rows].contiguous())
+        want, terms = opref.product(*opref.quantize(x[:rows].double()), up, up_s)
+        # below 2^-126 a scale has fewer bits: the smallest f32 step, 2^-149, on 448 * 448 * 128 terms
+        assert ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * terms + 2.0 ** -149 * 448 * 448 * 128).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+def test_a_few_tokens_with_shared_and_absent_experts(lib, rows):
+    plan, w, g = expert_layer(lib, 12, 416, 288, 6, 4, 8)
+    x, res = bf16(g, rows, 416), bf16(g, rows, 416)
+    probs = torch.rand((rows, 4), device="cuda", generator=g)
+    for pattern in ([0, 1, 2, 3], [5, -1, 5, 6], [-1, -1, -1, -1], [-1, 2, -1, 2**31 - 1], [3, 3, 3, 3]):
+        ids = torch.tensor([pattern] * rows, dtype=torch.int32, device="cuda").roll(1, 1).contiguous()
+        p = probs.clone()
+        p[(ids < 0) | (ids >= 6)] = float("nan")                              # never read
+        out = torch.empty_like(res)
+        plan.forward(x, ids, p, res, rows, out=out)
+        plan.poll()
+        ffn_near(out, experts_want(w, x, ids, probs, res), 2.0 ** -8)
+        if not ((ids >= 0) & (ids < 6)).any():
+            assert torch.equal(out, res)
+
+
+@pytest.mark.parametrize("E,K,rows", [(5, 5, 1000), (130, 8, 700), (512, 16, 300)])
+def test_many_routes(lib, E, K, rows):
+    """More routes than one CTA orders: every route once, in any order inside its expert, absent ones nowhere."""
+    H, F = 64, 64
+    plan, w, g = expert_layer(lib, 13, H, F, E, K, rows)
+    x, res = bf16(g, rows, H), bf16(g, rows, H)
+    ids = torch.randint(-1, E, (rows, K), device="cuda", generator=g).to(torch.int32)
+    probs = torch.rand((rows, K), device="cuda", generator=g)
+    out = torch.empty_like(res)
+    plan.forward(x, ids, probs, res, rows, out=out)
+    plan.poll()
+    ffn_near(out, experts_want(w, x, ids, probs, res), 2.0 ** -8)
+
+
+def test_overlap_is_refused(lib):
+    g = gen(14)
+    up, up_s = opref.weights(g, (), 128, 128)
+    x = bf16(g, 8, 128)
+    plan, _ = projection(lib, up, up_s, x)
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        plan.forward(x, x, 8)
+    fresh = lib.moe.F8ExpertPlan.new(128, 128, 4, 2)
+    with pytest.raises(_lib.OcoError, match="reserve"):
+        fresh.forward(x, torch.zeros((8, 2), dtype=torch.int32, device="cuda"), torch.ones((8, 2), device="cuda"), x, 8)

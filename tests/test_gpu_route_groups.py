@@ -245,3 +245,38 @@ def test_refused_tensors(moe):
     shifted = torch.zeros(4 * 256 + 1, device="cuda", dtype=torch.bfloat16)[1:]
     with pytest.raises(_lib.OcoError, match="aligned"):
         r.forward(shifted, ids, probs, 4)
+
+
+@pytest.mark.parametrize("experts", [3, 40, 100, 200, 511])
+@pytest.mark.parametrize("rows", [1, 4, 5, 16, 17, 129])
+def test_experts_that_fill_no_tile(moe, experts, rows):
+    shape = (experts, min(experts, 7), "softmax", 1, 1, 1, True, True, 1.0)
+    r, w, b, g = make(moe, shape, 640, rows, 20 + rows)
+    x = torch.randn((rows, 640), device="cuda", generator=g).to(torch.bfloat16)
+    ids, probs = outputs(shape, rows)
+    for _ in range(2):                                   # the counters of the last arrival are back at zero
+        ids.fill_(-7)
+        r.forward(x, ids, probs, rows)
+        want, p = expect(shape, x.double() @ w.double().t(), b)
+        assert np.array_equal(ids.cpu().numpy(), want)
+        np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=2.0 ** -16)
+    r.poll()
+
+
+def test_a_bias_that_is_nan_or_leaves_too_few(moe):
+    """NaN and -inf biases rank last, in the order of their indexes where nothing else is left."""
+    shape = (64, 6, "sigmoid", 1, 1, 1, True, True, 1.0)
+    r, _, b, g = make(moe, shape, 0, 9, 30)
+    b = torch.full((64,), -float("inf"), device="cuda")
+    b[[9, 33, 50]] = 0.0
+    r.bind(None, b)
+    logits = torch.randn((9, 64), device="cuda", generator=g)
+    ids, probs = outputs(shape, 9)
+    r.select(logits, ids, probs, 9)
+    got = ids.cpu().numpy()
+    assert (np.sort(got[:, :3], 1) == [9, 33, 50]).all() and (got[:, 3:] == [0, 1, 2]).all() and np.isfinite(probs.cpu().numpy()).all()
+    b[::2] = float("nan")
+    b[1::2] = 0.0
+    r.bind(None, b)
+    r.select(logits, ids, probs, 9)
+    assert (ids.cpu().numpy() % 2 == 1).all()
