@@ -402,7 +402,7 @@ struct F8Thin {
     // (64 tokens over 128 experts: 136 -> 114 us).
     static constexpr int kRoom = (NT == 16 && FORM == kF8Tiles ? (GATED ? 70 : 54) : 108) * 1024;
     static constexpr int kStages = (kRoom - kOwn) / kStage > 2 ? (kRoom - kOwn) / kStage : 2;
-    static constexpr int kBufs = 2, kTmemUsed = kBufs * kMats * NT;
+    static constexpr int kBufs = NT == 16 ? 4 : 2, kTmemUsed = kBufs * kMats * NT;   // narrow tiles: MMAs of more blocks ahead of the sums
     static constexpr int kTmem = kTmemUsed <= 32 ? 32 : kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : 256;
     static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
     static constexpr int kCtrl = 512;

