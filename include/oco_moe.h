@@ -333,7 +333,7 @@ void oco_moe_graph_destroy(oco_moe_graph* graph);
 
 /* The dense products either side of the MoE layer: the reference's DenseMatrix::apply
  * (src/weights/compute/matrix.rs:130-278) composed as its callers compose it.
- *   OCO_DENSE_PROJECTION     y[rows, ffn] = up_w . x, stored as bf16 (any of the three weight formats)
+ *   OCO_DENSE_PROJECTION     y[rows, ffn] = up_w . x, stored as bf16 (any weight format)
  *   OCO_DENSE_FFN_RELU2      Nemotron's always-on expert (compute/nemotron.rs:302-315 for rows > 1,
  *                            :460-509 for one token): up -> relu^2 -> down, Q4_0; y[rows, hidden]
  *   OCO_DENSE_FFN_SILU_GATE  the gated feed-forward of dense layers (Compute::feed_forward,
@@ -366,7 +366,8 @@ int oco_dense_bind_workspace(oco_dense_plan* plan, void* workspace, size_t bytes
 int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* weights);
 /* OCO_FMT_F8_E4M3 (OCO_DENSE_PROJECTION and OCO_DENSE_FFN_SILU_GATE; hidden and ffn multiples of 32, codes 16-byte
  * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes. The arithmetic
- * is that of the oco_moe_f8_plan calls at every row count: no single-token numerics of its own. */
+ * is that of the oco_moe_f8_plan calls at every row count: no single-token numerics of its own. 0 rows are no work; a
+ * projection's y must not overlap x. */
 typedef struct {
     const float* up_s;
     const float* gate_s;
@@ -464,8 +465,9 @@ int oco_moe_block_norm(const oco_moe_block_norm_args* args, int rows, void* cuda
  * elements: scale = largest / 448, code = e4m3(x * 448 / largest). Products of codes are summed in f32 over the
  * 128 elements of a block on the tensor cores, the blocks' sums in f32 under the product of their scales:
  *     g = gate . x, u = up . x, a = silu(g) * u (f32), rounded to e4m3 as the rows are, y = down . a
- *     out[t] = residual[t] + sum_r prob[t, r] * y[t, r]        (y is rounded to bf16, the sum is f32, one rounding)
- * The ids may come from any router; an id outside 0 .. experts-1 is a route of another shard or of padding and is
+ *     out[t] = residual[t] + sum_r prob[t, r] * y[t, r]        (f32, one rounding; in calls of more than three tokens y
+ *                                                              travels through memory as bf16)
+ * The ids may come from any router, one expert twice for a token included; an id outside 0 .. experts-1 is a route of another shard or of padding and is
  * left out (its weight is not read). A row without any route keeps its residual. */
 typedef struct {
     int32_t hidden;      /* multiple of 32 */
@@ -485,8 +487,10 @@ void oco_moe_f8_plan_destroy(oco_moe_f8_plan* plan);
 size_t oco_moe_f8_workspace_bytes(const oco_moe_f8_plan* plan, int max_rows);
 int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t bytes, int max_rows);
 int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* weights);
-/* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual); ids u32, probs f32 [rows, top_k].
- * Only enqueues; 0 rows are no work. */
+/* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual or x); ids u32, probs f32 [rows, top_k].
+ * Only enqueues; 0 rows are no work. Weights are fetched ahead of the kernels before them in the stream: a kernel or
+ * copy that writes them and lies before the call in stream order is waited for, as long as it does not itself let
+ * its successor start early. */
 int oco_moe_f8_forward(oco_moe_f8_plan* plan, const uint16_t* x_bf16, const uint32_t* ids, const float* probs,
                        const uint16_t* residual_bf16, uint16_t* out_bf16, int rows, void* cuda_stream);
 int oco_moe_f8_poll(oco_moe_f8_plan* plan, void* cuda_stream);
