@@ -18,7 +18,7 @@ namespace oco {
 struct RouterTile {
     static constexpr int kTile = 128 * 128, kStage = 4 * kTile, kStages = 3;
     static constexpr int kRun = 4;                       // stages between two readings of the accumulator
-    static constexpr int kPitch = 129;                   // f32 of a row of the parts: neighbouring rows in other banks
+    static constexpr int kPitch = 132;                   // f32 of a row of the parts: eight rows' 16-byte pieces fill the banks
     static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
     static constexpr int kCtrl = 256, kSmem = kStages * kStage + kCtrl + 1024;
     static_assert(128 * kPitch * 4 <= kStages * kStage, "the parts lie where the stages were");
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         }
         // every MMA of this CTA is done: the parts go where the stages were
 #pragma unroll
-        for (int j = 0; j < 128; j++) part[tid * S::kPitch + j] = sum[j];
+        for (int j = 0; j < 128; j += 4) *reinterpret_cast<float4*>(part + tid * S::kPitch + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
     } else if (warp == S::kTmaWarp) {
         if (lane == 0) {
             int g = 0;
@@ -153,15 +153,24 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         __syncthreads();
     }
     if (split > 1) cluster_sync_all();
-    // join: this CTA's share of the rows, a warp per row
-    const int live = min(128, rows - row0), cols = min(128, E - e0);
+    // join: this CTA's share of the rows, a warp per row, four experts a lane
+    const int live = min(128, rows - row0), cols = min(128, E - e0), c = 4 * lane;
+    const bool wide = (E & 3) == 0 && ((uintptr_t)logits & 15u) == 0;
     for (int r = rank + split * warp; r < live; r += split * (S::kThreads / 32)) {
-        for (int c = lane; c < cols; c += 32) {
-            float v = 0.f;
-            if (split == 1) v = part[r * S::kPitch + c];
-            else
-                for (int q = 0; q < split; q++) v += peer_f32(base + 4u * (uint32_t)(r * S::kPitch + c), (uint32_t)q);
-            logits[(size_t)(row0 + r) * E + e0 + c] = v;
+        const uint32_t at = base + 4u * (uint32_t)(r * S::kPitch + c);
+        float4 v = peer_f32x4(at, 0);
+#pragma unroll 7
+        for (int q = 1; q < split; q++) {
+            const float4 w = peer_f32x4(at, (uint32_t)q);
+            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+        }
+        float* dst = logits + (size_t)(row0 + r) * E + e0 + c;
+        if (wide && c < cols) *reinterpret_cast<float4*>(dst) = v;
+        else {
+            if (c < cols) dst[0] = v.x;
+            if (c + 1 < cols) dst[1] = v.y;
+            if (c + 2 < cols) dst[2] = v.z;
+            if (c + 3 < cols) dst[3] = v.w;
         }
     }
     tc_fence_before();
