@@ -60,7 +60,7 @@ struct F8Wide {
     static constexpr int kA = 128 * 128, kB = (PAIR ? 128 : 256) * 128, kStage = kA + kB, kStages = PAIR ? 4 : 3;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10, kThreads = 384;
     static constexpr int kScaleRun = 4, kScales = 3;                    // scales travel in runs of four blocks, three runs
-    static constexpr int kScaleBytes = (128 + 4) * 4;                   // of a block: 128 rows, gate and up block
+    static constexpr int kScaleBytes = 128 * 2 * 4;                     // of a block: 128 rows under two blocks of features
     static constexpr int kOutPitch = 256 + 16;                          // a row's 128 results, spread over the banks
     static constexpr int kOut = kStages * kStage, kCtrlAt = kOut + 8 * 32 * kOutPitch;
     static constexpr int kTops = 512, kRing = kTops + 2 * 128 * 4, kCtrl = kRing + kScales * kScaleRun * kScaleBytes;
@@ -72,13 +72,6 @@ template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-__device__ __forceinline__ void cp_async4(uint32_t smem_dst, const void* gsrc) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(gsrc) : "memory");
-}
-// One arrival on `bar` when this thread's copies so far have landed (counted among the barrier's expected arrivals).
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ float lds_f32(uint32_t at) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
@@ -109,7 +102,7 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
     auto tempty = [&](int b) { return ctrl + 8u * (2 * S::kStages + b); };   // of the issuing CTA: both have read
     auto sfull = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + q); };
     auto sempty = [&](int q) { return ctrl + 8u * (2 * S::kStages + 2 + S::kScales + q); };
-    auto ring = [&](int q, int k) { return ctrl + S::kRing + (uint32_t)(q * S::kScaleRun + k) * S::kScaleBytes; };   // [128] rows, gate, up
+    auto ring = [&](int q, int k) { return ctrl + S::kRing + (uint32_t)(q * S::kScaleRun + k) * S::kScaleBytes; };   // [row][gate, up or first, second block]
     uint32_t* slot = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + 8 * (2 * S::kStages + 2 + 2 * S::kScales));
     volatile uint32_t* abort_flag = slot + 1;
     uint32_t* tops = reinterpret_cast<uint32_t*>(gen + S::kCtrlAt + S::kTops);   // [2][128]
@@ -184,8 +177,8 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
             auto scales = [&](int kb) {
                 const int k = kb % S::kScaleRun, q = run % S::kScales;
                 if (k == 0) mbar_wait(sfull(q), (uint32_t)(run / S::kScales) & 1u, abort_flag, p.status);
-                const float x = lds_f32(ring(q, k) + 4u * erow);
-                const float s0 = x * lds_f32(ring(q, k) + 512u + (GATED ? 0u : 4u * half)), s1 = GATED ? x * lds_f32(ring(q, k) + 516u) : s0;
+                const uint32_t at = ring(q, k) + 8u * erow;
+                const float s0 = lds_f32(at + (GATED ? 0u : 4u * half)), s1 = GATED ? lds_f32(at + 4u) : s0;
                 t0 = f32x2(s0, s0);
                 t1 = f32x2(s1, s1);
                 if (k == S::kScaleRun - 1 || kb == nkb - 1) {
@@ -292,26 +285,34 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
     } else {
         fewer_registers<56>();
         if (warp == S::kScaleWarp) {
-            // ===== scales: four rows a lane and the two blocks of the weights, a block of K at a time ====================
+            // ===== scales: four rows a lane times the two blocks of the weights, a run of blocks of K at a time ==========
             int run = 0;
             for (int i = first; i < total; i += step) {
                 const Item it = item_of(i);
                 const int fb = it.f0 / 128;
-                const float* ws = lane == 0 || !GATED ? p.s0 : p.s1;   // lane 0: gate or the first block, lane 1: up or the second
-                ws += ((size_t)it.expert * nfb + (GATED ? fb : min(fb + lane, nfb - 1))) * nkb;
+                const float* w0 = p.s0 + ((size_t)it.expert * nfb + fb) * nkb;
+                const float* w1 = GATED ? p.s1 + ((size_t)it.expert * nfb + fb) * nkb : p.s0 + ((size_t)it.expert * nfb + min(fb + 1, nfb - 1)) * nkb;
                 for (int kb = 0; kb < nkb; kb += S::kScaleRun, run++) {
                     const int q = run % S::kScales;
-                    mbar_wait(sempty(q), ((uint32_t)(run / S::kScales) & 1u) ^ 1u, abort_flag, p.status);
-                    for (int k = 0; k < S::kScaleRun && kb + k < nkb; k++) {
-                        const float* xs = p.row_scales + (size_t)(kb + k) * p.pitch;
+                    float x[S::kScaleRun][4], a[S::kScaleRun], b[S::kScaleRun];
 #pragma unroll
-                        for (int r = 0; r < 4; r++) cp_async4(ring(q, k) + 4u * (lane + 32 * r), xs + min(it.row0 + lane + 32 * r, p.pitch - 1));
-                        if (lane < 2) cp_async4(ring(q, k) + 512u + 4u * lane, ws + kb + k);
+                    for (int k = 0; k < S::kScaleRun; k++) {
+                        const int at = min(kb + k, nkb - 1);
+                        const float* xs = p.row_scales + (size_t)at * p.pitch;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) x[k][r] = xs[min(it.row0 + lane + 32 * r, p.pitch - 1)];
+                        a[k] = w0[at];
+                        b[k] = w1[at];
                     }
-                    cp_async_arrive(sfull(q));
+                    mbar_wait(sempty(q), ((uint32_t)(run / S::kScales) & 1u) ^ 1u, abort_flag, p.status);
+#pragma unroll
+                    for (int k = 0; k < S::kScaleRun; k++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(ring(q, k) + 8u * (lane + 32 * r)), "f"(x[k][r] * a[k]), "f"(x[k][r] * b[k]) : "memory");
+                    mbar_arrive(sfull(q));
                 }
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         } else if (warp == S::kTmaWarp && lane == 0) {
             // ===== operands: this CTA's 128 rows, and its half (PAIR) or all of the features ==============================
             int g = 0;
