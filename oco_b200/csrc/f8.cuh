@@ -105,32 +105,49 @@ struct F8Divider {
         const float q = top * kPart;
         return plain ? fmaf(fmaf(-q, 448.0f, top), kPart, q) : __fdiv_rn(top, 448.0f);
     }
-    __device__ __forceinline__ float operator()(float x) const {
+    // Eight bf16 elements -> codes, two at a time in packed f32 arithmetic.
+    __device__ __forceinline__ uint2 codes(const uint4& x) const {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        float v[8];
         if (plain) {
-            const float n = x * 448.0f, q = n * rcp;
-            return fmaf(fmaf(-q, top, n), rcp, q);
+            const uint64_t lift = f32x2(448.0f, 448.0f), r2 = f32x2(rcp, rcp), minus = f32x2(-top, -top);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint64_t n = mul_f32x2(f32x2_bits(w[j] << 16, w[j] & 0xffff0000u), lift), q = mul_f32x2(n, r2);
+                f32x2_split(fma_f32x2(fma_f32x2(q, minus, n), r2, q), v[2 * j], v[2 * j + 1]);
+            }
+        } else {
+            const float by = top == 0.0f ? 1.0f : top;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[2 * j] = __fdiv_rn(__uint_as_float(w[j] << 16) * 0.875f, by) * 512.0f;
+                v[2 * j + 1] = __fdiv_rn(__uint_as_float(w[j] & 0xffff0000u) * 0.875f, by) * 512.0f;
+            }
         }
-        return __fdiv_rn(x * 0.875f, top == 0.0f ? 1.0f : top) * 512.0f;
+        return make_uint2(f8x4(v[0], v[1], v[2], v[3]), f8x4(v[4], v[5], v[6], v[7]));
     }
 };
 
-// Half a warp's block of 128 bf16 elements (eight a lane) -> codes and their scale. `half`: the lanes' mask.
-__device__ __forceinline__ float f8_block(const uint4& q, uint32_t half, uint2& codes) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    // the largest as bits: for non-negative floats the order of the bits, a NaN above everything
+// N (1 or 2) blocks of 128 bf16 elements of half a warp, eight of each a lane -> codes and scales. All 32 lanes take part.
+// The largest magnitude is found on the upper 16 bits of f32 values (for non-negative floats the order of the bits, a NaN
+// above everything), two of them in a word: both blocks share the four exchanges.
+template <int N>
+__device__ __forceinline__ void f8_blocks(const uint4 (&x)[N], uint2 (&codes)[N], float (&scale)[N]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) m = max(m, max((w[j] << 16) & 0x7fff0000u, w[j] & 0x7fff0000u));
-    m = __reduce_max_sync(half, m);
-    const F8Divider code(__uint_as_float(m));
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        v[2 * j] = code(__uint_as_float(w[j] << 16));
-        v[2 * j + 1] = code(__uint_as_float(w[j] & 0xffff0000u));
+    for (int b = 0; b < N; b++) {
+        constexpr uint32_t kMagnitude = 0x7fff7fffu;
+        const uint32_t t = __vmaxu2(__vmaxu2(x[b].x & kMagnitude, x[b].y & kMagnitude), __vmaxu2(x[b].z & kMagnitude, x[b].w & kMagnitude));
+        m |= max(t & 0xffffu, t >> 16) << (16 * b);
     }
-    codes = make_uint2(f8x4(v[0], v[1], v[2], v[3]), f8x4(v[4], v[5], v[6], v[7]));
-    return code.scale();
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+#pragma unroll
+    for (int b = 0; b < N; b++) {
+        const F8Divider by(__uint_as_float(b ? m & 0xffff0000u : m << 16));
+        codes[b] = by.codes(x[b]);
+        scale[b] = by.scale();
+    }
 }
 
 // Rows to codes: half a warp per token and two blocks of 128 elements, eight elements of each a lane (two loads on their
@@ -141,21 +158,19 @@ __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();   // only now: the next kernel reads weights before it waits for this one
     const int lane = threadIdx.x & 15, npairs = (K + 255) / 256;
-    const uint32_t half = 0xffffu << (threadIdx.x & 16);
     const uint32_t units = (uint32_t)tokens * (uint32_t)npairs, step = gridDim.x * 16;
-    for (uint32_t u = blockIdx.x * 16 + (threadIdx.x >> 4); u < units; u += step) {
-        const uint32_t token = u / (uint32_t)npairs;
+    for (uint32_t first = blockIdx.x * 16 + (threadIdx.x >> 5) * 2; first < units; first += step) {
+        const uint32_t u = first + ((threadIdx.x >> 4) & 1), token = u / (uint32_t)npairs;
         const int pair = (int)(u - token * (uint32_t)npairs), k = pair * 256 + 8 * lane;
         const uint16_t* src = x + (size_t)token * K + k;
-        const bool in[2] = {k < K, k + 128 < K};
+        const bool in[2] = {u < units && k < K, u < units && k + 128 < K};
         uint4 q[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) q[b] = in[b] ? __ldg(reinterpret_cast<const uint4*>(src + 128 * b)) : make_uint4(0, 0, 0, 0);
         uint2 c[2];
         float scale[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++) scale[b] = f8_block(q[b], half, c[b]);
-        for (int r = 0; r < top_k; r++) {
+        f8_blocks(q, c, scale);
+        for (int r = 0; r < top_k && in[0]; r++) {
             const uint32_t row = row_of_route ? __ldg(row_of_route + (size_t)token * top_k + r) : token;
             if (row == 0xffffffffu) continue;
 #pragma unroll

@@ -500,7 +500,6 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
             if (FORM == kF8Rows) {
                 // ===== rows to codes: half a warp per row and block (the swizzled layout that TMA would have written) =======
                 const int hl = lane & 15, nb = q1 - q0, units = nv * nb;
-                const uint32_t half = 0xffffu << (lane & 16);
                 auto fetch = [&](int u) {
                     if (u >= units) return make_uint4(0, 0, 0, 0);
                     const int c = u / nb, k = (q0 + u - c * nb) * 128 + 8 * hl;
@@ -508,15 +507,18 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
                     return k < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + row * p.K + k)) : make_uint4(0, 0, 0, 0);
                 };
                 uint4 next = fetch(tid >> 4);
-                for (int u = tid >> 4; u < units; u += 8) {
-                    const uint4 v = next;
+                for (int both = 2 * warp; both < units; both += 8) {   // all lanes of the warp stay together
+                    const int u = both + (lane >> 4);
+                    const uint4 v[1] = {next};
                     next = fetch(u + 8);
-                    uint2 code;
-                    const float scale = f8_block(v, half, code);
+                    uint2 code[1];
+                    float scale[1];
+                    f8_blocks(v, code, scale);
+                    if (u >= units) continue;
                     const int c = u / nb, i = u - c * nb;
                     const uint32_t at = own + (uint32_t)(i * NT * 128 + (c >> 3) * 1024 + (c & 7) * 128) + ((((uint32_t)hl >> 1) ^ (uint32_t)(c & 7)) << 4) + 8u * (hl & 1);
-                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(code.x), "r"(code.y) : "memory");
-                    if (hl == 0) reinterpret_cast<float*>(gen + (own - base) + S::kBlocks * NT * 128)[i * NT + c] = scale;
+                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at), "r"(code[0].x), "r"(code[0].y) : "memory");
+                    if (hl == 0) reinterpret_cast<float*>(gen + (own - base) + S::kBlocks * NT * 128)[i * NT + c] = scale[0];
                 }
                 fence_proxy_async_smem();
                 asm volatile("bar.sync 2, 160;" ::: "memory");          // with the MMA warp
