@@ -202,7 +202,7 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
         OCO_CK(plan, launch_dependent_clusters(f8_plan_kernel, ctas, dim3(ctas), dim3(1024), 0, st, pp));
         plan->launches++;
     }
-    const unsigned row_ctas = (unsigned)std::min<long long>(((long long)rows * ((H + 255) / 256) + 15) / 16, 8LL * plan->sm_count);
+    const unsigned row_ctas = (unsigned)(((long long)rows * ((H + 255) / 256) + 15) / 16);
     OCO_CK(plan, launch_dependent(f8_rows_kernel, dim3(row_ctas), dim3(256), 0, st, x, routed ? ws.row_of_route : nullptr, d.top_k, rows, H, ws.xq, ws.xs, ws.pitch));
     plan->launches++;
     if (routed) { p.tiles = ws.tiles; p.tile_count = ws.tile_count; p.offsets = ws.offsets; }
