@@ -434,8 +434,8 @@ const char* oco_moe_router_last_error(const oco_moe_router* router);
  *     layer: (v - mean(v)) * rsqrt(var(v) + epsilon) * (weight_offset + w) + bias
  * (oco_moe_add_norm_forward holds the plain case, with the reference's rounding, in front of a layer.) Sums are
  * f32; x is made from h before h is rounded. pre_w NULL: x is not weighted. block NULL: h = residual_scale *
- * hidden. hidden_out may be hidden and norm_out may be block (with the same strides); other overlaps are not
- * allowed. Rows of zeros give zeros (epsilon > 0); a NaN or infinity spoils its own row only. */
+ * hidden. hidden_out may be hidden and norm_out may be block (with the same strides); other overlaps of rows
+ * are refused. Rows of zeros give zeros (epsilon > 0); a NaN or infinity spoils its own row only. */
 typedef enum { OCO_NORM_RMS = 0, OCO_NORM_LAYER = 1 } oco_moe_norm_kind;
 typedef enum { OCO_GATE_NONE = 0, OCO_GATE_BF16 = 1, OCO_GATE_F32 = 2 } oco_moe_gate_type;
 typedef enum { OCO_GATE_PLAIN = 0, OCO_GATE_SIGMOID = 1, OCO_GATE_TANH = 2 } oco_moe_gate_act;
@@ -487,7 +487,8 @@ void oco_moe_f8_plan_destroy(oco_moe_f8_plan* plan);
 size_t oco_moe_f8_workspace_bytes(const oco_moe_f8_plan* plan, int max_rows);
 int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t bytes, int max_rows);
 int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* weights);
-/* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual or x); ids u32, probs f32 [rows, top_k].
+/* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual or x;
+ * a part of the residual it must not be); ids u32, probs f32 [rows, top_k].
  * Only enqueues; 0 rows are no work. Weights are fetched ahead of the kernels before them in the stream: a kernel or
  * copy that writes them and lies before the call in stream order is waited for, as long as it does not itself let
  * its successor start early. */

@@ -57,6 +57,8 @@ __device__ __forceinline__ uint4 pack8(const Oct& r) {
 __device__ __forceinline__ Oct load8(const float* p) {
     return pairs8(__ldg(reinterpret_cast<const uint4*>(p)), __ldg(reinterpret_cast<const uint4*>(p) + 1));
 }
+// The same of an array that a kernel before in the stream may have written.
+__device__ __forceinline__ Oct fetch8(const float* p) { return pairs8(*reinterpret_cast<const uint4*>(p), *(reinterpret_cast<const uint4*>(p) + 1)); }
 __device__ __forceinline__ uint64_t both(float v) { return f32x2(v, v); }
 __device__ __forceinline__ float sum2(uint64_t v) {
     float lo, hi;
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
             if (WIDE) raw[i][WIDE ? 1 : 0] = *reinterpret_cast<const uint4*>(src + 16);
             if (p.block) braw[i] = *reinterpret_cast<const uint4*>(p.block + (long long)row * p.block_stride + at);
             // a gate in bf16 may be as long as the rows: it travels with them
-            if (p.gate_type == OCO_GATE_BF16) graw[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + grow + at));
+            if (p.gate_type == OCO_GATE_BF16) graw[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + grow + at);
         }
     }
     if (p.block) {
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
 #pragma unroll
             for (int i = 0; i < ITER; i++) {
                 if (live[i]) {
-                    Oct g = p.gate_type == OCO_GATE_F32 ? load8(reinterpret_cast<const float*>(p.gate) + grow + col0 + i * THREADS * 8) : unpack8(graw[i]);
+                    Oct g = p.gate_type == OCO_GATE_F32 ? fetch8(reinterpret_cast<const float*>(p.gate) + grow + col0 + i * THREADS * 8) : unpack8(graw[i]);
                     if (p.gate_act != OCO_GATE_PLAIN) {
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
@@ -209,9 +211,23 @@ int say(char* err, size_t len, int code, const char* text) {
     return code;
 }
 
+// Rows in memory: `count` rows of `width` bytes every `pitch` bytes.
+struct Rows {
+    uintptr_t at;
+    size_t pitch, width, count;
+    uintptr_t end() const { return at + (count - 1) * pitch + width; }
+};
+// Whether two sets of rows share a byte. Interleaved rows of one pitch are told apart; of two pitches they count as shared.
+bool overlap(const Rows& a, const Rows& b) {
+    if (!a.at || !b.at || a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.pitch != b.pitch || a.count == 1 || b.count == 1) return true;
+    const size_t d = b.at >= a.at ? (b.at - a.at) % a.pitch : (a.pitch - (a.at - b.at) % a.pitch) % a.pitch;
+    return d < a.width || a.pitch - d < b.width;
+}
+
 template <int THREADS, int ITER>
 cudaError_t launch(const NormParams& p, bool layer, bool wide, cudaStream_t st) {
-    const dim3 grid(THREADS == 32 ? (p.rows + 3) / 4 : p.rows), block(THREADS == 32 ? 128 : THREADS);
+    const dim3 grid(THREADS == 32 ? (unsigned)((p.rows + 3LL) / 4) : (unsigned)p.rows), block(THREADS == 32 ? 128 : THREADS);
     if (layer) return wide ? launch_dependent(block_norm_kernel<THREADS, ITER, true, true>, grid, block, 0, st, p)
                            : launch_dependent(block_norm_kernel<THREADS, ITER, true, false>, grid, block, 0, st, p);
     return wide ? launch_dependent(block_norm_kernel<THREADS, ITER, false, true>, grid, block, 0, st, p)
@@ -251,6 +267,14 @@ extern "C" int oco_moe_block_norm(const oco_moe_block_norm_args* a, int rows, vo
     p.n = a->width; p.rows = rows; p.gate_type = a->gate_type; p.gate_rows = a->gate_rows; p.gate_act = a->gate_act;
     p.eps = a->epsilon; p.offset = a->weight_offset; p.residual_scale = a->residual_scale; p.block_scale = a->block_scale;
     const bool layer = a->kind == OCO_NORM_LAYER, wide = a->wide != 0;
+    const size_t n = (size_t)a->width, es = wide ? 4 : 2, gs = a->gate_type == OCO_GATE_F32 ? 4 : 2, R = (size_t)rows;
+    const Rows hidden{(uintptr_t)p.hidden, p.hidden_stride * es, n * es, R}, block{(uintptr_t)p.block, (size_t)p.block_stride * 2, n * 2, R},
+        gate{(uintptr_t)p.gate, p.gate_stride * gs, n * gs, p.gate_rows ? (R - 1) / p.gate_rows + 1 : 1}, h_out{(uintptr_t)p.hidden_out, p.hidden_out_stride * es, n * es, R},
+        x_out{(uintptr_t)p.norm_out, (size_t)p.norm_out_stride * 2, n * 2, R};
+    auto same = [](const Rows& x, const Rows& y) { return x.at == y.at && x.pitch == y.pitch && x.width == y.width; };   // each element is read by its writer
+    if ((overlap(h_out, hidden) && !same(h_out, hidden)) || (overlap(x_out, block) && !same(x_out, block)) || overlap(h_out, block) || overlap(x_out, hidden) ||
+        overlap(h_out, gate) || overlap(x_out, gate) || overlap(h_out, x_out))
+        return say(err, err_len, OCO_INVALID_ARGUMENT, "outputs overlap inputs or each other (hidden_out may be hidden, norm_out may be block)");
     const int pieces = a->width / 8;
     cudaStream_t st = (cudaStream_t)cuda_stream;
     cudaError_t e;

@@ -343,6 +343,10 @@ int oco_moe_f8_forward(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t*
     if (!x || !ids || !probs || !residual || !out) return plan->fail(OCO_INVALID_ARGUMENT, "null x, ids, probs, residual or out");
     if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)out) & 15u) return plan->fail(OCO_INVALID_ARGUMENT, "x, residual and out must be 16-byte aligned");
     if (((uintptr_t)ids | (uintptr_t)probs) & 3u) return plan->fail(OCO_INVALID_ARGUMENT, "ids and probs must be 4-byte aligned");
+    // out = residual: every element is read by its writer
+    const size_t bytes = (size_t)rows * plan->d.hidden * 2;
+    if (out != residual && (uintptr_t)out < (uintptr_t)residual + bytes && (uintptr_t)residual < (uintptr_t)out + bytes)
+        return plan->fail(OCO_INVALID_ARGUMENT, "out must not overlap a part of the residual");
     return run_rows(plan, x, ids, probs, residual, out, rows, (cudaStream_t)cuda_stream);
 }
 

@@ -152,9 +152,9 @@ __device__ __forceinline__ void f8_blocks(const uint4 (&x)[N], uint2 (&codes)[N]
 
 // Rows to codes: half a warp per token and two blocks of 128 elements, eight elements of each a lane (two loads on their
 // way). A routed token is read and rounded once and its codes written to the row of each of its routes. Scales lie
-// [block][row]. One pass over a grid of all rows: CTAs that loop took 25.5 us where this takes 22.6 (8192 rows of 4096).
-__global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict__ x, const uint32_t* __restrict__ row_of_route, int top_k,
-                                                      int tokens, int K, uint8_t* __restrict__ codes, float* __restrict__ scales, int scale_pitch) {
+// [block][row]. One pass over a grid of all rows: CTAs that loop take 3 us more (8192 rows of 4096: 24 us).
+__global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* x, const uint32_t* row_of_route, int top_k, int tokens, int K, uint8_t* codes,
+                                                      float* scales, int scale_pitch) {
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();   // only now: the next kernel reads weights before it waits for this one
     const int lane = threadIdx.x & 15, npairs = (K + 255) / 256;
@@ -165,12 +165,13 @@ __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict
     const bool in[2] = {u < units && k < K, u < units && k + 128 < K};
     uint4 q[2];
 #pragma unroll
-    for (int b = 0; b < 2; b++) q[b] = in[b] ? __ldg(reinterpret_cast<const uint4*>(src + 128 * b)) : make_uint4(0, 0, 0, 0);
+    for (int b = 0; b < 2; b++) q[b] = in[b] ? *reinterpret_cast<const uint4*>(src + 128 * b) : make_uint4(0, 0, 0, 0);
     uint2 c[2];
     float scale[2];
+    const uint32_t mine = row_of_route && u < units && lane < top_k ? row_of_route[(size_t)token * top_k + lane] : token;   // lane r: of route r
     f8_blocks(q, c, scale);
-    for (int r = 0; r < top_k && in[0]; r++) {
-        const uint32_t row = row_of_route ? __ldg(row_of_route + (size_t)token * top_k + r) : token;
+    for (int r = 0; r < top_k; r++) {
+        const uint32_t row = __shfl_sync(0xffffffffu, mine, r, 16);
         if (row == 0xffffffffu) continue;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* __restrict
 // ---- weighted combination --------------------------------------------------------------------------------------------
 // out[t] = residual[t] + sum_r prob[t, r] y[t, r], one rounding; routes without an expert of this plan are left out. A
 // thread takes eight columns of a row.
-__global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* __restrict__ y, const uint32_t* __restrict__ ids, const float* __restrict__ probs,
+__global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* y, const uint32_t* ids, const float* probs,
                                                          const uint16_t* residual, uint16_t* out, int rows, int top_k, int H, int E) {
     pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
     pdl_wait();                // the kernel before has completed and its writes are visible
@@ -197,9 +198,9 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* __restr
             float pr[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const bool live = r0 + r < top_k && __ldg(ids + (size_t)t * top_k + r0 + r) < (uint32_t)E;
-                pr[r] = live ? __ldg(probs + (size_t)t * top_k + r0 + r) : 0.f;
-                v[r] = live ? __ldg(reinterpret_cast<const uint4*>(y + ((size_t)t * top_k + r0 + r) * H + c)) : make_uint4(0, 0, 0, 0);
+                const bool live = r0 + r < top_k && ids[(size_t)t * top_k + r0 + r] < (uint32_t)E;
+                pr[r] = live ? probs[(size_t)t * top_k + r0 + r] : 0.f;
+                v[r] = live ? *reinterpret_cast<const uint4*>(y + ((size_t)t * top_k + r0 + r) * H + c) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) {

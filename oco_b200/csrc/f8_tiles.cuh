@@ -42,9 +42,9 @@ struct F8TileParams {
 
 __device__ __forceinline__ float silu_times(float g, float u) { return sigmoid_times(g, 1.0f) * g * u; }
 // Scale and factor of a block of activations whose largest magnitude is `top`: code = e4m3(a * lift * factor). `lift`
-// keeps 448 / top finite where top is tiny.
+// keeps 448 / top finite where top is tiny and the quotient's divisor in its range (below 2^126) where it is vast.
 __device__ __forceinline__ void f8_act_scale(float top, float& scale, float& lift, float& factor) {
-    lift = top < 1e-30f ? 1.2676506e30f : 1.0f;
+    lift = top < 1e-30f ? 1.2676506e30f : top > 1e30f ? 7.8886091e-31f : 1.0f;   // 2^100, 2^-100
     factor = top == 0.0f ? 1.0f : __fdividef(448.0f, top * lift);
     scale = top * (1.0f / 448.0f);
 }
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
                     if (u >= units) return make_uint4(0, 0, 0, 0);
                     const int c = u / nb, k = (q0 + u - c * nb) * 128 + 8 * hl;
                     const size_t row = p.ids ? (size_t)(tile / p.top_k) : (size_t)(row0 + c);
-                    return k < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + row * p.K + k)) : make_uint4(0, 0, 0, 0);
+                    return k < p.K ? *reinterpret_cast<const uint4*>(p.x + row * p.K + k) : make_uint4(0, 0, 0, 0);
                 };
                 uint4 next = fetch(tid >> 4);
                 for (int both = 2 * warp; both < units; both += 8) {   // all lanes of the warp stay together

@@ -60,7 +60,7 @@ constexpr int kRowsMax = 16;
 // The selection; fused: with the product before it, for few rows.
 int launch_select(oco_moe_router* r, const SelectParams& p, bool fused, cudaStream_t st) {
     const int per_lane = (p.E + 31) / 32;
-    const dim3 grid = fused ? dim3((p.rows + 3) / 4, (p.E + 7) / 8) : dim3((p.rows + 7) / 8), block(256);
+    const dim3 grid = fused ? dim3((p.rows + 3) / 4, (p.E + 7) / 8) : dim3((unsigned)((p.rows + 7LL) / 8)), block(256);
     auto launch = [&](auto select, auto route) {
         return fused ? launch_dependent(route, grid, block, 0, st, p, const_cast<float*>(p.logits), r->arrivals) : launch_dependent(select, grid, block, 0, st, p);
     };
@@ -114,6 +114,7 @@ int oco_moe_router_bind_workspace(oco_moe_router* r, void* workspace, size_t byt
     if (!r) return OCO_INVALID_ARGUMENT;
     if (!workspace || max_rows < 1) return r->fail(OCO_INVALID_ARGUMENT, "null workspace or max_rows < 1");
     if ((uintptr_t)workspace & 255u) return r->fail(OCO_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    if (max_rows > 1 << 28) return r->fail(OCO_UNSUPPORTED_SHAPE, "max_rows is more than 2^28");   // tiles are counted in 32 bits
     const RouterSpace s = carve(r->d, max_rows);
     if (bytes < s.total) return r->fail(OCO_INVALID_ARGUMENT, "workspace too small: %zu < %zu", bytes, s.total);
     OCO_CK(r, cudaDeviceSynchronize());     // whoever had this memory before is done with it

@@ -71,7 +71,7 @@ __device__ __forceinline__ void dots_share(const SelectParams& p, SelectShared* 
 #pragma unroll 2
     for (int k = threadIdx.x; k < p.H / 4; k += 256) {
         const float4 u = __ldg(wa + k), v = __ldg(wb + k);
-        const uint2 q = __ldg(xr + k);
+        const uint2 q = xr[k];
         const double x0 = (double)__uint_as_float(q.x << 16), x1 = (double)__uint_as_float(q.x & 0xffff0000u);
         const double x2 = (double)__uint_as_float(q.y << 16), x3 = (double)__uint_as_float(q.y & 0xffff0000u);
         a0 = fma((double)u.x, x0, a0); a1 = fma((double)u.y, x1, a1); a0 = fma((double)u.z, x2, a0); a1 = fma((double)u.w, x3, a1);
@@ -658,8 +658,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, f
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        last = atomicAdd(&arrivals[blockIdx.x], 1u) == gridDim.y - 1;
-        if (last) arrivals[blockIdx.x] = 0u;
+        last = atomicInc(&arrivals[blockIdx.x], gridDim.y - 1) == gridDim.y - 1;   // the last one sets the counter back to zero
         __threadfence();
     }
     __syncthreads();

@@ -360,9 +360,12 @@ def f8_matrix(codes, scales, lead, n: int, k: int, device, name: str):
     codes, scales = _staged(codes, device), _staged(scales, device)
     if scales.dtype == torch.uint8 and scales.numel() == 4 * blocks:      # bytes of a host array
         scales = scales.view(torch.float32)
-    for t, size, want, what in ((codes, 1, count, "codes"), (scales, 4, blocks, "scales")):
-        if t.numel() != want or t.element_size() != size or not t.is_contiguous():
-            raise OcoError(_lib.INVALID_ARGUMENT, f"{name} {what}: {want} contiguous elements of {size} bytes are needed, got {tuple(t.shape)} {t.dtype}")
+    for t, types, want, what in ((codes, (torch.float8_e4m3fn, torch.uint8, torch.int8), count, "codes"), (scales, (torch.float32,), blocks, "scales")):
+        if t.numel() != want or t.dtype not in types or not t.is_contiguous():
+            raise OcoError(_lib.INVALID_ARGUMENT, f"{name} {what}: {want} contiguous elements of {types[0]} are needed, got {tuple(t.shape)} {t.dtype}")
+    for t, what in ((codes, "codes"), (scales, "scales")):
+        if t.get_device() != _current_device():
+            raise OcoError(_lib.INVALID_ARGUMENT, f"{name} {what}: on {t.device}, the current device is cuda:{_current_device()}")
     return codes, scales
 
 
@@ -543,6 +546,8 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
         if t is None or t.is_contiguous():
             strides.append(0)
         elif t.stride(1) == 1:
+            if 0 < rows != 1 and t.stride(0) < width:      # expanded rows: a stride of 0 would be read as the width
+                refuse("the rows must not overlap")
             strides.append(t.stride(0) if rows > 1 else 0)
         else:
             refuse("the elements of a row must be neighbours")
@@ -560,6 +565,8 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
             if rows and (per < 1 or (rows - 1) // per >= gates):
                 refuse("gate: fewer gate rows than the rows need")
             gs = gate.stride(0) if gates > 1 else 0
+            if gates > 1 and gs == 0:                      # an expanded row: one gate for all
+                per = 0
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     args = _NORM_ARGS.pack(width, NORMS[kind], wide, gate_type, per, GATE_ACTS[gate_act], epsilon, weight_offset, residual_scale, block_scale,
                            hidden.data_ptr(), at(block), at(post_weight), at(post_bias), at(pre_weight), at(pre_bias), at(gate), at(hidden_out), at(norm_out),

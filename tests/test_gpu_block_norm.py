@@ -161,3 +161,31 @@ def test_no_rows_streams_graphs_and_refusals(moe):
         moe.block_norm(a["hidden"][:, :100].contiguous(), norm_out=no[:, :100].contiguous())       # 100 is no multiple of 8
     with pytest.raises(_lib.OcoError):
         moe.block_norm(a["hidden"][:, 4:132], norm_out=torch.empty((8, 128), dtype=torch.bfloat16, device="cuda"))   # rows start on 8 bytes
+
+
+def test_expanded_rows_and_overlaps(moe):
+    """An expanded gate is one gate for all rows; expanded rows and outputs that share rows with other inputs are refused."""
+    a = case(31, 6, 256, gate="none")
+    g = torch.randn((1, 256), device="cuda", generator=torch.Generator("cuda").manual_seed(5)).to(torch.bfloat16)
+    outs = []
+    for gate in (g, g[0], g.expand(6, 256), g.expand(3, 256)):
+        a["gate"] = gate
+        outs.append(run(moe, a, "rms", "sigmoid", 0.0, 1.0, 1.0, 1e-5))
+    for ho, no in outs[1:]:
+        assert torch.equal(ho, outs[0][0]) and torch.equal(no, outs[0][1])
+    out = torch.empty_like(a["hidden"])
+    one = a["block"][:1].expand(6, 256)
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        moe.block_norm(a["hidden"], one, norm_out=out)
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        moe.block_norm(one, norm_out=out)
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        moe.block_norm(a["hidden"], a["block"], norm_out=a["hidden"])
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        moe.block_norm(a["hidden"][1:], a["block"][1:], hidden_out=a["hidden"][:5])
+    both = torch.cat((a["hidden"], a["block"]), 1)                       # interleaved rows share no element
+    ho, no = torch.empty_like(both), None
+    moe.block_norm(both[:, :256], both[:, 256:], hidden_out=ho[:, :256], norm_out=ho[:, 256:], epsilon=1e-5)
+    a["gate"] = a["post_w"] = a["pre_w"] = None
+    want = run(moe, a, "rms", "none", 0.0, 1.0, 1.0, 1e-5)
+    assert torch.equal(ho[:, :256], want[0]) and torch.equal(ho[:, 256:], want[1])

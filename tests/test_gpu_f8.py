@@ -426,3 +426,46 @@ def test_overlap_is_refused(lib):
     fresh = lib.moe.F8ExpertPlan.new(128, 128, 4, 2)
     with pytest.raises(_lib.OcoError, match="reserve"):
         fresh.forward(x, torch.zeros((8, 2), dtype=torch.int32, device="cuda"), torch.ones((8, 2), device="cuda"), x, 8)
+
+
+@pytest.mark.parametrize("rows", [3, 24, 300])
+def test_activations_near_the_ends_of_f32(lib, rows):
+    """Activations of 1e38 and of 1e-38: their scale and quotient stay in range; down scales bring the results back."""
+    H = F = 128
+    g = gen(rows)
+    gate, gate_s = opref.weights(g, (), F, H)
+    gate_s = gate_s * 20                                    # silu(gate) is larger than one for a part of the features
+    up, up_s = opref.weights(g, (), F, H)
+    down, down_s = opref.weights(g, (), H, F)
+    x = bf16(g, rows, H)
+    for size in (1e35, 1e-35):
+        scale = up_s * size
+        unit = opref.ffn(x.double(), gate, gate_s, up, scale, down, down_s)
+        if size > 1:                                        # up to the largest activation that f32 holds with room for the products' sums
+            c, s = opref.quantize(x.double())
+            a, _ = opref.product(c, s, gate, gate_s)
+            u, _ = opref.product(c, s, up, scale)
+            scale = scale * float(2.0 ** torch.floor(torch.log2(2.5e38 / torch.maximum(u.abs().max(), (a * torch.sigmoid(a) * u).abs().max()))))
+        plan = lib.dense.DensePlan(lib.dense.FFN_SILU_GATE, synth.FMT_F8_E4M3, H, F)
+        plan.reserve(rows)
+        back = down_s * float(2.0 ** -torch.floor(torch.log2(unit.abs().max())))
+        if size > 1:
+            back = back / 2.0 ** 10
+        plan.bind(up, gate, down, up_scale=scale, gate_scale=gate_s, down_scale=back)
+        y = torch.empty_like(x)
+        plan.forward(x, y, rows)
+        plan.poll()
+        ffn_near(y, opref.ffn(x.double(), gate, gate_s, up, scale, down, back))
+
+
+def test_a_part_of_the_residual_is_refused(lib):
+    plan, w, g = expert_layer(lib, 15, 128, 128, 4, 2, 8)
+    buf, x = bf16(g, 9, 128), bf16(g, 8, 128)
+    ids, probs = torch.zeros((8, 2), dtype=torch.int32, device="cuda"), torch.ones((8, 2), device="cuda")
+    with pytest.raises(_lib.OcoError, match="overlap"):
+        plan.forward(x, ids, probs, buf[:8], 8, out=buf[1:])
+    want = torch.empty_like(x)
+    plan.forward(x, ids, probs, buf[:8], 8, out=want)
+    into = x.clone()
+    plan.forward(into, ids, probs, buf[:8], 8, out=into)    # onto x, which has been read by then
+    assert torch.equal(into, want)

@@ -151,3 +151,31 @@ def test_the_plain_forms_of_the_tests():
     x[0, 0], x[0, 1], x[0, 129] = 448.0, 17.0, -3.0
     codes, scales = opref.quantize(x)
     assert codes[0, 1] == 16.0 and codes[0, 129] == -448.0 and scales.tolist() == [[1.0, 3.0 / 448.0]]
+
+
+def test_f8_matrices_of_other_types(lib):
+    """Codes are e4m3 or bytes and scales f32: other types of the same size would be read as something else."""
+    from oco_b200 import moe
+    codes, scales = torch.zeros((64, 128), dtype=torch.uint8), torch.ones((1, 1))
+    for c, s in ((codes.view(torch.float8_e5m2), scales), (codes.view(torch.bool), scales), (codes, scales.view(torch.int32))):
+        with pytest.raises(_lib.OcoError, match="contiguous elements"):
+            moe.f8_matrix(c, s, (), 64, 128, "cpu", "up")
+    with pytest.raises(_lib.OcoError, match="current device"):
+        moe.f8_matrix(codes, scales, (), 64, 128, "cpu", "up")
+
+
+def test_block_norm_overlaps(lib):
+    """Rows that an output shares with an input of other rows; interleaved rows are no overlap. Refused before any CUDA call."""
+    B = 1 << 20
+    base = dict(width=64, kind=0, gate_type=1, gate_rows=1, gate_act=0, epsilon=1e-6, residual_scale=1.0, block_scale=1.0, hidden=B, block=2 * B, gate=3 * B,
+                hidden_out=4 * B, norm_out=5 * B)
+    err = C.create_string_buffer(160)
+    refused = lambda **kw: (lib.oco_moe_block_norm(C.byref(_lib.BlockNormArgs(**{**base, **kw})), 8, None, err, len(err)) == _lib.INVALID_ARGUMENT  # noqa: E731
+                            and b"overlap" in err.value)
+    assert refused(hidden_out=B + 128) and refused(hidden_out=B, hidden_stride=128) and refused(norm_out=B) and refused(norm_out=2 * B + 16)
+    assert refused(hidden_out=2 * B) and refused(hidden_out=3 * B + 7 * 128) and refused(norm_out=4 * B + 64) and refused(hidden_out=2 * B - 16)
+    assert refused(hidden_out=B + 64, hidden_stride=128, hidden_out_stride=128) and refused(hidden_out=B - 64, hidden_stride=128, hidden_out_stride=128)
+    halves = dict(hidden_stride=128, hidden_out_stride=128)
+    if not torch.cuda.is_available():      # these go on to the launch, which has no device
+        assert not refused() and not refused(hidden_out=B) and not refused(norm_out=2 * B) and not refused(hidden_out=3 * B + 8 * 128)
+        assert not refused(hidden_out=B + 128, **halves) and not refused(hidden_out=B - 128, **halves)
