@@ -325,18 +325,22 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     const int E = p.E, gs = E / p.G, K = p.K;
     const float* lrow = p.logits + (size_t)row * E;                     // read past L1: other CTAs of this kernel may have written them
     const bool soft = p.score == OCO_SCORE_SOFTMAX;
-    float l[VPL];
-    if (VPL >= 4 && E % 4 == 0 && ((uintptr_t)p.logits & 15u) == 0) {
+    // this lane's elements of E values, zero behind the last; four a load where they lie so (one a load touches every line VPL times)
+    auto lane_part = [&](const float* from, float (&v)[VPL], auto load4, auto load1) {
+        if (VPL >= 4 && E % 4 == 0 && ((uintptr_t)from & 15u) == 0) {
 #pragma unroll
-        for (int i = 0; i < VPL; i += 4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane * VPL + i < E) v = __ldcg(reinterpret_cast<const float4*>(lrow + lane * VPL + i));
-            l[i] = v.x; l[(i + 1) % VPL] = v.y; l[(i + 2) % VPL] = v.z; l[(i + 3) % VPL] = v.w;
+            for (int i = 0; i < VPL; i += 4) {
+                float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (lane * VPL + i < E) q = load4(reinterpret_cast<const float4*>(from + lane * VPL + i));
+                v[i] = q.x; v[(i + 1) % VPL] = q.y; v[(i + 2) % VPL] = q.z; v[(i + 3) % VPL] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; i++) v[i] = lane * VPL + i < E ? load1(from + lane * VPL + i) : 0.f;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPL; i++) l[i] = lane * VPL + i < E ? __ldcg(lrow + lane * VPL + i) : 0.f;
-    }
+    };
+    float l[VPL];
+    lane_part(lrow, l, [](const float4* a) { return __ldcg(a); }, [](const float* a) { return __ldcg(a); });
     uint32_t big = 0;                                                  // largest magnitude of a logit, as bits
 #pragma unroll
     for (int i = 0; i < VPL; i++) big = max(big, __float_as_uint(fabsf(l[i])));
@@ -379,10 +383,11 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         if (soft) inv = 1.0f / warp_sum_f(z);
     }
     if (p.bias) {
+        float bias[VPL];
+        lane_part(p.bias, bias, [](const float4* a) { return __ldg(a); }, [](const float* a) { return __ldg(a); });
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
-            const int x = lane * VPL + i;
-            r[i] = r[i] * inv + (x < E ? __ldg(p.bias + x) : 0.f);
+            r[i] = r[i] * inv + bias[i];
             wide = max(wide, __float_as_uint(fabsf(r[i])));
         }
         wide = warp_max(wide);
