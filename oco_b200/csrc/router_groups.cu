@@ -1,6 +1,7 @@
 // Routing with groups of experts: the router product and the selection (select.cuh) behind oco_moe_router_*.
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "host.cuh"
 #include "router_tiles.cuh"
@@ -61,15 +62,17 @@ constexpr int kRowsMax = 16;
 int launch_select(oco_moe_router* r, const SelectParams& p, bool fused, cudaStream_t st) {
     const int per_lane = (p.E + 31) / 32;
     const dim3 grid = fused ? dim3((p.rows + 3) / 4, (p.E + 7) / 8) : dim3((unsigned)((p.rows + 7LL) / 8)), block(256);
-    auto launch = [&](auto select, auto route) {
-        return fused ? launch_dependent(route, grid, block, 0, st, p, const_cast<float*>(p.logits), r->arrivals) : launch_dependent(select, grid, block, 0, st, p);
+    auto launch = [&](auto width) {
+        constexpr int VPL = decltype(width)::value;
+        if (fused) return launch_dependent(route_rows_kernel<VPL>, grid, block, 0, st, p, const_cast<float*>(p.logits), r->arrivals);
+        return p.x ? launch_dependent(select_kernel<VPL, true>, grid, block, 0, st, p) : launch_dependent(select_kernel<VPL, false>, grid, block, 0, st, p);
     };
     cudaError_t e;
-    if (per_lane <= 1) e = launch(select_kernel<1>, route_rows_kernel<1>);
-    else if (per_lane <= 2) e = launch(select_kernel<2>, route_rows_kernel<2>);
-    else if (per_lane <= 4) e = launch(select_kernel<4>, route_rows_kernel<4>);
-    else if (per_lane <= 8) e = launch(select_kernel<8>, route_rows_kernel<8>);
-    else e = launch(select_kernel<16>, route_rows_kernel<16>);
+    if (per_lane <= 1) e = launch(std::integral_constant<int, 1>());
+    else if (per_lane <= 2) e = launch(std::integral_constant<int, 2>());
+    else if (per_lane <= 4) e = launch(std::integral_constant<int, 4>());
+    else if (per_lane <= 8) e = launch(std::integral_constant<int, 8>());
+    else e = launch(std::integral_constant<int, 16>());
     if (e != cudaSuccess) return r->fail(OCO_CUDA_ERROR, "select: %s", cudaGetErrorString(e));
     r->launches++;
     return OCO_OK;

@@ -602,13 +602,13 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
 template <int VPL>
 __device__ __noinline__ void settle_row(const SelectParams& p, int row, int lane, SelectShared* sh) { select_row<VPL, true>(p, row, lane, sh); }
 
-// The tokens of a CTA of 256 threads, one per warp (row < 0: none).
-template <int VPL>
+// The tokens of a CTA of 256 threads, one per warp (row < 0: none). PRODUCT: the logits come from rows and weights.
+template <int VPL, bool PRODUCT>
 __device__ __forceinline__ void select_tokens(const SelectParams& p, int row, SelectShared& sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int left = row >= 0 ? select_row<VPL, false>(p, row, lane, nullptr) : 0;
     if (left == 1) settle_row<VPL>(p, row, lane, nullptr);
-    if (!p.x || !__syncthreads_or(left == 2)) return;
+    if (!PRODUCT || !__syncthreads_or(left == 2)) return;
     if (lane == 0) sh.rows[warp] = left == 2 ? row : -1;
     __syncthreads();
     if (warp == 0) {
@@ -620,14 +620,17 @@ __device__ __forceinline__ void select_tokens(const SelectParams& p, int row, Se
     }
 }
 
-template <int VPL>
-__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2) select_kernel(const SelectParams p) {
+// CTAs an SM: what is bound by the latency of one row after the other gains from more warps than the registers of the
+// usual path allow for (given logits, 32768 rows of 256 experts, 4 / 5 / 6: 49.8 / 47.7 / 46.5 us); behind the product,
+// where CTAs wait for exact logits, the spills weigh more (8192 rows with their product 85.2 / 85.9 / 87.8 us).
+template <int VPL, bool PRODUCT>
+__global__ void __launch_bounds__(256, VPL > 8 ? 2 : PRODUCT ? 4 : 6) select_kernel(const SelectParams p) {
     __shared__ SelectShared sh;
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();
     if (__syncthreads_or(p.status && threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u)) return;
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    select_tokens<VPL>(p, row < p.rows ? row : -1, sh);
+    select_tokens<VPL, PRODUCT>(p, row < p.rows ? row : -1, sh);
 }
 
 // Few rows: the product and the selection in one launch. A warp per expert and four tokens makes the logits (f32); the CTA
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, f
     }
     __syncthreads();
     if (!last) return;
-    select_tokens<VPL>(p, warp < 4 && t0 + warp < p.rows ? t0 + warp : -1, sh);
+    select_tokens<VPL, true>(p, warp < 4 && t0 + warp < p.rows ? t0 + warp : -1, sh);
 }
 
 }  // namespace oco
