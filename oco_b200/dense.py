@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib, synth
-from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr, f8_matrix, need
+from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr, f8_matrix, need, same_device
 
 PROJECTION, FFN_RELU2, FFN_SILU_GATE = 0, 1, 2
 
@@ -44,7 +44,10 @@ class DensePlan:
         if self.workspace is not None and max_rows <= self.max_rows:
             return
         nbytes = _lib.lib().oco_dense_workspace_bytes(self.handle, max_rows)
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        if self.fmt == synth.FMT_F8_E4M3:
+            same_device(self._weights, workspace)
+        self.workspace = workspace
         self._check(_lib.lib().oco_dense_bind_workspace(self.handle, _ptr(self.workspace), nbytes, max_rows))
         self.max_rows = max_rows
         self.device = self.workspace.get_device()

@@ -344,6 +344,15 @@ def _current_device() -> int:
     return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
 
 
+def same_device(weights, workspace: torch.Tensor):
+    """Refuses a workspace on another device than the weights that are bound already (a dict or tuple of tensors, or of
+    pairs of them)."""
+    for t in (weights.values() if isinstance(weights, dict) else weights or ()):
+        for part in t if isinstance(t, tuple) else (t,):
+            if part is not None and part.get_device() != workspace.get_device():
+                raise OcoError(_lib.INVALID_ARGUMENT, f"the workspace is on {workspace.device}, the weights are on another device")
+
+
 def _staged(a, device) -> torch.Tensor:
     if isinstance(a, np.ndarray):
         return _dev_bytes(a, device)
@@ -392,6 +401,7 @@ class _GroupPlan:
             return
         nbytes = self._fn["workspace_bytes"](self.handle, max_rows)
         ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        same_device(self._weights, ws)
         self._check(self._fn["bind_workspace"](self.handle, _ptr(ws), nbytes, max_rows))
         self.workspace, self.max_rows, self.device = ws, max_rows, ws.get_device()
 

@@ -179,3 +179,18 @@ def test_block_norm_overlaps(lib):
     if not torch.cuda.is_available():      # these go on to the launch, which has no device
         assert not refused() and not refused(hidden_out=B) and not refused(norm_out=2 * B) and not refused(hidden_out=3 * B + 8 * 128)
         assert not refused(hidden_out=B + 128, **halves) and not refused(hidden_out=B - 128, **halves)
+
+
+def test_a_workspace_on_another_device_than_the_weights(lib):
+    from oco_b200 import dense, moe, synth
+
+    class OnSecondDevice:
+        def get_device(self):
+            return 1
+    there = OnSecondDevice()
+    plans = moe.RouterPlan.new(256, 8, 2), moe.F8ExpertPlan.new(128, 128, 4, 2), dense.DensePlan(dense.PROJECTION, synth.FMT_F8_E4M3, 128, 64)
+    for plan, held in zip(plans, ((there, None), {"gate_w": there}, {"up": (there, there)})):
+        plan._weights = held
+        with pytest.raises(_lib.OcoError, match="another device"):
+            plan.reserve(8, device="cpu")
+        assert plan.workspace is None
