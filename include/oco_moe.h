@@ -465,8 +465,7 @@ int oco_moe_block_norm(const oco_moe_block_norm_args* args, int rows, void* cuda
  * elements: scale = largest / 448, code = e4m3(x * 448 / largest). Products of codes are summed in f32 over the
  * 128 elements of a block on the tensor cores, the blocks' sums in f32 under the product of their scales:
  *     g = gate . x, u = up . x, a = silu(g) * u (f32), rounded to e4m3 as the rows are, y = down . a
- *     out[t] = residual[t] + sum_r prob[t, r] * y[t, r]        (f32, one rounding; in calls of more than three tokens y
- *                                                              travels through memory as bf16)
+ *     out[t] = residual[t] + sum_r prob[t, r] * y[t, r]        (f32, one rounding)
  * The ids may come from any router, one expert twice for a token included; an id outside 0 .. experts-1 is a route of another shard or of padding and is
  * left out (its weight is not read). A row without any route keeps its residual. */
 typedef struct {

@@ -31,7 +31,7 @@ struct F8Space {
     float* xs = nullptr;          // their scales [H blocks][pitch]
     uint8_t* aq = nullptr;        // codes of the activations [R][F]
     float* as = nullptr;
-    uint16_t* y = nullptr;        // bf16 [R][H], route order
+    float* y = nullptr;           // f32 [R][H], route order
     int pitch = 0;
     size_t total = 0;
 };
@@ -73,7 +73,7 @@ F8Space carve(int kind, const oco_moe_f8_desc& d, int max_rows, unsigned char* b
         w.aq = take(R * F);
         w.as = (float*)take((F + 127) / 128 * w.pitch * 4);
     }
-    if (kind == kF8Experts) w.y = (uint16_t*)take(R * H * 2);
+    if (kind == kF8Experts) w.y = (float*)take(R * H * 4);
     w.total = off;
     return w;
 }
@@ -214,7 +214,8 @@ int run_rows(oco_moe_f8_plan* plan, const uint16_t* x, const uint32_t* ids, cons
     p.s0 = plan->w.gate_s; p.s1 = plan->w.up_s; p.codes = ws.aq; p.code_scales = ws.as;
     if (int rc = product<true>(plan, p, plan->map_x, plan->map_gate, plan->map_up, index, tiles, expected, st)) return rc;
     q.row_scales = ws.as; q.K = F; q.n = H; q.s0 = plan->w.down_s;
-    q.out = routed ? ws.y : out; q.route_of_row = routed ? ws.route_of_row : nullptr;
+    if (routed) { q.sums = ws.y; q.route_of_row = ws.route_of_row; }
+    else q.out = out;
     if (int rc = product<false>(plan, q, plan->map_a, plan->map_down, plan->map_down, index, tiles, expected, st)) return rc;
     if (routed) {
         const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (H / 8) + 255) / 256, 16LL * plan->sm_count);

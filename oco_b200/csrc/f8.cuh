@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) f8_rows_kernel(const uint16_t* x, const u
 // ---- weighted combination --------------------------------------------------------------------------------------------
 // out[t] = residual[t] + sum_r prob[t, r] y[t, r], one rounding; routes without an expert of this plan are left out. A
 // thread takes eight columns of a row.
-__global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* y, const uint32_t* ids, const float* probs,
+__global__ void __launch_bounds__(256) f8_combine_kernel(const float* y, const uint32_t* ids, const float* probs,
                                                          const uint16_t* residual, uint16_t* out, int rows, int top_k, int H, int E) {
     pdl_launch_dependents();   // the next kernel of the step may be set up beside this one
     pdl_wait();                // the kernel before has completed and its writes are visible
@@ -194,21 +194,24 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const uint16_t* y, cons
         const uint4 q = *reinterpret_cast<const uint4*>(residual + (size_t)t * H + c);
         float sum[8] = {};
         for (int r0 = 0; r0 < top_k; r0 += 4) {                        // four routes' rows on their way at a time
-            uint4 v[4];
+            float4 v[4][2];
             float pr[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const bool live = r0 + r < top_k && ids[(size_t)t * top_k + r0 + r] < (uint32_t)E;
                 pr[r] = live ? probs[(size_t)t * top_k + r0 + r] : 0.f;
-                v[r] = live ? *reinterpret_cast<const uint4*>(y + ((size_t)t * top_k + r0 + r) * H + c) : make_uint4(0, 0, 0, 0);
+                const float4* from = reinterpret_cast<const float4*>(y + ((size_t)t * top_k + r0 + r) * H + c);
+#pragma unroll
+                for (int j = 0; j < 2; j++) v[r][j] = live ? from[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const uint32_t u[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    sum[2 * j] = fmaf(pr[r], __uint_as_float(u[j] << 16), sum[2 * j]);
-                    sum[2 * j + 1] = fmaf(pr[r], __uint_as_float(u[j] & 0xffff0000u), sum[2 * j + 1]);
+                for (int j = 0; j < 2; j++) {
+                    sum[4 * j] = fmaf(pr[r], v[r][j].x, sum[4 * j]);
+                    sum[4 * j + 1] = fmaf(pr[r], v[r][j].y, sum[4 * j + 1]);
+                    sum[4 * j + 2] = fmaf(pr[r], v[r][j].z, sum[4 * j + 2]);
+                    sum[4 * j + 3] = fmaf(pr[r], v[r][j].w, sum[4 * j + 3]);
                 }
             }
         }

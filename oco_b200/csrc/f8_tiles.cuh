@@ -29,6 +29,7 @@ struct F8TileParams {
     const uint32_t* offsets;
     const uint32_t* route_of_row;   // result rows (not gated); null: in place
     uint16_t* out;                  // bf16 [..][n]
+    float* sums;                    // instead of out, where results are summed afterwards: f32 [..][n]
     uint8_t* codes;                 // gated: codes of the activations [row][n]
     float* code_scales;             // and their scales [ceil(n / 128)][pitch]
     uint32_t* status;
@@ -61,7 +62,7 @@ struct F8Wide {
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10, kThreads = 384;
     static constexpr int kScaleRun = 4, kScales = 3;                    // scales travel in runs of four blocks, three runs
     static constexpr int kScaleBytes = 128 * 2 * 4;                     // of a block: 128 rows under two blocks of features
-    static constexpr int kOutPitch = 256 + 16;                          // a row's 128 results, spread over the banks
+    static constexpr int kOutPitch = 256 + 16;                          // a row's 128 results (64 in f32), spread over the banks
     static constexpr int kOut = kStages * kStage, kCtrlAt = kOut + 8 * 32 * kOutPitch;
     static constexpr int kTops = 512, kRing = kTops + 2 * 128 * 4, kCtrl = kRing + kScales * kScaleRun * kScaleBytes;
     static constexpr int kSmem = kCtrlAt + kCtrl + 1024;
@@ -266,19 +267,36 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
             } else {
                 const int f = it.f0 + 128 * half;
                 const size_t row = !live ? 0 : p.route_of_row ? p.route_of_row[it.row0 + erow] : (uint32_t)(it.row0 + erow);
+                if (!PAIR && p.sums) {                                // f32: 64 features at a time
 #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    uint32_t w[4];
+                    for (int h = 0; h < 2; h++) {
+                        if (h) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float v0, v1;
-                        f32x2_split(acc[4 * c + k], v0, v1);
-                        const __nv_bfloat162 o = __floats2bfloat162_rn(v0, v1);
-                        w[k] = *reinterpret_cast<const uint32_t*>(&o);
+                        for (int c = 0; c < 16; c++) {
+                            float v[4];
+                            f32x2_split(acc[32 * h + 2 * c], v[0], v[1]);
+                            f32x2_split(acc[32 * h + 2 * c + 1], v[2], v[3]);
+                            const uint32_t w[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                            store16(c, w);
+                        }
+                        const int fh = f + 64 * h;
+                        send(p.sums + row * p.n + fh, 4u * (uint32_t)max(0, min(64, p.n - fh)), live && fh < p.n);
                     }
-                    store16(c, w);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            float v0, v1;
+                            f32x2_split(acc[4 * c + k], v0, v1);
+                            const __nv_bfloat162 o = __floats2bfloat162_rn(v0, v1);
+                            w[k] = *reinterpret_cast<const uint32_t*>(&o);
+                        }
+                        store16(c, w);
+                    }
+                    send(p.out + row * p.n + f, 2u * (uint32_t)max(0, min(128, p.n - f)), live && f < p.n);
                 }
-                send(p.out + row * p.n + f, 2u * (uint32_t)max(0, min(128, p.n - f)), live && f < p.n);
             }
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -675,6 +693,10 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
                     const uint2 q = *reinterpret_cast<const uint2*>(p.residual + row * p.n + f);
                     v[0].x += __uint_as_float(q.x << 16); v[0].y += __uint_as_float(q.x & 0xffff0000u);
                     v[0].z += __uint_as_float(q.y << 16); v[0].w += __uint_as_float(q.y & 0xffff0000u);
+                }
+                if (FORM == kF8Tiles && p.sums) {
+                    *reinterpret_cast<float4*>(p.sums + row * p.n + f) = v[0];
+                    continue;
                 }
                 const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0].x, v[0].y), hi = __floats2bfloat162_rn(v[0].z, v[0].w);
                 *reinterpret_cast<uint2*>(p.out + row * p.n + f) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));

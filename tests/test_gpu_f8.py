@@ -469,3 +469,36 @@ def test_a_part_of_the_residual_is_refused(lib):
     into = x.clone()
     plan.forward(into, ids, probs, buf[:8], 8, out=into)    # onto x, which has been read by then
     assert torch.equal(into, want)
+
+
+@pytest.mark.parametrize("H,F", [(128, 1024), (416, 1056)])
+@pytest.mark.parametrize("rows", [1, 3, 4, 40, 300, 1500])
+def test_routes_are_summed_before_they_are_rounded(lib, rows, H, F):
+    """Two experts whose results nearly cancel: down codes of opposite sign, but for one of each feature's. What is left is
+    about 2 / sqrt(F) of either, and is off by its own rounding, 2^-8, by activations on the other side of a border
+    between codes (ffn_near: 2^-8), and by the f32 sums: a block's four MMAs cut off up to 33 addends at 2^-25 of the
+    largest and the sum at 2^-23, 4 * 18.5 * 2^-24, its nine blocks add 2 * 9 * 2^-24: below 2^-17 of the terms' sizes.
+    Results rounded to bf16 on their way would leave 2^-8 / sqrt(3) * 0.7 * sqrt(2) * sqrt(F) / 2 = 0.037 and more."""
+    g = gen(rows + F)
+    w = {}
+    for n, shape in (("gate", (F, H)), ("up", (F, H)), ("down", (H, F))):
+        w[n], w[n + "_s"] = (t.repeat(2, 1, 1) for t in opref.weights(g, (1,), *shape))
+    kept = torch.randint(0, F, (H, 1), device="cuda", generator=g)
+    w["down"][1] = (w["down"][0].float() * torch.full((H, F), -1.0, device="cuda").scatter_(1, kept, 1.0)).to(torch.float8_e4m3fn)
+    plan = lib.moe.F8ExpertPlan.new(H, F, 2, 2)
+    plan.reserve(rows)
+    plan.bind(lib.moe.F8Experts(w["gate"], w["gate_s"], w["up"], w["up_s"], w["down"], w["down_s"]))
+    x, res = bf16(g, rows, H), torch.zeros((rows, H), dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([[0, 1]] * rows, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(res)
+    plan.forward(x, ids, torch.ones((rows, 2), device="cuda"), res, rows, out=out)
+    plan.poll()
+    one = {n: w[n][0] for n in w}
+    c, s = opref.quantize(x.double())
+    gg, uu = opref.product(c, s, one["gate"], one["gate_s"])[0], opref.product(c, s, one["up"], one["up_s"])[0]
+    ac, as_ = opref.quantize(gg * torch.sigmoid(gg) * uu)
+    y0, terms = opref.product(ac, as_, one["down"], one["down_s"])
+    y1 = opref.product(ac, as_, w["down"][1], w["down_s"][1])[0]
+    want = y0 + y1
+    err = (out.double() - want).norm()
+    assert err <= (2.0 ** -8 + 2.0 ** -8) * want.norm() + 2.0 ** -17 * 2 * terms.norm(), err / want.norm()
