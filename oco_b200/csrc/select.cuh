@@ -55,7 +55,8 @@ constexpr float kLogitError = 1.5e-6f;
 // quotient's two units: below 4e-7.
 // A softmax score relative to the largest one: the same and the rounding of l - top (x e^-x < 0.37), the sum and its
 // reciprocal. kHalfUlp: the rounding of score + bias.
-constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f;
+// kLeast: 2^-126, below which the last bits of a value (an index stands there in a sorted key) weigh more than its size tells.
+constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f, kLeast = 1.1754944e-38f;
 
 // ---- exact logits, summed by a whole CTA ------------------------------------------------------------------------------
 struct SelectShared {
@@ -422,7 +423,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     sort_keys(key);
     // the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
     auto value = [&](uint32_t k) { return k < 0x00800000u ? -INFINITY : key_rank(k); };
-    auto margin = [&](float v) { return 2.f * ek + (VPL > 1 ? 2.f * VPL * kHalfUlp * 2.f * fabsf(v) : 0.f); };
+    auto margin = [&](float v) { return 2.f * ek + (VPL > 1 ? 2.f * VPL * kHalfUlp * 2.f * fabsf(v) + kLeast : 0.f); };
     // two values, the first not below the second, that are not told apart (also two of -inf)
     auto too_near = [&](float a, float b) { return (VPL > 1 || ek > 0.f) && !(a - b > margin(a)); };
     auto expert_of = [&](uint32_t k, int from) { return from * VPL + (int)(kIndex - (k & kIndex)); };
@@ -498,7 +499,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         const float wa = key_rank(kt), wb = key_rank(k2);
         // error of a worth: of one value, or of two and the rounding of their sum
         const float size = !pairs ? fabsf(wa) : p.bias ? __uint_as_float(wide) : 1.f;
-        const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size : 0.f) + kHalfUlp * size;
+        const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size + kLeast : 0.f) + kHalfUlp * size;
         const float near_w = pairs ? 4.f * one : 2.f * one;
         if ((VPL > 1 || ek > 0.f || pairs) && !(wa - wb > near_w) && !any_bad) {
             // the border lies between two groups: their exact worths decide, unless a third one is as near or what a group

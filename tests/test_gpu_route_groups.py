@@ -280,3 +280,23 @@ def test_a_bias_that_is_nan_or_leaves_too_few(moe):
     r.bind(None, b)
     r.select(logits, ids, probs, 9)
     assert (ids.cpu().numpy() % 2 == 1).all()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,K,groups,top_groups,best", [(64, 1, 1, 1, 1), (256, 1, 1, 1, 1), (256, 2, 1, 1, 1), (512, 2, 1, 1, 1), (32, 1, 1, 1, 1),
+                                                         (64, 1, 4, 1, 1), (256, 2, 8, 2, 1), (512, 1, 16, 1, 1), (270, 1, 5, 1, 1), (256, 1, 8, 1, 2)])
+@pytest.mark.parametrize("size", [0.0, 1e-42, 1e-38])
+def test_two_equal_values_near_zero(moe, score, E, K, groups, top_groups, best, size):
+    """Two logits of the same value at and near zero (+0 and -0 among them), the others below: the lower index comes first."""
+    shape = (E, K, score, groups, top_groups, best, False, True, 1.0)
+    rows = 96
+    r, _, _, g = make(moe, shape, 0, rows, 40)
+    at = torch.rand((rows, E), device="cuda", generator=g).topk(2, 1).indices
+    logits = torch.full((rows, E), -1.0, device="cuda").scatter_(1, at, size)
+    if size == 0.0:
+        logits[torch.arange(0, rows, 2, device="cuda"), at[::2, 0]] = -0.0
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    want, p = expect(shape, logits.double(), None)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
