@@ -363,8 +363,11 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
             if (lane * VPL + i < E) m = fmaxf(m, l[i]);
         top = key_rank(warp_max(rank_key(m)));
     }
-    // What is ranked: score + bias; without a bias the logit itself, which has the same order. ek: the largest error of a
-    // ranking value, es: of a score (a softmax's relative to the largest score, which is inv).
+    // What is ranked: score + bias; without a bias the logit itself, which has the same order, or, where a softmax's groups
+    // are worth two scores, its distance from the largest (a score is made of the ranked value then, and its error is that
+    // value's: a common offset of the logits must not enter it). ek: the largest error of a ranking value but for what
+    // grows with its size, es: of a score (a softmax's relative to the largest score, which is inv).
+    const bool shifted = soft && pairs && !p.bias;
     float ek = dl;
     const float es = soft ? kScoreError + dl : kSigmoidError + 0.25f * dl;
     float r[VPL];
@@ -404,7 +407,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         ek = (soft ? inv * es : es) + kHalfUlp * __uint_as_float(wide);
     } else {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) r[i] = l[i];
+        for (int i = 0; i < VPL; i++) r[i] = shifted ? l[i] - top : l[i];
     }
     uint32_t key[VPL];
     if (any_bad || bad_bias) {                               // a NaN among the values, or a logit that ranks last
@@ -423,9 +426,9 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     sort_keys(key);
     // the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
     auto value = [&](uint32_t k) { return k < 0x00800000u ? -INFINITY : key_rank(k); };
-    auto margin = [&](float v) { return 2.f * ek + (VPL > 1 ? 2.f * VPL * kHalfUlp * 2.f * fabsf(v) + kLeast : 0.f); };
+    auto margin = [&](float v) { return 2.f * ek + 2.f * kHalfUlp * fabsf(v) * ((VPL > 1 ? 2.f * VPL : 0.f) + (shifted ? 1.f : 0.f)) + (VPL > 1 ? kLeast : 0.f); };
     // two values, the first not below the second, that are not told apart (also two of -inf)
-    auto too_near = [&](float a, float b) { return (VPL > 1 || ek > 0.f) && !(a - b > margin(a)); };
+    auto too_near = [&](float a, float b) { return (VPL > 1 || ek > 0.f || shifted) && !(a - b > margin(a)); };
     auto expert_of = [&](uint32_t k, int from) { return from * VPL + (int)(kIndex - (k & kIndex)); };
     double z64 = 0.0;                                                  // the softmax's sum in 64 bits, made when it is needed
     auto sum64 = [&]() {
@@ -459,10 +462,10 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
                 if (lane == from) { m[0] = m[1]; m[1] = m[2]; m[2] = 0; }
             }
         };
-        auto worth_of = [&](float a, float b) {                        // without a bias of scores, a softmax's relative to the largest
+        auto worth_of = [&](float a, float b) {                        // of ranking values; without a bias a softmax's scores relative to the largest
             if (!pairs) return a;
             if (p.bias) return a + b;
-            return soft ? expf(a - top) + expf(b - top) : __fdividef(1.0f, 1.0f + expf(fminf(-a, 80.0f))) + __fdividef(1.0f, 1.0f + expf(fminf(-b, 80.0f)));
+            return soft ? expf(a) + expf(b) : __fdividef(1.0f, 1.0f + expf(fminf(-a, 80.0f))) + __fdividef(1.0f, 1.0f + expf(fminf(-b, 80.0f)));
         };
         float worth = -INFINITY;                                       // lane g: group g
         const int lanes = gs / VPL;
@@ -499,7 +502,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         const float wa = key_rank(kt), wb = key_rank(k2);
         // error of a worth: of one value, or of two and the rounding of their sum
         const float size = !pairs ? fabsf(wa) : p.bias ? __uint_as_float(wide) : 1.f;
-        const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size + kLeast : 0.f) + kHalfUlp * size;
+        const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size + kLeast : 0.f) + (shifted ? 2.f : 1.f) * kHalfUlp * size;
         const float near_w = pairs ? 4.f * one : 2.f * one;
         if ((VPL > 1 || ek > 0.f || pairs) && !(wa - wb > near_w) && !any_bad) {
             // the border lies between two groups: their exact worths decide, unless a third one is as near or what a group

@@ -300,3 +300,25 @@ def test_two_equal_values_near_zero(moe, score, E, K, groups, top_groups, best, 
     want, p = expect(shape, logits.double(), None)
     assert np.array_equal(ids.cpu().numpy(), want)
     np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
+
+
+@pytest.mark.parametrize("offset", [0.0, 100.0, -100.0, 300.0, -300.0])
+@pytest.mark.parametrize("E,K,groups,top_groups", [(256, 8, 8, 4), (64, 4, 4, 2), (32, 4, 4, 1), (512, 16, 32, 5), (270, 9, 5, 2)])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_a_common_offset_does_not_choose_the_groups(moe, offset, E, K, groups, top_groups, normalize):
+    """Softmax without a bias, groups worth two scores: groups of the same logits in another order, one of each a step or a
+    few larger, so that their worths lie within 1e-4 of each other and far logits have few bits for it."""
+    shape = (E, K, "softmax", groups, top_groups, 2, False, normalize, 1.0)
+    rows, size = 200, E // groups
+    r, _, _, g = make(moe, shape, 0, rows, 41)
+    base = torch.randn((rows, 1, size), device="cuda", generator=g).expand(rows, groups, size)
+    order = torch.rand((rows, groups, size), device="cuda", generator=g).argsort(2)
+    logits = torch.gather(base, 2, order) + offset
+    steps = torch.randint(0, 9, (rows, groups, 1), device="cuda", generator=g)
+    logits = logits + (logits == logits.amax(2, keepdim=True)) * steps * 2.0 ** -20 * max(1.0, abs(offset) / 8)
+    logits = logits.reshape(rows, E).contiguous()
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    want, p = expect(shape, logits.double(), None)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
