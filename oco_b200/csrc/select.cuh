@@ -104,142 +104,145 @@ __device__ __forceinline__ void dots_end(SelectShared* sh) {
 }
 
 // ---- 64-bit path ---------------------------------------------------------------------------------------------------
-struct Best { double v; int i; float e; };
+struct Best { double v; int i; };
 // The largest value of the warp, the lowest index among equals; i = -1: no candidate.
 __device__ __forceinline__ Best warp_best(Best b) {
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) {
         const double v = __shfl_xor_sync(0xffffffffu, b.v, d);
         const int i = __shfl_xor_sync(0xffffffffu, b.i, d);
-        const float e = __shfl_xor_sync(0xffffffffu, b.e, d);
-        if (i >= 0 && (b.i < 0 || v > b.v || (v == b.v && i < b.i))) { b.v = v; b.i = i; b.e = e; }
+        if (i >= 0 && (b.i < 0 || v > b.v || (v == b.v && i < b.i))) { b.v = v; b.i = i; }
     }
     return b;
 }
 
-// Writes ids and weights of one token; called by a whole warp. `l`: the lane's logits, `bad`: lanes' elements whose logit
-// is not finite never come here. Not inlined: it is rare and would cost the 32-bit path registers.
+// Writes ids and weights of one token; called by a whole warp. `d`: the largest error of a logit (0 without `sh`). Every
+// value is held with its error, and what is decided between two values is settled when their intervals do not overlap;
+// the logits of those that do are summed again. Ranked is score + bias, without a bias the logit itself: scores that
+// have run into 0 or 1 keep the order of their logits. Not inlined: it is rare and would cost the 32-bit path registers.
 template <int VPL>
-__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, SelectShared* sh) {
+__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, double d, SelectShared* sh) {
     const int E = p.E, gs = p.E / p.G;
     const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = sh != nullptr;
-    double l[VPL], s[VPL], r[VPL];
-    float e[VPL];
-    uint32_t precise = 0;                                              // bit i: element i's logit is exact
-    double top = -1e300;
-    float big = 0.f;
+    const bool scored = !p.bias && p.best == 2 && gs > 1;              // groups are worth scores, experts are ranked by logits
+    double l[VPL], s[VPL], r[VPL], er[VPL], w[VPL], ew[VPL];           // logit, score, rank and part of a group's worth with their errors
+    uint32_t precise = remake ? 0u : 0xffffffffu;                      // bit i: element i's logit is exact
+    double top = -1.0 / 0.0;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         const int x = lane * VPL + i;
         l[i] = x < E ? (double)__ldcg(lrow + x) : 0.0;
-        if (x < E) { top = fmax(top, l[i]); big = fmaxf(big, fabsf((float)l[i])); }
+        if (x < E) top = fmax(top, l[i]);
     }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float d = kLogitError * __uint_as_float(warp_max(__float_as_uint(big)));
-    if (!remake) precise = 0xffffffffu;
+    for (int k = 16; k >= 1; k >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, k));
     while (true) {
-        // scores and ranks from the present logits
-        double z = 1.0;
+        // scores, ranks and errors from the present logits
+        double z = 0.0;
         bool all = true;
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
             const int x = lane * VPL + i;
             if (x < E && !((precise >> i) & 1u)) all = false;
             s[i] = soft ? exp(l[i] - top) : 1.0 / (1.0 + exp(-l[i]));
+            if (x < E) z += s[i];
         }
         all = __all_sync(0xffffffffu, all);
-        if (soft) {
-            z = 0.0;
-#pragma unroll
-            for (int i = 0; i < VPL; i++)
-                if (lane * VPL + i < E) z += s[i];
-            z = warp_sum_d(z);
-        }
+        z = soft ? warp_sum_d(z) : 1.0;
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
             const int x = lane * VPL + i;
+            const double dl = (precise >> i) & 1u ? 0.0 : d;
+            // d ln s / dl lies between 0 and 1, and so does the slope of a sigmoid's s (1 - s) in those terms; scores lie in 0 .. 1
+            const double e = soft ? (d > 1.0 ? (dl > 0.0 ? 1.0 / 0.0 : 0.0) : s[i] * expm1(dl))
+                                  : (d > 1.0 ? (dl > 0.0 ? 1.0 : 0.0) : dl * fmin(0.25, s[i] * (1.0 - s[i]) * exp(dl)));
+            w[i] = s[i]; ew[i] = e;                                    // of a softmax before its division, which is the same for all
             s[i] /= z;
-            const float sf = (float)s[i];
-            e[i] = ((precise >> i) & 1u) ? 0.f : sf * (1.f - sf) * d * 1.01f;
-            // the sum of the softmax is not exact before all logits are; it shifts ranks only against a bias
-            if (soft && p.bias && !all) e[i] += sf * kLogitError * 0.25f;
-            r[i] = s[i];
-            if (p.bias && x < E) { r[i] = s[i] + (double)p.bias[x]; if (r[i] != r[i]) r[i] = -1.0 / 0.0; }
+            r[i] = l[i]; er[i] = dl;
+            if (p.bias) {
+                r[i] = x < E ? s[i] + (double)p.bias[x] : 0.0;
+                if (r[i] != r[i]) r[i] = -1.0 / 0.0;
+                er[i] = !soft ? e : all ? 0.0 : d > 1.0 ? 1.0 : s[i] * expm1(dl + d);   // the sum is exact when all logits are
+            }
+            if (!scored) { w[i] = r[i]; ew[i] = er[i]; }
         }
         bool open = false;                                             // a decision that exact logits could turn
         uint32_t want = 0;
-        auto group_best = [&](int g, uint32_t not_i) {                 // best element of group g, not_i: expert left out
-            Best b{0.0, -1, 0.f};
+        // sum of the p.best largest w + f * ew of group g; `last`: the smaller one of them
+        auto worth_of = [&](int g, double f, double& last) {
+            int first = -1;
+            double sum = 0.0;
+            for (int t = 0; t < min(p.best, gs); t++) {
+                Best b{0.0, -1};
 #pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                const int x = lane * VPL + i;
-                if (x < E && x / gs == g && x != (int)not_i && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = x; b.e = e[i]; }
+                for (int i = 0; i < VPL; i++) {
+                    const int x = lane * VPL + i;
+                    const double v = f == 0.0 ? w[i] : w[i] + f * ew[i];
+                    if (x < E && x / gs == g && x != first && (b.i < 0 || v > b.v)) { b.v = v; b.i = x; }
+                }
+                b = warp_best(b);
+                first = b.i;
+                last = b.v;
+                sum += b.v;
             }
-            return warp_best(b);
+            return sum;
         };
         uint32_t groups = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u;
         if (p.TG < p.G) {
-            double worth = 0.0, edge = 0.0;                            // lane g: group g
-            float err = 0.f;
+            double worth = 0.0, low = 0.0, high = 0.0, edge = 0.0;     // lane g: group g
             for (int g = 0; g < p.G; g++) {
-                const Best a = group_best(g, 0xffffffffu);
-                Best b{0.0, -1, 0.f};
-                if (p.best == 2 && gs > 1) b = group_best(g, (uint32_t)a.i);
-                if (lane == g) { worth = a.v + b.v; err = a.e + b.e; edge = b.i >= 0 ? b.v : a.v; }
+                double last, e;
+                const double a = worth_of(g, 0.0, last), b = worth_of(g, -1.0, e), c = worth_of(g, 1.0, last);
+                if (lane == g) { worth = a; low = b; high = c; edge = e; }
             }
             uint32_t left = groups;
-            Best last{0.0, -1, 0.f}, next;
-            for (int t = 0; t < p.TG; t++) {
-                last = warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1, err});
-                left &= ~(1u << last.i);
-            }
-            next = warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1, err});
+            for (int t = 0; t < p.TG; t++) left &= ~(1u << warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1}).i);
             groups &= ~left;
-            if (last.v - next.v <= (double)(last.e + next.e) && last.e + next.e > 0.f) {
+            const double out = warp_best(Best{high, ((left >> lane) & 1u) ? lane : -1}).v;
+            const double in = -warp_best(Best{-low, ((groups >> lane) & 1u) ? lane : -1}).v;
+            if (in < out) {
                 open = true;
-                for (int g = 0; g < p.G; g++) {                        // every group that could lie at the border
-                    const double wg = __shfl_sync(0xffffffffu, worth, g), eg = __shfl_sync(0xffffffffu, edge, g);
-                    const float er = __shfl_sync(0xffffffffu, err, g);
-                    if (fabs(wg - last.v) > (double)(er + 2.f * (last.e + next.e))) continue;
+                for (int g = 0; g < p.G; g++) {                        // every group at the border: what could be among its best
+                    const double lg = __shfl_sync(0xffffffffu, low, g), hg = __shfl_sync(0xffffffffu, high, g), eg = __shfl_sync(0xffffffffu, edge, g);
+                    if ((groups >> g) & 1u ? !(lg < out) : !(hg > in)) continue;
 #pragma unroll
                     for (int i = 0; i < VPL; i++) {
                         const int x = lane * VPL + i;
-                        if (x < E && x / gs == g && r[i] + e[i] >= eg - (double)er) want |= 1u << i;
+                        if (x < E && x / gs == g && w[i] + ew[i] >= eg) want |= 1u << i;
                     }
                 }
             }
         }
         uint32_t taken = 0;
-        Best prev{0.0, -1, 0.f};
         int my_id = -1;
         double my_s = 0.0;
-        for (int j = 0; j <= p.K; j++) {
-            Best b{0.0, -1, 0.f};
+        for (int j = 0; j < p.K; j++) {
+            Best b{0.0, -1};
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
                 const int x = lane * VPL + i;
-                if (x < E && ((groups >> (x / gs)) & 1u) && !((taken >> i) & 1u) && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = x; b.e = e[i]; }
+                if (x < E && ((groups >> (x / gs)) & 1u) && !((taken >> i) & 1u) && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = x; }
             }
             b = warp_best(b);
-            if (b.i < 0) break;                                        // fewer experts than K + 1
-            if (j > 0 && prev.v - b.v <= (double)(prev.e + b.e) && prev.e + b.e > 0.f) {
-                open = true;
-#pragma unroll
-                for (int i = 0; i < VPL; i++) {
-                    const int x = lane * VPL + i;
-                    // at the border anything as near as the next one could be meant
-                    if (x == prev.i || x == b.i || (j == p.K && x < E && ((groups >> (x / gs)) & 1u) && fabs(r[i] - prev.v) <= (double)(prev.e + e[i])))
-                        want |= 1u << i;
-                }
-            }
-            double sv = 0.0;
+            double sv = 0.0, low = 0.0;
 #pragma unroll
             for (int i = 0; i < VPL; i++)
-                if (lane * VPL + i == b.i) { taken |= 1u << i; sv = s[i]; }
+                if (lane * VPL + i == b.i) { taken |= 1u << i; sv = s[i]; low = r[i] - er[i]; }
             sv = __shfl_sync(0xffffffffu, sv, b.i / VPL);
-            if (lane == j && j < p.K) { my_id = b.i; my_s = sv; }
-            prev = b;
+            low = __shfl_sync(0xffffffffu, low, b.i / VPL);
+            if (lane == j) { my_id = b.i; my_s = sv; }
+            bool passes = false;                                       // one that is not taken yet could be the larger one
+#pragma unroll
+            for (int i = 0; i < VPL; i++) {
+                const int x = lane * VPL + i;
+                if (x < E && ((groups >> (x / gs)) & 1u) && !((taken >> i) & 1u) && r[i] + er[i] > low) { passes = true; want |= 1u << i; }
+            }
+            if (__any_sync(0xffffffffu, passes)) {
+                open = true;
+#pragma unroll
+                for (int i = 0; i < VPL; i++)
+                    if (lane * VPL + i == b.i) want |= 1u << i;
+            }
         }
         want &= ~precise;
         if (open && !all && !__any_sync(0xffffffffu, want != 0)) want = ~precise;   // only the softmax's sum is left to doubt
@@ -281,14 +284,15 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
 }
 
 // ---- 32-bit path -----------------------------------------------------------------------------------------------------
-// The ranking values r and scores s (64 bits) of two experts, made by a whole warp. `z`: the softmax's sum.
+// The ranking values r (score + bias, without a bias the logit) and scores s of two experts in 64 bits, made by a whole
+// warp. `z`: the softmax's sum.
 __device__ __noinline__ void exact_pair(const SelectParams& p, SelectShared* sh, int row, const float* lrow, int lane, int a, int b, double top, double z, double (&r)[2], double (&s)[2]) {
     double la = (double)__ldcg(lrow + a), lb = (double)__ldcg(lrow + b);
     if (sh) dots_ask(p, sh, row, a, b, la, lb);
     // lane 0 takes a, lane 1 takes b
     const double l = lane == 0 ? la : lb;
     const double v = p.score == OCO_SCORE_SOFTMAX ? exp(l - top) / z : 1.0 / (1.0 + exp(-l));
-    const double w = p.bias ? v + (double)p.bias[lane == 0 ? a : b] : v;
+    const double w = p.bias ? v + (double)p.bias[lane == 0 ? a : b] : l;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         r[i] = __shfl_sync(0xffffffffu, w, i);
@@ -522,7 +526,8 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
                     double r1[2], v1[2], r2[2] = {0.0, 0.0}, v2[2] = {0.0, 0.0};
                     exact_pair(p, sh, row, lrow, lane, ia[0], ib[0], (double)top, z64, r1, v1);
                     if (pairs) exact_pair(p, sh, row, lrow, lane, ia[1], ib[1], (double)top, z64, r2, v2);
-                    const double da = r1[0] + r2[0], db = r1[1] + r2[1];
+                    const bool scored = pairs && !p.bias;
+                    const double da = scored ? v1[0] + v2[0] : r1[0] + r2[0], db = scored ? v1[1] + v2[1] : r1[1] + r2[1];
                     // the softmax's sum is not exact where the logits are not: it shifts the scores' difference
                     if (sh && soft && p.bias && fabs(da - db) <= (double)dl * fabs((v1[0] + v2[0]) - (v1[1] + v2[1]))) open = true;
                     else if (db > da || (db == da && at2 < at)) left = (left | (1u << at)) & ~(1u << at2);
@@ -583,7 +588,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         }
     }
     if (EXACT && open) {
-        select_exact<VPL>(p, row, lrow, lane, sh);
+        select_exact<VPL>(p, row, lrow, lane, (double)dl, sh);
         return 0;
     }
     float s = 0.f;

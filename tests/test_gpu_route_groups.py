@@ -322,3 +322,29 @@ def test_a_common_offset_does_not_choose_the_groups(moe, offset, E, K, groups, t
     want, p = expect(shape, logits.double(), None)
     assert np.array_equal(ids.cpu().numpy(), want)
     np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,K,groups,top_groups", [(64, 4, 1, 1), (256, 16, 1, 1), (512, 8, 1, 1), (256, 8, 8, 2), (32, 4, 4, 2), (270, 9, 5, 1)])
+@pytest.mark.parametrize("far", [60.0, 700.0, -760.0, -1500.0])
+def test_scores_that_have_run_into_their_ends(moe, score, E, K, groups, top_groups, far):
+    """Without a bias the logits are what is ranked: beyond 37 a sigmoid is 1 in 64 bits too, below -745 it is 0, and so is
+    a softmax's score that far under the largest. Neighbours a few steps of f32 apart keep the order of their logits."""
+    shape = (E, K, score, groups, top_groups, 1, False, False, 1.0)
+    rows = 64
+    r, _, _, g = make(moe, shape, 0, rows, 42)
+    logits = far + torch.randint(0, 40, (rows, E), device="cuda", generator=g) * 2.0 ** -14
+    if far < 0:
+        logits[:, 7] = 0.0                                             # the softmax's largest, and one expert with a score
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    l = logits.double().cpu().numpy()
+    worth = l.reshape(rows, groups, -1).max(2)
+    kept = np.argsort(-worth, axis=1, kind="stable")[:, :top_groups]
+    open_ = np.zeros((rows, groups), bool)
+    np.put_along_axis(open_, kept, True, 1)
+    want = np.argsort(-np.where(np.repeat(open_, E // groups, 1), l, -np.inf), axis=1, kind="stable")[:, :K]
+    assert np.array_equal(ids.cpu().numpy(), want)
+    with np.errstate(over="ignore", under="ignore"):
+        s = 1.0 / (1.0 + np.exp(-l)) if score == "sigmoid" else np.exp(l - l.max(1, keepdims=True)) / np.exp(l - l.max(1, keepdims=True)).sum(1, keepdims=True)
+    np.testing.assert_allclose(probs.cpu().numpy(), np.take_along_axis(s, want, 1), rtol=REL, atol=2.0 ** -126)
