@@ -390,9 +390,10 @@ const char* oco_dense_last_error(const oco_dense_plan* plan);
  *     prob = s[id] / max(sum of the winners' s, 2^-14) if normalize, else s[id]; times scale
  * Rankings are decided in 64 bits wherever two values lie within the error of the 32-bit ones (then the
  * logits concerned are summed again in 64 bits from x and the weights), so the ids of a token do not depend
- * on the number of rows in the call. A non-finite logit makes the token's weights NaN while its ids stay
- * valid and distinct (a non-finite logit ranks last). A bias may be -inf: such an expert is chosen only when
- * nothing else is left. */
+ * on the number of rows in the call. A logit of -inf masks its expert for the token: s = 0, which ranks as 0 + bias,
+ * without a bias last, and a chosen one has the weight 0. A NaN or +inf among a token's logits, or nothing but
+ * -inf, makes the token's weights NaN while its ids stay valid and distinct (what is not finite ranks last). A bias
+ * may be -inf: such an expert is chosen only when nothing else is left. */
 typedef enum { OCO_SCORE_SIGMOID = 0, OCO_SCORE_SOFTMAX = 1 } oco_moe_score;
 typedef struct {
     int32_t hidden;      /* row width, a multiple of 32 up to 16384; 0: the plan selects from given logits only */

@@ -152,7 +152,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
             const int x = lane * VPL + i;
-            const double dl = (precise >> i) & 1u ? 0.0 : d;
+            const double dl = (precise >> i) & 1u || l[i] == -1.0 / 0.0 ? 0.0 : d;   // a masked expert is one for sure
             // d ln s / dl lies between 0 and 1, and so does the slope of a sigmoid's s (1 - s) in those terms; scores lie in 0 .. 1
             const double e = soft ? (d > 1.0 ? (dl > 0.0 ? 1.0 / 0.0 : 0.0) : s[i] * expm1(dl))
                                   : (d > 1.0 ? (dl > 0.0 ? 1.0 : 0.0) : dl * fmin(0.25, s[i] * (1.0 - s[i]) * exp(dl)));
@@ -350,11 +350,26 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
 #pragma unroll
     for (int i = 0; i < VPL; i++) big = max(big, __float_as_uint(fabsf(l[i])));
     big = warp_max(big);
-    const bool any_bad = big >= 0x7f800000u;                           // a logit is infinite or NaN: the weights will be NaN
-    if (any_bad) {
+    // A logit of -inf masks its expert: its score is 0. A NaN or +inf among the logits, or nothing but -inf, makes the
+    // weights NaN.
+    bool any_bad = false;
+    if (big >= 0x7f800000u) {
+        bool bad = false, alive = false;
+        uint32_t finite = 0;
 #pragma unroll
-        for (int i = 0; i < VPL; i++)
-            if (nonfinite(l[i])) l[i] = -3.4e38f;
+        for (int i = 0; i < VPL; i++) {
+            if (lane * VPL + i >= E) continue;
+            bad = bad || !(l[i] < INFINITY);
+            alive = alive || l[i] > -INFINITY;
+            if (!nonfinite(l[i])) finite = max(finite, __float_as_uint(fabsf(l[i])));
+        }
+        any_bad = __any_sync(0xffffffffu, bad) || !__any_sync(0xffffffffu, alive);
+        big = warp_max(finite);
+        if (any_bad) {
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (nonfinite(l[i])) l[i] = -3.4e38f;
+        }
     }
     // largest error of a logit of this row (0: they are exact as given)
     const float dl = p.x && !any_bad ? kLogitError * __uint_as_float(big) : 0.f;   // rows of zeros have exact ones

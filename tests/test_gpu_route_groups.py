@@ -348,3 +348,41 @@ def test_scores_that_have_run_into_their_ends(moe, score, E, K, groups, top_grou
     with np.errstate(over="ignore", under="ignore"):
         s = 1.0 / (1.0 + np.exp(-l)) if score == "sigmoid" else np.exp(l - l.max(1, keepdims=True)) / np.exp(l - l.max(1, keepdims=True)).sum(1, keepdims=True)
     np.testing.assert_allclose(probs.cpu().numpy(), np.take_along_axis(s, want, 1), rtol=REL, atol=2.0 ** -126)
+
+
+@pytest.mark.parametrize("shape", SHAPES[:10], ids=str)
+@pytest.mark.parametrize("share", [0.05, 0.5, 0.9])
+def test_masked_experts(moe, shape, share):
+    """Logits of -inf among finite ones: scores of 0, finite weights, the ids of the definition; rows with one expert left."""
+    E, rows = shape[0], 80
+    r, _, b, g = make(moe, shape, 0, rows, 43)
+    logits = torch.randn((rows, E), device="cuda", generator=g) * 1.5
+    gone = torch.rand((rows, E), device="cuda", generator=g) < share
+    gone[:10] = True
+    gone[torch.arange(rows, device="cuda"), torch.randint(0, E, (rows,), device="cuda", generator=g)] = False
+    logits = logits.masked_fill(gone, -float("inf"))
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    with np.errstate(over="ignore"):
+        want, p = expect(shape, logits.double(), b)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL, atol=0)
+
+
+def test_masked_experts_of_a_product(moe):
+    """A weight row of -inf behind positive rows: the expert is masked, whichever kernel makes the logits."""
+    for score, bias in (("sigmoid", True), ("softmax", False)):
+        shape = (96, 4, score, 4, 2, 2, bias, True, 1.0)
+        r, w, b, g = make(moe, shape, 256, 60, 44)
+        w[[5, 40]] = -float("inf")
+        w[60, 3] = -float("inf")
+        r.bind(w, b)
+        x = (torch.rand((60, 256), device="cuda", generator=g) + 0.1).to(torch.bfloat16)
+        exact = x.double() @ w.double().t()
+        with np.errstate(over="ignore"):
+            want, p = expect(shape, exact, b)
+        for rows in (3, 60):
+            ids, probs = outputs(shape, rows)
+            r.forward(x[:rows].contiguous(), ids, probs, rows)
+            assert np.array_equal(ids.cpu().numpy(), want[:rows])
+            np.testing.assert_allclose(probs.cpu().numpy(), p[:rows], rtol=2.0 ** -16)
