@@ -15,7 +15,9 @@ struct oco_moe_router : PlanBase {
     const float* bias = nullptr;
     uint32_t* status = nullptr;
     uint32_t* arrivals = nullptr;     // route_rows_kernel's counters, left at zero by every call
+    float* w_norm = nullptr;          // the largest norm of an expert's weights
     float* logits = nullptr;
+    float* errors = nullptr;          // of the logits of a row, for each 128 experts
     uint16_t* pieces = nullptr;       // the weights as three bf16 pieces [3][experts rounded up to 128][hidden]
     CUtensorMap map_w;
     bool laid_out = false;            // pieces and map match the bound weights and workspace
@@ -25,13 +27,14 @@ namespace {
 
 int padded(int experts) { return (experts + 127) / 128 * 128; }
 
-struct RouterSpace { size_t status, logits, pieces, total; };
+struct RouterSpace { size_t status, logits, errors, pieces, total; };
 RouterSpace carve(const oco_moe_router_desc& d, int max_rows) {
     RouterSpace s{};
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off = align_up(off + bytes, 256); return at; };
     s.status = take(256);
     s.logits = take(d.hidden ? (size_t)max_rows * d.experts * 4 : 0);
+    s.errors = take(d.hidden ? (size_t)max_rows * (padded(d.experts) / 128) * 4 : 0);
     s.pieces = take((size_t)3 * padded(d.experts) * d.hidden * 2);
     s.total = off;
     return s;
@@ -46,6 +49,9 @@ int lay_out(oco_moe_router* r) {
     const int Ep = padded(d.experts);
     OCO_CK(r, cudaDeviceSynchronize());     // the weights have been written, on whatever stream
     router_pieces_kernel<<<4 * r->sm_count, 256>>>(r->w, r->pieces, d.experts, Ep, d.hidden);
+    OCO_CK(r, cudaGetLastError());
+    OCO_CK(r, cudaMemset(r->w_norm, 0, 4));
+    router_norms_kernel<<<d.experts, 256>>>(r->w, (uint32_t*)r->w_norm, d.hidden);
     OCO_CK(r, cudaGetLastError());
     OCO_CK(r, cudaDeviceSynchronize());
     const CUresult e = encode_rows(&r->map_w, r->pieces, (uint64_t)3 * Ep, (uint64_t)d.hidden, 2, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
@@ -127,7 +133,9 @@ int oco_moe_router_bind_workspace(oco_moe_router* r, void* workspace, size_t byt
     unsigned char* base = (unsigned char*)workspace;
     r->status = (uint32_t*)(base + s.status);
     r->arrivals = r->status + 16;
+    r->w_norm = (float*)(r->status + 32);
     r->logits = (float*)(base + s.logits);
+    r->errors = (float*)(base + s.errors);
     r->pieces = (uint16_t*)(base + s.pieces);
     r->max_rows = max_rows;
     r->have_ws = true;
@@ -158,7 +166,7 @@ int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint3
     float* lg = logits ? logits : r->logits;
     const oco_moe_router_desc& d = r->d;
     SelectParams p = select_params(r, lg, rows, ids, probs);
-    p.x = x; p.w = r->w; p.status = r->status;
+    p.x = x; p.w = r->w; p.status = r->status; p.errors = r->errors; p.w_norm = r->w_norm;
     if (rows > kRowsMax) {
         CUtensorMap map_x;
         const CUresult e = encode_rows(&map_x, (void*)x, (uint64_t)rows, (uint64_t)d.hidden, 2, 128);
@@ -168,7 +176,7 @@ int oco_moe_router_forward(oco_moe_router* r, const uint16_t* x, int rows, uint3
         unsigned split = 1;      // parts of the contraction, four stages of 64 or more each, while they find idle SMs
         while (split < 8 && items * (int)split * 2 <= r->sm_count && chunks >= 8 * (int)split) split *= 2;
         OCO_CK(r, launch_dependent_clusters(router_tile_kernel, split, dim3((unsigned)items * split), dim3(RouterTile::kThreads), RouterTile::kSmem, st, map_x, r->map_w,
-                                            lg, rows, d.experts, Ep, d.hidden, r->status));
+                                            lg, r->errors, r->w_norm, rows, d.experts, Ep, d.hidden, r->status));
         r->launches++;
     }
     return launch_select(r, p, rows <= kRowsMax, st);

@@ -2,24 +2,31 @@
 //
 // The rows are bf16; an f32 weight is the exact sum of three bf16 pieces of falling size (8 bits of its 24 each), laid
 // out once when the weights are bound. Three kind::f16 products with bf16 operands then add exact terms into f32
-// accumulators. What is left is the rounding of the sums, which tensor memory cuts off instead of rounding to nearest
-// (with one accumulator read out every 512 terms, 96 additions, the logits came out 1.6e-6 too small): the largest pieces
-// have an accumulator of their own, and after every 256 terms (16 additions to it) both are read out and added, rounding
-// to nearest, to sums in registers.
+// accumulators. What is left is the rounding of the sums, which tensor memory cuts off instead of rounding to nearest:
+// an MMA adds 16 products and the accumulator, each cut at 2^-25 of the largest one's power of two, and cuts the sum to
+// 24 bits (seen on single terms of falling size beside one of size 1). So the largest pieces have an accumulator of their
+// own, and after every 64 terms (four additions to it) both are read out and added, rounding to nearest, to sums in
+// registers.
+//
+// The selection has to know how far a logit may be off. In units of 2^-24 |x| |w|: 17 / 2 + 2 for each of the four MMAs,
+// 2^-8 of twice that for the smaller pieces, one for the sum of both accumulators: 44. The sums in registers and of the
+// parts: 2^-24 of the largest partial sum of a row, which is kept, for each addition. The rows' norms are taken from the
+// tiles in shared memory by the warps that wait for the MMAs anyway.
 //
 // One item = 128 rows x 128 experts; a contraction is split over the CTAs of a cluster while items do not fill the SMs,
 // and the parts are added through distributed shared memory in the order of their ranks. Each stage of shared memory
 // holds 64 columns of the rows and of the three pieces (64 KB). All waits are bounded (mbar_wait).
 #pragma once
 #include "cluster.cuh"
+#include "select.cuh"
 
 namespace oco {
 
 struct RouterTile {
     static constexpr int kTile = 128 * 128, kStage = 4 * kTile, kStages = 3;
-    static constexpr int kRun = 4;                       // stages between two readings of the accumulator
-    static constexpr int kPitch = 132;                   // f32 of a row of the parts: eight rows' 16-byte pieces fill the banks
-    static constexpr int kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
+    static constexpr int kPitch = 132;                   // f32 of a row of the parts: eight rows' 16-byte pieces fill the banks; then squares and the largest sum of both halves
+    static constexpr float kUnits = 45.f;                // of 2^-24 |x| |w|: the error of what tensor memory has summed
+    static constexpr int kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;   // warps 0 .. 7 hold the sums
     static constexpr int kCtrl = 256, kSmem = kStages * kStage + kCtrl + 1024;
     static_assert(128 * kPitch * 4 <= kStages * kStage, "the parts lie where the stages were");
 };
@@ -38,8 +45,27 @@ __global__ void __launch_bounds__(256) router_pieces_kernel(const float* __restr
     }
 }
 
+// The largest Euclidean norm of an expert's weights, rounded up (`largest`: zero before). An expert with a weight that is
+// not finite has no finite logit.
+__global__ void __launch_bounds__(256) router_norms_kernel(const float* __restrict__ w, uint32_t* __restrict__ largest, int H) {
+    __shared__ double part[8];
+    double s = 0.0;
+    for (int k = threadIdx.x; k < H; k += 256) {
+        const double v = (double)w[(size_t)blockIdx.x * H + k];
+        s = fma(v, v, s);
+    }
+    s = warp_sum_d(s);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    s = 0.0;
+    for (int i = 0; i < 8; i++) s += part[i];
+    if (s < INFINITY) atomicMax(largest, __float_as_uint(__double2float_ru(sqrt(s))));
+}
+
 __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
-                                                                             float* __restrict__ logits, int rows, int E, int Ep, int H, uint32_t* status) {
+                                                                             float* __restrict__ logits, float* __restrict__ errors, const float* __restrict__ w_norm,
+                                                                             int rows, int E, int Ep, int H, uint32_t* status) {
     using S = RouterTile;
     extern __shared__ unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -56,8 +82,8 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
     const int chunks = (H + 63) / 64, per = (chunks + split - 1) / split, c0 = min(chunks, rank * per), c1 = min(chunks, c0 + per);
     const int etiles = Ep / 128, item = (int)blockIdx.x / split, row0 = item / etiles * 128, e0 = item % etiles * 128;
     if (tid == 0) {
-        for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(tfull(b), 1); mbar_init(tempty(b), 4); }
+        for (int s = 0; s < S::kStages; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 9); }   // the MMAs, and the warps that read the rows
+        for (int b = 0; b < 2; b++) { mbar_init(tfull(b), 1); mbar_init(tempty(b), 8); }
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -80,34 +106,70 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
     pdl_launch_dependents();
 
     float* part = reinterpret_cast<float*>(gen);
-    if (warp < 4) {
-        // thread = row
-        float sum[128];
+    if (warp < 8) {
+        // thread = row 32 * (warp & 3) + lane, half of the columns
+        const int row = (warp & 3) * 32 + lane, col0 = warp < 4 ? 0 : 64;
+        uint64_t sum[32];
+        float big = 0.f;                                                   // largest magnitude of a partial sum
+        uint64_t squares = 0;                                              // of half of the row's elements
+        uint32_t some = 0;
 #pragma unroll
-        for (int j = 0; j < 128; j++) sum[j] = 0.f;
-        const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
-        for (int c = c0, run = 0; c < c1; c += S::kRun, run++) {
-            const int b = run & 1;
-            mbar_wait(tfull(b), (uint32_t)(run >> 1) & 1u, abort_flag, status);
+        for (int j = 0; j < 32; j++) sum[j] = 0;
+        const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)col0;
+        for (int c = c0, g = 0; c < c1; c++, g++) {
+            const int s = g % S::kStages, b = g & 1;
+            mbar_wait(full(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, status);
+            const unsigned char* mine = gen + s * S::kStage + row * 128;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {                                  // in an order that keeps eight rows on different banks
+                const uint4 q = *reinterpret_cast<const uint4*>(mine + (((j + (warp & 4)) ^ (row & 7)) << 4));
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint64_t v = f32x2_bits(w[k] << 16, w[k] & 0xffff0000u);
+                    squares = fma_f32x2(v, v, squares);
+                }
+                some |= q.x | q.y | q.z | q.w;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+            mbar_wait(tfull(b), (uint32_t)(g >> 1) & 1u, abort_flag, status);
             tc_fence_after();
+            const uint32_t at = taddr + 256u * b;
+            uint32_t r[2][16], u[2][16];
+            tmem_ld16(at, r[0]);
+            tmem_ld16(at + 128u, u[0]);
 #pragma unroll
-            for (int j0 = 0; j0 < 128; j0 += 32) {
-                uint32_t r[32], u[32];
-                tmem_ld32(taddr + 256u * b + j0, r);
-                tmem_ld32(taddr + 256u * b + 128u + j0, u);
+            for (int i = 0; i < 4; i++) {
                 tmem_ld_wait();
-                if (j0 == 96) {
+                if (i < 3) {                                               // the next columns travel while these are added
+                    tmem_ld16(at + 16u * (i + 1), r[(i + 1) & 1]);
+                    tmem_ld16(at + 16u * (i + 1) + 128u, u[(i + 1) & 1]);
+                } else {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tempty(b));
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j++) sum[j0 + j] += __uint_as_float(r[j]) + __uint_as_float(u[j]);
+                for (int j = 0; j < 8; j++) {
+                    uint64_t both;                                         // volatile: not before the wait above
+                    asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(both) : "l"(f32x2_bits(r[i & 1][2 * j], r[i & 1][2 * j + 1])),
+                                 "l"(f32x2_bits(u[i & 1][2 * j], u[i & 1][2 * j + 1])));
+                    uint64_t& t = sum[8 * i + j];
+                    t = add_f32x2(t, both);
+                    float lo, hi;
+                    f32x2_split(t, lo, hi);
+                    big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+                }
             }
         }
-        // every MMA of this CTA is done: the parts go where the stages were
+        // every MMA of this CTA is done, and the rows have been read: the parts go where the stages were
+        asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
-        for (int j = 0; j < 128; j += 4) *reinterpret_cast<float4*>(part + tid * S::kPitch + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+        for (int j = 0; j < 32; j += 2) *reinterpret_cast<ulonglong2*>(part + row * S::kPitch + col0 + 2 * j) = make_ulonglong2(sum[j], sum[j + 1]);
+        float even, odd;
+        f32x2_split(squares, even, odd);
+        *reinterpret_cast<float2*>(part + row * S::kPitch + 128 + 2 * (warp >> 2)) = make_float2(even + odd + (some & 0x7fff7fffu ? kLostSquares : 0.f), big);
     } else if (warp == S::kTmaWarp) {
         if (lane == 0) {
             int g = 0;
@@ -128,9 +190,8 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t x0 = umma_desc(base), w0 = umma_desc(base + S::kTile);
         for (int c = c0, g = 0; c < c1; c++, g++) {
-            const int s = g % S::kStages, run = g / S::kRun, b = run & 1;
-            const bool begins = g % S::kRun == 0, ends = g % S::kRun == S::kRun - 1 || c == c1 - 1;
-            if (begins) mbar_wait(tempty(b), ((uint32_t)(run >> 1) & 1u) ^ 1u, abort_flag, status);
+            const int s = g % S::kStages, b = g & 1;
+            mbar_wait(tempty(b), ((uint32_t)(g >> 1) & 1u) ^ 1u, abort_flag, status);
             mbar_wait(full(s), (uint32_t)(g / S::kStages) & 1u, abort_flag, status);
             tc_fence_after();
             if (elect_one()) {
@@ -140,9 +201,9 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         umma_f16(d0 + 256u * b + (q ? 128u : 0u), x0 + at + 2u * k, w0 + at + (uint64_t)(q * (S::kTile >> 4)) + 2u * k, idesc,
-                                 begins && q < 2 && k == 0 ? 0u : 1u);
+                                 q < 2 && k == 0 ? 0u : 1u);
                 umma_commit(empty(s));
-                if (ends) umma_commit(tfull(b));
+                umma_commit(tfull(b));
             }
             __syncwarp();
         }
@@ -164,6 +225,18 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
             const float4 w = peer_f32x4(at, (uint32_t)q);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
         }
+        float squares = 0.f, big = 0.f;
+        if (lane < split) {
+            const float4 both = peer_f32x4(base + 4u * (uint32_t)(r * S::kPitch + 128), (uint32_t)lane);
+            squares = both.x + both.z;
+            big = fmaxf(both.y, both.w);
+        }
+#pragma unroll
+        for (int d = 4; d >= 1; d >>= 1) {                                 // split is at most 8
+            squares += __shfl_xor_sync(0xffffffffu, squares, d);
+            big += __shfl_xor_sync(0xffffffffu, big, d);
+        }
+        if (lane == 0) errors[(size_t)(e0 / 128) * rows + row0 + r] = product_error(S::kUnits, squares, *w_norm) + 1.01f * 5.9604645e-8f * (float)(per + split) * big;
         float* dst = logits + (size_t)(row0 + r) * E + e0 + c;
         if (wide && c < cols) *reinterpret_cast<float4*>(dst) = v;
         else {

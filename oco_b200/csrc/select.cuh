@@ -5,9 +5,12 @@
 //
 // Everything is first done in 32 bits. Two ranking values that lie within each other's error (rounding of the score, of
 // score + bias, and the error of the logit where it came from the router product) leave their order open; such a token
-// is settled in 64 bits, where the logits that matter are summed again from x and the weights by the whole CTA (one warp
-// alone took 10 to 20 us for it). With continuous logits that is a token in a few hundred.
+// is settled in 64 bits, where the logits that matter are summed again from x and the weights. With continuous logits that
+// is a token in a few hundred where logits are given or rows are few, one in twenty behind the tensor cores, whose sums
+// have the wider bound.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace oco {
@@ -22,6 +25,8 @@ struct SelectParams {
     uint32_t* ids;
     float* probs;
     uint32_t* status;        // null, or a status word: set = nothing is written
+    const float* errors;     // behind the product: largest error of a row's logits, [tiles of 128 experts][rows]
+    const float* w_norm;     // largest Euclidean norm of an expert's weights
     int rows, E, H, K, G, TG, best, score, normalize;
     float scale;
 };
@@ -48,29 +53,32 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 
-// Error of a logit that came from the router product, relative to the largest logit of its row: a sum of exact products
-// whose partial sums are of the size of the row's logits, in 32-bit accumulators.
-constexpr float kLogitError = 1.5e-6f;
+// Error of a logit that a product of 32-bit sums has made. Its partial sums are as large as the terms make them, however
+// small the logit is where large terms cancel, so the bound is one on sums of |x w|: roundings of 2^-24 each (`units` of
+// them at most on the way of a term) times |x| |w| (Euclidean norms: no smaller than the sum of |x w|). Where the sum of
+// squares overflows nothing is known of the logits. 1.01: the rounding of all this. kLostSquares: what squares below 2^-126
+// may have lost in a row of 16384; rows of zeros go without, their logits are exact.
+constexpr float kLostSquares = 2e-34f;
+__device__ __forceinline__ float product_error(float units, float squares, float w_norm) {
+    const float e = 1.01f * units * 5.9604645e-8f * w_norm * sqrtf(squares);
+    return e < 1e30f ? e : INFINITY;
+}
 // A sigmoid in 32 bits: s (1 - s) 2^-22 from the exponential's two units in the last place, the sum's rounding and the
 // quotient's two units: below 4e-7.
 // A softmax score relative to the largest one: the same and the rounding of l - top (x e^-x < 0.37), the sum and its
 // reciprocal. kHalfUlp: the rounding of score + bias.
-// kLeast: 2^-126, below which the last bits of a value (an index stands there in a sorted key) weigh more than its size tells.
-constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f, kLeast = 1.1754944e-38f;
+// kFarError: up to here e^d - 1 is d but for a twentieth. kLeast: 2^-126, below which the last bits of a value (an index stands there in a sorted key) weigh more than its size tells.
+constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f, kFarError = 0.01f, kLeast = 1.1754944e-38f;
 
-// ---- exact logits, summed by a whole CTA ------------------------------------------------------------------------------
-struct SelectShared {
-    int rows[8];                 // rows of the CTA's warps that need exact logits, -1: none
-    int row, a, b, work;         // what is asked for: the logits of experts a and b of a row; work 0: nothing more
-    double part[2][8];
-};
-__device__ __forceinline__ void dots_share(const SelectParams& p, SelectShared* sh) {
-    const float4* wa = reinterpret_cast<const float4*>(p.w + (size_t)sh->a * p.H);
-    const float4* wb = reinterpret_cast<const float4*>(p.w + (size_t)sh->b * p.H);
-    const uint2* xr = reinterpret_cast<const uint2*>(p.x + (size_t)sh->row * p.H);
+// ---- exact logits ----------------------------------------------------------------------------------------------------
+// Partial sums of two experts' logits in 64 bits: thread t of T takes the columns 4 t .. 4 t + 3 of every 4 T.
+__device__ __forceinline__ void exact_parts(const SelectParams& p, int row, int t, int T, int a, int b, double& la, double& lb) {
+    const float4* wa = reinterpret_cast<const float4*>(p.w + (size_t)a * p.H);
+    const float4* wb = reinterpret_cast<const float4*>(p.w + (size_t)b * p.H);
+    const uint2* xr = reinterpret_cast<const uint2*>(p.x + (size_t)row * p.H);
     double a0 = 0, a1 = 0, b0 = 0, b1 = 0;
-#pragma unroll 2
-    for (int k = threadIdx.x; k < p.H / 4; k += 256) {
+#pragma unroll 4
+    for (int k = t; k < p.H / 4; k += T) {
         const float4 u = __ldg(wa + k), v = __ldg(wb + k);
         const uint2 q = xr[k];
         const double x0 = (double)__uint_as_float(q.x << 16), x1 = (double)__uint_as_float(q.x & 0xffff0000u);
@@ -78,60 +86,64 @@ __device__ __forceinline__ void dots_share(const SelectParams& p, SelectShared* 
         a0 = fma((double)u.x, x0, a0); a1 = fma((double)u.y, x1, a1); a0 = fma((double)u.z, x2, a0); a1 = fma((double)u.w, x3, a1);
         b0 = fma((double)v.x, x0, b0); b1 = fma((double)v.y, x1, b1); b0 = fma((double)v.z, x2, b0); b1 = fma((double)v.w, x3, b1);
     }
-    const double da = warp_sum_d(a0 + a1), db = warp_sum_d(b0 + b1);
-    if ((threadIdx.x & 31) == 0) { sh->part[0][threadIdx.x >> 5] = da; sh->part[1][threadIdx.x >> 5] = db; }
+    la = warp_sum_d(a0 + a1);
+    lb = warp_sum_d(b0 + b1);
 }
-// Warp 0 asks, the other warps wait in dots_serve.
-__device__ __noinline__ void dots_ask(const SelectParams& p, SelectShared* sh, int row, int a, int b, double& da, double& db) {
-    if (threadIdx.x == 0) { sh->row = row; sh->a = a; sh->b = b; sh->work = 1; }
-    __syncthreads();
-    dots_share(p, sh);
-    __syncthreads();
-    da = db = 0.0;
-    for (int w = 0; w < 8; w++) { da += sh->part[0][w]; db += sh->part[1][w]; }
-}
-__device__ __noinline__ void dots_serve(const SelectParams& p, SelectShared* sh) {
-    while (true) {
-        __syncthreads();
-        if (!sh->work) return;
-        dots_share(p, sh);
-        __syncthreads();
-    }
-}
-__device__ __forceinline__ void dots_end(SelectShared* sh) {
-    if (threadIdx.x == 0) sh->work = 0;
+// By one warp: 6 us for 4096 columns, most of it the way of the loads.
+__device__ __noinline__ void exact_logits(const SelectParams& p, int row, int lane, int a, int b, double& la, double& lb) { exact_parts(p, row, lane, 32, a, b, la, lb); }
+
+// By the eight warps of a CTA, for all of its open rows together: an eighth of every sum each.
+struct SelectShared {
+    int row[8], count[8];        // of each warp: its row, and how many logits it wants
+    int want[8][32];             // of which experts
+    double part[8][8][32];       // [warp that summed][warp that wants][place]
+};
+__device__ __noinline__ void exact_wanted(const SelectParams& p, SelectShared& sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int w = 0; w < 8; w++)
+        for (int i = 0, n = sh.count[w]; i < n; i += 2) {
+            const int j = min(i + 1, n - 1);
+            double la, lb;
+            exact_parts(p, sh.row[w], threadIdx.x, 256, sh.want[w][i], sh.want[w][j], la, lb);
+            if (lane == 0) { sh.part[warp][w][i] = la; sh.part[warp][w][j] = lb; }
+        }
     __syncthreads();
 }
 
 // ---- 64-bit path ---------------------------------------------------------------------------------------------------
 struct Best { double v; int i; };
-// The largest value of the warp, the lowest index among equals; i = -1: no candidate.
+// The largest value of the warp, of the lowest lane among equals; i = -1: no candidate. Two reductions over the halves of
+// a key that is ordered as the value is (a tree of exchanges of doubles takes three times as long).
 __device__ __forceinline__ Best warp_best(Best b) {
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
-        const double v = __shfl_xor_sync(0xffffffffu, b.v, d);
-        const int i = __shfl_xor_sync(0xffffffffu, b.i, d);
-        if (i >= 0 && (b.i < 0 || v > b.v || (v == b.v && i < b.i))) { b.v = v; b.i = i; }
-    }
-    return b;
+    const long long u = __double_as_longlong(b.v + 0.0);
+    const unsigned long long k = (unsigned long long)(u ^ (u >> 63)) ^ (u < 0 ? 0ull : 0x8000000000000000ull);
+    const bool in = b.i >= 0;
+    const uint32_t hi = warp_max(in ? (uint32_t)(k >> 32) : 0u);
+    const bool first = in && (uint32_t)(k >> 32) == hi;
+    const uint32_t lo = warp_max(first ? (uint32_t)k : 0u), lanes = __ballot_sync(0xffffffffu, first && (uint32_t)k == lo);
+    if (!lanes) return Best{0.0, -1};
+    const int from = __ffs((int)lanes) - 1;
+    return Best{__shfl_sync(0xffffffffu, b.v, from), __shfl_sync(0xffffffffu, b.i, from)};
 }
 
-// Writes ids and weights of one token; called by a whole warp. `d`: the largest error of a logit (0 without `sh`). Every
+// Writes ids and weights of one token; called by a whole warp. `d`: the largest error of a logit. Every
 // value is held with its error, and what is decided between two values is settled when their intervals do not overlap;
 // the logits of those that do are summed again. Ranked is score + bias, without a bias the logit itself: scores that
 // have run into 0 or 1 keep the order of their logits. Not inlined: it is rare and would cost the 32-bit path registers.
 template <int VPL>
-__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, double d, SelectShared* sh) {
+__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, double d) {
     const int E = p.E, gs = p.E / p.G;
-    const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = sh != nullptr;
+    const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = d > 0.0;
     const bool scored = !p.bias && p.best == 2 && gs > 1;              // groups are worth scores, experts are ranked by logits
     double l[VPL], s[VPL], r[VPL], er[VPL], w[VPL], ew[VPL];           // logit, score, rank and part of a group's worth with their errors
+    int group[VPL];                                                    // -1: behind the last expert
     uint32_t precise = remake ? 0u : 0xffffffffu;                      // bit i: element i's logit is exact
     double top = -1.0 / 0.0;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         const int x = lane * VPL + i;
         l[i] = x < E ? (double)__ldcg(lrow + x) : 0.0;
+        group[i] = x < E ? x / gs : -1;
         if (x < E) top = fmax(top, l[i]);
     }
 #pragma unroll
@@ -168,22 +180,26 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
         }
         bool open = false;                                             // a decision that exact logits could turn
         uint32_t want = 0;
-        // sum of the p.best largest w + f * ew of group g; `last`: the smaller one of them
-        auto worth_of = [&](int g, double f, double& last) {
+        // sum of the p.best largest values of group g, with their errors on top (f = 1); without (f = 0) also the sum of
+        // their lower ends, and the least of these
+        auto worth_of = [&](int g, double f, double& low, double& edge) {
             int first = -1;
             double sum = 0.0;
+            low = 0.0;
             for (int t = 0; t < min(p.best, gs); t++) {
                 Best b{0.0, -1};
+                double e = 0.0;
 #pragma unroll
                 for (int i = 0; i < VPL; i++) {
-                    const int x = lane * VPL + i;
-                    const double v = f == 0.0 ? w[i] : w[i] + f * ew[i];
-                    if (x < E && x / gs == g && x != first && (b.i < 0 || v > b.v)) { b.v = v; b.i = x; }
+                    const double v = f == 0.0 ? w[i] : w[i] + ew[i];
+                    if (group[i] == g && lane * VPL + i != first && (b.i < 0 || v > b.v)) { b.v = v; b.i = lane * VPL + i; e = ew[i]; }
                 }
-                b = warp_best(b);
-                first = b.i;
-                last = b.v;
-                sum += b.v;
+                const Best best = warp_best(b);
+                e = __shfl_sync(0xffffffffu, e, best.i / VPL);
+                first = best.i;
+                edge = t ? fmin(edge, best.v - e) : best.v - e;
+                low += best.v - e;
+                sum += best.v;
             }
             return sum;
         };
@@ -191,8 +207,8 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
         if (p.TG < p.G) {
             double worth = 0.0, low = 0.0, high = 0.0, edge = 0.0;     // lane g: group g
             for (int g = 0; g < p.G; g++) {
-                double last, e;
-                const double a = worth_of(g, 0.0, last), b = worth_of(g, -1.0, e), c = worth_of(g, 1.0, last);
+                double b, e, none, least;
+                const double a = worth_of(g, 0.0, b, e), c = remake ? worth_of(g, 1.0, none, least) : a;
                 if (lane == g) { worth = a; low = b; high = c; edge = e; }
             }
             uint32_t left = groups;
@@ -207,8 +223,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
                     if ((groups >> g) & 1u ? !(lg < out) : !(hg > in)) continue;
 #pragma unroll
                     for (int i = 0; i < VPL; i++) {
-                        const int x = lane * VPL + i;
-                        if (x < E && x / gs == g && w[i] + ew[i] >= eg) want |= 1u << i;
+                        if (group[i] == g && w[i] + ew[i] >= eg) want |= 1u << i;
                     }
                 }
             }
@@ -220,8 +235,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
             Best b{0.0, -1};
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
-                const int x = lane * VPL + i;
-                if (x < E && ((groups >> (x / gs)) & 1u) && !((taken >> i) & 1u) && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = x; }
+                if (group[i] >= 0 && ((groups >> group[i]) & 1u) && !((taken >> i) & 1u) && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = lane * VPL + i; }
             }
             b = warp_best(b);
             double sv = 0.0, low = 0.0;
@@ -234,8 +248,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
             bool passes = false;                                       // one that is not taken yet could be the larger one
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
-                const int x = lane * VPL + i;
-                if (x < E && ((groups >> (x / gs)) & 1u) && !((taken >> i) & 1u) && r[i] + er[i] > low) { passes = true; want |= 1u << i; }
+                if (group[i] >= 0 && ((groups >> group[i]) & 1u) && !((taken >> i) & 1u) && r[i] + er[i] > low) { passes = true; want |= 1u << i; }
             }
             if (__any_sync(0xffffffffu, passes)) {
                 open = true;
@@ -268,7 +281,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
                 lanes &= lanes - 1;
                 if (first < 0) { first = x; continue; }
                 double da, db;
-                dots_ask(p, sh, row, first, x, da, db);
+                exact_logits(p, row, lane, first, x, da, db);
                 keep(first, da);
                 keep(x, db);
                 first = -1;
@@ -276,7 +289,7 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
         }
         if (first >= 0) {
             double da, db;
-            dots_ask(p, sh, row, first, first, da, db);
+            exact_logits(p, row, lane, first, first, da, db);
             keep(first, da);
         }
         precise |= want;
@@ -284,20 +297,73 @@ __device__ __noinline__ void select_exact(const SelectParams& p, int row, const 
 }
 
 // ---- 32-bit path -----------------------------------------------------------------------------------------------------
-// The ranking values r (score + bias, without a bias the logit) and scores s of two experts in 64 bits, made by a whole
-// warp. `z`: the softmax's sum.
-__device__ __noinline__ void exact_pair(const SelectParams& p, SelectShared* sh, int row, const float* lrow, int lane, int a, int b, double top, double z, double (&r)[2], double (&s)[2]) {
-    double la = (double)__ldcg(lrow + a), lb = (double)__ldcg(lrow + b);
-    if (sh) dots_ask(p, sh, row, a, b, la, lb);
-    // lane 0 takes a, lane 1 takes b
-    const double l = lane == 0 ? la : lb;
-    const double v = p.score == OCO_SCORE_SOFTMAX ? exp(l - top) / z : 1.0 / (1.0 + exp(-l));
-    const double w = p.bias ? v + (double)p.bias[lane == 0 ? a : b] : l;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        r[i] = __shfl_sync(0xffffffffu, w, i);
-        s[i] = __shfl_sync(0xffffffffu, v, i);
+// A lane's keys carry the element's index in place of their last bits (VPL - 1 - i, so that of equal ones the lower index
+// comes first): sorted once, a lane's best is its first key, and taking it is a shift. What the bits hid belongs to the
+// margin below which two values are not told apart here.
+template <int VPL>
+__device__ __forceinline__ int expert_of(uint32_t k, int from) { return from * VPL + (int)((uint32_t)(VPL - 1) - (k & (uint32_t)(VPL - 1))); }
+// the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
+__device__ __forceinline__ float key_value(uint32_t k) { return k < 0x00800000u ? -INFINITY : key_rank(k); }
+
+// What two values of a token have to differ by to be told apart in 32 bits.
+struct Margin {
+    float error, relative, least;            // 2 * (error of a ranking value), of its size, and near zero
+    bool none;                               // the values are exact
+    __device__ __forceinline__ bool near(float a, float b) const { return !none && !(a - b > error + relative * fabsf(a) + least); }   // a >= b; also two of -inf
+};
+// A token's row: its logits, their error, the softmax's largest one.
+struct OpenRow {
+    const float* logits;
+    int row;
+    bool bad;                                // the weights are NaN, and nothing is settled
+    float error, top, inv;                   // inv: the largest score of a softmax, or 1
+};
+// The sum of a softmax's scores in 64 bits, where it matters: beside a bias.
+template <int VPL>
+__device__ __forceinline__ double softmax_sum(const SelectParams& p, const OpenRow& o, int lane) {
+    if (p.score != OCO_SCORE_SOFTMAX || !p.bias) return 1.0;
+    double z = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < VPL; i++)
+        if (lane * VPL + i < p.E) z += exp((double)__ldcg(o.logits + lane * VPL + i) - (double)o.top);
+    return warp_sum_d(z);
+}
+// What a token still needs: the exact logits of the experts `want` of its lanes, and with them to
+enum OpenKind {
+    kDone,
+    kWinners,        // put in order the winners that are too near: lane j's is not told apart from lane j - 1's where bit j of `near` is set
+    kGroups,         // decide between the last group that stays (`at`) and the first that goes (`at2`); lanes 0, 1 and 2, 3 want their best
+    kAll             // go through select_exact
+};
+struct Open {
+    int kind, want, my_id, at, at2;
+    uint32_t near, out;
+};
+// The lanes' exact logits where no CTA has summed them: as given, or summed by this warp.
+__device__ __forceinline__ double exact_of_lanes(const SelectParams& p, const OpenRow& o, int lane, int want) {
+    if (!(o.error > 0.f)) return want >= 0 ? (double)__ldcg(o.logits + want) : 0.0;
+    double l = 0.0;
+    for (uint32_t rest = __ballot_sync(0xffffffffu, want >= 0); rest;) {
+        const int j = __ffs((int)rest) - 1;
+        rest &= rest - 1;
+        const int k = rest ? __ffs((int)rest) - 1 : j;
+        rest &= rest - 1;
+        double a, b;
+        exact_logits(p, o.row, lane, __shfl_sync(0xffffffffu, want, j), __shfl_sync(0xffffffffu, want, k), a, b);
+        if (lane == j) l = a;
+        if (lane == k) l = b;
     }
+    return l;
+}
+// Ranking value (score + bias, without a bias the logit) and score of a lane's expert in 64 bits. `z`: the softmax's sum.
+__device__ __forceinline__ void exact_values(const SelectParams& p, const OpenRow& o, int want, double l, double z, double& r, double& v) {
+    v = p.score == OCO_SCORE_SOFTMAX ? exp(l - (double)o.top) / z : 1.0 / (1.0 + exp(-l));
+    r = !p.bias ? l : want >= 0 ? v + (double)p.bias[want] : 0.0;
+}
+// The softmax's sum is not exact where the logits are not: what it does to the difference of two values that have scores
+// va and vb in them.
+__device__ __forceinline__ bool sum_matters(const SelectParams& p, const OpenRow& o, double difference, double va, double vb) {
+    return o.error > 0.f && p.score == OCO_SCORE_SOFTMAX && p.bias && (o.error > kFarError || fabs(difference) <= 1.05 * (double)o.error * fabs(va - vb));
 }
 
 // Largest first (Batcher's merge exchange).
@@ -318,16 +384,177 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
                     }
 }
 
-// A lane's keys carry the element's index in place of their last bits (VPL - 1 - i, so that of equal ones the lower index
-// comes first): sorted once, a lane's best is its first key, and taking it is a shift. What the bits hid belongs to the
-// margin below which two values are not told apart here.
-//
-// Returns 0, or, before anything is written, what an open decision needs (only where !EXACT): 1 the exact values of the
-// logits as they are, 2 exact logits too. EXACT settles it: with `sh`, warp 0 while the others serve, else any warp.
-template <int VPL, bool EXACT>
-__device__ __forceinline__ int select_row(const SelectParams& p, int row, int lane, SelectShared* sh) {
+// Ids and weights of a token whose lane j has the j-th winner.
+__device__ __forceinline__ void write_row(const SelectParams& p, const OpenRow& o, int lane, int my_id) {
+    const bool soft = p.score == OCO_SCORE_SOFTMAX;
+    float s = 0.f;
+    if (lane < p.K) {
+        const float v = __ldcg(o.logits + my_id);
+        s = soft ? expf(v - o.top) * o.inv : 1.0f / (1.0f + expf(-v));
+    }
+    float sum = 1.0f;
+    if (p.normalize) {
+        sum = warp_sum_f(s);
+        if (!soft || p.bias) sum = fmaxf(sum, 6.103515625e-5f);        // of a softmax's largest scores: never below top_k / experts
+    }
+    if (lane < p.K) {
+        p.ids[(size_t)o.row * p.K + lane] = (uint32_t)my_id;
+        p.probs[(size_t)o.row * p.K + lane] = o.bad ? qnan() : s / sum * p.scale;
+    }
+}
+
+// A run of near winners that crosses the border takes in what is near behind it (`key`: the sorted keys that are left).
+template <int VPL>
+__device__ __noinline__ Open behind_border(const SelectParams& p, int lane, Margin margin, uint32_t (&key)[VPL], Open q, float mine) {
+    int n = p.K + 1;
+    while ((q.near >> (n - 1)) & 1u) {
+        const uint32_t m = warp_max(key[0]);
+        const float last = __shfl_sync(0xffffffffu, mine, n - 1), v = key_value(m);
+        if (!m || !margin.near(last, v)) break;
+        if (n == 32) { q.kind = kAll; break; }
+        const int from = __ffs((int)__ballot_sync(0xffffffffu, key[0] == m)) - 1;
+        if (lane == n) { q.my_id = expert_of<VPL>(m, from); mine = v; }
+        if (lane == from) {
+#pragma unroll
+            for (int i = 0; i + 1 < VPL; i++) key[i] = key[i + 1];
+            key[VPL - 1] = 0u;
+        }
+        q.near |= 1u << n++;
+    }
+    return q;
+}
+
+// The choice from sorted keys, without the groups in q.out; written, or left open.
+template <int VPL>
+__device__ __forceinline__ Open choose(const SelectParams& p, const OpenRow& o, int lane, const Margin& margin, uint32_t (&key)[VPL], Open q) {
+    const int K = p.K;
+    if (p.TG < p.G) {
+        const int gs = p.E / p.G;
+        if (gs % VPL == 0) {                                           // a lane's experts are all of one group
+            if ((q.out >> min(31, lane * VPL / gs)) & 1u) {
+#pragma unroll
+                for (int i = 0; i < VPL; i++) key[i] = 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (key[i] && ((q.out >> (expert_of<VPL>(key[i], lane) / gs)) & 1u)) key[i] = 0u;
+            sort_keys(key);
+        }
+    }
+    // top-k: lane j keeps the j-th key and the lane it came from
+    uint32_t my_key = 0;
+    int my_from = 0;
+    for (int j = 0; j <= K; j++) {
+        const uint32_t m = warp_max(key[0]);
+        const int from = __ffs((int)__ballot_sync(0xffffffffu, key[0] == m)) - 1;
+        if (lane == j) { my_key = m; my_from = from; }
+        if (lane == from) {
+#pragma unroll
+            for (int i = 0; i + 1 < VPL; i++) key[i] = key[i + 1];
+            key[VPL - 1] = 0u;
+        }
+    }
+    q.my_id = expert_of<VPL>(my_key, my_from);
+    const float mine = my_key ? key_value(my_key) : 0.f, before = __shfl_up_sync(0xffffffffu, mine, 1);
+    q.near = __ballot_sync(0xffffffffu, lane > 0 && lane <= K && my_key && margin.near(before, mine));
+    if (q.near && !o.bad) {
+        q.kind = kWinners;
+        if ((q.near >> K) & 1u) {
+            uint32_t left[VPL];                                        // a copy that may lie in memory
+#pragma unroll
+            for (int i = 0; i < VPL; i++) left[i] = key[i];
+            q = behind_border<VPL>(p, lane, margin, left, q, mine);
+        }
+        q.want = ((q.near | (q.near >> 1)) >> lane) & 1u ? q.my_id : -1;
+        return q;
+    }
+    q.kind = kDone;
+    write_row(p, o, lane, q.my_id);
+    return q;
+}
+
+// Takes an open token to its end; `l`: the exact logits of the lanes' experts. `key`: the sorted keys (kGroups).
+template <int VPL>
+__device__ __noinline__ void settle(const SelectParams& p, OpenRow o, int lane, Margin margin, uint32_t (&key)[VPL], Open q, double l) {
+    const double z = softmax_sum<VPL>(p, o, lane);
+    double r, v;
+    exact_values(p, o, q.want, l, z, r, v);
+    if (q.kind == kGroups) {
+        const bool two = p.best == 2 && p.E > p.G;
+        const double part = two && !p.bias ? v : r;                    // of a group's worth
+        auto both = [&](double t, int at) { const double first = __shfl_sync(0xffffffffu, t, at), second = __shfl_sync(0xffffffffu, t, at + 1); return two ? first + second : first; };
+        const double a = both(part, 0), b = both(part, 2);
+        if (sum_matters(p, o, a - b, both(v, 0), both(v, 2))) q.kind = kAll;
+        else {
+            if (b > a || (b == a && q.at2 < q.at)) q.out = (q.out | (1u << q.at)) & ~(1u << q.at2);
+            q = choose<VPL>(p, o, lane, margin, key, q);
+            if (q.kind == kWinners) exact_values(p, o, q.want, exact_of_lanes(p, o, lane, q.want), z, r, v);
+        }
+    }
+    if (q.kind == kWinners) {
+        const uint32_t members = q.near | (q.near >> 1);
+        const uint32_t begins = ~q.near & ((2u << lane) - 1u);         // a run's first lane is the last one up to here that is not linked to the one before
+        const int first = 31 - __clz((int)begins);
+        int place = first;
+        bool doubt = false;
+        for (uint32_t rest = members; rest; rest &= rest - 1) {
+            const int t = __ffs((int)rest) - 1;
+            const int start = __shfl_sync(0xffffffffu, first, t), it = __shfl_sync(0xffffffffu, q.my_id, t);
+            const double rt = __shfl_sync(0xffffffffu, r, t), vt = __shfl_sync(0xffffffffu, v, t);
+            if (start != first || t == lane || !((members >> lane) & 1u)) continue;
+            place += rt > r || (rt == r && it < q.my_id);
+            doubt = doubt || sum_matters(p, o, r - rt, v, vt);
+        }
+        if (__any_sync(0xffffffffu, doubt)) q.kind = kAll;
+        else {
+            int id = q.my_id;
+            for (uint32_t rest = members; rest; rest &= rest - 1) {
+                const int t = __ffs((int)rest) - 1, to = __shfl_sync(0xffffffffu, place, t), it = __shfl_sync(0xffffffffu, q.my_id, t);
+                if (lane == to) id = it;
+            }
+            write_row(p, o, lane, id);
+        }
+    }
+    if (q.kind == kAll) select_exact<VPL>(p, o.row, o.logits, lane, (double)o.error);
+}
+
+// What a decision between two groups needs: their best experts. Groups whose best are not clear go through select_exact.
+template <int VPL>
+__device__ __noinline__ Open best_of_groups(const SelectParams& p, int lane, Margin margin, const uint32_t (&key)[VPL], Open q) {
+    const int gs = p.E / p.G, best = min(p.best, gs);
+    q.kind = kGroups;
+    for (int s = 0; s < 2; s++) {
+        // the three best of the group: values, and the experts of the first two
+        const int g = s ? q.at2 : q.at;
+        uint32_t m[3] = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (key[i] && expert_of<VPL>(key[i], lane) / gs == g) {
+                if (!m[0]) m[0] = key[i];
+                else if (!m[1]) m[1] = key[i];
+                else if (!m[2]) m[2] = key[i];
+            }
+        float v[3];
+#pragma unroll
+        for (int t = 0; t < 3; t++) {
+            const uint32_t a = warp_max(m[0]);
+            const int from = __ffs((int)__ballot_sync(0xffffffffu, m[0] == a)) - 1;
+            v[t] = a ? key_value(a) : -INFINITY;
+            if (t < best && lane == 2 * s + t) q.want = expert_of<VPL>(a, from);
+            if (lane == from) { m[0] = m[1]; m[1] = m[2]; m[2] = 0; }
+        }
+        if (gs > best && (best == 2 ? margin.near(v[1], v[2]) : margin.near(v[0], v[1]))) q.kind = kAll;
+    }
+    return q;
+}
+
+// One token by one warp: written, or left open (`kept`: its sorted keys where the groups are). `error`: the largest error
+// of its logits (0: they are exact as given).
+template <int VPL>
+__device__ __forceinline__ Open select_row(const SelectParams& p, int row, float error, int lane, OpenRow& o, Margin& margin, uint32_t (&kept)[VPL]) {
     constexpr uint32_t kIndex = VPL - 1;
-    const int E = p.E, gs = E / p.G, K = p.K;
+    const int E = p.E, gs = E / p.G;
     const float* lrow = p.logits + (size_t)row * E;                     // read past L1: other CTAs of this kernel may have written them
     const bool soft = p.score == OCO_SCORE_SOFTMAX;
     // this lane's elements of E values, zero behind the last; four a load where they lie so (one a load touches every line VPL times)
@@ -371,8 +598,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
                 if (nonfinite(l[i])) l[i] = -3.4e38f;
         }
     }
-    // largest error of a logit of this row (0: they are exact as given)
-    const float dl = p.x && !any_bad ? kLogitError * __uint_as_float(big) : 0.f;   // rows of zeros have exact ones
+    const float dl = any_bad ? 0.f : error;                            // largest error of a logit of this row (0: they are exact as given)
     const bool pairs = p.TG < p.G && p.best == 2 && gs > 1;            // groups are worth two scores
     float top = 0.f, inv = 1.f;
     if (soft) {
@@ -388,7 +614,7 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
     // grows with its size, es: of a score (a softmax's relative to the largest score, which is inv).
     const bool shifted = soft && pairs && !p.bias;
     float ek = dl;
-    const float es = soft ? kScoreError + dl : kSigmoidError + 0.25f * dl;
+    const float es = !soft ? kSigmoidError + 0.25f * dl : dl > kFarError ? INFINITY : kScoreError + 2.1f * dl;   // a softmax's: of its logit and of the sum
     float r[VPL];
     uint32_t wide = 0;                                                 // largest magnitude of score + bias, as bits
     bool bad_bias = false;
@@ -443,44 +669,12 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
         }
     }
     sort_keys(key);
-    // the value a key stands for, to within VPL units in the last place; -inf and NaN: -inf
-    auto value = [&](uint32_t k) { return k < 0x00800000u ? -INFINITY : key_rank(k); };
-    auto margin = [&](float v) { return 2.f * ek + 2.f * kHalfUlp * fabsf(v) * ((VPL > 1 ? 2.f * VPL : 0.f) + (shifted ? 1.f : 0.f)) + (VPL > 1 ? kLeast : 0.f); };
-    // two values, the first not below the second, that are not told apart (also two of -inf)
-    auto too_near = [&](float a, float b) { return (VPL > 1 || ek > 0.f || shifted) && !(a - b > margin(a)); };
-    auto expert_of = [&](uint32_t k, int from) { return from * VPL + (int)(kIndex - (k & kIndex)); };
-    double z64 = 0.0;                                                  // the softmax's sum in 64 bits, made when it is needed
-    auto sum64 = [&]() {
-        if (!soft || z64 != 0.0) return;
-        double z = 0.0;
-#pragma unroll
-        for (int i = 0; i < VPL; i++)
-            if (lane * VPL + i < E) z += exp((double)__ldcg(lrow + lane * VPL + i) - (double)top);
-        z64 = warp_sum_d(z);
-    };
-
-    bool open = false;                                                 // left to select_exact
+    margin = Margin{2.f * ek, 2.f * kHalfUlp * ((VPL > 1 ? 2.f * VPL : 0.f) + (shifted ? 1.f : 0.f)), VPL > 1 ? kLeast : 0.f, VPL == 1 && ek == 0.f && !shifted};
+    o = OpenRow{lrow, row, any_bad, dl, top, inv};
+    Open q{kDone, -1, 0, 0, 0, 0u, 0u};
+    uint32_t out = 0;                                                  // groups that do not stay
     if (p.TG < p.G) {
         const bool whole = gs % VPL == 0;                              // a lane's experts are all of one group
-        // the three best of group g: values, and the experts of the first two
-        auto best_of = [&](int g, float (&v)[3], int (&id)[2]) {
-            uint32_t m[3] = {0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < VPL; i++)
-                if (key[i] && expert_of(key[i], lane) / gs == g) {
-                    if (!m[0]) m[0] = key[i];
-                    else if (!m[1]) m[1] = key[i];
-                    else if (!m[2]) m[2] = key[i];
-                }
-#pragma unroll
-            for (int t = 0; t < 3; t++) {
-                const uint32_t a = warp_max(m[0]);
-                const int from = __ffs((int)__ballot_sync(0xffffffffu, m[0] == a)) - 1;
-                v[t] = a ? value(a) : -INFINITY;
-                if (t < 2) id[t] = a ? expert_of(a, from) : g * gs;
-                if (lane == from) { m[0] = m[1]; m[1] = m[2]; m[2] = 0; }
-            }
-        };
         auto worth_of = [&](float a, float b) {                        // of ranking values; without a bias a softmax's scores relative to the largest
             if (!pairs) return a;
             if (p.bias) return a + b;
@@ -496,178 +690,113 @@ __device__ __forceinline__ int select_row(const SelectParams& p, int row, int la
                 m2 = max(max(m2, o2), min(m1, o1));
                 m1 = max(m1, o1);
             }
-            worth = __shfl_sync(0xffffffffu, worth_of(value(m1), value(m2)), min(31, lane * lanes));
+            worth = __shfl_sync(0xffffffffu, worth_of(key_value(m1), key_value(m2)), min(31, lane * lanes));
         } else {
             for (int g = 0; g < p.G; g++) {
-                float v[3];
-                int id[2];
-                best_of(g, v, id);
-                const float w = worth_of(v[0], v[1]);
+                uint32_t m1 = 0, m2 = 0;                               // the two best of group g
+#pragma unroll
+                for (int i = 0; i < VPL; i++)
+                    if (key[i] && expert_of<VPL>(key[i], lane) / gs == g) {
+                        if (!m1) m1 = key[i];
+                        else if (!m2) m2 = key[i];
+                    }
+                const uint32_t a = warp_max(m1);
+                const int from = __ffs((int)__ballot_sync(0xffffffffu, m1 == a)) - 1;
+                const uint32_t b = pairs ? warp_max(lane == from ? m2 : m1) : 0u;
+                const float w = worth_of(key_value(a), key_value(b));
                 if (lane == g) worth = w;
             }
         }
         const uint32_t wkey = lane < p.G ? rank_key(worth) : 0u;
-        uint32_t left = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u, kprev = 0, kt = 0;
+        uint32_t kprev = 0, kt = 0;
         int at = 0;
+        out = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u;
         for (int t = 0; t < p.TG; t++) {
-            const uint32_t mine = (left >> lane) & 1u ? wkey : 0u;
+            const uint32_t mine = (out >> lane) & 1u ? wkey : 0u;
             kprev = kt;
             kt = warp_max(mine);
-            at = __ffs((int)__ballot_sync(0xffffffffu, mine == kt && ((left >> lane) & 1u))) - 1;
-            left &= ~(1u << at);
+            at = __ffs((int)__ballot_sync(0xffffffffu, mine == kt && ((out >> lane) & 1u))) - 1;
+            out &= ~(1u << at);
         }
-        const uint32_t mine = (left >> lane) & 1u ? wkey : 0u, k2 = warp_max(mine);
-        const int at2 = __ffs((int)__ballot_sync(0xffffffffu, mine == k2 && ((left >> lane) & 1u))) - 1;
+        const uint32_t mine = (out >> lane) & 1u ? wkey : 0u, k2 = warp_max(mine);
+        const int at2 = __ffs((int)__ballot_sync(0xffffffffu, mine == k2 && ((out >> lane) & 1u))) - 1;
         const float wa = key_rank(kt), wb = key_rank(k2);
         // error of a worth: of one value, or of two and the rounding of their sum
         const float size = !pairs ? fabsf(wa) : p.bias ? __uint_as_float(wide) : 1.f;
         const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size + kLeast : 0.f) + (shifted ? 2.f : 1.f) * kHalfUlp * size;
         const float near_w = pairs ? 4.f * one : 2.f * one;
         if ((VPL > 1 || ek > 0.f || pairs) && !(wa - wb > near_w) && !any_bad) {
-            // the border lies between two groups: their exact worths decide, unless a third one is as near or what a group
-            // is worth is not clear
-            if constexpr (!EXACT) return dl > 0.f ? 2 : 1;
-            const uint32_t k3 = warp_max((left >> lane) & 1u && lane != at2 ? wkey : 0u);
-            open = (p.TG > 1 && !(key_rank(kprev) - wb > near_w)) || (k3 != 0u && !(wa - key_rank(k3) > near_w));
-            if (!open) {
-                float a[3], b[3];
-                int ia[2], ib[2];
-                best_of(at, a, ia);
-                best_of(at2, b, ib);
-                const int t = pairs ? 1 : 0;
-                open = (gs > t + 1 && (too_near(a[t], a[t + 1]) || too_near(b[t], b[t + 1])));
-                if (!open) {
-                    sum64();
-                    double r1[2], v1[2], r2[2] = {0.0, 0.0}, v2[2] = {0.0, 0.0};
-                    exact_pair(p, sh, row, lrow, lane, ia[0], ib[0], (double)top, z64, r1, v1);
-                    if (pairs) exact_pair(p, sh, row, lrow, lane, ia[1], ib[1], (double)top, z64, r2, v2);
-                    const bool scored = pairs && !p.bias;
-                    const double da = scored ? v1[0] + v2[0] : r1[0] + r2[0], db = scored ? v1[1] + v2[1] : r1[1] + r2[1];
-                    // the softmax's sum is not exact where the logits are not: it shifts the scores' difference
-                    if (sh && soft && p.bias && fabs(da - db) <= (double)dl * fabs((v1[0] + v2[0]) - (v1[1] + v2[1]))) open = true;
-                    else if (db > da || (db == da && at2 < at)) left = (left | (1u << at)) & ~(1u << at2);
-                }
-            }
-        }
-        if (whole) {
-            if ((left >> min(31, lane * VPL / gs)) & 1u) {
+            // the border lies between two groups, or more
+            const uint32_t k3 = warp_max((out >> lane) & 1u && lane != at2 ? wkey : 0u);
+            q.at = at; q.at2 = at2; q.out = out;
+            if ((p.TG > 1 && !(key_rank(kprev) - wb > near_w)) || (k3 != 0u && !(wa - key_rank(k3) > near_w))) { q.kind = kAll; return q; }
 #pragma unroll
-                for (int i = 0; i < VPL; i++) key[i] = 0u;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VPL; i++)
-                if (key[i] && ((left >> (expert_of(key[i], lane) / gs)) & 1u)) key[i] = 0u;
-            sort_keys(key);
+            for (int i = 0; i < VPL; i++) kept[i] = key[i];
+            return best_of_groups<VPL>(p, lane, margin, kept, q);
         }
     }
-
-    // top-k: lane j keeps the j-th key and the lane it came from
-    uint32_t my_key = 0;
-    int my_from = 0;
-    for (int j = 0; j <= K; j++) {
-        const uint32_t m = warp_max(key[0]);
-        const int from = __ffs((int)__ballot_sync(0xffffffffu, key[0] == m)) - 1;
-        if (lane == j) { my_key = m; my_from = from; }
-        if (lane == from) {
-#pragma unroll
-            for (int i = 0; i + 1 < VPL; i++) key[i] = key[i + 1];
-            key[VPL - 1] = 0u;
-        }
-    }
-    int my_id = expert_of(my_key, my_from);
-    const float mine = my_key ? value(my_key) : 0.f, before = __shfl_up_sync(0xffffffffu, mine, 1);
-    uint32_t near = __ballot_sync(0xffffffffu, lane > 0 && lane <= K && my_key && too_near(before, mine));   // bit j: not told apart from j - 1
-    if (near && !any_bad && !open) {
-        if constexpr (!EXACT) return dl > 0.f ? 2 : 1;
-        // neighbours that are too near change places if their exact values say so; three in a row go to select_exact
-        open = (near & (near << 1)) != 0u;
-        if ((near >> K) & 1u) {
-            const uint32_t m = warp_max(key[0]);                       // the next one behind the border
-            open = open || (m != 0u && too_near(__shfl_sync(0xffffffffu, mine, K), value(m)));
-        }
-        if (!open) {
-            sum64();
-            while (near) {
-                const int j = __ffs((int)near) - 1;
-                near &= near - 1;
-                const int a = __shfl_sync(0xffffffffu, my_id, j - 1), b = __shfl_sync(0xffffffffu, my_id, j);
-                double rr[2], v[2];
-                exact_pair(p, sh, row, lrow, lane, a, b, (double)top, z64, rr, v);
-                if (sh && soft && p.bias && fabs(rr[0] - rr[1]) <= (double)dl * fabs(v[0] - v[1])) open = true;
-                if (rr[1] > rr[0] || (rr[1] == rr[0] && b < a)) {
-                    if (lane == j - 1) my_id = b;
-                    if (lane == j) my_id = a;
-                }
-            }
-        }
-    }
-    if (EXACT && open) {
-        select_exact<VPL>(p, row, lrow, lane, (double)dl, sh);
-        return 0;
-    }
-    float s = 0.f;
-    if (lane < K) {
-        const float v = __ldcg(lrow + my_id);
-        s = soft ? expf(v - top) * inv : 1.0f / (1.0f + expf(-v));
-    }
-    float sum = 1.0f;
-    if (p.normalize) {
-        sum = warp_sum_f(s);
-        if (!soft || p.bias) sum = fmaxf(sum, 6.103515625e-5f);        // of a softmax's largest scores: never below top_k / experts
-    }
-    if (lane < K) {
-        p.ids[(size_t)row * K + lane] = (uint32_t)my_id;
-        p.probs[(size_t)row * K + lane] = any_bad ? qnan() : s / sum * p.scale;
-    }
-    return 0;
+    q.out = out;
+    return choose<VPL>(p, o, lane, margin, key, q);
 }
 
-template <int VPL>
-__device__ __noinline__ void settle_row(const SelectParams& p, int row, int lane, SelectShared* sh) { select_row<VPL, true>(p, row, lane, sh); }
-
-// The tokens of a CTA of 256 threads, one per warp (row < 0: none). PRODUCT: the logits come from rows and weights.
+// The tokens of a CTA of 256 threads, one per warp (row < 0: none). PRODUCT: logits with errors, for which the CTA sums
+// what its open tokens want. Without it a warp settles its token on the spot.
 template <int VPL, bool PRODUCT>
-__device__ __forceinline__ void select_tokens(const SelectParams& p, int row, SelectShared& sh) {
+__device__ __forceinline__ void select_tokens(const SelectParams& p, int row, float error, SelectShared* sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int left = row >= 0 ? select_row<VPL, false>(p, row, lane, nullptr) : 0;
-    if (left == 1) settle_row<VPL>(p, row, lane, nullptr);
-    if (!PRODUCT || !__syncthreads_or(left == 2)) return;
-    if (lane == 0) sh.rows[warp] = left == 2 ? row : -1;
-    __syncthreads();
-    if (warp == 0) {
-        for (int w = 0; w < 8; w++)
-            if (sh.rows[w] >= 0) settle_row<VPL>(p, sh.rows[w], lane, &sh);
-        dots_end(&sh);
+    OpenRow o;
+    Margin margin;
+    uint32_t kept[VPL];
+    Open q{kDone, -1, 0, 0, 0, 0u, 0u};
+    if (row >= 0) q = select_row<VPL>(p, row, error, lane, o, margin, kept);
+    double l = 0.0;
+    if (PRODUCT) {
+        if (!__syncthreads_or(q.kind != kDone)) return;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, (q.kind == kWinners || q.kind == kGroups) && q.want >= 0);
+        const int at = __popc(lanes & ((1u << lane) - 1u));
+        if (lane == 0) { sh->row[warp] = row; sh->count[warp] = __popc(lanes); }
+        if ((lanes >> lane) & 1u) sh->want[warp][at] = q.want;
+        __syncthreads();
+        exact_wanted(p, *sh);
+        if (q.kind == kDone) return;
+        if ((lanes >> lane) & 1u)
+            for (int w = 0; w < 8; w++) l += sh->part[w][warp][at];
     } else {
-        dots_serve(p, &sh);
+        if (q.kind == kDone) return;
+        if (q.want >= 0) l = (double)__ldcg(o.logits + q.want);
     }
+    settle<VPL>(p, o, lane, margin, kept, q, l);
 }
 
-// CTAs an SM: what is bound by the latency of one row after the other gains from more warps than the registers of the
-// usual path allow for (given logits, 32768 rows of 256 experts, 4 / 5 / 6: 49.8 / 47.7 / 46.5 us); behind the product,
-// where CTAs wait for exact logits, the spills weigh more (8192 rows with their product 85.2 / 85.9 / 87.8 us).
+// CTAs an SM: what is bound by the latency of one row after the other gains a little from more warps than the registers of
+// the usual path allow for (given logits, 32768 rows of 256 experts, 4 / 5 / 6: 44.8 / 43.9 / 43.6 us); behind the product,
+// where CTAs sum exact logits, the spills weigh more (8192 rows, 3 / 4 / 5: 39.4 / 39.4 / 41.5 us).
 template <int VPL, bool PRODUCT>
 __global__ void __launch_bounds__(256, VPL > 8 ? 2 : PRODUCT ? 4 : 6) select_kernel(const SelectParams p) {
-    __shared__ SelectShared sh;
+    __shared__ typename std::conditional<PRODUCT, SelectShared, int>::type sh;
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();
     if (__syncthreads_or(p.status && threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u)) return;
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    select_tokens<VPL, PRODUCT>(p, row < p.rows ? row : -1, sh);
+    float error = 0.f;
+    if (PRODUCT && row < p.rows)
+        for (int t = 0; t < (p.E + 127) / 128; t++) error = fmaxf(error, __ldcg(p.errors + (size_t)t * p.rows + row));
+    select_tokens<VPL, PRODUCT>(p, row < p.rows ? row : -1, error, reinterpret_cast<SelectShared*>(&sh));
 }
 
-// Few rows: the product and the selection in one launch. A warp per expert and four tokens makes the logits (f32); the CTA
-// that comes last for its four tokens (counted in `arrivals`, which it leaves at zero) selects for them. No CTA waits.
+// Few rows: the product and the selection in one launch. A warp per expert and four tokens makes the logits: four terms at
+// a time in 32 bits, their sums in 64, which leaves a term five roundings (four, and the logit's). The CTA that comes last
+// for its four tokens (counted in `arrivals`, which it leaves at zero) selects for them. No CTA waits.
 template <int VPL>
 __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, float* logits, uint32_t* arrivals) {
     __shared__ SelectShared sh;
     __shared__ int last;
+    __shared__ float squares[8];
     pdl_wait();                // the kernel before has completed and its writes are visible
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.y * 8 + warp, t0 = blockIdx.x * 4;
     if (e < p.E) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        double acc[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 4
         for (int k = lane * 4; k < p.H; k += 128) {
             const float4 v = __ldg(reinterpret_cast<const float4*>(p.w + (size_t)e * p.H + k));
@@ -675,17 +804,40 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, f
             for (int t = 0; t < 4; t++) {
                 if (t0 + t >= p.rows) continue;
                 const uint2 q = *reinterpret_cast<const uint2*>(p.x + (size_t)(t0 + t) * p.H + k);
-                acc[t] = fmaf(v.x, __uint_as_float(q.x << 16), acc[t]);
-                acc[t] = fmaf(v.y, __uint_as_float(q.x & 0xffff0000u), acc[t]);
-                acc[t] = fmaf(v.z, __uint_as_float(q.y << 16), acc[t]);
-                acc[t] = fmaf(v.w, __uint_as_float(q.y & 0xffff0000u), acc[t]);
+                acc[t] += (double)fmaf(v.w, __uint_as_float(q.y & 0xffff0000u), fmaf(v.z, __uint_as_float(q.y << 16),
+                               fmaf(v.y, __uint_as_float(q.x & 0xffff0000u), v.x * __uint_as_float(q.x << 16))));
             }
         }
+        // the four sums together: half of the lanes go on with two of them, a quarter with one
+        const bool upper = lane & 16, odd = lane & 8;
+        double a = (upper ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, upper ? acc[0] : acc[2], 16);
+        double b = (upper ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, upper ? acc[1] : acc[3], 16);
+        a = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const float s = warp_sum_f(acc[t]);
-            if (lane == 0 && t0 + t < p.rows) logits[(size_t)(t0 + t) * p.E + e] = s;
+        for (int d = 4; d >= 1; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+        const int t = lane >> 3;
+        if ((lane & 7) == 0 && t0 + t < p.rows) logits[(size_t)(t0 + t) * p.E + e] = (float)a;
+    }
+    // the rows' squares, two warps a row (which lies in L1 by now)
+    {
+        const int t = t0 + (warp & 3), half = warp >> 2;
+        float sq = 0.f;
+        uint32_t some = 0;
+        if (t < p.rows) {
+#pragma unroll 4
+            for (int k = (half * 32 + lane) * 8; k < p.H; k += 512) {
+                const uint4 q = *reinterpret_cast<const uint4*>(p.x + (size_t)t * p.H + k);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xffff0000u);
+                    sq = fmaf(hi, hi, fmaf(lo, lo, sq));
+                    some |= w[i];
+                }
+            }
         }
+        sq = warp_sum_f(sq) + (__any_sync(0xffffffffu, (some & 0x7fff7fffu) != 0u) ? kLostSquares : 0.f);
+        if (lane == 0) squares[warp] = sq;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -695,7 +847,8 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, f
     }
     __syncthreads();
     if (!last) return;
-    select_tokens<VPL, true>(p, warp < 4 && t0 + warp < p.rows ? t0 + warp : -1, sh);
+    const bool mine = warp < 4 && t0 + warp < p.rows;
+    select_tokens<VPL, true>(p, mine ? t0 + warp : -1, mine ? product_error(5.1f, squares[warp] + squares[warp + 4], __ldcg(p.w_norm)) : 0.f, &sh);
 }
 
 }  // namespace oco

@@ -386,3 +386,74 @@ def test_masked_experts_of_a_product(moe):
             r.forward(x[:rows].contiguous(), ids, probs, rows)
             assert np.array_equal(ids.cpu().numpy(), want[:rows])
             np.testing.assert_allclose(probs.cpu().numpy(), p[:rows], rtol=2.0 ** -16)
+
+
+@pytest.mark.parametrize("shape", [(512, 8, "sigmoid", 1, 1, 1, True, True, 1.0), (256, 8, "sigmoid", 8, 4, 2, True, True, 2.5), (128, 8, "softmax", 1, 1, 1, False, True, 1.0),
+                                   (64, 4, "softmax", 8, 3, 2, False, True, 1.0), (270, 9, "softmax", 5, 2, 2, True, True, 1.0), (160, 6, "sigmoid", 5, 2, 2, False, True, 1.0)],
+                         ids=str)
+@pytest.mark.parametrize("H,at,size,weight", [(4096, (0, 2050), 4096.0, 1.0), (4096, (5, 4090), 45.0, 0.5), (1024, (3, 40), 2000.0, 1.0), (2080, (64, 2079), 1e6, 0.25),
+                                              (256, (17, 18), 512.0, 1.0)])
+def test_large_terms_that_cancel(moe, shape, H, at, size, weight):
+    """Two large terms of opposite sign in every logit leave their rounding in 32-bit sums: the ids are the definition's all
+    the same, at any number of rows."""
+    E, rows = shape[0], 200
+    r, w, b, g = make(moe, shape, H, rows, 45)
+    x = torch.randn((rows, H), device="cuda", generator=g).to(torch.bfloat16)
+    for k, sign in zip(at, (1.0, -1.0)):
+        x[:, k] = size * sign
+        w[:, k] = weight
+    r.bind(w, b)
+    exact = x.double() @ w.double().t()
+    want, p = expect(shape, exact, b)
+    logits = torch.empty((rows, E), device="cuda")
+    for n in (1, 16, 17, 200):
+        ids, probs = outputs(shape, n)
+        r.forward(x[:n], ids, probs, n, logits=logits)
+        r.poll()
+        assert np.array_equal(ids.cpu().numpy(), want[:n]), n
+        # logits within what the selection allows for: 45 units of 2^-24 of the norms, and the sums of up to 64 stages
+        bound = 2.0 ** -24 * (45 + 2 * 64) * x[:n].double().norm(dim=1, keepdim=True) * w.double().norm(dim=1).max()
+        err = (logits[:n].double() - exact[:n]).abs()
+        assert (err <= bound).all()
+        # a logit's error d changes a weight by at most e^(2d) where a softmax or a sum of sigmoids divides it
+        np.testing.assert_allclose(probs.cpu().numpy(), p[:n], rtol=2.0 ** -16 + 3.0 * float(err.max()))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("xs,ws", [(1e-30, 1.0), (1e20, 1e-20), (1e25, 1e-15), (1e-38, 1e10)])
+def test_rows_whose_squares_leave_the_range(moe, rows, xs, ws):
+    """Squares of rows below 2^-126 or beyond the range of f32: the error bound of the logits still holds."""
+    for shape in ((64, 4, "sigmoid", 1, 1, 1, False, True, 1.0), (64, 4, "softmax", 8, 2, 1, False, True, 1.0)):
+        r, w, b, g = make(moe, shape, 512, rows, 46)
+        w = w[:16].repeat(4, 1)                                        # near ties that the product cannot tell apart
+        w *= 1.0 + (torch.rand((64, 512), device="cuda", generator=g) - 0.5) * 2e-7
+        w *= ws
+        r.bind(w, None)
+        x = (torch.randn((rows, 512), device="cuda", generator=g).to(torch.bfloat16).float() * xs).to(torch.bfloat16)
+        x[1] = 0.0
+        exact = x.double() @ w.double().t()
+        ids, probs = outputs(shape, rows)
+        r.forward(x, ids, probs, rows)
+        l = exact.cpu().numpy()
+        worth = l.reshape(rows, shape[3], -1).max(2)
+        kept = np.argsort(-worth, axis=1, kind="stable")[:, :shape[4]]
+        open_ = np.zeros((rows, shape[3]), bool)
+        np.put_along_axis(open_, kept, True, 1)
+        want = np.argsort(-np.where(np.repeat(open_, 64 // shape[3], 1), l, -np.inf), axis=1, kind="stable")[:, :4]
+        assert np.array_equal(ids.cpu().numpy(), want)
+
+
+def test_norm_of_the_weights_follows_a_new_binding(moe):
+    """The error bound belongs to the weights that are bound: larger ones after smaller ones."""
+    shape = (256, 8, "sigmoid", 8, 4, 2, True, True, 1.0)
+    r, w, b, g = make(moe, shape, 1024, 100, 47)
+    small = w * 1e-6
+    x = torch.randn((100, 1024), device="cuda", generator=g).to(torch.bfloat16)
+    x[:, 3], x[:, 700] = 3000.0, -3000.0
+    w[:, 3] = w[:, 700] = 1.0
+    ids, probs = outputs(shape, 100)
+    for weights in (small, w):
+        r.bind(weights, b)
+        r.forward(x, ids, probs, 100)
+        want, _ = expect(shape, x.double() @ weights.double().t(), b)
+        assert np.array_equal(ids.cpu().numpy(), want)
