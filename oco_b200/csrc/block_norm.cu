@@ -168,9 +168,11 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) block_norm_kern
                         for (int j = 0; j < 4; j++) {
                             float lo, hi;
                             f32x2_split(g.v[j], lo, hi);
-                            // beyond 80 a sigmoid is e^-80 in all but name, and 1 + e^80 is still in the range of the quotient
-                            if (p.gate_act == OCO_GATE_SIGMOID)
-                                g.v[j] = f32x2(__fdividef(1.0f, 1.0f + __expf(fminf(-lo, 80.0f))), __fdividef(1.0f, 1.0f + __expf(fminf(-hi, 80.0f))));
+                            // beyond 80 a sigmoid is e^-80 in all but name, and 1 + e^80 is still in the range of the quotient; a NaN stays one
+                            if (p.gate_act == OCO_GATE_SIGMOID) {
+                                const float el = __expf(lo < -80.0f ? 80.0f : -lo), eh = __expf(hi < -80.0f ? 80.0f : -hi);
+                                g.v[j] = f32x2(__fdividef(1.0f, 1.0f + el), __fdividef(1.0f, 1.0f + eh));
+                            }
                             else g.v[j] = f32x2(tanhf(lo), tanhf(hi));
                         }
                     }

@@ -189,3 +189,21 @@ def test_expanded_rows_and_overlaps(moe):
     a["gate"] = a["post_w"] = a["pre_w"] = None
     want = run(moe, a, "rms", "none", 0.0, 1.0, 1.0, 1e-5)
     assert torch.equal(ho[:, :256], want[0]) and torch.equal(ho[:, 256:], want[1])
+
+
+@pytest.mark.parametrize("act", ["none", "sigmoid", "tanh"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_a_bad_gate_spoils_its_row(moe, act, dtype, kind):
+    """A NaN in the gate reaches its element of the residual rows and all of the row's norm; infinities are the ends of sigmoid and tanh."""
+    a = case(32, 5, 520, kind, gate="row", wide=True)
+    gate = a["gate"].to(dtype)
+    gate[1, 7] = float("nan")
+    gate[3, 500] = -float("nan")
+    gate[2, 3], gate[2, 4] = float("inf"), -float("inf")
+    a["gate"] = gate
+    ho, no = run(moe, a, kind, act, 0.0, 1.0, 1.0, 1e-5)
+    h, x = opref.block_norm(a["hidden"], a["block"], a["pre_w"], a["pre_b"], a["post_w"], a["post_b"], gate, act, kind)
+    assert torch.equal(ho.isnan(), h.isnan()) and torch.equal(no.isnan(), x.isnan()) and ho[1, 7].isnan() and no[3].isnan().all()
+    rows = [0, 4] if act == "none" else [0, 2, 4]
+    near(ho[rows], h[rows], h[rows].abs().amax(1, keepdim=True) + 1, 520)
