@@ -207,3 +207,15 @@ def test_a_bad_gate_spoils_its_row(moe, act, dtype, kind):
     assert torch.equal(ho.isnan(), h.isnan()) and torch.equal(no.isnan(), x.isnan()) and ho[1, 7].isnan() and no[3].isnan().all()
     rows = [0, 4] if act == "none" else [0, 2, 4]
     near(ho[rows], h[rows], h[rows].abs().amax(1, keepdim=True) + 1, 520)
+
+
+def test_sigmoid_gates_far_below_zero(moe):
+    """f32 rows that are the gate alone: exponential and quotient (two units of 2^-23 each), their sum and two products (half
+    a unit each) are within 2^-20 of the value, down to e^-85, where a cheaper exponential is off by a hundred units."""
+    width = 1024
+    gate = torch.linspace(-85.0, 10.0, width, device="cuda")
+    hidden = torch.zeros((3, width), device="cuda")
+    out = torch.empty_like(hidden)
+    moe.block_norm(hidden, torch.ones((3, width), dtype=torch.bfloat16, device="cuda"), hidden_out=out, gate=gate, gate_act="sigmoid")
+    want = torch.sigmoid(gate.double()).expand(3, width)
+    assert ((out.double() - want).abs() <= 2.0 ** -20 * want).all(), ((out.double() - want).abs() / want).max()
