@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const F8PlanParams p) {
 // rounded reciprocal, corrected once by its exact residual (Markstein's method: the correction of a correctly rounded
 // reciprocal's product rounds correctly while nothing leaves the normal range; a block outside 2^-100 .. 2^100 divides).
 // A block whose largest is NaN or infinite gives NaN codes or a scale that makes its products NaN.
+// Activations are f32: their x * 448 is rounded as well, and near either end of f32 both sides are moved by 2^100 first.
 struct F8Divider {
     float top, rcp;
     bool plain;
@@ -105,17 +106,33 @@ struct F8Divider {
         const float q = top * kPart;
         return plain ? fmaf(fmaf(-q, 448.0f, top), kPart, q) : __fdiv_rn(top, 448.0f);
     }
-    // Eight bf16 elements -> codes, two at a time in packed f32 arithmetic.
+    // Two quotients in packed f32 arithmetic; plain only.
+    __device__ __forceinline__ uint64_t two(uint64_t x) const {
+        const uint64_t r2 = f32x2(rcp, rcp), n = mul_f32x2(x, f32x2(448.0f, 448.0f)), q = mul_f32x2(n, r2);
+        return fma_f32x2(fma_f32x2(q, f32x2(-top, -top), n), r2, q);
+    }
+    // Four f32 elements -> codes.
+    __device__ __forceinline__ uint32_t codes(uint64_t a, uint64_t b) const {
+        float v[4];
+        if (plain) {
+            f32x2_split(two(a), v[0], v[1]);
+            f32x2_split(two(b), v[2], v[3]);
+        } else {
+            const float lift = top < 1.0f ? 1.2676506e30f : 7.8886091e-31f, by = top == 0.0f ? 1.0f : top * lift;   // 2^100, 2^-100
+            f32x2_split(a, v[0], v[1]);
+            f32x2_split(b, v[2], v[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = __fdiv_rn(v[i] * lift * 0.875f, by) * 512.0f;
+        }
+        return f8x4(v[0], v[1], v[2], v[3]);
+    }
+    // Eight bf16 elements -> codes.
     __device__ __forceinline__ uint2 codes(const uint4& x) const {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         float v[8];
         if (plain) {
-            const uint64_t lift = f32x2(448.0f, 448.0f), r2 = f32x2(rcp, rcp), minus = f32x2(-top, -top);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint64_t n = mul_f32x2(f32x2_bits(w[j] << 16, w[j] & 0xffff0000u), lift), q = mul_f32x2(n, r2);
-                f32x2_split(fma_f32x2(fma_f32x2(q, minus, n), r2, q), v[2 * j], v[2 * j + 1]);
-            }
+            for (int j = 0; j < 4; j++) f32x2_split(two(f32x2_bits(w[j] << 16, w[j] & 0xffff0000u)), v[2 * j], v[2 * j + 1]);
         } else {
             const float by = top == 0.0f ? 1.0f : top;
 #pragma unroll

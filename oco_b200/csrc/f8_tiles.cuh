@@ -42,14 +42,6 @@ struct F8TileParams {
 };
 
 __device__ __forceinline__ float silu_times(float g, float u) { return sigmoid_times(g, 1.0f) * g * u; }
-// Scale and factor of a block of activations whose largest magnitude is `top`: code = e4m3(a * lift * factor). `lift`
-// keeps 448 / top finite where top is tiny and the quotient's divisor in its range (below 2^126) where it is vast.
-__device__ __forceinline__ void f8_act_scale(float top, float& scale, float& lift, float& factor) {
-    lift = top < 1e-30f ? 1.2676506e30f : top > 1e30f ? 7.8886091e-31f : 1.0f;   // 2^100, 2^-100
-    factor = top == 0.0f ? 1.0f : __fdividef(448.0f, top * lift);
-    scale = top * (1.0f / 448.0f);
-}
-
 // ---- many rows --------------------------------------------------------------------------------------------------------
 // PAIR: two SMs multiply one tile of 256 rows (tcgen05.mma.cta_group::2): each brings its own 128 rows and half of the 256
 // features, so that an SM fetches 32 KB instead of 48 KB for the same 128 x 256 products of 128 terms.
@@ -243,25 +235,15 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");       // the two warps that share the rows
                 top = max(top, tops[(half ^ 1) * 128 + erow]);
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-                float scale, lift, factor;
-                f8_act_scale(__uint_as_float(top), scale, lift, factor);
+                const F8Divider by(__uint_as_float(top));
                 const size_t row = (size_t)it.row0 + erow;
-                if (live && half == 0) p.code_scales[(size_t)(it.f0 / 128) * p.pitch + row] = scale;
-                {
+                if (live && half == 0) p.code_scales[(size_t)(it.f0 / 128) * p.pitch + row] = by.scale();
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t w[4];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            float v[4];
-                            f32x2_split(acc[8 * c + 2 * k], v[0], v[1]);
-                            f32x2_split(acc[8 * c + 2 * k + 1], v[2], v[3]);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) v[e] = v[e] * lift * factor;
-                            w[k] = f8x4(v[0], v[1], v[2], v[3]);
-                        }
-                        store16(c, w);
-                    }
+                    for (int k = 0; k < 4; k++) w[k] = by.codes(acc[8 * c + 2 * k], acc[8 * c + 2 * k + 1]);
+                    store16(c, w);
                 }
                 send(p.codes + row * p.n + f, (uint32_t)max(0, min(64, p.n - f)), live && f < p.n);
             } else {
@@ -681,11 +663,9 @@ __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_
                                     in ? silu_times(v[0].w, u.w) : 0.f};
                 const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(fabsf(a[0])), __float_as_uint(fabsf(a[1]))),
                                                                         max(__float_as_uint(fabsf(a[2])), __float_as_uint(fabsf(a[3])))));
-                float scale, lift, factor;
-                f8_act_scale(__uint_as_float(top), scale, lift, factor);
-                if (in) *reinterpret_cast<uint32_t*>(p.codes + (size_t)(row0 + c) * p.n + f) =
-                    f8x4(a[0] * lift * factor, a[1] * lift * factor, a[2] * lift * factor, a[3] * lift * factor);
-                if (lane == 0) p.code_scales[(size_t)(f0 / 128) * p.pitch + row0 + c] = scale;
+                const F8Divider by(__uint_as_float(top));
+                if (in) *reinterpret_cast<uint32_t*>(p.codes + (size_t)(row0 + c) * p.n + f) = by.codes(f32x2(a[0], a[1]), f32x2(a[2], a[3]));
+                if (lane == 0) p.code_scales[(size_t)(f0 / 128) * p.pitch + row0 + c] = by.scale();
             } else if (f < p.n) {
                 size_t row = FORM == kF8Concat ? (size_t)tile : (size_t)(row0 + c);
                 if (FORM == kF8Tiles && p.route_of_row) row = p.route_of_row[row0 + c];

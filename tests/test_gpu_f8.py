@@ -502,3 +502,31 @@ def test_routes_are_summed_before_they_are_rounded(lib, rows, H, F):
     want = y0 + y1
     err = (out.double() - want).norm()
     assert err <= (2.0 ** -8 + 2.0 ** -8) * want.norm() + 2.0 ** -17 * 2 * terms.norm(), err / want.norm()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 16, 20, 70, 300, 1100])
+def test_rounding_of_activations_halfway_between_codes(lib, rows):
+    """Activations that are whole numbers, halfway between two codes of their block, and the identity as the down matrix:
+    every stage is exact but the rounding itself. Row r: gate 64 (its sigmoid is 1 in 32 bits), up k * (16 + 1), k * (18 + 1),
+    .. and k * 448 for the largest, k small and not a power of two: codes of exactly 17, 19, .. before they are rounded."""
+    H = F = 128
+    k = torch.tensor([3, 5, 7, 9, 11, 13, 15], dtype=torch.float64).repeat(rows // 7 + 1)[:rows]
+    x = torch.zeros((rows, H), dtype=torch.float64)
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = 448.0, 64.0, k, k                       # the scale is 1
+    gate, up = torch.zeros((F, H), dtype=torch.float64), torch.zeros((F, H), dtype=torch.float64)
+    gate[:, 1] = 1.0
+    up[0, 2] = 448.0
+    for f in range(1, F):
+        m, size = 16 + 2 * (f % 8), 2.0 ** (f // 8 % 5 - 1)
+        up[f, 2], up[f, 3] = m * size * (-1) ** f, size * (-1) ** f
+    one = torch.ones((1, 1), device="cuda")
+    as_codes = lambda t: t.float().to(torch.float8_e4m3fn).cuda()  # noqa: E731
+    plan = lib.dense.DensePlan(lib.dense.FFN_SILU_GATE, synth.FMT_F8_E4M3, H, F)
+    plan.reserve(rows)
+    plan.bind(as_codes(up), as_codes(gate), as_codes(torch.eye(H)), up_scale=one, gate_scale=one, down_scale=one)
+    y = torch.empty((rows, H), dtype=torch.bfloat16, device="cuda")
+    plan.forward(x.to(torch.bfloat16).cuda(), y, rows)
+    plan.poll()
+    codes, scales = opref.quantize(64.0 * (x @ up.t()))
+    assert torch.equal(scales[:, 0], 64.0 * k) and codes.abs().max() == 448.0
+    assert torch.equal(y.double().cpu(), codes * scales)
