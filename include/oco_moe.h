@@ -420,7 +420,8 @@ int oco_moe_router_bind_weights(oco_moe_router* router, const float* router_w, c
  * logits f32 [rows, experts]. Only enqueues; 0 rows are no work. */
 int oco_moe_router_forward(oco_moe_router* router, const uint16_t* x_bf16, int rows, uint32_t* ids, float* probs, float* logits,
                            void* cuda_stream);
-/* The selection alone, from logits f32 [rows, experts] of any origin (any number of rows). */
+/* The selection alone, from logits f32 [rows, experts] of any origin (any number of rows), on the current device: the
+ * one the bias was bound on, if there is one. */
 int oco_moe_router_select(oco_moe_router* router, const float* logits, int rows, uint32_t* ids, float* probs, void* cuda_stream);
 int oco_moe_router_poll(oco_moe_router* router, void* cuda_stream);
 int oco_moe_router_last_launch_count(const oco_moe_router* router);

@@ -229,6 +229,8 @@ int ready(oco_moe_f8_plan* plan, int rows) {
     plan->launches = 0;
     if (!plan->have_ws || !plan->have_w) return plan->fail(OCO_INVALID_ARGUMENT, "bind a workspace, weights and scales first");
     if (int rc = plan->check_device()) return rc;
+    if (plan->weights_device != plan->device)
+        return plan->fail(OCO_INVALID_ARGUMENT, "the weights were bound on device %d, the workspace on device %d", plan->weights_device, plan->device);
     if (rows < 0 || rows > plan->max_rows) return plan->fail(OCO_INVALID_ARGUMENT, "rows %d outside 0..%d", rows, plan->max_rows);
     return OCO_OK;
 }
@@ -265,6 +267,7 @@ int f8_dense_bind_scales(oco_moe_f8_plan* p, const oco_dense_scales& s) {
     if (p->kind == kF8Gated) { p->w.gate_s = s.gate_s; p->w.down_s = s.down_s; }
     if (int rc = check_scales(p)) return rc;
     if (int rc = make_maps(p)) return rc;
+    if (int rc = p->note_weights()) return rc;
     p->have_w = true;
     return OCO_OK;
 }
@@ -332,6 +335,7 @@ int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* w) 
     if (int rc = check_codes(plan)) return rc;
     if (int rc = check_scales(plan)) return rc;
     if (int rc = make_maps(plan)) return rc;
+    if (int rc = plan->note_weights()) return rc;
     plan->have_w = true;
     return OCO_OK;
 }

@@ -96,7 +96,7 @@ inline CUresult encode_rows(CUtensorMap* map, void* base, uint64_t rows, uint64_
 // count of the last call and the last message.
 struct PlanBase {
     bool have_ws = false, have_w = false;
-    int max_rows = 0, device = -1, sm_count = 148, launches = 0;
+    int max_rows = 0, device = -1, weights_device = -1, sm_count = 148, launches = 0;
     char err[256] = {0};
 
     int fail(int code, const char* fmt, ...) {
@@ -110,6 +110,11 @@ struct PlanBase {
         int dev = -1;
         if (cudaGetDevice(&dev) != cudaSuccess || dev != device)
             return fail(OCO_INVALID_ARGUMENT, "the plan's workspace was bound on device %d, the current device is %d", device, dev);
+        return OCO_OK;
+    }
+    // The weights that are bound belong to the device that is current then.
+    int note_weights() {
+        if (cudaGetDevice(&weights_device) != cudaSuccess) return fail(OCO_CUDA_ERROR, "cudaGetDevice failed");
         return OCO_OK;
     }
     int note_device() {

@@ -46,6 +46,8 @@ int lay_out(oco_moe_router* r) {
     const oco_moe_router_desc& d = r->d;
     if (!r->have_ws || !r->have_w || !d.hidden) return OCO_OK;
     if (int rc = r->check_device()) return rc;
+    if (r->weights_device != r->device)
+        return r->fail(OCO_INVALID_ARGUMENT, "the weights were bound on device %d, the workspace on device %d", r->weights_device, r->device);
     const int Ep = padded(d.experts);
     OCO_CK(r, cudaDeviceSynchronize());     // the weights have been written, on whatever stream
     router_pieces_kernel<<<4 * r->sm_count, 256>>>(r->w, r->pieces, d.experts, Ep, d.hidden);
@@ -146,6 +148,9 @@ int oco_moe_router_bind_weights(oco_moe_router* r, const float* w, const float* 
     if (!r) return OCO_INVALID_ARGUMENT;
     if ((r->d.hidden != 0) != (w != nullptr)) return r->fail(OCO_INVALID_ARGUMENT, "router_w goes with hidden: both or neither");
     if (((uintptr_t)w & 15u) || ((uintptr_t)bias & 3u)) return r->fail(OCO_INVALID_ARGUMENT, "router_w must be 16-byte aligned, bias 4-byte");
+    r->have_w = false;
+    if (w || bias)
+        if (int rc = r->note_weights()) return rc;
     r->w = w; r->bias = bias;
     r->have_w = true;
     return lay_out(r);
@@ -190,6 +195,11 @@ int oco_moe_router_select(oco_moe_router* r, const float* logits, int rows, uint
     if (rows == 0) return OCO_OK;
     if (!logits || !ids || !probs) return r->fail(OCO_INVALID_ARGUMENT, "null logits, ids or probs");
     if (((uintptr_t)logits | (uintptr_t)ids | (uintptr_t)probs) & 3u) return r->fail(OCO_INVALID_ARGUMENT, "logits, ids and probs must be 4-byte aligned");
+    if (r->bias) {
+        int dev = -1;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev != r->weights_device)
+            return r->fail(OCO_INVALID_ARGUMENT, "the bias was bound on device %d, the current device is %d", r->weights_device, dev);
+    }
     return launch_select(r, select_params(r, logits, rows, ids, probs), false, (cudaStream_t)cuda_stream);
 }
 

@@ -63,6 +63,8 @@ class DensePlan:
             if not gated and any(t is not None for t in (gate_w, down_w, gate_scale, down_scale)):
                 raise OcoError(_lib.INVALID_ARGUMENT, "a projection has one matrix")
             got = {name: f8_matrix(codes, scales, (), n, k, device, name) for name, codes, scales, (n, k) in shapes}
+            if self.workspace is not None:
+                same_device(got, self.workspace)
             ptr = lambda name, i: C.c_void_p(got[name][i].data_ptr()) if name in got else None  # noqa: E731
             cw = _lib.DenseWeights(*[C.cast(ptr(n, 0), C.POINTER(C.c_uint8)) if n in got else None for n in ("up", "gate", "down")])
             self._check(_lib.lib().oco_dense_bind_weights(self.handle, C.byref(cw)))

@@ -345,8 +345,8 @@ def _current_device() -> int:
 
 
 def same_device(weights, workspace: torch.Tensor):
-    """Refuses a workspace on another device than the weights that are bound already (a dict or tuple of tensors, or of
-    pairs of them)."""
+    """Refuses a workspace on another device than the weights (a dict or tuple of tensors, or of pairs of them), whichever
+    of the two came first."""
     for t in (weights.values() if isinstance(weights, dict) else weights or ()):
         for part in t if isinstance(t, tuple) else (t,):
             if part is not None and part.get_device() != workspace.get_device():
@@ -386,7 +386,7 @@ class _GroupPlan:
         self.desc, self.handle = desc, C.c_void_p()
         self._fn = {n: getattr(_lib.lib(), self._prefix + n) for n in ("workspace_bytes", "bind_workspace", "bind_weights", "forward", "poll",
                                                                       "last_error", "last_launch_count")}
-        self.workspace, self.max_rows, self._weights = None, 0, None
+        self.workspace, self.max_rows, self._weights, self._bias = None, 0, None, None
         self.device = -2                                                   # of the workspace
         rc = create(C.byref(desc), C.byref(self.handle))
         if rc != _lib.OK:
@@ -447,7 +447,7 @@ class RouterPlan(_GroupPlan):
             if t is not None:
                 need(t, name, 4, count, self.device if self.workspace is not None else _current_device())
         self._check(self._fn["bind_weights"](self.handle, _ptr(router_w), _ptr(bias)))
-        self._weights = (router_w, bias)
+        self._weights, self._bias = (router_w, bias), bias
 
     def forward(self, x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int, logits: Optional[torch.Tensor] = None):
         """x bf16 [rows, hidden] -> ids (32-bit) and probs f32 [rows, active], and the logits f32 [rows, experts] if asked for."""
@@ -466,6 +466,8 @@ class RouterPlan(_GroupPlan):
     def select(self, logits: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, rows: int):
         """The selection alone, from logits f32 [rows, experts] of any origin."""
         d, dev = self.desc, _current_device()
+        if self._bias is not None and self._bias.get_device() != dev:
+            raise OcoError(_lib.INVALID_ARGUMENT, f"the bias is on {self._bias.device}, the current device is cuda:{dev}")
         k = rows * d.top_k
         need(logits, "logits", 4, rows * d.experts, dev)
         need(ids, "ids", 4, k, dev)
@@ -502,6 +504,8 @@ class F8ExpertPlan(_GroupPlan):
         got = {}
         for name, n, k in (("gate", d.ffn, d.hidden), ("up", d.ffn, d.hidden), ("down", d.hidden, d.ffn)):
             got[name + "_w"], got[name + "_s"] = f8_matrix(getattr(w, name + "_w"), getattr(w, name + "_s"), (d.experts,), n, k, device, name)
+        if self.workspace is not None:
+            same_device(got, self.workspace)
         cw = _lib.F8Weights(**{n: t.data_ptr() for n, t in got.items()})
         self._check(self._fn["bind_weights"](self.handle, C.byref(cw)))
         self._weights = got

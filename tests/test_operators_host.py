@@ -194,3 +194,28 @@ def test_a_workspace_on_another_device_than_the_weights(lib):
         with pytest.raises(_lib.OcoError, match="another device"):
             plan.reserve(8, device="cpu")
         assert plan.workspace is None
+
+
+def test_weights_on_another_device_than_the_workspace(lib, monkeypatch):
+    """The other order: reserved on one device, bound while another one is current; and a bias that the current device has not."""
+    from oco_b200 import dense, moe, synth
+
+    class On:
+        def __init__(self, number):
+            self.number, self.device = number, f"cuda:{number}"
+
+        def get_device(self):
+            return self.number
+    for module in (moe, dense):
+        monkeypatch.setattr(module, "f8_matrix", lambda *a: (On(1), On(1)))
+    experts, projection = moe.F8ExpertPlan.new(128, 128, 4, 2), dense.DensePlan(dense.PROJECTION, synth.FMT_F8_E4M3, 128, 64)
+    for plan, args in ((experts, (moe.F8Experts(*[None] * 6),)), (projection, (None,))):
+        plan.workspace = On(0)
+        with pytest.raises(_lib.OcoError, match="another device"):
+            plan.bind(*args)
+        assert not plan._weights
+    router = moe.RouterPlan.new(0, 8, 2)
+    router._weights, router._bias = (None, On(1)), On(1)
+    monkeypatch.setattr(moe, "_current_device", lambda: 0)
+    with pytest.raises(_lib.OcoError, match="bias is on cuda:1"):
+        router.select(None, None, None, 1)
