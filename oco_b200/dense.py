@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib, synth
-from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr, f8_matrix, need, same_device
+from .moe import OcoError, _dev_bytes, _ptr, _stream_ptr, BF16, f8_matrix, need, same_device
 
 PROJECTION, FFN_RELU2, FFN_SILU_GATE = 0, 1, 2
 
@@ -79,8 +79,8 @@ class DensePlan:
     def forward(self, x: torch.Tensor, y: torch.Tensor, rows: int):
         """x: bf16 bit patterns [rows, hidden]; y receives [rows, ffn] (projection) or [rows, hidden]."""
         if self.fmt == synth.FMT_F8_E4M3 and rows > 0:
-            need(x, "x", 2, rows * self.hidden, self.device)
-            need(y, "y", 2, rows * (self.ffn if self.kind == PROJECTION else self.hidden), self.device)
+            need(x, "x", BF16, rows * self.hidden, self.device)
+            need(y, "y", BF16, rows * (self.ffn if self.kind == PROJECTION else self.hidden), self.device)
         rc = _lib.lib().oco_dense_forward(self.handle, x.data_ptr(), y.data_ptr(), rows, _stream_ptr())
         if rc:
             self._check(rc)

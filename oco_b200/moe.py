@@ -330,13 +330,16 @@ class Routing:
         return out
 
 
-def need(t: torch.Tensor, name: str, size: int, count: int, device: int):
-    """Refuses a tensor that the kernels could not read as `count` contiguous elements of `size` bytes on the CUDA device
-    of that number."""
-    if t.get_device() != device or t.element_size() != size or not t.is_contiguous() or t.numel() < count:
+BF16, F32, IDS = (torch.bfloat16,), (torch.float32,), (torch.int32, torch.uint32)
+
+
+def need(t: torch.Tensor, name: str, types: tuple, count: int, device: int):
+    """Refuses a tensor that is not `count` or more contiguous elements of one of the types on the CUDA device of that
+    number."""
+    if t.get_device() != device or t.dtype not in types or not t.is_contiguous() or t.numel() < count:
         if device < 0 and t.is_cuda:
             raise OcoError(_lib.INVALID_ARGUMENT, "reserve a workspace first")
-        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {size} bytes on cuda:{device} is needed, "
+        raise OcoError(_lib.INVALID_ARGUMENT, f"{name}: a contiguous CUDA tensor of {count} elements of {types[0]} on cuda:{device} is needed, "
                                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
@@ -445,7 +448,7 @@ class RouterPlan(_GroupPlan):
         d = self.desc
         for t, name, count in ((router_w, "router_w", d.experts * d.hidden), (bias, "bias", d.experts)):
             if t is not None:
-                need(t, name, 4, count, self.device if self.workspace is not None else _current_device())
+                need(t, name, F32, count, self.device if self.workspace is not None else _current_device())
         self._check(self._fn["bind_weights"](self.handle, _ptr(router_w), _ptr(bias)))
         self._weights, self._bias = (router_w, bias), bias
 
@@ -453,11 +456,11 @@ class RouterPlan(_GroupPlan):
         """x bf16 [rows, hidden] -> ids (32-bit) and probs f32 [rows, active], and the logits f32 [rows, experts] if asked for."""
         d, dev = self.desc, self.device
         k = rows * d.top_k
-        need(x, "x", 2, rows * d.hidden, dev)
-        need(ids, "ids", 4, k, dev)
-        need(probs, "probs", 4, k, dev)
+        need(x, "x", BF16, rows * d.hidden, dev)
+        need(ids, "ids", IDS, k, dev)
+        need(probs, "probs", F32, k, dev)
         if logits is not None:
-            need(logits, "logits", 4, rows * d.experts, dev)
+            need(logits, "logits", F32, rows * d.experts, dev)
             logits = logits.data_ptr()
         rc = self._fn["forward"](self.handle, x.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), logits, _stream_ptr())
         if rc:
@@ -469,9 +472,9 @@ class RouterPlan(_GroupPlan):
         if self._bias is not None and self._bias.get_device() != dev:
             raise OcoError(_lib.INVALID_ARGUMENT, f"the bias is on {self._bias.device}, the current device is cuda:{dev}")
         k = rows * d.top_k
-        need(logits, "logits", 4, rows * d.experts, dev)
-        need(ids, "ids", 4, k, dev)
-        need(probs, "probs", 4, k, dev)
+        need(logits, "logits", F32, rows * d.experts, dev)
+        need(ids, "ids", IDS, k, dev)
+        need(probs, "probs", F32, k, dev)
         rc = _lib.lib().oco_moe_router_select(self.handle, logits.data_ptr(), rows, ids.data_ptr(), probs.data_ptr(), _stream_ptr())
         if rc:
             self._check(rc)
@@ -516,11 +519,11 @@ class F8ExpertPlan(_GroupPlan):
         d, dev = self.desc, self.device
         out = residual if out is None else out
         n, k = rows * d.hidden, rows * d.top_k
-        need(x, "x", 2, n, dev)
-        need(ids, "ids", 4, k, dev)
-        need(probs, "probs", 4, k, dev)
-        need(residual, "residual", 2, n, dev)
-        need(out, "out", 2, n, dev)
+        need(x, "x", BF16, n, dev)
+        need(ids, "ids", IDS, k, dev)
+        need(probs, "probs", F32, k, dev)
+        need(residual, "residual", BF16, n, dev)
+        need(out, "out", BF16, n, dev)
         rc = self._fn["forward"](self.handle, x.data_ptr(), ids.data_ptr(), probs.data_ptr(), residual.data_ptr(), out.data_ptr(), rows, _stream_ptr())
         if rc:
             self._check(rc)
@@ -567,7 +570,7 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
             refuse("the elements of a row must be neighbours")
     for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
         if t is not None:
-            need(t, name, 4, width, dev)
+            need(t, name, F32, width, dev)
     gs = gate_type = per = 0
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.dtype not in (torch.bfloat16, torch.float32) or gate.get_device() != dev or gate.shape[-1] != width or gate.stride(-1) != 1:

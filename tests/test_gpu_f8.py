@@ -530,3 +530,25 @@ def test_rounding_of_activations_halfway_between_codes(lib, rows):
     codes, scales = opref.quantize(64.0 * (x @ up.t()))
     assert torch.equal(scales[:, 0], 64.0 * k) and codes.abs().max() == 448.0
     assert torch.equal(y.double().cpu(), codes * scales)
+
+
+def test_other_types_of_the_same_size(lib):
+    """Every entry point of the newer operators: fp16 rows are not bf16, floats are no ids, whole numbers no weights."""
+    plan, w, g = expert_layer(lib, 16, 128, 128, 4, 2, 8)
+    x, ids, probs = bf16(g, 8, 128), torch.zeros((8, 2), dtype=torch.int32, device="cuda"), torch.ones((8, 2), device="cuda")
+    router = lib.moe.RouterPlan.new(128, 4, 2)
+    router.reserve(8)
+    rw, rb = torch.zeros((4, 128), device="cuda"), torch.zeros(4, device="cuda")
+    router.bind(rw, rb)
+    dense, y = projection(lib, w["up"][0], w["up_s"][0], x)
+    logits = torch.zeros((8, 4), device="cuda")
+    out = torch.empty_like(x)
+    whole = lambda t: t.to(torch.int32)  # noqa: E731
+    for call in (lambda: plan.forward(x.half(), ids, probs, x, 8, out=out), lambda: plan.forward(x, ids.float(), probs, x, 8, out=out), lambda: plan.forward(x, ids, whole(probs), x, 8, out=out),
+                 lambda: plan.forward(x, ids, probs, x.half(), 8, out=out), lambda: plan.forward(x, ids, probs, x, 8, out=out.half()), lambda: router.bind(whole(rw), rb), lambda: router.bind(rw, whole(rb)),
+                 lambda: router.forward(x.half(), ids, probs, 8), lambda: router.forward(x, ids.float(), probs, 8), lambda: router.forward(x, ids, whole(probs), 8),
+                 lambda: router.forward(x, ids, probs, 8, logits=whole(logits)), lambda: router.select(whole(logits), ids, probs, 8), lambda: router.select(logits, ids.float(), probs, 8),
+                 lambda: dense.forward(x.half(), y, 8), lambda: dense.forward(x, y.half(), 8), lambda: lib.moe.block_norm(x, norm_out=out, pre_weight=whole(torch.ones(128, device="cuda")))):
+        with pytest.raises(_lib.OcoError, match="is needed"):
+            call()
+    router.forward(x, ids.view(torch.uint32), probs, 8)

@@ -219,3 +219,15 @@ def test_weights_on_another_device_than_the_workspace(lib, monkeypatch):
     monkeypatch.setattr(moe, "_current_device", lambda: 0)
     with pytest.raises(_lib.OcoError, match="bias is on cuda:1"):
         router.select(None, None, None, 1)
+
+
+def test_other_types_of_the_same_size(lib):
+    """A tensor whose elements are as large as the right ones is refused all the same."""
+    from oco_b200 import moe
+    for types, good, bad in ((moe.BF16, (torch.bfloat16,), (torch.float16, torch.int16, torch.uint16)), (moe.F32, (torch.float32,), (torch.int32, torch.uint32)),
+                             (moe.IDS, (torch.int32, torch.uint32), (torch.float32,))):
+        for t in good:
+            moe.need(torch.zeros(4, dtype=t), "x", types, 4, -1)
+        for t in bad:
+            with pytest.raises(_lib.OcoError, match="is needed"):
+                moe.need(torch.zeros(4, dtype=t), "x", types, 4, -1)
