@@ -7,17 +7,13 @@
 
 namespace oco {
 
-constexpr int kF8MaxExperts = 512, kF8MaxTopK = 16, kF8Block = 128;
+constexpr int kF8MaxExperts = 512, kF8MaxTopK = 16;
 
 // Four f32 values as e4m3 codes in one word (round to nearest even; beyond the range: the largest; NaN stays NaN).
 __device__ __forceinline__ uint32_t f8x4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
-}
-__device__ __forceinline__ float f8_value(uint8_t c) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3);
-    return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
 // ---- expert-sorted order of the routes ----------------------------------------------------------------------------
