@@ -94,15 +94,8 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t adesc, u
 __device__ __forceinline__ uint32_t umma_idesc_f16_pair(uint32_t n) {
     return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
-// One arrival, when the MMAs issued so far have retired, on the barrier at `bar` of both CTAs (one instruction
-// per CTA; a single instruction that signals both measured the same).
+// One arrival, when the MMAs issued so far have retired, on the barrier at `bar` of both CTAs.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-    const uint32_t b0 = map_to_cta(bar, 0), b1 = map_to_cta(bar, 1);
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b0) : "memory");
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b1) : "memory");
-}
-// The same as one instruction that signals both CTAs.
-__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 // This CTA's box of route rows into its own shared memory; the bytes are counted on the barrier at `cluster_bar`

@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(F8Wide<PAIR>::kThreads, 1) f8_wide_kernel(cons
                         if (PAIR) umma_f8f6f4_pair(d0 + 256u * b, a + 2u * k, w + 2u * k, idesc, k ? 1u : 0u);
                         else umma_f8f6f4(d0 + 256u * b, a + 2u * k, w + 2u * k, idesc, k ? 1u : 0u);
                     }
-                    if (PAIR) umma_commit_both(done(s));
+                    if (PAIR) umma_commit_pair(done(s));
                     else umma_commit(done(s));
                 }
                 __syncwarp();
