@@ -38,9 +38,15 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
-def _stream_ptr():
-    """The current stream of the current device. (torch.cuda.current_stream() builds an object for it, 3 us a call.)"""
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+# torch.cuda.current_stream() builds an object for the handle, 3 us a call; torch's own shortcut is not a public name
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_ptr(device: Optional[int] = None):
+    """The current stream of the current device (`device`: its number, where the caller has it already)."""
+    if _raw_stream is None:
+        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(_raw_stream(torch.cuda.current_device() if device is None else device))
 
 
 def _dev_bytes(a: Optional[np.ndarray], device, misalign: int = 0) -> Optional[torch.Tensor]:
@@ -344,7 +350,7 @@ def need(t: torch.Tensor, name: str, types: tuple, count: int, device: int):
 
 
 def _current_device() -> int:
-    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    return torch.cuda.current_device() if torch.cuda.is_initialized() else -2
 
 
 def same_device(weights, workspace: torch.Tensor):
@@ -549,8 +555,8 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
     wide = hidden.dtype is torch.float32
     if hidden.dim() != 2 or dev < 0 or not (wide or hidden.dtype is torch.bfloat16):
         refuse("hidden: CUDA rows [rows, width], bf16 or f32")
-    if dev != _current_device():
-        refuse(f"hidden is on {hidden.device}, the current device is cuda:{_current_device()}")
+    if dev != (current := _current_device()):
+        refuse(f"hidden is on {hidden.device}, the current device is cuda:{current}")
     rows, width = shape = hidden.shape
     if kind not in NORMS or gate_act not in GATE_ACTS:
         refuse(f"kind is one of {sorted(NORMS)}, gate_act one of {sorted(GATE_ACTS)}")
@@ -590,11 +596,11 @@ def block_norm(hidden: torch.Tensor, block: Optional[torch.Tensor] = None, *, hi
                            strides[0], strides[1], gs, strides[2], strides[3])
     if rows == 0:      # an empty tensor has no address
         return
-    rc = _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(), None, 0)
+    rc = _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(dev), None, 0)
     if rc:
         err = C.create_string_buffer(160)
         if rc in (_lib.INVALID_ARGUMENT, _lib.UNSUPPORTED_SHAPE):      # refused before anything ran: asked again for the reason
-            _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(), err, len(err))
+            _lib.lib().oco_moe_block_norm(args, rows, _stream_ptr(dev), err, len(err))
         raise OcoError(rc, err.value.decode())
 
 

@@ -231,3 +231,17 @@ def test_other_types_of_the_same_size(lib):
         for t in bad:
             with pytest.raises(_lib.OcoError, match="is needed"):
                 moe.need(torch.zeros(4, dtype=t), "x", types, 4, -1)
+
+
+def test_streams_without_torch_s_shortcut(monkeypatch):
+    """The handle of the current stream by the public call, where torch has no other."""
+    from oco_b200 import moe
+
+    class Stream:
+        cuda_stream = 0x7100
+    monkeypatch.setattr(moe, "_raw_stream", None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: Stream)
+    assert moe._stream_ptr().value == 0x7100
+    monkeypatch.setattr(moe, "_raw_stream", lambda device: 0x7200 + device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    assert moe._stream_ptr().value == 0x7203
