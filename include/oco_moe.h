@@ -365,7 +365,7 @@ size_t oco_dense_workspace_bytes(const oco_dense_plan* plan, int max_rows);
 int oco_dense_bind_workspace(oco_dense_plan* plan, void* workspace, size_t bytes, int max_rows);
 int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* weights);
 /* OCO_FMT_F8_E4M3 (OCO_DENSE_PROJECTION and OCO_DENSE_FFN_SILU_GATE; hidden and ffn multiples of 32, codes 16-byte
- * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes. The arithmetic
+ * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes (binding waits as oco_moe_f8_bind_weights does). The arithmetic
  * is that of the oco_moe_f8_plan calls at every row count: no single-token numerics of its own. 0 rows are no work; a
  * projection's y must not overlap x. */
 typedef struct {
@@ -490,9 +490,9 @@ int oco_moe_f8_bind_workspace(oco_moe_f8_plan* plan, void* workspace, size_t byt
 int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* weights);
 /* x, residual, out: bf16 [rows, hidden], 16-byte aligned (out may be residual or x;
  * a part of the residual it must not be); ids u32, probs f32 [rows, top_k].
- * Only enqueues; 0 rows are no work. Weights are fetched ahead of the kernels before them in the stream: a kernel or
- * copy that writes them and lies before the call in stream order is waited for, as long as it does not itself let
- * its successor start early. */
+ * Only enqueues; 0 rows are no work. Weights are immutable while they are bound: a call may fetch them before the work
+ * ahead of it in the stream has ended. Binding waits until what was enqueued on the device before it, such as the
+ * kernels that write the weights, has ended; bind again after rewriting them. */
 int oco_moe_f8_forward(oco_moe_f8_plan* plan, const uint16_t* x_bf16, const uint32_t* ids, const float* probs,
                        const uint16_t* residual_bf16, uint16_t* out_bf16, int rows, void* cuda_stream);
 int oco_moe_f8_poll(oco_moe_f8_plan* plan, void* cuda_stream);

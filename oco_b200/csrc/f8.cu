@@ -268,6 +268,7 @@ int f8_dense_bind_scales(oco_moe_f8_plan* p, const oco_dense_scales& s) {
     if (int rc = check_scales(p)) return rc;
     if (int rc = make_maps(p)) return rc;
     if (int rc = p->note_weights()) return rc;
+    OCO_CK(p, cudaDeviceSynchronize());     // calls fetch weights ahead of the work before them: what writes them has ended
     p->have_w = true;
     return OCO_OK;
 }
@@ -336,6 +337,7 @@ int oco_moe_f8_bind_weights(oco_moe_f8_plan* plan, const oco_moe_f8_weights* w) 
     if (int rc = check_scales(plan)) return rc;
     if (int rc = make_maps(plan)) return rc;
     if (int rc = plan->note_weights()) return rc;
+    OCO_CK(plan, cudaDeviceSynchronize());  // as in f8_dense_bind_scales
     plan->have_w = true;
     return OCO_OK;
 }

@@ -415,9 +415,10 @@ struct F8Thin {
 // One item (a tile of up to NT rows of one expert, 128 features) per cluster; CTA r of its S takes the blocks
 // [r * per, ..) of the contraction. x = S * (item), items: feature tile fastest.
 //
-// Weights travel before the kernel before is waited for: they, the tiles and (kF8Concat) the ids come from before the call
-// or from a kernel that has ended when this one may start, since every kernel of a call lets the next one start only after
-// its own wait. kF8Rows with ids (a router may just have written them) waits first.
+// Weights travel before the kernel before is waited for: they have been there since they were bound (one row through 4096
+// -> 6144 features: 5.8 us, after the wait 6.9), and the tiles and (kF8Concat) the ids come from a kernel that has ended
+// when this one may start, since every kernel of a call lets the next one start only after its own wait. kF8Rows with ids
+// (a router may just have written them) waits first.
 template <int NT, bool GATED, int FORM>
 __global__ void __launch_bounds__(F8Thin<NT, GATED, FORM>::kThreads, 2) f8_thin_kernel(const F8TileParams p, const __grid_constant__ CUtensorMap rows_map,
                                                                                    const __grid_constant__ CUtensorMap w0_map,

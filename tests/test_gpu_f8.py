@@ -552,3 +552,29 @@ def test_other_types_of_the_same_size(lib):
         with pytest.raises(_lib.OcoError, match="is needed"):
             call()
     router.forward(x, ids.view(torch.uint32), probs, 8)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_weights_written_just_before_they_are_bound(lib, rows):
+    """Codes that kernels of another stream are still making when they are bound: binding waits for them, as calls fetch
+    weights ahead of the work before them."""
+    H, F = 2048, 4096
+    g = gen(rows)
+    wide = torch.randn((F, H), device="cuda", generator=g)
+    x = bf16(g, rows, H)
+    one = torch.full((F // 128, H // 128), 2e-4, device="cuda")
+    plan = lib.dense.DensePlan(lib.dense.PROJECTION, synth.FMT_F8_E4M3, H, F)
+    plan.reserve(rows)
+    y = torch.empty((rows, F), dtype=torch.bfloat16, device="cuda")
+    codes = torch.zeros((F, H), dtype=torch.float8_e4m3fn, device="cuda")
+    slow = torch.randn((8192, 8192), device="cuda", generator=g)
+    slow_out = slow @ slow
+    torch.cuda.synchronize()
+    for size in (105.0, 50.0):                               # and once more after rewriting them
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(4):                               # some tens of milliseconds
+                torch.mm(slow, slow, out=slow_out)
+            codes.copy_((wide * size).clamp(-448, 448))
+        plan.bind(codes, up_scale=one)
+        plan.forward(x, y, rows)
+        within(y, *opref.product(*opref.quantize(x.double()), (wide * size).clamp(-448, 448).to(torch.float8_e4m3fn), one))
