@@ -126,174 +126,180 @@ __device__ __forceinline__ Best warp_best(Best b) {
     return Best{__shfl_sync(0xffffffffu, b.v, from), __shfl_sync(0xffffffffu, b.i, from)};
 }
 
-// Writes ids and weights of one token; called by a whole warp. `d`: the largest error of a logit. Every
-// value is held with its error, and what is decided between two values is settled when their intervals do not overlap;
-// the logits of those that do are summed again. Ranked is score + bias, without a bias the logit itself: scores that
-// have run into 0 or 1 keep the order of their logits. Not inlined: it is rare and would cost the 32-bit path registers.
+// One token in 64 bits, by a warp. `l`: the lane's logits, `precise`: bit i: element i's is exact, `d`: the largest error of
+// the others (0: none). Every value is held with its error, and what is decided between two values is settled when their
+// intervals do not overlap. Returns the lane's elements whose exact logits could turn a decision; none in the whole warp:
+// ids and weights are written. Ranked is score + bias, without a bias the logit itself: scores that have run into 0 or 1
+// keep the order of their logits. Not inlined: it is rare and would cost the 32-bit path registers.
 template <int VPL>
-__device__ __noinline__ void select_exact(const SelectParams& p, int row, const float* lrow, int lane, double d) {
+__device__ __noinline__ uint32_t exact_step(const SelectParams& p, int row, int lane, double d, const double (&l)[VPL], uint32_t precise) {
     const int E = p.E, gs = p.E / p.G;
-    const bool soft = p.score == OCO_SCORE_SOFTMAX, remake = d > 0.0;
-    const bool scored = !p.bias && p.best == 2 && gs > 1;              // groups are worth scores, experts are ranked by logits
-    double l[VPL], s[VPL], r[VPL], er[VPL], w[VPL], ew[VPL];           // logit, score, rank and part of a group's worth with their errors
-    int group[VPL];                                                    // -1: behind the last expert
-    uint32_t precise = remake ? 0u : 0xffffffffu;                      // bit i: element i's logit is exact
-    double top = -1.0 / 0.0;
+    const bool soft = p.score == OCO_SCORE_SOFTMAX, two = p.best == 2 && gs > 1;
+    const bool scored = !p.bias && two;                                // groups are worth scores, experts are ranked by logits
+    const bool far = d > 0.5;                                          // up to here e^d - 1 is below d (1 + d); scores lie in 0 .. 1 in any case
+    double s[VPL], r[VPL], er[VPL], w[VPL], ew[VPL];                   // score, rank and part of a group's worth with their errors
+    double top = -1.0 / 0.0, z = 0.0;
+    uint32_t in = 0;                                                   // bit i: an expert that can be chosen
+    bool all = true;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
-        const int x = lane * VPL + i;
-        l[i] = x < E ? (double)__ldcg(lrow + x) : 0.0;
-        group[i] = x < E ? x / gs : -1;
-        if (x < E) top = fmax(top, l[i]);
+        if (lane * VPL + i >= E) continue;
+        in |= 1u << i;
+        top = fmax(top, l[i]);
+        all = all && ((precise >> i) & 1u);
     }
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, k));
-    while (true) {
-        // scores, ranks and errors from the present logits
-        double z = 0.0;
-        bool all = true;
+    all = __all_sync(0xffffffffu, all);
 #pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            const int x = lane * VPL + i;
-            if (x < E && !((precise >> i) & 1u)) all = false;
-            s[i] = soft ? exp(l[i] - top) : 1.0 / (1.0 + exp(-l[i]));
-            if (x < E) z += s[i];
+    for (int i = 0; i < VPL; i++) {
+        s[i] = soft ? exp(l[i] - top) : 1.0 / (1.0 + exp(-l[i]));
+        if ((in >> i) & 1u) z += s[i];
+    }
+    if (soft) z = warp_sum_d(z);
+#pragma unroll
+    for (int i = 0; i < VPL; i++) {
+        const double dl = ((precise >> i) & 1u) || l[i] == -1.0 / 0.0 ? 0.0 : d;   // a masked expert is one for sure
+        // d ln s / dl lies between 0 and 1, and so does the slope of a sigmoid's s (1 - s) in those terms
+        const double e = dl == 0.0 ? 0.0 : soft ? (far ? 1.0 / 0.0 : s[i] * dl * (1.0 + dl)) : far ? 1.0 : dl * fmin(0.25, s[i] * (1.0 - s[i]) * (1.0 + dl * (1.0 + dl)));
+        w[i] = s[i]; ew[i] = e;                                        // of a softmax before its division, which is the same for all
+        if (soft) s[i] /= z;
+        r[i] = l[i]; er[i] = dl;
+        if (p.bias) {
+            r[i] = (in >> i) & 1u ? s[i] + (double)p.bias[lane * VPL + i] : 0.0;
+            if (r[i] != r[i]) r[i] = -1.0 / 0.0;
+            er[i] = !soft ? e : all ? 0.0 : far ? 1.0 : s[i] * (dl + d) * (1.0 + dl + d);   // the sum is exact when all logits are
         }
-        all = __all_sync(0xffffffffu, all);
-        z = soft ? warp_sum_d(z) : 1.0;
+        if (!scored) { w[i] = r[i]; ew[i] = er[i]; }
+    }
+    bool open = false;                                                 // a decision that exact logits could turn
+    uint32_t want = 0;
+    if (p.TG < p.G) {
+        double worth = 0.0, low = 0.0, high = 0.0, edge = 0.0;         // lane g: group g, the ends of its interval, the least lower end among its best
+        const int lanes = gs / VPL;
+        const double none = -1.0 / 0.0;
+        if (gs % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+            // a group is 2^n lanes: the two best values (with their errors) and the two best upper ends of every group at once
+            double a1 = none, a2 = none, e1 = 0.0, e2 = 0.0, h1 = none, h2 = none;
+            auto take = [&](double v, double e) {
+                if (v > a1) { a2 = a1; e2 = e1; a1 = v; e1 = e; }
+                else if (v > a2) { a2 = v; e2 = e; }
+            };
+            auto lift = [&](double h) {
+                if (h > h1) { h2 = h1; h1 = h; }
+                else if (h > h2) h2 = h;
+            };
 #pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            const int x = lane * VPL + i;
-            const double dl = (precise >> i) & 1u || l[i] == -1.0 / 0.0 ? 0.0 : d;   // a masked expert is one for sure
-            // d ln s / dl lies between 0 and 1, and so does the slope of a sigmoid's s (1 - s) in those terms; scores lie in 0 .. 1
-            const double e = soft ? (d > 1.0 ? (dl > 0.0 ? 1.0 / 0.0 : 0.0) : s[i] * expm1(dl))
-                                  : (d > 1.0 ? (dl > 0.0 ? 1.0 : 0.0) : dl * fmin(0.25, s[i] * (1.0 - s[i]) * exp(dl)));
-            w[i] = s[i]; ew[i] = e;                                    // of a softmax before its division, which is the same for all
-            s[i] /= z;
-            r[i] = l[i]; er[i] = dl;
-            if (p.bias) {
-                r[i] = x < E ? s[i] + (double)p.bias[x] : 0.0;
-                if (r[i] != r[i]) r[i] = -1.0 / 0.0;
-                er[i] = !soft ? e : all ? 0.0 : d > 1.0 ? 1.0 : s[i] * expm1(dl + d);   // the sum is exact when all logits are
+            for (int i = 0; i < VPL; i++) { take(w[i], ew[i]); lift(w[i] + ew[i]); }
+            for (int k = 1; k < lanes; k <<= 1) {
+                const double b1 = __shfl_xor_sync(0xffffffffu, a1, k), b2 = __shfl_xor_sync(0xffffffffu, a2, k), f1 = __shfl_xor_sync(0xffffffffu, e1, k), f2 = __shfl_xor_sync(0xffffffffu, e2, k);
+                const double g1 = __shfl_xor_sync(0xffffffffu, h1, k), g2 = __shfl_xor_sync(0xffffffffu, h2, k);
+                take(b1, f1); take(b2, f2);
+                lift(g1); lift(g2);
             }
-            if (!scored) { w[i] = r[i]; ew[i] = er[i]; }
-        }
-        bool open = false;                                             // a decision that exact logits could turn
-        uint32_t want = 0;
-        // sum of the p.best largest values of group g, with their errors on top (f = 1); without (f = 0) also the sum of
-        // their lower ends, and the least of these
-        auto worth_of = [&](int g, double f, double& low, double& edge) {
-            int first = -1;
-            double sum = 0.0;
-            low = 0.0;
-            for (int t = 0; t < min(p.best, gs); t++) {
-                Best b{0.0, -1};
-                double e = 0.0;
-#pragma unroll
-                for (int i = 0; i < VPL; i++) {
-                    const double v = f == 0.0 ? w[i] : w[i] + ew[i];
-                    if (group[i] == g && lane * VPL + i != first && (b.i < 0 || v > b.v)) { b.v = v; b.i = lane * VPL + i; e = ew[i]; }
-                }
-                const Best best = warp_best(b);
-                e = __shfl_sync(0xffffffffu, e, best.i / VPL);
-                first = best.i;
-                edge = t ? fmin(edge, best.v - e) : best.v - e;
-                low += best.v - e;
-                sum += best.v;
-            }
-            return sum;
-        };
-        uint32_t groups = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u;
-        if (p.TG < p.G) {
-            double worth = 0.0, low = 0.0, high = 0.0, edge = 0.0;     // lane g: group g
+            const int from = min(31, lane * lanes);
+            worth = __shfl_sync(0xffffffffu, two ? a1 + a2 : a1, from);
+            low = __shfl_sync(0xffffffffu, two ? (a1 - e1) + (a2 - e2) : a1 - e1, from);
+            edge = __shfl_sync(0xffffffffu, two ? fmin(a1 - e1, a2 - e2) : a1 - e1, from);
+            high = __shfl_sync(0xffffffffu, two ? h1 + h2 : h1, from);
+        } else {
             for (int g = 0; g < p.G; g++) {
-                double b, e, none, least;
-                const double a = worth_of(g, 0.0, b, e), c = remake ? worth_of(g, 1.0, none, least) : a;
-                if (lane == g) { worth = a; low = b; high = c; edge = e; }
-            }
-            uint32_t left = groups;
-            for (int t = 0; t < p.TG; t++) left &= ~(1u << warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1}).i);
-            groups &= ~left;
-            const double out = warp_best(Best{high, ((left >> lane) & 1u) ? lane : -1}).v;
-            const double in = -warp_best(Best{-low, ((groups >> lane) & 1u) ? lane : -1}).v;
-            if (in < out) {
-                open = true;
-                for (int g = 0; g < p.G; g++) {                        // every group at the border: what could be among its best
-                    const double lg = __shfl_sync(0xffffffffu, low, g), hg = __shfl_sync(0xffffffffu, high, g), eg = __shfl_sync(0xffffffffu, edge, g);
-                    if ((groups >> g) & 1u ? !(lg < out) : !(hg > in)) continue;
+                double sum = 0.0, lower = 0.0, upper = 0.0, least = 0.0;
+                for (int f = 0; f < 2; f++) {                          // values, then upper ends
+                    int first = -1;
+                    for (int t = 0; t <= (int)two; t++) {
+                        Best b{0.0, -1};
+                        double e = 0.0;
 #pragma unroll
-                    for (int i = 0; i < VPL; i++) {
-                        if (group[i] == g && w[i] + ew[i] >= eg) want |= 1u << i;
+                        for (int i = 0; i < VPL; i++) {
+                            const double v = f ? w[i] + ew[i] : w[i];
+                            const int x = lane * VPL + i;
+                            if (((in >> i) & 1u) && x / gs == g && x != first && (b.i < 0 || v > b.v)) { b.v = v; b.i = x; e = ew[i]; }
+                        }
+                        b = warp_best(b);
+                        e = __shfl_sync(0xffffffffu, e, b.i / VPL);
+                        first = b.i;
+                        if (f) upper += b.v;
+                        else {
+                            sum += b.v;
+                            lower += b.v - e;
+                            least = t ? fmin(least, b.v - e) : b.v - e;
+                        }
                     }
                 }
+                if (lane == g) { worth = sum; low = lower; high = upper; edge = least; }
             }
         }
-        uint32_t taken = 0;
-        int my_id = -1;
-        double my_s = 0.0;
-        for (int j = 0; j < p.K; j++) {
-            Best b{0.0, -1};
-#pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                if (group[i] >= 0 && ((groups >> group[i]) & 1u) && !((taken >> i) & 1u) && (b.i < 0 || r[i] > b.v)) { b.v = r[i]; b.i = lane * VPL + i; }
-            }
-            b = warp_best(b);
-            double sv = 0.0, low = 0.0;
-#pragma unroll
-            for (int i = 0; i < VPL; i++)
-                if (lane * VPL + i == b.i) { taken |= 1u << i; sv = s[i]; low = r[i] - er[i]; }
-            sv = __shfl_sync(0xffffffffu, sv, b.i / VPL);
-            low = __shfl_sync(0xffffffffu, low, b.i / VPL);
-            if (lane == j) { my_id = b.i; my_s = sv; }
-            bool passes = false;                                       // one that is not taken yet could be the larger one
-#pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                if (group[i] >= 0 && ((groups >> group[i]) & 1u) && !((taken >> i) & 1u) && r[i] + er[i] > low) { passes = true; want |= 1u << i; }
-            }
-            if (__any_sync(0xffffffffu, passes)) {
-                open = true;
+        uint32_t left = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u, groups = left;
+        for (int t = 0; t < p.TG; t++) left &= ~(1u << warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1}).i);
+        groups &= ~left;
+        const double outside = warp_best(Best{high, ((left >> lane) & 1u) ? lane : -1}).v;
+        const double inside = -warp_best(Best{-low, ((groups >> lane) & 1u) ? lane : -1}).v;
+        if (inside < outside) {                                        // every group at the border: what could be among its best
+            open = true;
+            const uint32_t border = __ballot_sync(0xffffffffu, ((groups >> lane) & 1u) ? low < outside : ((left >> lane) & 1u) && high > inside);
+            for (uint32_t rest = border; rest; rest &= rest - 1) {
+                const int g = __ffs((int)rest) - 1;
+                const double at = __shfl_sync(0xffffffffu, edge, g);
 #pragma unroll
                 for (int i = 0; i < VPL; i++)
-                    if (lane * VPL + i == b.i) want |= 1u << i;
+                    if (((in >> i) & 1u) && (lane * VPL + i) / gs == g && w[i] + ew[i] >= at) want |= 1u << i;
             }
         }
-        want &= ~precise;
-        if (open && !all && !__any_sync(0xffffffffu, want != 0)) want = ~precise;   // only the softmax's sum is left to doubt
-        if (!open || !remake || all) {
-            const double sum = p.normalize ? fmax(warp_sum_d(lane < p.K ? my_s : 0.0), 6.103515625e-5) : 1.0;
-            if (lane < p.K) {
-                p.ids[(size_t)row * p.K + lane] = (uint32_t)my_id;
-                p.probs[(size_t)row * p.K + lane] = (float)(my_s / sum * (double)p.scale);
-            }
-            return;
-        }
-        // sum the wanted logits again, two at a time
-        int first = -1;
-        auto keep = [&](int x, double v) {
 #pragma unroll
-            for (int q = 0; q < VPL; q++)
-                if (lane * VPL + q == x) l[q] = v;
-        };
-        for (int i = 0; i < VPL; i++) {
-            uint32_t lanes = __ballot_sync(0xffffffffu, ((want >> i) & 1u) && lane * VPL + i < E);
-            while (lanes) {
-                const int x = (__ffs((int)lanes) - 1) * VPL + i;
-                lanes &= lanes - 1;
-                if (first < 0) { first = x; continue; }
-                double da, db;
-                exact_logits(p, row, lane, first, x, da, db);
-                keep(first, da);
-                keep(x, db);
-                first = -1;
-            }
-        }
-        if (first >= 0) {
-            double da, db;
-            exact_logits(p, row, lane, first, first, da, db);
-            keep(first, da);
-        }
-        precise |= want;
+        for (int i = 0; i < VPL; i++)
+            if (((in >> i) & 1u) && !((groups >> ((lane * VPL + i) / gs)) & 1u)) in &= ~(1u << i);
     }
+    Best mine{0.0, -1};                                                // the lane's best that is left
+    auto scan = [&]() {
+        mine.i = -1;
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (((in >> i) & 1u) && (mine.i < 0 || r[i] > mine.v)) { mine.v = r[i]; mine.i = lane * VPL + i; }
+    };
+    scan();
+    int my_id = -1;
+    double my_s = 0.0;
+    for (int j = 0; j < p.K; j++) {
+        const Best b = warp_best(mine);
+        const int from = b.i / VPL;
+        double sv = 0.0, low = 0.0;
+        if (lane == from) {
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (lane * VPL + i == b.i) { in &= ~(1u << i); sv = s[i]; low = r[i] - er[i]; }
+            scan();
+        }
+        sv = __shfl_sync(0xffffffffu, sv, from);
+        if (lane == j) { my_id = b.i; my_s = sv; }
+        if (all) continue;
+        low = __shfl_sync(0xffffffffu, low, from);
+        bool passes = false;                                           // one that is not taken yet could be the larger one
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (((in >> i) & 1u) && r[i] + er[i] > low) { passes = true; want |= 1u << i; }
+        if (__any_sync(0xffffffffu, passes)) {
+            open = true;
+            if (lane == from) want |= 1u << (b.i - from * VPL);
+        }
+    }
+    if (!open || all) {
+        const double sum = p.normalize ? fmax(warp_sum_d(lane < p.K ? my_s : 0.0), 6.103515625e-5) : 1.0;
+        if (lane < p.K) {
+            p.ids[(size_t)row * p.K + lane] = (uint32_t)my_id;
+            p.probs[(size_t)row * p.K + lane] = (float)(my_s / sum * (double)p.scale);
+        }
+        return 0u;
+    }
+    want &= ~precise;
+    if (!__any_sync(0xffffffffu, want != 0)) {                         // only the softmax's sum is left to doubt
+        want = ~precise;
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (lane * VPL + i >= E) want &= ~(1u << i);
+        want &= (1u << VPL) - 1u;
+    }
+    return want;
 }
 
 // ---- 32-bit path -----------------------------------------------------------------------------------------------------
@@ -333,7 +339,7 @@ enum OpenKind {
     kDone,
     kWinners,        // put in order the winners that are too near: lane j's is not told apart from lane j - 1's where bit j of `near` is set
     kGroups,         // decide between the last group that stays (`at`) and the first that goes (`at2`); lanes 0, 1 and 2, 3 want their best
-    kAll             // go through select_exact
+    kAll             // go through exact_step, as often as that wants more exact logits
 };
 struct Open {
     int kind, want, my_id, at, at2;
@@ -474,9 +480,9 @@ __device__ __forceinline__ Open choose(const SelectParams& p, const OpenRow& o, 
     return q;
 }
 
-// Takes an open token to its end; `l`: the exact logits of the lanes' experts. `key`: the sorted keys (kGroups).
+// Takes an open token to its end, or to kAll; `l`: the exact logits of the lanes' experts. `key`: the sorted keys (kGroups).
 template <int VPL>
-__device__ __noinline__ void settle(const SelectParams& p, OpenRow o, int lane, Margin margin, uint32_t (&key)[VPL], Open q, double l) {
+__device__ __noinline__ bool settle(const SelectParams& p, OpenRow o, int lane, Margin margin, uint32_t (&key)[VPL], Open q, double l) {
     const double z = softmax_sum<VPL>(p, o, lane);
     double r, v;
     exact_values(p, o, q.want, l, z, r, v);
@@ -516,10 +522,10 @@ __device__ __noinline__ void settle(const SelectParams& p, OpenRow o, int lane, 
             write_row(p, o, lane, id);
         }
     }
-    if (q.kind == kAll) select_exact<VPL>(p, o.row, o.logits, lane, (double)o.error);
+    return q.kind == kAll;
 }
 
-// What a decision between two groups needs: their best experts. Groups whose best are not clear go through select_exact.
+// What a decision between two groups needs: their best experts. Groups whose best are not clear go through exact_step.
 template <int VPL>
 __device__ __noinline__ Open best_of_groups(const SelectParams& p, int lane, Margin margin, const uint32_t (&key)[VPL], Open q) {
     const int gs = p.E / p.G, best = min(p.best, gs);
@@ -749,23 +755,52 @@ __device__ __forceinline__ void select_tokens(const SelectParams& p, int row, fl
     uint32_t kept[VPL];
     Open q{kDone, -1, 0, 0, 0, 0u, 0u};
     if (row >= 0) q = select_row<VPL>(p, row, error, lane, o, margin, kept);
+    if (PRODUCT ? !__syncthreads_or(q.kind != kDone) : q.kind == kDone) return;
     double l = 0.0;
-    if (PRODUCT) {
-        if (!__syncthreads_or(q.kind != kDone)) return;
-        const uint32_t lanes = __ballot_sync(0xffffffffu, (q.kind == kWinners || q.kind == kGroups) && q.want >= 0);
-        const int at = __popc(lanes & ((1u << lane) - 1u));
+    uint32_t lanes = 0;
+    int at = 0;
+    // `wanted` experts of the lanes, up to 32 of a warp, are summed by the CTA; each lane gets its own
+    auto sum_wanted = [&](bool wants, int expert) {
+        lanes = __ballot_sync(0xffffffffu, wants);
+        at = __popc(lanes & ((1u << lane) - 1u));
         if (lane == 0) { sh->row[warp] = row; sh->count[warp] = __popc(lanes); }
-        if ((lanes >> lane) & 1u) sh->want[warp][at] = q.want;
+        if (wants) sh->want[warp][at] = expert;
         __syncthreads();
         exact_wanted(p, *sh);
-        if (q.kind == kDone) return;
-        if ((lanes >> lane) & 1u)
-            for (int w = 0; w < 8; w++) l += sh->part[w][warp][at];
-    } else {
-        if (q.kind == kDone) return;
-        if (q.want >= 0) l = (double)__ldcg(o.logits + q.want);
+        double v = 0.0;
+        if (wants)
+            for (int w = 0; w < 8; w++) v += sh->part[w][warp][at];
+        return v;
+    };
+    const bool some = (q.kind == kWinners || q.kind == kGroups) && q.want >= 0;
+    if (PRODUCT) l = sum_wanted(some, q.want);
+    else if (some) l = (double)__ldcg(o.logits + q.want);
+    bool open = q.kind == kAll;
+    if (q.kind == kWinners || q.kind == kGroups) open = settle<VPL>(p, o, lane, margin, kept, q, l);
+    if (PRODUCT ? !__syncthreads_or(open) : !open) return;
+    double all[VPL];
+    uint32_t precise = 0, want = 0;
+    if (open) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) all[i] = lane * VPL + i < p.E ? (double)__ldcg(o.logits + lane * VPL + i) : 0.0;
+        if (!(o.error > 0.f)) precise = 0xffffffffu;
     }
-    settle<VPL>(p, o, lane, margin, kept, q, l);
+    while (true) {
+        if (open && !__any_sync(0xffffffffu, want != 0u)) {
+            want = exact_step<VPL>(p, row, lane, (double)o.error, all, precise);
+            open = __any_sync(0xffffffffu, want != 0u);
+        }
+        if (PRODUCT ? !__syncthreads_or(open) : true) return;
+        const int i = __ffs((int)want) - 1;                            // one element of a lane at a time
+        l = sum_wanted(open && i >= 0, lane * VPL + i);
+        if (i >= 0) {
+#pragma unroll
+            for (int k = 0; k < VPL; k++)
+                if (k == i) all[k] = l;
+            want &= want - 1;
+            precise |= 1u << i;
+        }
+    }
 }
 
 // CTAs an SM: what is bound by the latency of one row after the other gains a little from more warps than the registers of
