@@ -338,11 +338,11 @@ __device__ __forceinline__ double softmax_sum(const SelectParams& p, const OpenR
 enum OpenKind {
     kDone,
     kWinners,        // put in order the winners that are too near: lane j's is not told apart from lane j - 1's where bit j of `near` is set
-    kGroups,         // decide between the last group that stays (`at`) and the first that goes (`at2`); lanes 0, 1 and 2, 3 want their best
+    kGroups,         // decide which `stay` of the groups in `near` do (`out`: the groups that go, all of those too); `group`: of the lane's expert
     kAll             // go through exact_step, as often as that wants more exact logits
 };
 struct Open {
-    int kind, want, my_id, at, at2;
+    int kind, want, my_id, group, stay;
     uint32_t near, out;
 };
 // The lanes' exact logits where no CTA has summed them: as given, or summed by this warp.
@@ -365,6 +365,7 @@ __device__ __forceinline__ double exact_of_lanes(const SelectParams& p, const Op
 __device__ __forceinline__ void exact_values(const SelectParams& p, const OpenRow& o, int want, double l, double z, double& r, double& v) {
     v = p.score == OCO_SCORE_SOFTMAX ? exp(l - (double)o.top) / z : 1.0 / (1.0 + exp(-l));
     r = !p.bias ? l : want >= 0 ? v + (double)p.bias[want] : 0.0;
+    if (r != r) r = -1.0 / 0.0;                                        // a bias that is NaN ranks last
 }
 // The softmax's sum is not exact where the logits are not: what it does to the difference of two values that have scores
 // va and vb in them.
@@ -489,11 +490,26 @@ __device__ __noinline__ bool settle(const SelectParams& p, OpenRow o, int lane, 
     if (q.kind == kGroups) {
         const bool two = p.best == 2 && p.E > p.G;
         const double part = two && !p.bias ? v : r;                    // of a group's worth
-        auto both = [&](double t, int at) { const double first = __shfl_sync(0xffffffffu, t, at), second = __shfl_sync(0xffffffffu, t, at + 1); return two ? first + second : first; };
-        const double a = both(part, 0), b = both(part, 2);
-        if (sum_matters(p, o, a - b, both(v, 0), both(v, 2))) q.kind = kAll;
+        double worth = 0.0, scores = 0.0;                              // lane g: of group g, and the scores in it
+        for (uint32_t rest = q.near; rest; rest &= rest - 1) {
+            const int g = __ffs((int)rest) - 1;
+            const Best a = warp_best(Best{part, q.want >= 0 && q.group == g ? lane : -1});
+            const Best b = warp_best(Best{part, two && q.want >= 0 && q.group == g && lane != a.i ? lane : -1});
+            const double sum = two ? __shfl_sync(0xffffffffu, v, a.i) + __shfl_sync(0xffffffffu, v, b.i & 31) : __shfl_sync(0xffffffffu, v, a.i);
+            if (lane == g) { worth = two ? a.v + b.v : a.v; scores = sum; }
+        }
+        const uint32_t border = q.near;
+        uint32_t left = border;
+        for (int t = 0; t < q.stay; t++) left &= ~(1u << warp_best(Best{worth, ((left >> lane) & 1u) ? lane : -1}).i);
+        bool doubt = false;                                            // between one that stays and one that goes
+        for (uint32_t rest = left; rest; rest &= rest - 1) {
+            const int g = __ffs((int)rest) - 1;
+            const double wg = __shfl_sync(0xffffffffu, worth, g), vg = __shfl_sync(0xffffffffu, scores, g);
+            doubt = doubt || (((border & ~left) >> lane) & 1u && sum_matters(p, o, worth - wg, scores, vg));
+        }
+        if (__any_sync(0xffffffffu, doubt)) q.kind = kAll;
         else {
-            if (b > a || (b == a && q.at2 < q.at)) q.out = (q.out | (1u << q.at)) & ~(1u << q.at2);
+            q.out = (q.out & ~border) | left;
             q = choose<VPL>(p, o, lane, margin, key, q);
             if (q.kind == kWinners) exact_values(p, o, q.want, exact_of_lanes(p, o, lane, q.want), z, r, v);
         }
@@ -525,32 +541,33 @@ __device__ __noinline__ bool settle(const SelectParams& p, OpenRow o, int lane, 
     return q.kind == kAll;
 }
 
-// What a decision between two groups needs: their best experts. Groups whose best are not clear go through exact_step.
+// What a decision between the groups in q.near needs: their best experts, and those that could be among these.
 template <int VPL>
 __device__ __noinline__ Open best_of_groups(const SelectParams& p, int lane, Margin margin, const uint32_t (&key)[VPL], Open q) {
     const int gs = p.E / p.G, best = min(p.best, gs);
     q.kind = kGroups;
-    for (int s = 0; s < 2; s++) {
-        // the three best of the group: values, and the experts of the first two
-        const int g = s ? q.at2 : q.at;
-        uint32_t m[3] = {0, 0, 0};
+    int n = 0;                                                         // lanes that want an expert
+    for (uint32_t rest = q.near; rest && q.kind == kGroups; rest &= rest - 1) {
+        const int g = __ffs((int)rest) - 1;
+        uint32_t k[VPL];
+        int m = 0;                                                     // the lane's keys of the group, still in order
 #pragma unroll
+        for (int i = 0; i < VPL; i++) k[i] = 0u;
+#pragma unroll 1
         for (int i = 0; i < VPL; i++)
-            if (key[i] && expert_of<VPL>(key[i], lane) / gs == g) {
-                if (!m[0]) m[0] = key[i];
-                else if (!m[1]) m[1] = key[i];
-                else if (!m[2]) m[2] = key[i];
-            }
-        float v[3];
-#pragma unroll
-        for (int t = 0; t < 3; t++) {
-            const uint32_t a = warp_max(m[0]);
-            const int from = __ffs((int)__ballot_sync(0xffffffffu, m[0] == a)) - 1;
-            v[t] = a ? key_value(a) : -INFINITY;
-            if (t < best && lane == 2 * s + t) q.want = expert_of<VPL>(a, from);
-            if (lane == from) { m[0] = m[1]; m[1] = m[2]; m[2] = 0; }
+            if (key[i] && expert_of<VPL>(key[i], lane) / gs == g) k[m++] = key[i];
+        m = 0;
+        float last = 0.f;
+        for (int t = 0;; t++) {
+            const uint32_t mine = m < VPL ? k[m] : 0u, a = warp_max(mine);
+            if (!a || (t >= best && !margin.near(last, key_value(a)))) break;
+            if (n == 32 || t == 6) { q.kind = kAll; break; }           // so many are near only where values are equal
+            const int from = __ffs((int)__ballot_sync(0xffffffffu, mine == a)) - 1;
+            if (lane == n) { q.want = expert_of<VPL>(a, from); q.group = g; }
+            if (lane == from) m++;
+            if (t < best) last = key_value(a);
+            n++;
         }
-        if (gs > best && (best == 2 ? margin.near(v[1], v[2]) : margin.near(v[0], v[1]))) q.kind = kAll;
     }
     return q;
 }
@@ -714,28 +731,24 @@ __device__ __forceinline__ Open select_row(const SelectParams& p, int row, float
             }
         }
         const uint32_t wkey = lane < p.G ? rank_key(worth) : 0u;
-        uint32_t kprev = 0, kt = 0;
-        int at = 0;
+        uint32_t kt = 0;
         out = p.G == 32 ? 0xffffffffu : (1u << p.G) - 1u;
         for (int t = 0; t < p.TG; t++) {
             const uint32_t mine = (out >> lane) & 1u ? wkey : 0u;
-            kprev = kt;
             kt = warp_max(mine);
-            at = __ffs((int)__ballot_sync(0xffffffffu, mine == kt && ((out >> lane) & 1u))) - 1;
-            out &= ~(1u << at);
+            out &= ~(1u << (__ffs((int)__ballot_sync(0xffffffffu, mine == kt && ((out >> lane) & 1u))) - 1));
         }
         const uint32_t mine = (out >> lane) & 1u ? wkey : 0u, k2 = warp_max(mine);
-        const int at2 = __ffs((int)__ballot_sync(0xffffffffu, mine == k2 && ((out >> lane) & 1u))) - 1;
         const float wa = key_rank(kt), wb = key_rank(k2);
         // error of a worth: of one value, or of two and the rounding of their sum
         const float size = !pairs ? fabsf(wa) : p.bias ? __uint_as_float(wide) : 1.f;
         const float one = (pairs && !p.bias ? es : ek) + (VPL > 1 ? 2.f * VPL * kHalfUlp * size + kLeast : 0.f) + (shifted ? 2.f : 1.f) * kHalfUlp * size;
         const float near_w = pairs ? 4.f * one : 2.f * one;
         if ((VPL > 1 || ek > 0.f || pairs) && !(wa - wb > near_w) && !any_bad) {
-            // the border lies between two groups, or more
-            const uint32_t k3 = warp_max((out >> lane) & 1u && lane != at2 ? wkey : 0u);
-            q.at = at; q.at2 = at2; q.out = out;
-            if ((p.TG > 1 && !(key_rank(kprev) - wb > near_w)) || (k3 != 0u && !(wa - key_rank(k3) > near_w))) { q.kind = kAll; return q; }
+            // every group that could be on the other side of the border
+            q.near = __ballot_sync(0xffffffffu, lane < p.G && ((out >> lane) & 1u ? !(wa - worth > near_w) : !(worth - wb > near_w)));
+            q.stay = __popc(q.near & ~out);
+            q.out = out;
 #pragma unroll
             for (int i = 0; i < VPL; i++) kept[i] = key[i];
             return best_of_groups<VPL>(p, lane, margin, kept, q);
