@@ -15,7 +15,7 @@ struct oco_moe_router : PlanBase {
     const float* bias = nullptr;
     uint32_t* status = nullptr;
     uint32_t* arrivals = nullptr;     // route_rows_kernel's counters, left at zero by every call
-    float* w_norm = nullptr;          // the largest norm of an expert's weights
+    float* w_norm = nullptr;          // the largest norms of an expert's weights (SelectParams)
     float* logits = nullptr;
     float* errors = nullptr;          // of the logits of a row, for each 128 experts
     uint16_t* pieces = nullptr;       // the weights as three bf16 pieces [3][experts rounded up to 128][hidden]
@@ -52,7 +52,7 @@ int lay_out(oco_moe_router* r) {
     OCO_CK(r, cudaDeviceSynchronize());     // the weights have been written, on whatever stream
     router_pieces_kernel<<<4 * r->sm_count, 256>>>(r->w, r->pieces, d.experts, Ep, d.hidden);
     OCO_CK(r, cudaGetLastError());
-    OCO_CK(r, cudaMemset(r->w_norm, 0, 4));
+    OCO_CK(r, cudaMemset(r->w_norm, 0, 20));
     router_norms_kernel<<<d.experts, 256>>>(r->w, (uint32_t*)r->w_norm, d.hidden);
     OCO_CK(r, cudaGetLastError());
     OCO_CK(r, cudaDeviceSynchronize());

@@ -8,10 +8,11 @@
 // own, and after every 64 terms (four additions to it) both are read out and added, rounding to nearest, to sums in
 // registers.
 //
-// The selection has to know how far a logit may be off. In units of 2^-24 |x| |w|: 17 / 2 + 2 for each of the four MMAs,
-// 2^-8 of twice that for the smaller pieces, one for the sum of both accumulators: 44. The sums in registers and of the
-// parts: 2^-24 of the largest partial sum of a row, which is kept, for each addition. The rows' norms are taken from the
-// tiles in shared memory by the warps that wait for the MMAs anyway.
+// The selection has to know how far a logit may be off. In units of 2^-24 |x| |w|: 17 / 2 + 2 for each MMA that a term is
+// in its accumulator for: four for those of the first, one for those of the last. So norms are taken of every fourth 16
+// columns. 2^-8 of eight MMAs for the smaller pieces and one unit for the sum of both accumulators: one and a half. The
+// sums in registers and of the parts: 2^-24 of the largest partial sum of a row, which is kept, for each addition. The
+// rows' norms are taken from the tiles in shared memory by the warps that wait for the MMAs anyway.
 //
 // One item = 128 rows x 128 experts; a contraction is split over the CTAs of a cluster while items do not fill the SMs,
 // and the parts are added through distributed shared memory in the order of their ranks. Each stage of shared memory
@@ -24,11 +25,11 @@ namespace oco {
 
 struct RouterTile {
     static constexpr int kTile = 128 * 128, kStage = 4 * kTile, kStages = 3;
-    static constexpr int kPitch = 132;                   // f32 of a row of the parts: eight rows' 16-byte pieces fill the banks; then squares and the largest sum of both halves
-    static constexpr float kUnits = 45.f;                // of 2^-24 |x| |w|: the error of what tensor memory has summed
+    static constexpr int kPitch = 132;                   // f32 of a row of the parts: eight rows' 16-byte pieces fill the banks
+    static constexpr int kRowsAt = 128 * kPitch;         // behind the parts: [row][4 sums of squares, the largest sums of both halves, -, -]
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;   // warps 0 .. 7 hold the sums
     static constexpr int kCtrl = 256, kSmem = kStages * kStage + kCtrl + 1024;
-    static_assert(128 * kPitch * 4 <= kStages * kStage, "the parts lie where the stages were");
+    static_assert((kRowsAt + 128 * 8) * 4 <= kStages * kStage, "the parts lie where the stages were");
 };
 
 // Weights -> three bf16 pieces [piece][Ep][H], Ep = experts rounded up to 128 (rows behind the last expert are zero).
@@ -45,22 +46,24 @@ __global__ void __launch_bounds__(256) router_pieces_kernel(const float* __restr
     }
 }
 
-// The largest Euclidean norm of an expert's weights, rounded up (`largest`: zero before). An expert with a weight that is
-// not finite has no finite logit.
+// The largest Euclidean norms of an expert's weights (SelectParams::w_norm), rounded up (`largest`: zero before). An expert
+// with a weight that is not finite has no finite logit.
 __global__ void __launch_bounds__(256) router_norms_kernel(const float* __restrict__ w, uint32_t* __restrict__ largest, int H) {
-    __shared__ double part[8];
+    __shared__ double part[16];
     double s = 0.0;
-    for (int k = threadIdx.x; k < H; k += 256) {
+    for (int k = threadIdx.x; k < H; k += 256) {           // a thread stays with its fourth
         const double v = (double)w[(size_t)blockIdx.x * H + k];
         s = fma(v, v, s);
     }
-    s = warp_sum_d(s);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if ((threadIdx.x & 15) == 0) part[threadIdx.x >> 4] = s;
     __syncthreads();
-    if (threadIdx.x != 0) return;
+    if (threadIdx.x >= 5) return;
     s = 0.0;
-    for (int i = 0; i < 8; i++) s += part[i];
-    if (s < INFINITY) atomicMax(largest, __float_as_uint(__double2float_ru(sqrt(s))));
+    for (int i = 0; i < 16; i++)
+        if (threadIdx.x == 4 || i % 4 == (int)threadIdx.x) s += part[i];
+    if (s < INFINITY) atomicMax(largest + threadIdx.x, __float_as_uint(__double2float_ru(sqrt(s))));
 }
 
 __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         const int row = (warp & 3) * 32 + lane, col0 = warp < 4 ? 0 : 64;
         uint64_t sum[32];
         float big = 0.f;                                                   // largest magnitude of a partial sum
-        uint64_t squares = 0;                                              // of half of the row's elements
+        uint64_t squares[2] = {0, 0};                                      // of half of the row's elements, in two of the four parts
         uint32_t some = 0;
 #pragma unroll
         for (int j = 0; j < 32; j++) sum[j] = 0;
@@ -127,7 +130,7 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint64_t v = f32x2_bits(w[k] << 16, w[k] & 0xffff0000u);
-                    squares = fma_f32x2(v, v, squares);
+                    squares[j / 2] = fma_f32x2(v, v, squares[j / 2]);
                 }
                 some |= q.x | q.y | q.z | q.w;
             }
@@ -167,9 +170,14 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
         asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 32; j += 2) *reinterpret_cast<ulonglong2*>(part + row * S::kPitch + col0 + 2 * j) = make_ulonglong2(sum[j], sum[j + 1]);
-        float even, odd;
-        f32x2_split(squares, even, odd);
-        *reinterpret_cast<float2*>(part + row * S::kPitch + 128 + 2 * (warp >> 2)) = make_float2(even + odd + (some & 0x7fff7fffu ? kLostSquares : 0.f), big);
+        float* of_row = part + S::kRowsAt + row * 8;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float even, odd;
+            f32x2_split(squares[i], even, odd);
+            of_row[2 * (warp >> 2) + i] = even + odd + (some & 0x7fff7fffu ? kLostSquares : 0.f);
+        }
+        of_row[4 + (warp >> 2)] = big;
     } else if (warp == S::kTmaWarp) {
         if (lane == 0) {
             int g = 0;
@@ -217,6 +225,19 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
     // join: this CTA's share of the rows, a warp per row, four experts a lane
     const int live = min(128, rows - row0), cols = min(128, E - e0), c = 4 * lane;
     const bool wide = (E & 3) == 0 && ((uintptr_t)logits & 15u) == 0;
+    if (tid < live && tid % split == rank) {                               // how far the row's logits may be off
+        float n[4] = {0.f, 0.f, 0.f, 0.f}, big0 = 0.f, big1 = 0.f;
+        for (int q = 0; q < split; q++) {
+            const uint32_t at = base + 4u * (uint32_t)(S::kRowsAt + tid * 8);
+            const float4 squares = peer_f32x4(at, (uint32_t)q), largest = peer_f32x4(at + 16u, (uint32_t)q);
+            n[0] += squares.x; n[1] += squares.y; n[2] += squares.z; n[3] += squares.w;
+            big0 += largest.x; big1 += largest.y;
+        }
+        float e = product_error(1.5f, n[0] + n[1] + n[2] + n[3], w_norm[4]) + 1.01f * 5.9604645e-8f * (float)(per + split) * fmaxf(big0, big1);
+#pragma unroll
+        for (int i = 0; i < 4; i++) e += product_error(10.6f * (float)(4 - i), n[i], w_norm[i]);
+        errors[(size_t)(e0 / 128) * rows + row0 + tid] = e;
+    }
     for (int r = rank + split * warp; r < live; r += split * (S::kThreads / 32)) {
         const uint32_t at = base + 4u * (uint32_t)(r * S::kPitch + c);
         float4 v = peer_f32x4(at, 0);
@@ -225,18 +246,6 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
             const float4 w = peer_f32x4(at, (uint32_t)q);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
         }
-        float squares = 0.f, big = 0.f;
-        if (lane < split) {
-            const float4 both = peer_f32x4(base + 4u * (uint32_t)(r * S::kPitch + 128), (uint32_t)lane);
-            squares = both.x + both.z;
-            big = fmaxf(both.y, both.w);
-        }
-#pragma unroll
-        for (int d = 4; d >= 1; d >>= 1) {                                 // split is at most 8
-            squares += __shfl_xor_sync(0xffffffffu, squares, d);
-            big += __shfl_xor_sync(0xffffffffu, big, d);
-        }
-        if (lane == 0) errors[(size_t)(e0 / 128) * rows + row0 + r] = product_error(S::kUnits, squares, *w_norm) + 1.01f * 5.9604645e-8f * (float)(per + split) * big;
         float* dst = logits + (size_t)(row0 + r) * E + e0 + c;
         if (wide && c < cols) *reinterpret_cast<float4*>(dst) = v;
         else {

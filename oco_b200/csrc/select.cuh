@@ -26,7 +26,7 @@ struct SelectParams {
     float* probs;
     uint32_t* status;        // null, or a status word: set = nothing is written
     const float* errors;     // behind the product: largest error of a row's logits, [tiles of 128 experts][rows]
-    const float* w_norm;     // largest Euclidean norm of an expert's weights
+    const float* w_norm;     // largest Euclidean norms of an expert's weights: of every fourth 16 columns from 0, 16, 32, 48 on, and of all
     int rows, E, H, K, G, TG, best, score, normalize;
     float scale;
 };
@@ -896,7 +896,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const SelectParams p, f
     __syncthreads();
     if (!last) return;
     const bool mine = warp < 4 && t0 + warp < p.rows;
-    select_tokens<VPL, true>(p, mine ? t0 + warp : -1, mine ? product_error(5.1f, squares[warp] + squares[warp + 4], __ldcg(p.w_norm)) : 0.f, &sh);
+    select_tokens<VPL, true>(p, mine ? t0 + warp : -1, mine ? product_error(5.1f, squares[warp] + squares[warp + 4], __ldcg(p.w_norm + 4)) : 0.f, &sh);
 }
 
 }  // namespace oco
