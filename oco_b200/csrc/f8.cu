@@ -14,9 +14,11 @@ namespace {
 // of as many rows, the pair's two of 128.
 constexpr int kTileRows[5] = {16, 32, 64, 128, 256}, kRowBoxes[4] = {16, 32, 64, 128};
 constexpr int kWideIndex = 3, kPairIndex = 4;
-// Rows up to which a dense product rounds them itself (one launch less; 4096 -> 6144 features, 1 / 4 / 8 / 16 rows: 7.1 / 8.8 /
-// 11.5 / 17.1 us against 10.2 / 9.6 / 9.5 / 9.9), and tokens of a routed call up to which every route is a tile of its own (two
-// launches instead of five; eight of 128 experts, 2 / 3 / 4 tokens: 23.5 / 26.8 / 36.9 us against 28.6 / 32.5 / 37.2).
+// Rows up to which a dense product rounds them itself (one launch less; 4 / 8 / 16 rows through 4096 -> 6144 features: 7.5 /
+// 9.5 / 13.3 us against 10.1 / 10.2 / 10.3, 8192 -> 1024: 6.9 / 8.5 / 12.0 against 10.1, 2048 -> 512: 5.2 / 5.1 / 5.9 against
+// 10), and tokens of a routed call up to which every route is a tile of its own (two launches instead of five; 2048 x 768,
+// eight of 128 experts, 1 / 2 / 3 tokens: 17.3 / 21.8 / 25.8 us against 24.7 / 27.6 / 33.4, 4096 x 1536, two of 128: 16.3 /
+// 22.6 / 36.4 against 22.3 / 28.1 / 39.7).
 constexpr int kOwnRows = 4, kOwnTokens = 3;
 enum F8Kind { kF8Projection = OCO_DENSE_PROJECTION, kF8Gated = OCO_DENSE_FFN_SILU_GATE, kF8Experts = 100 };
 

@@ -41,6 +41,8 @@ struct F8TileParams {
     int n, K, rows, pitch, top_k, experts;
 };
 
+// silu(g) * u. The sigmoid is that of the other formats' tiles, to about 1e-6: of activations that are rounded to four bits
+// right away.
 __device__ __forceinline__ float silu_times(float g, float u) { return sigmoid_times(g, 1.0f) * g * u; }
 // ---- many rows --------------------------------------------------------------------------------------------------------
 // PAIR: two SMs multiply one tile of 256 rows (tcgen05.mma.cta_group::2): each brings its own 128 rows and half of the 256

@@ -6,7 +6,7 @@
 // Everything is first done in 32 bits. Two ranking values that lie within each other's error (rounding of the score, of
 // score + bias, and the error of the logit where it came from the router product) leave their order open; such a token
 // is settled in 64 bits, where the logits that matter are summed again from x and the weights. With continuous logits that
-// is a token in a few hundred where logits are given or rows are few, one in twenty behind the tensor cores, whose sums
+// is a token in a few hundred where logits are given or rows are few, one in thirty behind the tensor cores, whose sums
 // have the wider bound.
 #pragma once
 #include <type_traits>
@@ -67,7 +67,8 @@ __device__ __forceinline__ float product_error(float units, float squares, float
 // quotient's two units: below 4e-7.
 // A softmax score relative to the largest one: the same and the rounding of l - top (x e^-x < 0.37), the sum and its
 // reciprocal. kHalfUlp: the rounding of score + bias.
-// kFarError: up to here e^d - 1 is d but for a twentieth. kLeast: 2^-126, below which the last bits of a value (an index stands there in a sorted key) weigh more than its size tells.
+// kFarError: up to here e^d - 1 is d but for a twentieth. kLeast: 2^-126, below which the last bits of a value (an index
+// stands there in a sorted key) weigh more than its size tells.
 constexpr float kSigmoidError = 4e-7f, kScoreError = 6e-7f, kHalfUlp = 6e-8f, kFarError = 0.01f, kLeast = 1.1754944e-38f;
 
 // ---- exact logits ----------------------------------------------------------------------------------------------------
@@ -772,7 +773,7 @@ __device__ __forceinline__ void select_tokens(const SelectParams& p, int row, fl
     double l = 0.0;
     uint32_t lanes = 0;
     int at = 0;
-    // `wanted` experts of the lanes, up to 32 of a warp, are summed by the CTA; each lane gets its own
+    // the CTA sums the logits that its lanes want; each lane gets its own
     auto sum_wanted = [&](bool wants, int expert) {
         lanes = __ballot_sync(0xffffffffu, wants);
         at = __popc(lanes & ((1u << lane) - 1u));
