@@ -457,3 +457,43 @@ def test_norm_of_the_weights_follows_a_new_binding(moe):
         r.forward(x, ids, probs, 100)
         want, _ = expect(shape, x.double() @ weights.double().t(), b)
         assert np.array_equal(ids.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("shape", [(512, 16, "softmax", 32, 7, 2, True, True, 1.0), (512, 16, "sigmoid", 1, 1, 1, False, True, 1.0), (384, 9, "softmax", 1, 1, 1, True, True, 1.0),
+                                   (256, 8, "sigmoid", 8, 4, 2, True, True, 2.5), (128, 8, "softmax", 4, 2, 2, False, False, 1.0), (64, 6, "sigmoid", 16, 5, 1, False, True, 1.0),
+                                   (32, 4, "softmax", 4, 2, 2, True, True, 1.0), (270, 9, "sigmoid", 5, 2, 2, False, True, 1.0)], ids=str)
+@pytest.mark.parametrize("copies", ["all", "quarters", "last bits"])
+def test_more_open_decisions_than_one(moe, shape, copies):
+    """Experts that are copies of one another, or differ in the last bits of their weights: more than a warp's lanes are too
+    near, at the border of the groups too. Rows of zeros among them. The ids are the definition's, from the product (rows on
+    both sides of its forms) and from logits."""
+    E, rows = shape[0], 40
+    r, w, b, g = make(moe, shape, 512, rows, 48)
+    few = {"all": 1, "quarters": max(1, E // 4), "last bits": max(1, E // 8)}[copies]
+    w = w[:few].repeat(-(-E // few), 1)[:E].contiguous()
+    if copies == "last bits":
+        w *= 1.0 + (torch.rand((E, 512), device="cuda", generator=g) - 0.5) * 2e-7
+    if b is not None:
+        b = b[:few].repeat(-(-E // few))[:E].contiguous()
+    r.bind(w, b)
+    # small whole numbers: with weights that are copies the sums are equal in any order; else far apart against 64 bits
+    x = torch.randint(-4, 5, (rows, 512), device="cuda", generator=g).to(torch.bfloat16)
+    x[3] = x[25] = 0
+    exact = x.double() @ w.double().t()
+    if copies != "last bits":
+        exact = exact[:, :few].repeat(1, -(-E // few))[:, :E]
+    want, p = expect(shape, exact, b)
+    for n in (5, 40):
+        ids, probs = outputs(shape, n)
+        r.forward(x[:n].contiguous(), ids, probs, n)
+        r.poll()
+        assert np.array_equal(ids.cpu().numpy(), want[:n]), n
+        np.testing.assert_allclose(probs.cpu().numpy(), p[:n], rtol=2.0 ** -14)
+    logits = exact.float()
+    want, p = expect(shape, logits.double(), b)
+    ids, probs = outputs(shape, rows)
+    r.select(logits, ids, probs, rows)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    # a score is the exponential of l - top, which is rounded by 2^-24 of the logits' spread (up to 30 here: 1.8e-6), and so is
+    # the sum that divides it
+    np.testing.assert_allclose(probs.cpu().numpy(), p, rtol=REL + 2.0 ** -23 * float(logits.max() - logits.min()))
