@@ -227,7 +227,9 @@ __global__ void __launch_bounds__(RouterTile::kThreads, 1) router_tile_kernel(co
     const bool wide = (E & 3) == 0 && ((uintptr_t)logits & 15u) == 0;
     if (tid < live && tid % split == rank) {                               // how far the row's logits may be off
         float n[4] = {0.f, 0.f, 0.f, 0.f}, big0 = 0.f, big1 = 0.f;
-        for (int q = 0; q < split; q++) {
+#pragma unroll
+        for (int q = 0; q < 8; q++) {                                      // all on their way at once
+            if (q >= split) continue;
             const uint32_t at = base + 4u * (uint32_t)(S::kRowsAt + tid * 8);
             const float4 squares = peer_f32x4(at, (uint32_t)q), largest = peer_f32x4(at + 16u, (uint32_t)q);
             n[0] += squares.x; n[1] += squares.y; n[2] += squares.z; n[3] += squares.w;
