@@ -365,9 +365,9 @@ size_t oco_dense_workspace_bytes(const oco_dense_plan* plan, int max_rows);
 int oco_dense_bind_workspace(oco_dense_plan* plan, void* workspace, size_t bytes, int max_rows);
 int oco_dense_bind_weights(oco_dense_plan* plan, const oco_dense_weights* weights);
 /* OCO_FMT_F8_E4M3 (OCO_DENSE_PROJECTION and OCO_DENSE_FFN_SILU_GATE; hidden and ffn multiples of 32, codes 16-byte
- * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes (binding waits as oco_moe_f8_bind_weights does). The arithmetic
- * is that of the oco_moe_f8_plan calls at every row count: no single-token numerics of its own. 0 rows are no work; a
- * projection's y must not overlap x. */
+ * aligned): f32 scales [ceil(rows / 128)][ceil(columns / 128)] of each matrix, bound after its codes (binding waits as
+ * oco_moe_f8_bind_weights does). The arithmetic is that of the oco_moe_f8_plan calls at every row count: no single-token
+ * numerics of its own. 0 rows are no work; a projection's y must not overlap x. */
 typedef struct {
     const float* up_s;
     const float* gate_s;
